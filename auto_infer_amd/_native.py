@@ -30,16 +30,24 @@ SIGNATURES = {
                      c_i64, c_vp],
     "aia_kv_write_nz": [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_i64,
                         c_vp],
+    "aia_kv_write_fp8": [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32,
+                         c_i32, c_i32, c_i64, c_vp],
     "aia_attn_workspace_bytes": [c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
                                  ctypes.POINTER(c_i64)],
     "aia_attn_workspace_layout": [c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
                                   ctypes.POINTER(c_i64), c_i32],
     "aia_attn_plan": [c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
                       c_vp, c_i64, c_vp],
+    "aia_attn_plan_prefix": [c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
+                             c_i32, c_i32, c_vp, c_i64, c_vp],
     "aia_paged_attention_gqa": [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp,
                                 c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_f32,
                                 c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_i32, c_i32,
                                 c_vp, c_i64, c_vp],
+    "aia_paged_attention_gqa_ex": [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp,
+                                   c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_f32,
+                                   c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp,
+                                   c_vp, c_vp, c_f32, c_i32, c_i32, c_vp, c_i64, c_vp],
     "aia_paged_attention_gqa_noalloc": [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_i32, c_vp,
                                         c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32,
                                         c_f32, c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64,
@@ -56,6 +64,8 @@ SIGNATURES = {
     "aia_splice_tokens": [c_vp, c_i32, c_vp, c_i64, c_vp],
     "aia_qk_norm_rope": [c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp, c_i64, c_vp, c_i64,
                          c_vp, c_vp, c_f32, c_vp],
+    "aia_rope_qk": [c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_i32, c_f32, c_i32, c_vp,
+                    c_vp, c_f32, c_vp, c_i64, c_vp, c_i64, c_vp],
     "aia_mla_kv_latent": [c_vp, c_i64, c_i32, c_vp, c_f32, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64,
                           c_vp],
     "aia_mla_q_latent": [c_vp, c_i64, c_i64, c_i32, c_i32, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp,

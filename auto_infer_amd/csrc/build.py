@@ -10,6 +10,8 @@ import os
 import subprocess
 import sys
 import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
@@ -17,8 +19,8 @@ ROOT = os.path.dirname(PKG)
 OUT_DIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(OUT_DIR, "libautoinfer_amd.so")
 PROBES = os.path.join(OUT_DIR, "libaia_probes.so")
-SOURCES = ["core.hip", "kv_write.hip", "paged_attention.hip", "noalloc.hip", "pack.hip", "qk_rope.hip",
-           "mtp_compact.hip", "mla_pre.hip"]
+SOURCES = ["core.hip", "kv_write.hip", "kv_write_fp8.hip", "paged_attention.hip", "gqa_scored.hip",
+           "gqa_fp8.hip", "noalloc.hip", "pack.hip", "qk_rope.hip", "rope.hip", "mtp_compact.hip", "mla_pre.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
@@ -57,13 +59,22 @@ def build_hostpack(verbose=False):
 def build(verbose=False):
     build_hostpack(verbose)
     os.makedirs(OUT_DIR, exist_ok=True)
-    srcs = [os.path.join(HERE, s) for s in SOURCES]
-    tmp = LIB + ".tmp"
-    cmd = [hipcc(), *HIPCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-I", HERE,
-           *srcs, "-o", tmp]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
+    flags = [*HIPCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-I", HERE]
+    with tempfile.TemporaryDirectory() as objs:
+        def compile_one(src):
+            obj = os.path.join(objs, src + ".o")
+            cmd = [hipcc(), *flags, "-c", os.path.join(HERE, src), "-o", obj]
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            subprocess.run(cmd, check=True)
+            return obj
+        with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+            built = list(pool.map(compile_one, SOURCES))
+        tmp = LIB + ".tmp"
+        cmd = [hipcc(), *HIPCC_FLAGS, *built, "-o", tmp]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
     tmp = PROBES + ".tmp"
     cmd = [hipcc(), *HIPCC_FLAGS, os.path.join(HERE, "probes.hip"), "-o", tmp]

@@ -34,40 +34,9 @@
 #include <mutex>
 #include <type_traits>
 
-#include "common.h"
+#include "gqa_attention.h"
 
 namespace {
-
-using aia::float4_t;
-using aia::short4_t;
-
-constexpr int kHeadDim = 128;
-constexpr int kTile = 16;         // keys per MFMA tile
-constexpr int kRows = 16;         // query rows per segment (MFMA N)
-// LDS row stride (elements) of a staged V tile: 288 bytes puts the 16 rows
-// of a transposing read in distinct banks
-constexpr int kVStride = 144;
-constexpr int kMaxBatch = 8192;   // planner keeps the request offsets in LDS
-constexpr int kDefaultWaves = 2048;
-constexpr int kMaxWaves = 16384;
-constexpr int kPlanThreads = 512;
-// Per-range work record: {segment, first tile, end tile, tiles per range,
-// the segment's 8-int record, first logical block, last segment of the
-// range, 2 pad, the first 16 block ids of the range} -- everything a
-// work-group needs to issue its first K/V loads after one load.
-constexpr int kRecInts = 32;
-constexpr int kRecBlocks = 16;
-
-constexpr int kMaxGroupWaves = 8;  // kv heads (waves) per work-group
-
-// A segment is (request, query block, kv-head group, head block): the
-// work-group that owns one of its key ranges runs one wave per kv head of
-// the group over the same keys, so every tile reads whole contiguous
-// (block_size x Hkv x D) cache slots.
-struct Geometry {
-  int32_t hkv, group, hb, nhb, qb, nw, nkvg, rb, qs, pf;
-  int32_t ncu;   // compute units of the current device (MLA range count and dealing)
-};
 
 // Compute units of the current device, queried once per device (256, the
 // MI355X's count, when no device is visible, e.g. a size query on a host
@@ -91,53 +60,6 @@ int32_t device_cus() {
   }
   return n;
 }
-
-// Prefill routing: a GQA request whose query rows (query tokens x group
-// heads) fill at least one prefill work item is planned for the prefill
-// kernel (all its rows' keys staged once per 128 rows in LDS) instead of
-// split-K segments.  AIA_PREFILL=0 builds the split-K-only planner.
-#ifndef AIA_PREFILL
-#define AIA_PREFILL 1
-#endif
-// AIA_MLA_PREFILL=0 keeps absorbed-MLA prefill steps on the split-K kernel.
-#ifndef AIA_MLA_PREFILL
-#define AIA_MLA_PREFILL 1
-#endif
-#ifndef AIA_PF_WAVES
-#define AIA_PF_WAVES 4
-#endif
-#ifndef AIA_PF_KEYS
-#define AIA_PF_KEYS 64
-#endif
-#ifndef AIA_PF_RT
-#define AIA_PF_RT 2
-#endif
-constexpr int kPfWaves = AIA_PF_WAVES;       // waves per prefill work-group
-constexpr int kPfRt = AIA_PF_RT;             // 16-row MFMA tiles per wave
-constexpr int kPfRows = 16 * kPfRt * kPfWaves;   // rows per prefill work item
-constexpr int kPfKeys = AIA_PF_KEYS;         // keys per staged K/V tile (32 or 64)
-// Items alone fill the chip when items x kv heads reach kPfTargetWgs (a
-// little under two resident work-groups per CU); below that, each item's key
-// tiles are cut into chunks of at least kPfMinChunk tiles, sized so all units
-// still fit in one round (fp16 partials scaled per row, merged with the
-// split-K partials' rule).  448 rather than 512: fewer, longer chunks write
-// fewer partials, and the CUs left with one work-group take the largest
-// units (configs[1] prefill chunks, us per call: 43.1 at 448 or 416, 44.6 at
-// 512, 44.1-44.5 at 384, 49.6-49.9 at 256-320; 416 is slower at 32K keys).
-#ifndef AIA_PF_TARGET
-#define AIA_PF_TARGET 448
-#endif
-constexpr int kPfTargetWgs = AIA_PF_TARGET;
-constexpr int kPfCutSlots = 512;     // most work-groups (units x kv heads) of a step with cut items
-static_assert(kPfTargetWgs <= kPlanThreads && kPfCutSlots <= kPlanThreads, "a thread per cut item and unit");
-constexpr int kPfRecBytes = 48;      // a dealt work-group's record: three int4
-static_assert(2 * kPfTargetWgs >= kPfCutSlots && (2 * kPfTargetWgs - kPfCutSlots) * kPfRows * 8 >=
-              kPfCutSlots * kPfRecBytes, "partials and records of a step with cut items");
-#ifndef AIA_MLA_LPT
-#define AIA_MLA_LPT 1
-#endif
-
-constexpr int kPfMinChunk = 8;
 
 constexpr int64_t kMlaRb2Rows = 2048;
 
@@ -179,23 +101,6 @@ Geometry geometry(int32_t hq, int32_t hkv, int32_t batch, int32_t tokens, int32_
   g.ncu = device_cus();
   return g;
 }
-
-#ifndef AIA_MIXED
-#define AIA_MIXED 1
-#endif
-// Prefill units and split-K ranges of a step run in one grid (gqa_mixed_kernel).
-__host__ __device__ inline bool mixed_grid(const Geometry& g, int32_t dv) {
-  return AIA_MIXED && g.pf && g.nw == kPfWaves && g.rb == 1 && dv == kHeadDim;
-}
-
-// Workspace layout (all offsets 256-byte aligned).
-struct Layout {
-  int64_t hdr, seg, wave, part_ml, part_o, req, mrg, pf, pfm, pfw, pf_o, pf_ml, total;
-  int64_t seg_cap, part_cap, mrg_cap, pf_cap, pf_unit_cap, pf_mrg_cap, pf_slots;
-};
-
-constexpr int kMergeDims = 16;   // output dims per merge element
-constexpr int kMrgInts = 8;      // merge record
 
 // Merge slices (64 elements of kMergeDims dims) per (segment, kv head) at most.
 int64_t merge_slices(const Geometry& g, int32_t dv) {
@@ -393,8 +298,11 @@ __device__ __forceinline__ int range_last_seg(const int* tb, int nseg, int lo, i
   return lo2;
 }
 
+// PREFIX: the first prefix[b] keys of request b are seen by all its rows.
+template <bool PREFIX>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ kvlen,
+    const int32_t* __restrict__ prefix,
     const int32_t* __restrict__ block_table, int64_t bt_stride, int32_t block_size,
     int32_t batch, Geometry g, int32_t waves, int32_t dv,
     int32_t* __restrict__ hdr, int32_t* __restrict__ seg, int32_t* __restrict__ wave_rec,
@@ -498,7 +406,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(
       const int nitems = (lq * g.group + kPfRows - 1) / kPfRows;
       r0 = (nitems - 1 - (f - item_off[b])) * kPfRows;
       const int last = min(lq * g.group, r0 + kPfRows) - 1;
-      const int kend = max(0, min(lk, lk - lq + last / g.group + 1));
+      int kend = max(0, min(lk, lk - lq + last / g.group + 1));
+      if (PREFIX) kend = max(kend, min(prefix[b], lk));
       return (kend + kPfKeys - 1) / kPfKeys;
     };
     // Up to one item per thread: its request, row and tiles stay in registers
@@ -725,7 +634,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(
       const int q0 = qblk * g.qs;
       const int nq = min(g.qs, lq - q0);
       const int lim_base = lk - lq + q0;
-      const int visible = max(0, min(lk, lim_base + nq));
+      int visible = max(0, min(lk, lim_base + nq));
+      if (PREFIX) visible = max(visible, min(prefix[b], lk));
       // at least one (fully masked) tile, so the work-group that owns it
       // writes the zero output of rows that see no key
       ntiles = max(1, (visible + kTile - 1) / kTile);
@@ -866,7 +776,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(
       e_lo = range_first_seg(lds, nseg, t0);
       e_lo2 = range_last_seg(lds, nseg, e_lo, t1);
       const int4 r0 = srec[2 * e_lo], r1 = srec[2 * e_lo + 1];
-      const int nblk_vis = (max(0, r1.x + (r0.w & 0xff)) + block_size - 1) / block_size;
+      int visible = max(0, r1.x + (r0.w & 0xff));
+      if (PREFIX) visible = max(visible, min(prefix[r0.x], kvlen[r0.x]));
+      const int nblk_vis = (visible + block_size - 1) / block_size;
       e_blk = ((t0 - r1.y) * kTile) / block_size;
       const int32_t* btrow = block_table + (int64_t)r0.x * bt_stride;
 #pragma unroll
@@ -960,7 +872,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(
     o4[1] = r0;
     o4[2] = r1;
     const int b = r0.x, nq = r0.w & 0xff, lim_base = r1.x;
-    const int visible = max(0, lim_base + nq);
+    int visible = max(0, lim_base + nq);
+    if (PREFIX) visible = max(visible, min(prefix[b], kvlen[b]));
     const int nblk_vis = (visible + block_size - 1) / block_size;
     const int blk_base = ((t0 - r1.y) * kTile) / block_size;
     o4[3] = make_int4(blk_base, lo2, j, k);
@@ -1094,8 +1007,10 @@ __device__ __forceinline__ int wave_total(int x) {   // sum over the 64 lanes, i
   return __builtin_amdgcn_readlane(wave_incl_scan(x), 63);
 }
 
+template <bool PREFIX>
 __global__ __launch_bounds__(kSmallPlanThreads) void plan_small_kernel(
     const int32_t* __restrict__ cu_q, const int32_t* __restrict__ kvlen,
+    const int32_t* __restrict__ prefix,
     const int32_t* __restrict__ block_table, int64_t bt_stride, int32_t block_size,
     int32_t batch, Geometry g, int32_t waves, int32_t dv,
     int32_t* __restrict__ hdr, int32_t* __restrict__ seg, int32_t* __restrict__ wave_rec,
@@ -1146,7 +1061,8 @@ __global__ __launch_bounds__(kSmallPlanThreads) void plan_small_kernel(
         const int q0 = qblk * g.qs;
         const int nq = min(g.qs, lq - q0);
         lim_base = lkb - lq + q0;
-        const int visible = max(0, min(lkb, lim_base + nq));
+        int visible = max(0, min(lkb, lim_base + nq));
+        if (PREFIX) visible = max(visible, min(prefix[b], lkb));
         nt = max(1, (visible + kTile - 1) / kTile);
         rec0 = b; rec1 = kvg | (hb << 16) | ((q0 + nq == lq) << 30);
         rec2 = q_begin + q0; rec3 = nq | (q0 << 8);
@@ -1238,7 +1154,9 @@ __global__ __launch_bounds__(kSmallPlanThreads) void plan_small_kernel(
     }
     const int4 r0 = srec[lo][0], r1 = srec[lo][1];
     const int b = r0.x, nq = r0.w & 0xff;
-    const int nblk_vis = (max(0, r1.x + nq) + block_size - 1) / block_size;
+    int visible = max(0, r1.x + nq);
+    if (PREFIX) visible = max(visible, min(prefix[b], kvlen[b]));
+    const int nblk_vis = (visible + block_size - 1) / block_size;
     const int blk_base = ((t0 - r1.y) * kTile) / block_size;
     const int32_t* btrow = block_table + (int64_t)b * bt_stride;
     int bv[kRecBlocks];
@@ -1261,940 +1179,6 @@ __global__ __launch_bounds__(kSmallPlanThreads) void plan_small_kernel(
     if (nseg == 0 || i >= q8 + (x < rem8 ? 1 : 0))
       *reinterpret_cast<int4*>(wave_rec + (int64_t)w * kRecInts) = make_int4(-1, 0, 0, tpw);
   }
-}
-
-// ---------------------------------------------------------------- attention
-
-struct AttnArgs {
-  const uint16_t* q;
-  int64_t q_ts, q_hs;
-  uint16_t* kc;
-  uint16_t* vc;
-  // this step's new K/V rows (T, Hkv, D); when set, keys at the new
-  // positions are read from them and written into the cache by the kernel
-  const uint16_t* kn;
-  const uint16_t* vn;
-  int64_t kn_ts, vn_ts;
-  const int32_t* bt;
-  int64_t bt_stride;
-  int32_t hkv, group, hb, bs, nb, nw;
-  float scale_log2;
-  const int32_t* seg;
-  const int32_t* wave_rec;
-  uint16_t* part_o;          // split partials (fp16, scaled per row)
-  float2* part_ml;
-  uint16_t* out;
-  int64_t o_ts, o_hs;
-  int32_t waves;
-  const int32_t* hdr;
-  int32_t batch, tokens;
-};
-
-// A record is used only if it lies inside the plan (defence against a plan
-// read before its planner finished, e.g. from another stream).
-__device__ __forceinline__ bool rec_ok(const int* r, int nseg_tiles, int batch, int tokens,
-                                       int ngroups, int nhb) {
-  return r[0] >= 0 && r[0] < batch && (r[1] & 0xffff) < ngroups && ((r[1] >> 16) & 0x3fff) < nhb &&
-         r[2] >= 0 && (r[3] & 0xff) >= 1 && r[2] + (r[3] & 0xff) <= tokens && r[5] >= 0 && r[5] < r[6] &&
-         r[6] <= nseg_tiles;
-}
-
-using aia::kWaitVmcnt0;
-
-__device__ __forceinline__ short4_t as_s4(uint32_t a, uint32_t b) {
-  short4_t r;
-  r[0] = (short)(a & 0xffff); r[1] = (short)(a >> 16);
-  r[2] = (short)(b & 0xffff); r[3] = (short)(b >> 16);
-  return r;
-}
-
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef __attribute__((address_space(3))) short4_t lds_short4_t;
-
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
-  const half2_t v = {(_Float16)lo, (_Float16)hi};
-  return __builtin_bit_cast(uint32_t, v);
-}
-
-
-__device__ __forceinline__ u32x4_t as_u4(uint4 v) { return u32x4_t{v.x, v.y, v.z, v.w}; }
-
-__device__ __forceinline__ bf16x8_t as_b8(uint4 v) { return __builtin_bit_cast(bf16x8_t, as_u4(v)); }
-
-// S^T tile (16 keys x 16 rows) += K (16 keys x 32 dims) . Q^T: lane (key n,
-// group g) holds dims [32 j + 8 g, +8) of its key in kk and of its row in q.
-__device__ __forceinline__ float4_t qk_step(uint4 kk, uint4 q, float4_t acc) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_b8(kk), as_b8(q), acc, 0, 0, 0);
-}
-
-// A V tile is staged in LDS key-major (row stride kVStride elements): lane
-// (key n, group g) stores its 16-byte pieces at dims 32 j + 8 g.  The
-// transposing LDS read works within each 16-lane group: local lane l receives
-// element l % 4 of the 8 bytes addressed by local lanes 4 k + l / 4, k = 0..3.
-// Lane (n, g) addressing key 4 g + n / 4, dims 16 dt + 4 (n % 4) therefore
-// receives V^T[16 dt + n][keys 4 g .. 4 g + 3], the A fragment of the
-// 16x16x16 MFMA, in one instruction.  (The stores take vector values: an
-// aggregate copy of the tile registers keeps them in a private array, which
-// the compiler then places in LDS, serialising the load pipeline.)
-template <int KJ>
-__device__ __forceinline__ void stage_v(uint16_t* vs, int n, int g, const uint4 (&vv)[KJ]) {
-#pragma unroll
-  for (int j = 0; j < KJ; ++j) *reinterpret_cast<u32x4_t*>(vs + n * kVStride + 32 * j + 8 * g) = as_u4(vv[j]);
-}
-template <int STRIDE = kVStride>
-__device__ __forceinline__ short4_t vt_frag(const uint16_t* vs, int n, int g, int dt) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-      (lds_short4_t*)(vs + (4 * g + (n >> 2)) * STRIDE + 16 * dt + 4 * (n & 3)));
-}
-
-// Tiles kept in flight per GQA wave (registers: 32 VGPRs per tile).  One is
-// fastest: with random blocks, more outstanding tiles per CU lowers the
-// delivered bandwidth (measured on config-1 decode: 18.7 us at 1, 20.1 at 2,
-// 24.9 at 5), and the planner keeps ranges short instead.
-#ifndef AIA_PIPE
-#define AIA_PIPE 1
-#endif
-constexpr int kPipe = AIA_PIPE;
-
-// Processes key tiles [lt0, lt1) of one segment; rec = the segment record.
-// A segment holds RB blocks of 16 query rows: block r has the segment's
-// query tokens [r qb, r qb + qb), row n being token n / hb, head n % hb
-// (qb = 16 / hb).  Every K/V tile is loaded once and used by all blocks, so a
-// prefill chunk reads its keys 1/RB as often; blocks past the segment's last
-// token are skipped (a uniform branch), so a decode segment costs one block.
-// Cache layouts.  ND: (num_blocks, block_size, Hkv, D), a token slot's heads
-// contiguous.  NZ: the 16-wide fractal layout of the reference's graph-mode
-// caches (gqa.py:163,202-226): each block viewed (Hkv D / 16, block_size,
-// 16), so 16 dims of all of a block's tokens are contiguous.  kv_piece gives
-// the 16-byte index of piece p (8 dims) of head h of (block, offset).
-template <bool NZ>
-__device__ __forceinline__ int64_t kv_piece(int64_t blk, int off, int bs, int row_elems, int h,
-                                            int D, int p) {
-  if (!NZ) return (((blk * bs + off) * row_elems + (int64_t)h * D) >> 3) + p;
-  return ((blk * bs * row_elems) >> 3) +
-         (((int64_t)(h * (D / 16) + (p >> 1)) * bs + off) << 1) + (p & 1);
-}
-
-template <int RB, int D, bool NZ>
-__device__ __forceinline__ void gqa_segment(const AttnArgs& a, const int* rec, int s, int lt0,
-                                            int lt1, int w, int tpw, uint16_t* vt, int lane,
-                                            int wid, bool use_pre, int pre) {
-  constexpr int KJ = D / 32;   // 32-dim MFMA k-steps = 16-byte chunks per lane and row
-  constexpr int DT = D / 16;   // 16-dim output tiles
-  const int n = lane & 15, g = lane >> 4;
-  const int b = rec[0], kvh = (rec[1] & 0xffff) * a.nw + wid, hbi = (rec[1] >> 16) & 0x3fff;
-  const int qtok0 = rec[2], nq = rec[3] & 0xff, q0 = rec[3] >> 8, lim_base = rec[4];
-  const int tile_begin = rec[5], tile_end = rec[6], part_base = rec[7];
-  const int qb = kRows / a.hb;
-  const int nt = n / a.hb, hh = n - nt * a.hb;
-  const int nblk = (nq + qb - 1) / qb;               // row blocks holding tokens
-  const int head = kvh * a.group + hbi * a.hb + hh;
-  int qi[RB], lim[RB];
-  bool rv[RB];
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    qi[r] = r * qb + nt;
-    rv[r] = nt < qb && qi[r] < nq && hbi * a.hb + hh < a.group;
-    lim[r] = rv[r] ? lim_base + qi[r] : -1;
-  }
-  const int visible = max(0, lim_base + nq);
-  // smallest key limit of the valid rows (wave-uniform)
-  int lim_lo = 0x7fffffff;
-#pragma unroll
-  for (int r = 0; r < RB; ++r) lim_lo = rv[r] ? min(lim_lo, lim[r]) : lim_lo;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) lim_lo = min(lim_lo, __shfl_xor(lim_lo, d));
-  const int row_elems = a.hkv * D;
-  // this step's new keys sit at positions [new_start, Lk); the request's last
-  // query block (head block 0) owns writing them into the cache
-  const int new_start = a.kn ? lim_base - q0 : 0x7fffffff;
-  const int q_begin = qtok0 - q0;
-  const bool writer = a.kn && ((rec[1] >> 30) & 1) && hbi == 0;
-
-  const int32_t* btrow = a.bt + (int64_t)b * a.bt_stride;
-  const int nblk_vis = (visible + a.bs - 1) / a.bs;
-  int blk_base = 0, btv = 0, w1 = 0;
-  // 16-byte pieces between MFMA k-steps j and j + 1 of a cached key (4 pieces
-  // on in ND; two 16-dim chunks of block_size x 16 on in NZ)
-  const int64_t jstride = NZ ? 4 * (int64_t)a.bs : 4;
-
-  uint4 qf[RB][KJ];
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    if (rv[r]) {
-      const uint4* qp = reinterpret_cast<const uint4*>(
-          a.q + (int64_t)(qtok0 + qi[r]) * a.q_ts + (int64_t)head * a.q_hs);
-#pragma unroll
-      for (int j = 0; j < KJ; ++j) qf[r][j] = qp[4 * j + g];
-    } else {
-#pragma unroll
-      for (int j = 0; j < KJ; ++j) qf[r][j] = make_uint4(0, 0, 0, 0);
-    }
-  }
-
-  float4_t o[RB][DT];
-  float m[RB], lsum[RB];
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[r][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
-    m[r] = -1e30f;
-    lsum[r] = 0.f;
-  }
-
-  // Block ids are held one per lane for a window of 64 logical blocks; the
-  // window is (re)loaded only between pipelined runs, so the per-tile address
-  // shuffle never waits on an outstanding global load.
-  // Loads are issued unconditionally (tiles past the window read the
-  // window's first key row, K and V, again: an L1 hit, and a different row
-  // for every range, so no memory channel is hammered) so the load stream is
-  // straight-line and the compiler can wait for each tile with an exact count.
-  auto load = [&](int lt, uint4 (&kk)[KJ], uint4 (&vv)[KJ], int64_t& wdst) {
-    const bool live = lt < w1;
-    const int tok = live ? min(lt * kTile + n, visible - 1) : blk_base * a.bs;
-    const int bi = tok / a.bs;
-    // block ids outside the pool are clamped so a bad table cannot fault
-    const int blk = min(max(__shfl(btv, bi - blk_base), 0), a.nb - 1);
-    const int off = tok - bi * a.bs;
-    // 16-byte index of this lane's first piece (4 g + 0) in the cache; piece
-    // 4 j + g is jstride further on in either layout
-    const int64_t base = kv_piece<NZ>(blk, off, a.bs, row_elems, kvh, D, g);
-    const bool fresh = live && tok >= new_start;
-    const int64_t nrow = (int64_t)(q_begin + tok - new_start);
-    const uint4* kp = fresh ? reinterpret_cast<const uint4*>(a.kn + nrow * a.kn_ts + (int64_t)kvh * D) + g
-                            : reinterpret_cast<const uint4*>(a.kc) + base;
-    const uint4* vp = fresh ? reinterpret_cast<const uint4*>(a.vn + nrow * a.vn_ts + (int64_t)kvh * D) + g
-                            : reinterpret_cast<const uint4*>(a.vc) + base;
-    const int64_t js = fresh ? 4 : jstride;
-    // cache slot this lane writes after the tile arrives (-1: nothing)
-    wdst = (writer && fresh && lt * kTile + n < visible) ? base : (int64_t)-1;
-#pragma unroll
-    for (int j = 0; j < KJ; ++j) kk[j] = kp[j * js];
-#pragma unroll
-    for (int j = 0; j < KJ; ++j) vv[j] = vp[j * js];
-  };
-
-  auto compute = [&](int lt, const uint4 (&kk)[KJ], const uint4 (&vv)[KJ], int64_t wdst) {
-    if (wdst >= 0) {   // KV slot write of a new row (its bytes just arrived)
-      uint4* kd = reinterpret_cast<uint4*>(a.kc) + wdst;
-      uint4* vd = reinterpret_cast<uint4*>(a.vc) + wdst;
-#pragma unroll
-      for (int j = 0; j < KJ; ++j) { kd[j * jstride] = kk[j]; vd[j * jstride] = vv[j]; }
-    }
-    float4_t acc[RB];
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      acc[r] = float4_t{0.f, 0.f, 0.f, 0.f};
-      if (r == 0 || r < nblk) {
-#pragma unroll
-        for (int j = 0; j < KJ; ++j) acc[r] = qk_step(kk[j], qf[r][j], acc[r]);
-      }
-    }
-    stage_v(vt, n, g, vv);
-    const int tb = lt * kTile + 4 * g;
-    // keys past a valid row's limit exist only in tiles that reach past the
-    // smallest limit (causal diagonal, sequence end); rows that are not valid
-    // are never written, so their scores need no mask
-    const bool masked = lt * kTile + kTile - 1 > lim_lo;
-    short4_t pb[RB];
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      // raw scores; scale (> 0) is applied inside the exponent
-      float sv[4];
-#pragma unroll
-      for (int v = 0; v < 4; ++v) sv[v] = (!masked || tb + v <= lim[r]) ? acc[r][v] : -INFINITY;
-      float tmax = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
-      tmax = aia::group4_max(tmax);
-      const float mnew = fmaxf(m[r], tmax * a.scale_log2);
-      float p[4];
-#pragma unroll
-      for (int v = 0; v < 4; ++v) p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[v], a.scale_log2, -mnew));
-      const float psum = (p[0] + p[1]) + (p[2] + p[3]);
-      if (__any(mnew > m[r])) {   // rescale only when some row's max grew
-        const float alpha = __builtin_amdgcn_exp2f(m[r] - mnew);
-        lsum[r] = lsum[r] * alpha + psum;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[r][dt] *= alpha;
-      } else {
-        lsum[r] += psum;
-      }
-      m[r] = mnew;
-      pb[r] = as_s4(aia::pack_bf16x2(p[0], p[1]), aia::pack_bf16x2(p[2], p[3]));
-    }
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const short4_t va = vt_frag(vt, n, g, dt);
-#pragma unroll
-      for (int r = 0; r < RB; ++r)
-        if (r == 0 || r < nblk)
-          o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(va, pb[r], o[r][dt], 0, 0, 0);
-    }
-    __builtin_amdgcn_wave_barrier();
-  };
-
-  uint4 kbuf[kPipe][KJ], vbuf[kPipe][KJ];
-  int64_t wbuf[kPipe];
-  for (int w0 = lt0; w0 < lt1;) {
-    blk_base = (w0 * kTile) / a.bs;
-    // tiles whose keys all fall inside blocks [blk_base, blk_base + win);
-    // the first window of a range uses the block ids of its work record
-    const int win = use_pre ? kRecBlocks : 64;
-    w1 = min(lt1, ((blk_base + win) * a.bs - kTile) / kTile + 1);
-    if (use_pre) btv = lane < kRecBlocks ? pre : 0;
-    else btv = blk_base + lane < nblk_vis ? btrow[blk_base + lane] : 0;
-    use_pre = false;
-#pragma unroll
-    for (int i = 0; i < kPipe; ++i) {
-      load(w0 + i, kbuf[i], vbuf[i], wbuf[i]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    for (int base = w0; base < w1; base += kPipe) {
-#pragma unroll
-      for (int i = 0; i < kPipe; ++i) {
-        const int lt = base + i;
-        if (lt < w1) compute(lt, kbuf[i], vbuf[i], wbuf[i]);
-        load(lt + kPipe, kbuf[i], vbuf[i], wbuf[i]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    w0 = w1;
-  }
-
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    lsum[r] = aia::group4_sum(lsum[r]);
-  }
-  const int first_wave = tile_begin / tpw;
-  const int nparts = (tile_end - 1) / tpw - first_wave + 1;
-  constexpr int seg_rows = RB * kRows;
-  if (nparts == 1) {
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      if (!rv[r]) continue;
-      const float inv = lsum[r] > 0.f ? 1.f / lsum[r] : 0.f;
-      uint16_t* op = a.out + (int64_t)(qtok0 + qi[r]) * a.o_ts + (int64_t)head * a.o_hs;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        uint2 wv;
-        wv.x = aia::pack_bf16x2(o[r][dt][0] * inv, o[r][dt][1] * inv);
-        wv.y = aia::pack_bf16x2(o[r][dt][2] * inv, o[r][dt][3] * inv);
-        *reinterpret_cast<uint2*>(op + 16 * dt + 4 * g) = wv;
-      }
-    }
-  } else {
-    // fp16 partial y = O / c, c = the row's largest |O| (1 for a zero row),
-    // with (m + log2 c, l / c) in place of (m, l): the merge's weights
-    // exp2(m - M) carry c back, so y folds exactly as O would
-    const int part = part_base + (w - first_wave);
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      float cmax = 0.f;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) cmax = fmaxf(cmax, fabsf(o[r][dt][i]));
-      cmax = aia::group4_max(cmax);
-      if (!rv[r]) continue;
-      const float c = cmax > 0.f ? cmax : 1.f;
-      const float inv = 1.f / c;
-      const int64_t prow = ((int64_t)part * a.nw + wid) * seg_rows + r * kRows + n;
-      uint16_t* pp = a.part_o + prow * D;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        uint2 hv;
-        hv.x = pack_f16x2(o[r][dt][0] * inv, o[r][dt][1] * inv);
-        hv.y = pack_f16x2(o[r][dt][2] * inv, o[r][dt][3] * inv);
-        *reinterpret_cast<uint2*>(pp + 16 * dt + 4 * g) = hv;
-      }
-      if (g == 0) a.part_ml[prow] = make_float2(m[r] + __log2f(c), lsum[r] * inv);
-    }
-  }
-}
-
-// One work-group per key range, one wave per kv head of the segment's group.
-// D: head dim, 128 or 64.
-template <int NW, int RB, int D, bool NZ>
-#ifndef AIA_GQA_WAVES_PER_EU
-#define AIA_GQA_WAVES_PER_EU 2
-#endif
-__device__ __forceinline__ void gqa_attn_body(const AttnArgs& a, int bid,
-                                              uint16_t (*vt_all)[kTile * kVStride]) {
-  const int lane = threadIdx.x & 63;
-  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (bid >= a.waves) return;
-  // the planner placed the ranges in the slots, spread over the XCDs
-  const int* wr = a.wave_rec + (int64_t)bid * kRecInts;
-  const int pre = wr[16 + (lane & (kRecBlocks - 1))];   // issued with the header
-  const int nseg = a.hdr[0], total_tiles = a.hdr[1];
-  const int ngroups = (a.hkv + NW - 1) / NW, nhb = (a.group + a.hb - 1) / a.hb;
-  int s = wr[0];
-  int t = wr[1];
-  const int t_end = wr[2], tpw = wr[3], s_last = wr[13];
-  if (s < 0 || s >= nseg || t < 0 || t >= t_end || t_end > total_tiles || tpw < 1 ||
-      s_last < s || s_last >= nseg)
-    return;
-  const int w = t / tpw;                                  // the range's index
-  int rec[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) rec[i] = wr[4 + i];
-  uint16_t* vt = vt_all[wid];
-  bool first = true;
-  while (true) {
-    if (!rec_ok(rec, total_tiles, a.batch, a.tokens, ngroups, nhb)) return;
-    if (rec[6] > t) {
-      const int chunk_end = min(t_end, rec[6]);
-      if ((rec[1] & 0xffff) * NW + wid < a.hkv)
-        gqa_segment<RB, D, NZ>(a, rec, s, t - rec[5], chunk_end - rec[5], w, tpw, vt, lane, wid, first,
-                        pre);
-      first = false;
-      t = chunk_end;
-      if (t >= t_end) break;
-    }
-    if (++s > s_last) return;
-    const int* r = a.seg + (int64_t)s * 8;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) rec[i] = r[i];
-  }
-}
-
-template <int NW, int RB, int D, bool NZ>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(AIA_GQA_WAVES_PER_EU, AIA_GQA_WAVES_PER_EU)))
-void gqa_attn_kernel(AttnArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t vt_all[NW][kTile * kVStride];
-  gqa_attn_body<NW, RB, D, NZ>(a, blockIdx.x, vt_all);
-}
-
-// ---------------------------------------------------------------- prefill
-
-struct PrefillArgs {
-  const uint16_t* q;
-  int64_t q_ts, q_hs;
-  uint16_t* kc;
-  uint16_t* vc;
-  const uint16_t* kn;
-  const uint16_t* vn;
-  int64_t kn_ts, vn_ts;
-  const int32_t* bt;
-  int64_t bt_stride;
-  const int32_t* cu_q;
-  const int32_t* kvlen;
-  int32_t hkv, group, bs, nb, batch, tokens;
-  float scale_log2;
-  uint16_t* out;
-  int64_t o_ts, o_hs;
-  const int4* dealt;         // work-group b: {request, first row, first tile, end tile},
-                             // {first query token, query tokens, keys, first tile's block id},
-                             // {unit, kv head}
-  const int32_t* hdr;
-  uint16_t* part_o;          // partials of chunked items, two fp16 row blocks per (unit, kv head)
-  float2* part_ml;
-  int32_t part_units;        // units the partial buffer holds
-};
-
-// LDS rows of the staged K and V tiles are 2 D bytes, unpadded: the direct
-// loads write whole 1 KB runs, so the chunks of each row are swizzled
-// instead (see the loader).
-constexpr int kKStride = kHeadDim;   // the mixed kernel's (D = 128) buffer rows
-#ifndef AIA_PF_LAZY
-#define AIA_PF_LAZY 8.0f
-#endif
-// Instruction order of the QK^T and PV blocks (sched_group_barrier): LDS
-// reads kept kPfQkAhead 16-key sub-tiles (QK^T) and kPfPvAhead V^T fragments
-// (PV) ahead of their MFMAs.  Left to itself the scheduler reuses one V^T
-// fragment's registers and waits for each batch of reads before two MFMAs.
-// (configs[1] prefill chunks, µs per call: 48.2 unordered; QK 2 / PV 4 46.0;
-// PV 2, 6 or 8 and QK 3 or 4 the same within 0.1; QK 1 46.9; PV 16 46.6.)
-constexpr int kPfQkAhead = 2;
-constexpr int kPfPvAhead = 4;
-constexpr int kSgMfma = 0x008, kSgDsRead = 0x100;    // sched_group_barrier masks
-constexpr float kLazyLog2 = AIA_PF_LAZY;              // max growth (log2) before a rescale
-
-// Prefill attention: one work-group per (prefill item, kv head).  An item is
-// kPfRows consecutive rows of one request's (query token, group head) row
-// list, row = token * group + head-in-group; each of the 4 waves owns 32
-// rows (two 16-row MFMA tiles).  The work-group walks the keys its rows can
-// see in tiles of 64: every K/V tile is loaded once (straight into one of
-// two LDS buffers, one barrier per tile) and used by all 128 rows.
-//   S^T = K Q^T   v_mfma_f32_16x16x32_bf16, K fragments ds_read_b128 from LDS
-//                 (lane (key n, group g) reads dims 32 j + 8 g of key n), Q^T
-//                 fragments held in registers for the whole item;
-//   O^T += V^T P^T  v_mfma_f32_16x16x32_bf16 over 32 keys taken from two
-//                 16-key sub-tiles s0, s1: operand position 8 g + i holds key
-//                 16 s0 + 4 g + i (i < 4) or 16 s1 + 4 g + i - 4, which is
-//                 exactly where the S^T accumulators of s0 and s1 leave P,
-//                 and V^T comes from two transposing LDS reads.
-// Online softmax per row with the scale inside exp2; masks only in tiles
-// that reach past a wave's smallest row limit.  Outputs bf16 directly (a
-// work-group covers all keys of its rows).  With new K/V rows, keys at this
-// step's new positions are read from them, and the work-group writes the new
-// rows of the tokens whose first row it holds into the cache.
-#ifndef AIA_PF_WPE
-#define AIA_PF_WPE 2
-#endif
-template <bool ONE_BLOCK, bool FUSED, int D, bool NZ>
-__device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
-                                                 uint16_t* k0, uint16_t* k1,
-                                                 uint16_t* v0, uint16_t* v1) {
-  constexpr int KJ = D / 32;        // 32-dim MFMA k-steps
-  constexpr int DT = D / 16;        // 16-dim output tiles
-  constexpr int RC = D / 8;         // 16-byte chunks per K / V row
-  // The planner writes work-group b's record at dealt[b] (the grid is as long
-  // as the list can be); it is loaded beside the header rather than after it.
-  const int4* rec = a.dealt + 3 * (int64_t)wg;
-  const int4 it = rec[0], iq = rec[1], uk = rec[2];
-  const int count = a.hdr[6];
-  if (wg >= count * a.hkv) return;
-  const int unit = uk.x, kvh = uk.y;
-  if (unit < 0 || unit >= count) return;
-  const int b = it.x, row0 = it.y, t0 = it.z, t1 = it.w;
-  if (b < 0 || b >= a.batch || kvh < 0 || kvh >= a.hkv) return;
-  const int q_begin = iq.x, lq = iq.y, lk = iq.z, bid0 = iq.w;
-  const int G = a.group;
-  const int nrows = lq * G;
-  if (row0 < 0 || row0 >= nrows || q_begin < 0 || q_begin + lq > a.tokens) return;
-  const int ctx0 = lk - lq;                       // position of the first query token
-  const int row_end = min(nrows, row0 + kPfRows);
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = lane & 15, g = lane >> 4;
-  const int row_elems = a.hkv * D;
-  const int32_t* btrow = a.bt + (int64_t)b * a.bt_stride;
-
-  // new K/V rows of the tokens whose first row lies in this item (written by
-  // the item's first chunk)
-  if (FUSED && t0 == 0) {
-    const int t_lo = (row0 + G - 1) / G, t_hi = min(lq, (row_end - 1) / G + 1);
-    for (int e = tid; e < (t_hi - t_lo) * RC; e += kPfWaves * 64) {
-      const int t = t_lo + e / RC, c = e % RC;
-      const int p = ctx0 + t;
-      if (p < 0) continue;
-      const int blk = min(max(btrow[p / a.bs], 0), a.nb - 1);
-      const int64_t dst = kv_piece<NZ>(blk, p % a.bs, a.bs, row_elems, kvh, D, c);
-      const int64_t tok = q_begin + t;
-      reinterpret_cast<uint4*>(a.kc)[dst] =
-          reinterpret_cast<const uint4*>(a.kn + tok * a.kn_ts + (int64_t)kvh * D)[c];
-      reinterpret_cast<uint4*>(a.vc)[dst] =
-          reinterpret_cast<const uint4*>(a.vn + tok * a.vn_ts + (int64_t)kvh * D)[c];
-    }
-  }
-
-  // this wave's rows
-  int lim[kPfRt], tokr[kPfRt], headr[kPfRt];
-  bool rv[kPfRt];
-  int wlim_lo = 0x7fffffff, wlim_hi = -1;
-#pragma unroll
-  for (int rt = 0; rt < kPfRt; ++rt) {
-    const int row = row0 + (wid * kPfRt + rt) * kRows + n;
-    rv[rt] = row < row_end;
-    tokr[rt] = row / G;
-    headr[rt] = kvh * G + (row - tokr[rt] * G);
-    lim[rt] = rv[rt] ? min(ctx0 + tokr[rt], lk - 1) : -1;
-    if (rv[rt]) { wlim_lo = min(wlim_lo, lim[rt]); wlim_hi = max(wlim_hi, lim[rt]); }
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    wlim_lo = min(wlim_lo, __shfl_xor(wlim_lo, d));
-    wlim_hi = max(wlim_hi, __shfl_xor(wlim_hi, d));
-  }
-  uint4 qf[kPfRt][KJ];
-#pragma unroll
-  for (int rt = 0; rt < kPfRt; ++rt) {
-    if (rv[rt]) {
-      const uint4* qp = reinterpret_cast<const uint4*>(
-          a.q + (int64_t)(q_begin + tokr[rt]) * a.q_ts + (int64_t)headr[rt] * a.q_hs);
-#pragma unroll
-      for (int j = 0; j < KJ; ++j) qf[rt][j] = qp[4 * j + g];
-    } else {
-#pragma unroll
-      for (int j = 0; j < KJ; ++j) qf[rt][j] = make_uint4(0, 0, 0, 0);
-    }
-  }
-
-  // keys the work-group's last row sees
-  const int kend = max(0, min(lk, ctx0 + (row_end - 1) / G + 1));
-  const int ntiles = (kend + kPfKeys - 1) / kPfKeys;
-  // this unit's tiles [t0, t1) of the item's [0, ntiles); a unit that does
-  // not cover them all writes a partial
-  if (t0 < 0 || t1 < t0 || t1 > ntiles) return;
-  const bool whole = t0 == 0 && t1 == ntiles;
-  const bool wide = unit < a.hdr[11];
-  if (!whole && unit >= a.part_units) return;
-
-  // Loader: thread tid moves 16-byte chunk (tid % RC) of keys kLdKeys i + tid / RC
-  // (RC = D / 8 chunks per row) straight from global memory into LDS (no
-  // registers, no LDS stores).  Each wave's load writes one 1 KB run, 1024 /
-  // (2 D) key rows of 2 D bytes with lane l at byte 16 l; lane l fetches the
-  // chunk whose swizzled place that is: K chunk c of key r sits at
-  // c ^ (r % RC) and V chunk c at c ^ 2 (r % (RC / 2)), so the K fragment
-  // reads (16 keys, one chunk each) and the V^T transposing reads (8 keys, 32
-  // bytes each) spread over the banks without padded rows.
-  // When the block size is a multiple of the tile, a tile lies in one block
-  // and a key's address is one multiply-add: lane l of every wave holds the
-  // block id of tile tb + l, fetched 64 tiles at a time, and a tile takes its
-  // id with one readlane.  (Fetched per tile, the id's load was waited for at
-  // once to move it into a scalar register: a memory round trip every tile.)
-  // Other block sizes fetch each key's id one tile ahead, so those loads are
-  // in flight during a tile's math.  Keys past the last visible one re-read
-  // it (never a slot that may hold stale bytes); keys at this step's new
-  // positions come from the new rows.
-  const int lkey = tid / RC, lc = tid % RC;
-  const int64_t kvoff = (int64_t)kvh * D;
-  const uint16_t* kcb = a.kc + kvoff;
-  const uint16_t* vcb = a.vc + kvoff;
-  const uint16_t* knb = FUSED ? a.kn + kvoff : nullptr;
-  const uint16_t* vnb = FUSED ? a.vn + kvoff : nullptr;
-  constexpr int kWaveKeys = 64 / RC;                   // key rows per wave per round
-  constexpr int kLdKeys = kPfWaves * kWaveKeys;        // keys per loader round
-  constexpr int kLdRounds = kPfKeys / kLdKeys;
-  static_assert(kLdKeys % 16 == 0 && kPfKeys % kLdKeys == 0,
-                "loader rounds of whole 16-key swizzle groups");
-  int bid[kLdRounds];
-  int tb = -64, vbid = 0;
-  auto fetch_ids = [&](int t) {
-    if (!ONE_BLOCK) {
-#pragma unroll
-      for (int i = 0; i < kLdRounds; ++i) bid[i] = btrow[min(t * kPfKeys + kLdKeys * i + lkey, kend - 1) / a.bs];
-    }
-  };
-  auto tile_bid = [&](int t) {
-    if (t == t0) return bid0;      // from the unit record
-    if (t - tb >= 64) {
-      tb = t;
-      vbid = btrow[min((t + lane) * kPfKeys, kend - 1) / a.bs];
-    }
-    return __builtin_amdgcn_readlane(vbid, t - tb);
-  };
-  // key at position p, in block blk at offset boff
-  auto load_row = [&](int i, int p, int blk, int boff, uint16_t* kdst, uint16_t* vdst) {
-    // (rounds start at multiples of 16 keys, so lkey stands for the key mod RC)
-    const int ck = lc ^ (lkey & (RC - 1)), cv = lc ^ (2 * (lkey & (RC / 2 - 1)));
-    const uint16_t* kp;
-    const uint16_t* vp;
-    if (NZ) {
-      kp = a.kc + 8 * kv_piece<true>(blk, boff, a.bs, row_elems, kvh, D, ck);
-      vp = a.vc + 8 * kv_piece<true>(blk, boff, a.bs, row_elems, kvh, D, cv);
-    } else {
-      // (the slot in 32 bits: the entry points reject pools of 2^31 slots
-      // or more, as the int32 slot_mapping cannot address them; the 64-bit
-      // form of this address cost the 32K-key prefill 7%)
-      const int64_t e = (int64_t)(blk * a.bs + boff) * row_elems;
-      kp = kcb + e + 8 * ck;
-      vp = vcb + e + 8 * cv;
-    }
-    if (FUSED) {
-      const bool fresh = p >= ctx0;
-      const int64_t tok = q_begin + (p - ctx0);
-      kp = fresh ? knb + tok * a.kn_ts + 8 * ck : kp;
-      vp = fresh ? vnb + tok * a.vn_ts + 8 * cv : vp;
-    }
-    const int rb = (kLdKeys * i + kWaveKeys * wid) * D;     // the wave's first row
-    aia::lds_load16(kp, kdst + rb);
-    aia::lds_load16(vp, vdst + rb);
-  };
-  auto load = [&](int t, auto buf_tag) {
-    constexpr int B = decltype(buf_tag)::value;
-    uint16_t* kdst = B ? k1 : k0;
-    uint16_t* vdst = B ? v1 : v0;
-    const int kb = t * kPfKeys;
-    if (ONE_BLOCK) {
-      const int blk = min(max(tile_bid(t), 0), a.nb - 1);
-      const int boff0 = kb % a.bs;
-      const int last = kend - 1 - kb;
-#pragma unroll
-      for (int i = 0; i < kLdRounds; ++i) {
-        const int off = min(kLdKeys * i + lkey, last);
-        load_row(i, kb + off, blk, boff0 + off, kdst, vdst);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kLdRounds; ++i) {
-        const int p = min(kb + kLdKeys * i + lkey, kend - 1);
-        const int blk = min(max(bid[i], 0), a.nb - 1);
-        load_row(i, p, blk, p % a.bs, kdst, vdst);
-      }
-    }
-  };
-
-  float4_t o[kPfRt][DT];
-  float m[kPfRt], lsum[kPfRt];
-#pragma unroll
-  for (int rt = 0; rt < kPfRt; ++rt) {
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o[rt][dt] = float4_t{0.f, 0.f, 0.f, 0.f};
-    m[rt] = -INFINITY;
-    lsum[rt] = 0.f;
-  }
-
-  // issue_next() issues the next tile's loads after the QK^T MFMAs, so that
-  // the load addresses and issue overlap the MFMAs' execution: 0-1% faster
-  // than issuing them first.  (A raised wave priority around each MFMA block,
-  // 3% faster with register-staged loads, made this order 1-2% slower, and
-  // either order is as fast without it, so no priority is set.)
-  auto compute = [&](int t, auto buf_tag, auto mask_tag, auto issue_next) {
-    constexpr bool MASK = decltype(mask_tag)::value;
-    constexpr int B = decltype(buf_tag)::value;
-    const int kbase = t * kPfKeys;
-    if (MASK && kbase > wlim_hi) {               // no row of this wave sees these keys
-      issue_next();
-      return;
-    }
-    const uint16_t* kt = B ? k1 : k0;
-    const uint16_t* vt = B ? v1 : v0;
-    constexpr int kSt = kPfKeys / 16;      // 16-key sub-tiles
-    float4_t acc[kPfRt][kSt];
-    __builtin_amdgcn_sched_barrier(0);     // the block below is scheduled on its own
-#pragma unroll
-    for (int st = 0; st < kSt; ++st) {
-      uint4 kf[KJ];
-#pragma unroll
-      for (int j = 0; j < KJ; ++j)
-        kf[j] = *reinterpret_cast<const uint4*>(kt + (16 * st + n) * D + 8 * ((4 * j + g) ^ (n & (RC - 1))));
-#pragma unroll
-      for (int rt = 0; rt < kPfRt; ++rt) {
-        // (a row tile with no valid row computes rows that are never written)
-        acc[rt][st] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < KJ; ++j) acc[rt][st] = qk_step(kf[j], qf[rt][j], acc[rt][st]);
-      }
-    }
-    __builtin_amdgcn_sched_group_barrier(kSgDsRead, KJ * kPfQkAhead, 0);
-#pragma unroll
-    for (int st = 0; st < kSt; ++st) {
-      __builtin_amdgcn_sched_group_barrier(kSgMfma, KJ * kPfRt, 0);
-      if (st + kPfQkAhead < kSt) __builtin_amdgcn_sched_group_barrier(kSgDsRead, KJ, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    issue_next();
-    uint4 pb[kPfRt][kSt / 2];
-#pragma unroll
-    for (int rt = 0; rt < kPfRt; ++rt) {
-      float sv[kSt][4];
-      float tmax = -INFINITY;
-      if (MASK) {     // causal diagonal / sequence end: per-key limits
-        const int rel = lim[rt] - kbase - 4 * g;
-#pragma unroll
-        for (int st = 0; st < kSt; ++st)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) sv[st][v] = 16 * st + v <= rel ? acc[rt][st][v] : -INFINITY;
-      } else {
-#pragma unroll
-        for (int st = 0; st < kSt; ++st)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) sv[st][v] = acc[rt][st][v];
-      }
-#pragma unroll
-      for (int st = 0; st < kSt; ++st)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) tmax = fmaxf(tmax, sv[st][v]);
-      tmax = aia::group4_max(tmax);
-      // Lazy rescale: the running max m only moves when some row's tile max
-      // exceeds it by more than kLazyLog2, so P stays below 2^kLazyLog2 and O
-      // and l (which share m) need no rescale on most tiles.  m = -inf until
-      // a row sees a key; exp2(-inf) = 0 then.
-      const float tm = tmax * a.scale_log2;
-      const bool grow = __any(tm > m[rt] + kLazyLog2);
-      const float mnew = grow ? fmaxf(m[rt], tm) : m[rt];
-      const float msub = mnew == -INFINITY ? 0.f : mnew;
-      float p[kSt][4];
-      float psum = 0.f;
-#pragma unroll
-      for (int st = 0; st < kSt; ++st)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          p[st][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sv[st][v], a.scale_log2, -msub));
-          psum += p[st][v];
-        }
-      if (grow) {
-        const float alpha = __builtin_amdgcn_exp2f(m[rt] - msub);
-        lsum[rt] = lsum[rt] * alpha + psum;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= alpha;
-      } else {
-        lsum[rt] += psum;
-      }
-      m[rt] = mnew;
-#pragma unroll
-      for (int pp = 0; pp < kSt / 2; ++pp) {
-        pb[rt][pp].x = aia::pack_bf16x2(p[2 * pp][0], p[2 * pp][1]);
-        pb[rt][pp].y = aia::pack_bf16x2(p[2 * pp][2], p[2 * pp][3]);
-        pb[rt][pp].z = aia::pack_bf16x2(p[2 * pp + 1][0], p[2 * pp + 1][1]);
-        pb[rt][pp].w = aia::pack_bf16x2(p[2 * pp + 1][2], p[2 * pp + 1][3]);
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);     // the block below is scheduled on its own
-    // PV over V^T fragments f = (32-key pair pp, 16 dims dt), read kPfPvAhead
-    // fragments ahead of their MFMAs.  Lane (n, g) reads keys 4 g + n / 4
-    // (+ 16), dims 16 dt + 4 (n % 4), at their swizzled place (the
-    // transposing read as in vt_frag).
-    const int vrow = 4 * g + (n >> 2);
-#pragma unroll
-    for (int f = 0; f < kSt / 2 * DT; ++f) {
-      const int pp = f / DT, dt = f % DT;
-      const int vsw = 16 * (dt ^ (vrow & (RC / 2 - 1)));
-      const short4_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (lds_short4_t*)(vt + (32 * pp + vrow) * D + vsw + 4 * (n & 3)));
-      const short4_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (lds_short4_t*)(vt + (32 * pp + 16 + vrow) * D + vsw + 4 * (n & 3)));
-      const bf16x8_t va = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-      for (int rt = 0; rt < kPfRt; ++rt)
-        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, as_b8(pb[rt][pp]), o[rt][dt], 0, 0, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(kSgDsRead, 2 * kPfPvAhead, 0);
-#pragma unroll
-    for (int f = 0; f < kSt / 2 * DT; ++f) {
-      __builtin_amdgcn_sched_group_barrier(kSgMfma, kPfRt, 0);
-      if (f + kPfPvAhead < kSt / 2 * DT) __builtin_amdgcn_sched_group_barrier(kSgDsRead, 2, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  };
-
-  if (t1 > t0) {
-    using buf0 = std::integral_constant<int, 0>;
-    using buf1 = std::integral_constant<int, 1>;
-    if (ONE_BLOCK) {   // the next 64 tiles' ids, in flight beside the first tile
-      tb = t0;
-      vbid = btrow[min((t0 + lane) * kPfKeys, kend - 1) / a.bs];
-    }
-    fetch_ids(t0);
-    load(t0, buf0{});
-    fetch_ids(t0 + 1);
-    __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
-    __syncthreads();
-    // Tiles below the wave's smallest row limit need no mask; the two runs
-    // together take every tile, so all waves pass the same barriers.  The
-    // buffer of each step is a compile-time choice (separate LDS arrays), so
-    // the compiler sees that a step's reads and the next tile's direct loads
-    // touch different memory and holds no read back for those loads; with a
-    // buffer index chosen at run time it waits for the loads before each read.
-    // The loop keeps one copy of each buffer's step (unrolled copies cost more
-    // in instruction fetch than they save).
-    const int t_um = max(t0, min(t1, (wlim_lo + 1) / kPfKeys));
-    auto step = [&](int t, auto buf_tag, auto mask_tag) {
-      constexpr int B = decltype(buf_tag)::value;
-      using other = std::integral_constant<int, B ^ 1>;
-      auto issue_next = [&]() {
-        if (t + 1 < t1) {
-          load(t + 1, other{});
-          fetch_ids(t + 2);
-        }
-      };
-      compute(t, buf_tag, mask_tag, issue_next);
-      __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
-      __syncthreads();
-    };
-    auto run = [&](int t, int t_end, auto mask_tag) {
-      bool odd = ((t - t0) & 1) != 0;
-#pragma clang loop unroll(disable)
-      while (t < t_end) {
-        if (!odd) {
-          step(t, buf0{}, mask_tag);
-          if (++t >= t_end) break;
-        }
-        step(t, buf1{}, mask_tag);
-        ++t;
-        odd = false;
-      }
-    };
-    run(t0, t_um, std::false_type{});
-    run(t_um, t1, std::true_type{});
-  }
-
-#pragma unroll
-  for (int rt = 0; rt < kPfRt; ++rt) {
-    lsum[rt] = aia::group4_sum(lsum[rt]);
-    // a unit that does not cover all of its item's keys writes a partial:
-    // y = O / c in fp16, c = the row's largest |O| (1 for an all-zero row),
-    // with (m + log2 c, l / c) in place of (m, l).  The merge's log-sum-exp
-    // rule then folds c back exactly (its weights are exp2(m - M)), and the
-    // partials take half the bytes of fp32 ones.  The first hdr[11] units of
-    // the list keep O and (m, l) as they are, in fp32 (see the planner).
-    float cmax = 0.f;
-    if (!whole && !wide) {
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int v = 0; v < 4; ++v) cmax = fmaxf(cmax, fabsf(o[rt][dt][v]));
-      cmax = aia::group4_max(cmax);
-    }
-    if (!rv[rt]) continue;
-    if (!whole && wide) {
-      const int64_t prow = ((int64_t)unit * a.hkv + kvh) * kPfRows + (wid * kPfRt + rt) * kRows + n;
-      float* pp = reinterpret_cast<float*>(a.part_o) + prow * D;      // its block, whole
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float4_t*>(pp + 16 * dt + 4 * g) = o[rt][dt];
-      if (g == 0) a.part_ml[prow] = make_float2(m[rt], lsum[rt]);
-      continue;
-    }
-    if (!whole) {
-      const float c = cmax > 0.f ? cmax : 1.f, ic = 1.f / c;
-      const int64_t blk = (int64_t)unit * a.hkv + kvh, r = (wid * kPfRt + rt) * kRows + n;
-      uint16_t* pp = a.part_o + (2 * blk * kPfRows + r) * D;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        uint2 hv;
-        hv.x = pack_f16x2(o[rt][dt][0] * ic, o[rt][dt][1] * ic);
-        hv.y = pack_f16x2(o[rt][dt][2] * ic, o[rt][dt][3] * ic);
-        *reinterpret_cast<uint2*>(pp + 16 * dt + 4 * g) = hv;
-      }
-      if (g == 0) a.part_ml[blk * kPfRows + r] = make_float2(m[rt] + __log2f(c), lsum[rt] * ic);
-      continue;
-    }
-    const float inv = lsum[rt] > 0.f ? 1.f / lsum[rt] : 0.f;
-    uint16_t* op = a.out + (int64_t)(q_begin + tokr[rt]) * a.o_ts + (int64_t)headr[rt] * a.o_hs;
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      uint2 wv;
-      wv.x = aia::pack_bf16x2(o[rt][dt][0] * inv, o[rt][dt][1] * inv);
-      wv.y = aia::pack_bf16x2(o[rt][dt][2] * inv, o[rt][dt][3] * inv);
-      *reinterpret_cast<uint2*>(op + 16 * dt + 4 * g) = wv;
-    }
-  }
-}
-
-template <bool ONE_BLOCK, bool FUSED, int D, bool NZ>
-__global__ __launch_bounds__(kPfWaves * 64) __attribute__((amdgpu_waves_per_eu(AIA_PF_WPE, AIA_PF_WPE)))
-void gqa_prefill_kernel(PrefillArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t k0[kPfKeys * D];
-  __shared__ __attribute__((aligned(16))) uint16_t k1[kPfKeys * D];
-  __shared__ __attribute__((aligned(16))) uint16_t v0[kPfKeys * D];
-  __shared__ __attribute__((aligned(16))) uint16_t v1[kPfKeys * D];
-  gqa_prefill_body<ONE_BLOCK, FUSED, D, NZ>(a, blockIdx.x, k0, k1, v0, v1);
-}
-
-// Mixed steps (prefill items beside split-K decode ranges) in one grid, for
-// kPfWaves-wave decode groups (Hkv = kPfWaves).  Launched separately, the
-// two kernels barely share a CU: one prefill wave (212-232 VGPRs, allocated
-// in blocks of 8) plus two decode waves (2 x 144) fill or exceed a SIMD's
-// 512, so the second kernel mostly waits for the first to drain.  In one grid every
-// work-group gets the prefill budget and does one job or the other, so the
-// compute-bound prefill runs while the HBM-bound decode streams beside it.
-// The decode role stages its V^T tiles in the first K buffer.
-constexpr int kMixedK0 = kPfWaves * kTile * kVStride > kPfKeys * kKStride
-                             ? kPfWaves * kTile * kVStride : kPfKeys * kKStride;
-template <bool ONE_BLOCK, bool FUSED, bool NZ>
-__global__ __launch_bounds__(kPfWaves * 64) __attribute__((amdgpu_waves_per_eu(AIA_PF_WPE, AIA_PF_WPE)))
-void gqa_mixed_kernel(AttnArgs a, PrefillArgs pa, int npf) {
-  __shared__ __attribute__((aligned(16))) uint16_t k0[kMixedK0];
-  __shared__ __attribute__((aligned(16))) uint16_t k1[kPfKeys * kKStride];
-  __shared__ __attribute__((aligned(16))) uint16_t v0[kPfKeys * kKStride];
-  __shared__ __attribute__((aligned(16))) uint16_t v1[kPfKeys * kKStride];
-  // Prefill units take the first npf block ids and the decode ranges the
-  // rest: the units are dealt out first, one or two per CU, and the ranges
-  // fill the remaining slots and every slot a unit frees.  (Alternating the
-  // roles by block id measured slower: 590 us against 449 on configs[1] in
-  // runs of 8 ids, 459-462 in runs of 64; runs of 256 matched.)
-  const int b = blockIdx.x;
-  const bool prefill = b < npf;
-  const int idx = prefill ? b : b - npf;
-  if (prefill)
-    gqa_prefill_body<ONE_BLOCK, FUSED, kHeadDim, NZ>(pa, idx, k0, k1, v0, v1);
-  else
-    gqa_attn_body<kPfWaves, 1, kHeadDim, NZ>(a, idx,
-                                         reinterpret_cast<uint16_t(*)[kTile * kVStride]>(&k0[0]));
 }
 
 struct MergeArgs {
@@ -2699,7 +1683,7 @@ __device__ __forceinline__ void mla_segment(const MlaArgs& a, const int* rec, in
 
   auto load = [&](int lt, uint4 (&kk)[5]) {
     const bool live = lt < w1;
-    const int tok = live ? min(lt * kTile + n, visible - 1) : blk_base * a.bs;
+    const int tok = live ? max(min(lt * kTile + n, visible - 1), 0) : blk_base * a.bs;
     const int bi = tok / a.bs;
     const int blk = min(max(__shfl(btv, bi - blk_base), 0), a.nb - 1);
     const int off = tok - bi * a.bs;
@@ -3489,54 +2473,6 @@ bool small_plan(const Geometry& g, int32_t dv, int32_t batch, const Layout& L) {
   return !force_large && small_geometry(g, dv, batch, L.seg_cap);
 }
 
-// The attention launches of one call, for one cache layout.
-template <bool NZ>
-int launch_gqa(const AttnArgs& a, const PrefillArgs& pa, const Layout& L, const Geometry& g,
-               int32_t head_dim, int32_t waves, bool one_block, hipStream_t s) {
-  using aia::check_hip;
-  if (mixed_grid(g, head_dim)) {
-    const int npf = (int)(L.pf_unit_cap * g.hkv);
-    const dim3 grid((unsigned)(npf + waves));
-    if (one_block && pa.kn) gqa_mixed_kernel<true, true, NZ><<<grid, kPfWaves * 64, 0, s>>>(a, pa, npf);
-    else if (one_block) gqa_mixed_kernel<true, false, NZ><<<grid, kPfWaves * 64, 0, s>>>(a, pa, npf);
-    else if (pa.kn) gqa_mixed_kernel<false, true, NZ><<<grid, kPfWaves * 64, 0, s>>>(a, pa, npf);
-    else gqa_mixed_kernel<false, false, NZ><<<grid, kPfWaves * 64, 0, s>>>(a, pa, npf);
-    if (int rc = check_hip(hipGetLastError(), "gqa_mixed_kernel launch")) return rc;
-  } else {
-#define AIA_GQA_LAUNCH_D(NW, D)                                                   \
-  (g.rb == 2 ? gqa_attn_kernel<NW, 2, D, NZ><<<waves, 64 * NW, 0, s>>>(a)            \
-             : gqa_attn_kernel<NW, 1, D, NZ><<<waves, 64 * NW, 0, s>>>(a))
-#define AIA_GQA_LAUNCH(NW)                                                        \
-  (head_dim == 64 ? AIA_GQA_LAUNCH_D(NW, 64) : AIA_GQA_LAUNCH_D(NW, kHeadDim))
-    switch (g.nw) {
-      case 1: AIA_GQA_LAUNCH(1); break;
-      case 2: AIA_GQA_LAUNCH(2); break;
-      case 3: AIA_GQA_LAUNCH(3); break;
-      case 4: AIA_GQA_LAUNCH(4); break;
-      case 5: AIA_GQA_LAUNCH(5); break;
-      case 6: AIA_GQA_LAUNCH(6); break;
-      case 7: AIA_GQA_LAUNCH(7); break;
-      default: AIA_GQA_LAUNCH(8); break;
-    }
-#undef AIA_GQA_LAUNCH
-#undef AIA_GQA_LAUNCH_D
-    if (int rc = check_hip(hipGetLastError(), "gqa_attn_kernel launch")) return rc;
-    if (L.pf_cap > 0) {
-      const dim3 grid((unsigned)(L.pf_unit_cap * g.hkv));
-#define AIA_PF_LAUNCH(D)                                                                   \
-  (one_block && pa.kn ? gqa_prefill_kernel<true, true, D, NZ><<<grid, kPfWaves * 64, 0, s>>>(pa)   \
-   : one_block        ? gqa_prefill_kernel<true, false, D, NZ><<<grid, kPfWaves * 64, 0, s>>>(pa)  \
-   : pa.kn            ? gqa_prefill_kernel<false, true, D, NZ><<<grid, kPfWaves * 64, 0, s>>>(pa)  \
-                      : gqa_prefill_kernel<false, false, D, NZ><<<grid, kPfWaves * 64, 0, s>>>(pa))
-      if (head_dim == 64) AIA_PF_LAUNCH(64);
-      else AIA_PF_LAUNCH(kHeadDim);
-#undef AIA_PF_LAUNCH
-      if (int rc = check_hip(hipGetLastError(), "gqa_prefill_kernel launch")) return rc;
-    }
-  }
-  return AIA_OK;
-}
-
 int check_heads(const char* fn, int32_t hq, int32_t hkv) {
   if (hq <= 0 || hkv <= 0 || hq % hkv != 0)
     return aia::fail(AIA_ERR_INVALID, "%s: num_q_heads %d must be a positive multiple of num_kv_heads %d",
@@ -3574,39 +2510,42 @@ extern "C" int aia_attn_workspace_layout(int32_t batch, int32_t num_tokens, int3
   return AIA_OK;
 }
 
-extern "C" int aia_attn_plan(const int32_t* cu_seqlens_q, const int32_t* seqlens_kv,
-                             const int32_t* block_table, int32_t block_table_stride,
-                             int32_t block_size, int32_t batch,
-                             int32_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
-                             int32_t head_dim_v, int32_t num_waves, void* workspace,
-                             int64_t workspace_bytes, void* stream) {
+// aia_attn_plan and aia_attn_plan_prefix (fn: the one called, for its errors).
+static int attn_plan(const char* fn, const int32_t* cu_seqlens_q, const int32_t* seqlens_kv,
+                     const int32_t* prefix_lens, const int32_t* block_table,
+                     int32_t block_table_stride, int32_t block_size, int32_t batch,
+                     int32_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                     int32_t head_dim_v, int32_t num_waves, void* workspace,
+                     int64_t workspace_bytes, void* stream) {
   using namespace aia;
-  if (int rc = check_heads("aia_attn_plan", num_q_heads, num_kv_heads)) return rc;
+  if (int rc = check_heads(fn, num_q_heads, num_kv_heads)) return rc;
   if (batch < 0 || batch > kMaxBatch)
-    return fail(AIA_ERR_CAPACITY, "aia_attn_plan: batch %d exceeds planner limit %d", batch, kMaxBatch);
+    return fail(AIA_ERR_CAPACITY, "%s: batch %d exceeds planner limit %d", fn, batch, kMaxBatch);
   if (batch > 0 && (!cu_seqlens_q || !seqlens_kv || !block_table))
-    return fail(AIA_ERR_INVALID, "aia_attn_plan: null metadata");
-  if (block_size <= 0) return fail(AIA_ERR_INVALID, "aia_attn_plan: block_size %d", block_size);
-  if (!workspace) return fail(AIA_ERR_INVALID, "aia_attn_plan: null workspace");
+    return fail(AIA_ERR_INVALID, "%s: null metadata", fn);
+  if (block_size <= 0) return fail(AIA_ERR_INVALID, "%s: block_size %d", fn, block_size);
+  if (!workspace) return fail(AIA_ERR_INVALID, "%s: null workspace", fn);
   if ((uintptr_t)workspace & 255)
-    return fail(AIA_ERR_INVALID, "aia_attn_plan: workspace must be 256-byte aligned");
+    return fail(AIA_ERR_INVALID, "%s: workspace must be 256-byte aligned", fn);
   const Geometry g = geometry(num_q_heads, num_kv_heads, batch, num_tokens, head_dim_v);
   const int32_t waves = resolve_waves(num_waves, g, head_dim_v);
   const Layout L = layout(batch, num_tokens, g, head_dim_v, waves);
   if (workspace_bytes < L.total)
-    return fail(AIA_ERR_CAPACITY, "aia_attn_plan: workspace %lld bytes < %lld needed",
+    return fail(AIA_ERR_CAPACITY, "%s: workspace %lld bytes < %lld needed", fn,
                 (long long)workspace_bytes, (long long)L.total);
   char* ws = static_cast<char*>(workspace);
   if (small_plan(g, head_dim_v, batch, L)) {
-    plan_small_kernel<<<1, kSmallPlanThreads, 0, (hipStream_t)stream>>>(
-        cu_seqlens_q, seqlens_kv, block_table, block_table_stride, block_size, batch, g, waves,
+    auto* kernel = prefix_lens ? plan_small_kernel<true> : plan_small_kernel<false>;
+    kernel<<<1, kSmallPlanThreads, 0, (hipStream_t)stream>>>(
+        cu_seqlens_q, seqlens_kv, prefix_lens, block_table, block_table_stride, block_size, batch, g, waves,
         head_dim_v, reinterpret_cast<int32_t*>(ws + L.hdr),
         reinterpret_cast<int32_t*>(ws + L.seg), reinterpret_cast<int32_t*>(ws + L.wave),
         reinterpret_cast<int32_t*>(ws + L.mrg), (int32_t)L.seg_cap, (int32_t)L.part_cap);
     return check_hip(hipGetLastError(), "aia_attn_plan launch");
   }
-  plan_kernel<<<1, kPlanThreads, 0, (hipStream_t)stream>>>(
-      cu_seqlens_q, seqlens_kv, block_table, block_table_stride, block_size, batch, g, waves,
+  auto* kernel = prefix_lens ? plan_kernel<true> : plan_kernel<false>;
+  kernel<<<1, kPlanThreads, 0, (hipStream_t)stream>>>(
+      cu_seqlens_q, seqlens_kv, prefix_lens, block_table, block_table_stride, block_size, batch, g, waves,
       head_dim_v, reinterpret_cast<int32_t*>(ws + L.hdr),
       reinterpret_cast<int32_t*>(ws + L.seg), reinterpret_cast<int32_t*>(ws + L.wave),
       reinterpret_cast<int32_t*>(ws + L.req),
@@ -3618,51 +2557,97 @@ extern "C" int aia_attn_plan(const int32_t* cu_seqlens_q, const int32_t* seqlens
   return check_hip(hipGetLastError(), "aia_attn_plan launch");
 }
 
-extern "C" int aia_paged_attention_gqa(
-    const void* query, int64_t q_token_stride, int64_t q_head_stride, const void* key_cache,
-    const void* value_cache, const int32_t* block_table, int32_t block_table_stride,
-    const int32_t* cu_seqlens_q, const int32_t* seqlens_kv, int32_t batch, int32_t num_tokens,
-    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
-    int32_t num_blocks, float scale, void* out, int64_t out_token_stride, int64_t out_head_stride,
-    const void* key_new, const void* value_new, int64_t new_key_token_stride,
-    int64_t new_value_token_stride, int32_t num_waves, int32_t flags, void* workspace,
-    int64_t workspace_bytes, void* stream) {
+extern "C" int aia_attn_plan(const int32_t* cu_seqlens_q, const int32_t* seqlens_kv,
+                             const int32_t* block_table, int32_t block_table_stride,
+                             int32_t block_size, int32_t batch, int32_t num_tokens,
+                             int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim_v,
+                             int32_t num_waves, void* workspace, int64_t workspace_bytes,
+                             void* stream) {
+  return attn_plan("aia_attn_plan", cu_seqlens_q, seqlens_kv, nullptr, block_table, block_table_stride,
+                   block_size, batch, num_tokens, num_q_heads, num_kv_heads, head_dim_v, num_waves,
+                   workspace, workspace_bytes, stream);
+}
+
+extern "C" int aia_attn_plan_prefix(const int32_t* cu_seqlens_q, const int32_t* seqlens_kv,
+                                    const int32_t* prefix_lens, const int32_t* block_table,
+                                    int32_t block_table_stride, int32_t block_size, int32_t batch,
+                                    int32_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                                    int32_t head_dim_v, int32_t num_waves, void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+  if (batch > 0 && !prefix_lens)
+    return aia::fail(AIA_ERR_INVALID, "aia_attn_plan_prefix: null prefix_lens");
+  if (head_dim_v != kHeadDim && head_dim_v != 64)
+    return aia::fail(AIA_ERR_UNSUPPORTED, "aia_attn_plan_prefix: head_dim %d (128 or 64)", head_dim_v);
+  return attn_plan("aia_attn_plan_prefix", cu_seqlens_q, seqlens_kv, prefix_lens, block_table,
+                   block_table_stride, block_size, batch, num_tokens, num_q_heads, num_kv_heads,
+                   head_dim_v, num_waves, workspace, workspace_bytes, stream);
+}
+
+// What aia_paged_attention_gqa_ex takes beyond aia_paged_attention_gqa.
+struct GqaExtra {
+  const void* key_scale;
+  const void* value_scale;
+  const int32_t* prefix_lens;
+  const float* alibi_slopes;
+  float softcap;
+};
+
+static int attention_gqa(
+    const char* fn, const void* query, int64_t q_token_stride, int64_t q_head_stride,
+    const void* key_cache, const void* value_cache, const int32_t* block_table,
+    int32_t block_table_stride, const int32_t* cu_seqlens_q, const int32_t* seqlens_kv, int32_t batch,
+    int32_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t block_size, int32_t num_blocks, float scale, void* out, int64_t out_token_stride,
+    int64_t out_head_stride, const void* key_new, const void* value_new,
+    int64_t new_key_token_stride, int64_t new_value_token_stride, const GqaExtra& ex,
+    int32_t num_waves, int32_t flags, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace aia;
-  if (int rc = check_heads("aia_paged_attention_gqa", num_q_heads, num_kv_heads)) return rc;
+  if (int rc = check_heads(fn, num_q_heads, num_kv_heads)) return rc;
   if (head_dim != kHeadDim && head_dim != 64)
-    return fail(AIA_ERR_UNSUPPORTED, "aia_paged_attention_gqa: head_dim %d (128 or 64)", head_dim);
+    return fail(AIA_ERR_UNSUPPORTED, "%s: head_dim %d (128 or 64)", fn, head_dim);
   if (!(scale > 0.f))
-    return fail(AIA_ERR_INVALID, "aia_paged_attention_gqa: scale %g must be positive", (double)scale);
+    return fail(AIA_ERR_INVALID, "%s: scale %g must be positive", fn, (double)scale);
   if (block_size <= 0 || num_blocks <= 0)
-    return fail(AIA_ERR_INVALID, "aia_paged_attention_gqa: block_size %d / num_blocks %d",
+    return fail(AIA_ERR_INVALID, "%s: block_size %d / num_blocks %d", fn,
                 block_size, num_blocks);
   if ((int64_t)num_blocks * block_size > INT32_MAX)
-    return fail(AIA_ERR_INVALID, "aia_paged_attention_gqa: %d blocks of %d slots exceed the int32 slot range",
+    return fail(AIA_ERR_INVALID, "%s: %d blocks of %d slots exceed the int32 slot range", fn,
                 num_blocks, block_size);
   if (flags & ~AIA_ATTN_KV_NZ)
-    return fail(AIA_ERR_INVALID, "aia_paged_attention_gqa: unknown flags 0x%x", flags);
+    return fail(AIA_ERR_INVALID, "%s: unknown flags 0x%x", fn, flags);
+  const bool fp8 = ex.key_scale || ex.value_scale;
+  if (fp8 && !(ex.key_scale && ex.value_scale))
+    return fail(AIA_ERR_INVALID, "%s: key_scale and value_scale go together", fn);
+  if (fp8 && (flags & AIA_ATTN_KV_NZ))
+    return fail(AIA_ERR_UNSUPPORTED, "%s: 8-bit caches have no NZ layout", fn);
+  if (fp8 && (key_new || value_new))
+    return fail(AIA_ERR_INVALID, "%s: 8-bit caches are written by aia_kv_write_fp8 (no key_new / "
+                "value_new)", fn);
+  if (!(ex.softcap >= 0.f && ex.softcap < INFINITY))
+    return fail(AIA_ERR_INVALID, "%s: softcap %g must be finite and not negative (0: none)", fn,
+                (double)ex.softcap);
   if (num_tokens == 0 || batch == 0) return AIA_OK;    // empty step (zero-size tensors)
   if (!query || !key_cache || !value_cache || !block_table || !out || !workspace || !cu_seqlens_q ||
       !seqlens_kv)
-    return fail(AIA_ERR_INVALID, "aia_paged_attention_gqa: null pointer argument");
+    return fail(AIA_ERR_INVALID, "%s: null pointer argument", fn);
   if ((uintptr_t)workspace & 255)
-    return fail(AIA_ERR_INVALID, "aia_paged_attention_gqa: workspace must be 256-byte aligned");
+    return fail(AIA_ERR_INVALID, "%s: workspace must be 256-byte aligned", fn);
   if (q_token_stride % 8 || q_head_stride % 8 || out_token_stride % 4 || out_head_stride % 8 ||
       ((uintptr_t)query & 15) || ((uintptr_t)key_cache & 15) || ((uintptr_t)value_cache & 15) ||
       ((uintptr_t)out & 15))
-    return fail(AIA_ERR_INVALID, "aia_paged_attention_gqa: query/out/cache must be 16-byte aligned "
-                "with strides a multiple of 8 elements");
+    return fail(AIA_ERR_INVALID, "%s: query/out/cache must be 16-byte aligned "
+                "with strides a multiple of 8 elements", fn);
   if ((key_new == nullptr) != (value_new == nullptr))
-    return fail(AIA_ERR_INVALID, "aia_paged_attention_gqa: key_new and value_new go together");
+    return fail(AIA_ERR_INVALID, "%s: key_new and value_new go together", fn);
   if (key_new && (new_key_token_stride % 8 || new_value_token_stride % 8 ||
                   ((uintptr_t)key_new & 15) || ((uintptr_t)value_new & 15)))
-    return fail(AIA_ERR_INVALID, "aia_paged_attention_gqa: new K/V rows must be 16-byte aligned "
-                "with token strides a multiple of 8 elements");
+    return fail(AIA_ERR_INVALID, "%s: new K/V rows must be 16-byte aligned "
+                "with token strides a multiple of 8 elements", fn);
   const Geometry g = geometry(num_q_heads, num_kv_heads, batch, num_tokens, head_dim);
   const int32_t waves = resolve_waves(num_waves, g, head_dim);
   const Layout L = layout(batch, num_tokens, g, head_dim, waves);
   if (workspace_bytes < L.total)
-    return fail(AIA_ERR_CAPACITY, "aia_paged_attention_gqa: workspace %lld bytes < %lld needed",
+    return fail(AIA_ERR_CAPACITY, "%s: workspace %lld bytes < %lld needed", fn,
                 (long long)workspace_bytes, (long long)L.total);
   char* ws = static_cast<char*>(workspace);
   AttnArgs a;
@@ -3686,6 +2671,13 @@ extern "C" int aia_paged_attention_gqa(
   a.waves = waves;
   a.hdr = reinterpret_cast<const int32_t*>(ws + L.hdr);
   a.batch = batch; a.tokens = num_tokens;
+  a.sc.ks = static_cast<const uint8_t*>(ex.key_scale);
+  a.sc.vs = static_cast<const uint8_t*>(ex.value_scale);
+  a.sc.slopes = ex.alibi_slopes;
+  a.sc.prefix = ex.prefix_lens;
+  a.sc.kvlen = seqlens_kv;
+  a.sc.cap_in = ex.softcap > 0.f ? 2.f * a.scale_log2 / ex.softcap : 0.f;
+  a.sc.cap_out = ex.softcap * 1.4426950408889634f;
   hipStream_t s = (hipStream_t)stream;
   PrefillArgs pa = {};
   if (L.pf_cap > 0) {
@@ -3696,6 +2688,7 @@ extern "C" int aia_paged_attention_gqa(
     pa.hkv = g.hkv; pa.group = g.group; pa.bs = block_size; pa.nb = num_blocks;
     pa.batch = batch; pa.tokens = num_tokens;
     pa.scale_log2 = a.scale_log2;
+    pa.sc = a.sc;
     pa.out = a.out; pa.o_ts = a.o_ts; pa.o_hs = a.o_hs;
     pa.dealt = reinterpret_cast<const int4*>(ws + L.pfw);
     pa.hdr = a.hdr;
@@ -3704,11 +2697,53 @@ extern "C" int aia_paged_attention_gqa(
     pa.part_units = (int32_t)std::min<int64_t>(kPfCutSlots, L.pf_slots / 2) / g.hkv;
   }
   const bool one_block = block_size % kPfKeys == 0;
-  if (int rc = (flags & AIA_ATTN_KV_NZ) ? launch_gqa<true>(a, pa, L, g, head_dim, waves, one_block, s)
-                                        : launch_gqa<false>(a, pa, L, g, head_dim, waves, one_block, s))
+  const bool scored = ex.softcap > 0.f || ex.alibi_slopes || ex.prefix_lens;
+  const bool nz = flags & AIA_ATTN_KV_NZ;
+  const int rc =
+      fp8      ? launch_gqa_fp8(scored, a, pa, L, g, head_dim, waves, one_block, s)
+      : scored ? launch_gqa_scored(nz ? kKvNz : kKvNd, a, pa, L, g, head_dim, waves, one_block, s)
+      : nz     ? launch_gqa<kKvNz, false>(a, pa, L, g, head_dim, waves, one_block, s)
+               : launch_gqa<kKvNd, false>(a, pa, L, g, head_dim, waves, one_block, s);
+  if (rc)
     return rc;
   return launch_merge(ws, L, g, g.nw, head_dim, batch, num_tokens, waves, (int64_t)block_table_stride * block_size, a.part_o, a.part_ml, a.seg, a.out, a.o_ts, a.o_hs,
                       s);
+}
+
+extern "C" int aia_paged_attention_gqa(
+    const void* query, int64_t q_token_stride, int64_t q_head_stride, const void* key_cache,
+    const void* value_cache, const int32_t* block_table, int32_t block_table_stride,
+    const int32_t* cu_seqlens_q, const int32_t* seqlens_kv, int32_t batch, int32_t num_tokens,
+    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+    int32_t num_blocks, float scale, void* out, int64_t out_token_stride, int64_t out_head_stride,
+    const void* key_new, const void* value_new, int64_t new_key_token_stride,
+    int64_t new_value_token_stride, int32_t num_waves, int32_t flags, void* workspace,
+    int64_t workspace_bytes, void* stream) {
+  return attention_gqa("aia_paged_attention_gqa", query, q_token_stride, q_head_stride, key_cache,
+                       value_cache, block_table, block_table_stride, cu_seqlens_q, seqlens_kv, batch,
+                       num_tokens, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, scale,
+                       out, out_token_stride, out_head_stride, key_new, value_new,
+                       new_key_token_stride, new_value_token_stride, GqaExtra{}, num_waves, flags,
+                       workspace, workspace_bytes, stream);
+}
+
+extern "C" int aia_paged_attention_gqa_ex(
+    const void* query, int64_t q_token_stride, int64_t q_head_stride, const void* key_cache,
+    const void* value_cache, const int32_t* block_table, int32_t block_table_stride,
+    const int32_t* cu_seqlens_q, const int32_t* seqlens_kv, int32_t batch, int32_t num_tokens,
+    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+    int32_t num_blocks, float scale, void* out, int64_t out_token_stride, int64_t out_head_stride,
+    const void* key_new, const void* value_new, int64_t new_key_token_stride,
+    int64_t new_value_token_stride, const void* key_scale, const void* value_scale,
+    const int32_t* prefix_lens, const float* alibi_slopes, float softcap, int32_t num_waves, int32_t flags, void* workspace,
+    int64_t workspace_bytes, void* stream) {
+  return attention_gqa("aia_paged_attention_gqa_ex", query, q_token_stride, q_head_stride, key_cache,
+                       value_cache, block_table, block_table_stride, cu_seqlens_q, seqlens_kv, batch,
+                       num_tokens, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, scale,
+                       out, out_token_stride, out_head_stride, key_new, value_new,
+                       new_key_token_stride, new_value_token_stride,
+                       GqaExtra{key_scale, value_scale, prefix_lens, alibi_slopes, softcap}, num_waves,
+                       flags, workspace, workspace_bytes, stream);
 }
 
 extern "C" int aia_paged_attention_mla(

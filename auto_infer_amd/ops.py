@@ -5,12 +5,14 @@ check shapes/dtypes/devices on the host, then hand raw pointers and the
 current HIP stream to the C ABI.  Nothing here computes on the CPU.
 """
 import ctypes
+import math
 
 import torch
 
 from auto_infer_amd import _native
 
 _BF16 = torch.bfloat16
+FP8_KV, FP8_KV_SCALE = torch.float8_e4m3fn, torch.float8_e8m0fnu   # 8-bit KV caches
 
 
 # Pointers and streams go to the C-ABI as plain ints: every pointer
@@ -25,6 +27,16 @@ def _stream(device):
     if _raw_stream is not None and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def _call_on(device, name, *args):
+    """An entry point's launch with ``device`` current: its stream handle may be
+    the default stream's, which is that of the current device."""
+    if torch.cuda.current_device() == device.index:
+        _native.call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            _native.call(name, *args)
 
 
 def _ptr(t):
@@ -94,6 +106,134 @@ def qk_norm_rope(qkv, num_q_heads, num_kv_heads, cos, sin, q_norm_weight=None,
                  float(eps), _stream(qkv.device))
     q, k, v = qkv.split((num_q_heads * D, num_kv_heads * D, num_kv_heads * D), dim=-1)
     return q.view(T, num_q_heads, D), k.view(T, num_kv_heads, D), v.view(T, num_kv_heads, D)
+
+
+class RotaryEmbedding:
+    """Frequencies of rotary positions, for ``rope_qk``.
+
+    ``rotary_dim`` (default ``head_dim``): the leading dims of each head that
+    turn, a multiple of 16; ``interleaved``: pairs of neighbouring dims instead
+    of dims half of the rotated part apart.  Pair i turns by
+    ``base ** (-2 i / rotary_dim)`` per position, changed by ``scaling``:
+
+    * ``{"type": "linear", "factor": f}``: all frequencies divided by f;
+    * ``{"type": "yarn", "factor": f, "original_max_position": n}`` (optional
+      ``beta_fast`` 32, ``beta_slow`` 1, ``attention_factor`` 0.1 ln f + 1 for f
+      > 1): pairs that turn more than ``beta_fast`` times within n positions
+      stay, those that turn less than ``beta_slow`` times are divided by f, a
+      linear ramp over the pairs in between; cos and sin are multiplied by
+      ``attention_factor``;
+
+    or given as ``inv_freq`` (rotary_dim / 2 radians per position), with
+    ``attention_factor`` for the factor on cos and sin.  The frequencies are
+    kept on the device as 64-bit fractions of a turn (``turns``), so angles stay
+    exact at far positions.
+    """
+
+    def __init__(self, head_dim, rotary_dim=None, base=10000.0, interleaved=False, scaling=None,
+                 inv_freq=None, attention_factor=None, device="cuda"):
+        self.head_dim = int(head_dim)
+        self.rotary_dim = self.head_dim if rotary_dim is None else int(rotary_dim)
+        self.interleaved = bool(interleaved)
+        n = self.rotary_dim // 2
+        if self.head_dim not in (128, 64):
+            raise NotImplementedError(f"RotaryEmbedding: head_dim {head_dim} (128 or 64)")
+        if not 0 < self.rotary_dim <= self.head_dim or self.rotary_dim % 16:
+            raise NotImplementedError(f"RotaryEmbedding: rotary_dim {rotary_dim} (a multiple of 16 "
+                                      f"up to head_dim {head_dim})")
+        factor = 1.0
+        if inv_freq is not None:
+            _require(scaling is None, "inv_freq and scaling exclude each other")
+            freq = [float(f) for f in inv_freq]
+            _require(len(freq) == n and all(math.isfinite(f) for f in freq),
+                     f"inv_freq must hold {n} finite values")
+        else:
+            _require(base > 0, "base must be positive")
+            freq = [float(base) ** (-2.0 * i / self.rotary_dim) for i in range(n)]
+            if scaling is not None:
+                freq, factor = self._scaled(freq, float(base), dict(scaling))
+        if attention_factor is not None:
+            factor = float(attention_factor)
+        _require(math.isfinite(factor), "attention_factor must be finite")
+        self.inv_freq, self.attention_factor = freq, factor
+        # radians -> 2^-64 turns, modulo one turn, as a signed 64-bit word
+        words = [int(math.ldexp(f / (2 * math.pi), 64)) % (1 << 64) for f in freq]
+        self.turns = torch.tensor([w - (1 << 64) if w >> 63 else w for w in words],
+                                  dtype=torch.int64).to(device)
+
+    def _scaled(self, freq, base, sc):
+        kind, f = sc.pop("type", None), float(sc.pop("factor", 0.0))
+        _require(kind in ("linear", "yarn"), f"rotary scaling type {kind!r} (linear or yarn)")
+        _require(f > 0 and math.isfinite(f), f"{kind} scaling needs a positive factor")
+        if kind == "linear":
+            _require(not sc, f"unknown entries of linear scaling: {sorted(sc)}")
+            return [x / f for x in freq], 1.0
+        n = sc.pop("original_max_position", 0)
+        fast, slow = float(sc.pop("beta_fast", 32.0)), float(sc.pop("beta_slow", 1.0))
+        att = sc.pop("attention_factor", None)
+        _require(not sc, f"unknown entries of yarn scaling: {sorted(sc)}")
+        _require(n > 0, "yarn scaling needs original_max_position")
+        _require(fast >= slow > 0 and base > 1, "yarn scaling needs beta_fast >= beta_slow > 0 and "
+                 "base > 1")
+        d = self.rotary_dim
+
+        def pair(turns):        # the pair that turns so often within n positions
+            return d * math.log(n / (2 * math.pi * turns)) / (2 * math.log(base))
+        lo = max(math.floor(pair(fast)), 0)
+        hi = min(math.ceil(pair(slow)), d - 1)
+        out = []
+        for i, x in enumerate(freq):
+            r = min(max((i - lo) / max(hi - lo, 1e-3), 0.0), 1.0)
+            out.append(x * (1 - r) + x / f * r)
+        if att is None:
+            att = 0.1 * math.log(f) + 1.0 if f > 1 else 1.0
+        return out, float(att)
+
+
+def rope_qk(qkv, num_q_heads, num_kv_heads, positions, rope, q_norm_weight=None,
+            k_norm_weight=None, eps=1e-6, out=None):
+    """Rotary positions of the Q and K heads of a packed qkv projection (T, (Hq
+    + 2 Hkv) D), with an optional per-head RMSNorm in front, one launch.
+
+    ``positions`` (T,) int64, any values; ``rope`` a ``RotaryEmbedding`` of the
+    same head_dim.  In place by default; ``out`` = (q_out, k_out), tensors (T,
+    Hq, D) and (T, Hkv, D) that do not overlap ``qkv``, leaves ``qkv`` as it is.
+    Returns the rotated (q, k) and the V view, (T, heads, D) each.  Unlike
+    ``qk_norm_rope`` (cos/sin rows, bf16 roundings of the separate ops) it
+    computes the angles itself and rounds once."""
+    _check_device_tensor(qkv, "qkv", _BF16)
+    _require(qkv.dim() == 2 and qkv.stride(1) == 1, "qkv must be (T, width) with unit inner stride")
+    T, width = qkv.shape
+    _require(isinstance(rope, RotaryEmbedding), "rope must be a RotaryEmbedding")
+    D, device = rope.head_dim, qkv.device
+    if num_q_heads <= 0 or num_kv_heads <= 0 or width != (num_q_heads + 2 * num_kv_heads) * D:
+        raise ValueError(f"qkv width {width} != (Hq + 2 Hkv) x {D}")
+    _check_device_tensor(positions, "positions", torch.int64)
+    _require(positions.shape == (T,) and positions.is_contiguous(),
+             "positions must hold one contiguous entry per token")
+    _require(positions.device == device and rope.turns.device == device,
+             "qkv, positions and rope must be on the same GPU")
+    _require((q_norm_weight is None) == (k_norm_weight is None), "q and k norm weights go together")
+    for t, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
+        if t is not None:
+            _check_device_tensor(t, name, _BF16)
+            if t.numel() != D or not t.is_contiguous() or t.device != device:
+                raise ValueError(f"{name} must be {D} contiguous values on {device}")
+    q, k, v = qkv.split((num_q_heads * D, num_kv_heads * D, num_kv_heads * D), dim=-1)
+    v = v.view(T, num_kv_heads, D)
+    if out is None:
+        q, k = q.view(T, num_q_heads, D), k.view(T, num_kv_heads, D)
+    else:
+        q, k = out
+        _check_out(q, "q_out", (T, num_q_heads, D), device)
+        _check_out(k, "k_out", (T, num_kv_heads, D), device)
+    _call_on(device, "aia_rope_qk", _ptr(qkv), qkv.stride(0) if T > 1 else width, T, num_q_heads,
+                 num_kv_heads, D, _ptr(positions), _ptr(rope.turns), rope.rotary_dim,
+                 rope.attention_factor, int(rope.interleaved), _ptr(q_norm_weight),
+                 _ptr(k_norm_weight), float(eps), _ptr(q),
+                 _row_stride(q, "q_out") if T > 1 else num_q_heads * D, _ptr(k),
+                 _row_stride(k, "k_out") if T > 1 else num_kv_heads * D, _stream(device))
+    return q, k, v
 
 
 def _rope_rows(t, name, T, width):
@@ -297,6 +437,56 @@ def write_kv_nz(key, value, key_cache, value_cache, slot_mapping):
                  _stream(key.device))
 
 
+def _check_fp8_cache(cache, scale, name, device):
+    """An 8-bit cache (NB, bs, Hkv, D) and its scales (NB, Hkv)."""
+    _check_device_tensor(cache, f"{name}_cache", FP8_KV)
+    _check_device_tensor(scale, f"{name}_scale", FP8_KV_SCALE)
+    if cache.dim() != 4 or not cache.is_contiguous():
+        raise ValueError(f"{name}_cache must be a contiguous (num_blocks, block_size, Hkv, D) tensor")
+    if scale.shape != (cache.shape[0], cache.shape[2]) or not scale.is_contiguous():
+        raise ValueError(f"{name}_scale must be a contiguous (num_blocks, Hkv) tensor")
+    if cache.device != device or scale.device != device:
+        raise ValueError(f"{name}_cache and {name}_scale must be on {device}")
+
+
+def write_kv_fp8(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping):
+    """Scatter this step's bf16 K/V rows into 8-bit paged caches by slot index.
+
+    ``key`` / ``value`` (T, Hkv, D), D 128 or 64; caches (NB, bs, Hkv, D)
+    ``torch.float8_e4m3fn``; scales (NB, Hkv) ``torch.float8_e8m0fnu``, one power of two
+    per block and head: a cached value stands for value * scale.  A block whose
+    first slot is written starts anew (its other slots' contents are lost
+    until they are written, which a paged cache does in order); in any other
+    block the scale grows where the new rows need it and the block's other
+    rows are rescaled.  Values that are not finite become NaN.  ``value``, its
+    cache and its scale may be None.  Slots outside the cache are skipped; of
+    tokens with the same slot the last one stays."""
+    _check_device_tensor(key, "key", _BF16)
+    device = key.device
+    _check_fp8_cache(key_cache, key_scale, "key", device)
+    _check_device_tensor(slot_mapping, "slot_mapping", torch.int32)
+    nb, bs, hkv, d = key_cache.shape
+    _require(key.dim() == 3 and key.shape[1:] == (hkv, d),
+             "key rows do not match the key cache's (heads, dim)")
+    T = key.shape[0]
+    _require(slot_mapping.shape == (T,) and slot_mapping.is_contiguous() and
+             slot_mapping.device == device,
+             "slot_mapping must be a contiguous 1-D tensor with one slot per token")
+    kts, vts = _row_stride(key, "key") if T > 1 else hkv * d, 0
+    if value is not None:
+        _check_device_tensor(value, "value", _BF16)
+        _check_fp8_cache(value_cache, value_scale, "value", device)
+        _require(value_cache.shape == key_cache.shape, "value_cache must match key_cache")
+        _require(value.shape == key.shape and value.device == device, "value must match key")
+        vts = _row_stride(value, "value") if T > 1 else hkv * d
+    else:
+        _require(value_cache is None and value_scale is None,
+                 "value_cache or value_scale given without value")
+    _call_on(device, "aia_kv_write_fp8", _ptr(key), kts, _ptr(value), vts, _ptr(key_cache),
+                 _ptr(value_cache), _ptr(key_scale), _ptr(value_scale), _ptr(slot_mapping), T, hkv,
+                 d, bs, nb * bs, _stream(device))
+
+
 KV_LAYOUTS = {"nd": 0, "nz": 1}   # nz: AIA_ATTN_KV_NZ
 
 
@@ -333,10 +523,15 @@ class AttentionPlan:
     (forward_context.py:14-15), both int32 on the device.  The planner runs
     on the GPU, so device-produced metadata (the packing kernel) needs no
     host round trip.
+
+    ``prefix_lens`` (B,) int32 on the device: the first keys of each request
+    that all its rows see, in both directions (0 = none; more than the request
+    has = all its keys).  GQA only.
     """
 
     def __init__(self, block_table, cu_seqlens_q, seqlens_kv, num_tokens, num_q_heads,
-                 num_kv_heads, head_dim_v, block_size, num_waves=0, workspace=None, owned=None):
+                 num_kv_heads, head_dim_v, block_size, num_waves=0, workspace=None, owned=None,
+                 prefix_lens=None):
         _check_device_tensor(block_table, "block_table", torch.int32)
         _check_device_tensor(cu_seqlens_q, "cu_seqlens_q", torch.int32)
         _check_device_tensor(seqlens_kv, "seqlens_kv", torch.int32)
@@ -347,6 +542,12 @@ class AttentionPlan:
         _require(block_table.shape[0] >= batch, "block_table has fewer rows than requests")
         _require(cu_seqlens_q.is_contiguous() and seqlens_kv.is_contiguous(),
                  "metadata tensors must be contiguous")
+        if prefix_lens is not None:
+            _check_device_tensor(prefix_lens, "prefix_lens", torch.int32)
+            _require(prefix_lens.shape == (batch,) and prefix_lens.is_contiguous() and
+                     prefix_lens.device == block_table.device,
+                     "prefix_lens must hold one contiguous entry per request")
+        self.prefix_lens = prefix_lens
         self.block_table = block_table
         self.cu_seqlens_q = cu_seqlens_q
         self.seqlens_kv = seqlens_kv
@@ -380,11 +581,15 @@ class AttentionPlan:
         self.stream = torch.cuda.current_stream(device)
         self._on = (device, self.stream.cuda_stream)
         self._use_on(self.stream)
-        _native.call("aia_attn_plan", _ptr(self.cu_seqlens_q), _ptr(self.seqlens_kv),
-                     _ptr(self.block_table), self.block_table.stride(0), self.block_size,
-                     self.batch, self.num_tokens, self.num_q_heads, self.num_kv_heads,
-                     self.head_dim_v, self.num_waves, _ptr(self.workspace),
-                     self.workspace.numel(), self._on[1])
+        args = (_ptr(self.block_table), self.block_table.stride(0), self.block_size,
+                self.batch, self.num_tokens, self.num_q_heads, self.num_kv_heads,
+                self.head_dim_v, self.num_waves, _ptr(self.workspace),
+                self.workspace.numel(), self._on[1])
+        if self.prefix_lens is None:
+            _call_on(device, "aia_attn_plan", _ptr(self.cu_seqlens_q), _ptr(self.seqlens_kv), *args)
+        else:
+            _call_on(device, "aia_attn_plan_prefix", _ptr(self.cu_seqlens_q), _ptr(self.seqlens_kv),
+                         _ptr(self.prefix_lens), *args)
 
     def _use_on(self, stream):
         if stream not in self._streams:
@@ -467,7 +672,8 @@ def _check_out(out, name, shape, device):
 
 
 def paged_attention_gqa(query, key_cache, value_cache, plan, scale, out=None, flags=0,
-                        key_new=None, value_new=None, kv_layout="nd"):
+                        key_new=None, value_new=None, kv_layout="nd", key_scale=None,
+                        value_scale=None, softcap=0.0, alibi_slopes=None):
     """Paged GQA attention (reference base.py:48-61 FIA semantics).
 
     query (T, Hq, D) bf16 with D = 128 or 64; key/value caches (NB, bs, Hkv,
@@ -478,13 +684,28 @@ def paged_attention_gqa(query, key_cache, value_cache, plan, scale, out=None, fl
     ``kv_layout="nz"``: the caches hold the NZ layout of the reference's
     graph mode (see ``write_kv_nz``); results are the same as for the same
     values in the standard layout.
+
+    8-bit caches: ``torch.float8_e4m3fn`` tensors with their ``key_scale`` /
+    ``value_scale`` (see ``write_kv_fp8``, which also writes new rows: ``key_new``
+    and the NZ layout are for bf16 caches).
+    Modified scores, with query position i and key position j: ``softcap`` > 0
+    makes them ``softcap * tanh(scale * q.k / softcap)``; ``alibi_slopes`` (Hq,)
+    float32 subtracts ``slope * |i - j|``; a plan with ``prefix_lens`` lets all
+    rows of a request see its first keys.  Rows that see no key give zeros.
     """
     if kv_layout not in KV_LAYOUTS:
         raise ValueError(f"kv_layout must be one of {sorted(KV_LAYOUTS)}")
     flags |= KV_LAYOUTS[kv_layout]
     _check_device_tensor(query, "query", _BF16)
-    _check_device_tensor(key_cache, "key_cache", _BF16)
-    _check_device_tensor(value_cache, "value_cache", _BF16)
+    fp8 = key_scale is not None or value_scale is not None
+    if fp8:
+        _check_fp8_cache(key_cache, key_scale, "key", query.device)
+        _check_fp8_cache(value_cache, value_scale, "value", query.device)
+        _require(key_new is None and value_new is None,
+                 "8-bit caches are written by write_kv_fp8, not by key_new / value_new")
+    else:
+        _check_device_tensor(key_cache, "key_cache", _BF16)
+        _check_device_tensor(value_cache, "value_cache", _BF16)
     _require(query.dim() == 3 and query.stride(2) == 1, "query must be (T, Hq, D), D contiguous")
     shape = query.shape
     T, hq, d = shape
@@ -509,10 +730,25 @@ def paged_attention_gqa(query, key_cache, value_cache, plan, scale, out=None, fl
         _require(key_new.shape == rows and value_new.shape == rows,
                  "new K/V rows must be (tokens, Hkv, D)")
         kn_ts, vn_ts = _row_stride(key_new, "key_new"), _row_stride(value_new, "value_new")
+    scored = softcap != 0 or alibi_slopes is not None or plan.prefix_lens is not None
+    if alibi_slopes is not None:
+        _check_device_tensor(alibi_slopes, "alibi_slopes", torch.float32)
+        if alibi_slopes.shape != (hq,) or not alibi_slopes.is_contiguous() or alibi_slopes.device != device:
+            raise ValueError(f"alibi_slopes must hold {hq} contiguous values on {device}")
     stream = _ready(plan, device)
     q_ts, q_hs, _ = query.stride()
     o_ts, o_hs, _ = out.stride()
     table, ws = plan.block_table, plan.workspace
+    if fp8 or scored:
+        _require(table.device == device, "plan was made on another GPU")
+        _call_on(device, "aia_paged_attention_gqa_ex", query.data_ptr(), q_ts, q_hs,
+                     key_cache.data_ptr(), value_cache.data_ptr(), table.data_ptr(),
+                     table.stride(0), plan.cu_seqlens_q.data_ptr(), plan.seqlens_kv.data_ptr(),
+                     plan.batch, T, hq, hkv, d, bs, nb, float(scale), out.data_ptr(), o_ts,
+                     o_hs, _ptr(key_new), _ptr(value_new), kn_ts, vn_ts, _ptr(key_scale),
+                     _ptr(value_scale), _ptr(plan.prefix_lens), _ptr(alibi_slopes),
+                     float(softcap), plan.num_waves, flags, ws.data_ptr(), ws.numel(), stream)
+        return out
     _native.call("aia_paged_attention_gqa", query.data_ptr(), q_ts, q_hs,
                  key_cache.data_ptr(), value_cache.data_ptr(), table.data_ptr(),
                  table.stride(0), plan.cu_seqlens_q.data_ptr(), plan.seqlens_kv.data_ptr(),
@@ -547,6 +783,7 @@ def paged_attention_mla(q_latent, latent_cache, plan, scale, out=None, flags=0):
     _require(h == plan.num_q_heads and plan.num_kv_heads == 1 and plan.head_dim_v == MLA_LATENT
              and T == plan.num_tokens and bs == plan.block_size,
              "plan was not made for this MLA shape")
+    _require(plan.prefix_lens is None, "MLA attention takes no prefix_lens")
     if out is None:
         out = torch.empty(T, h, MLA_LATENT, dtype=_BF16, device=q_latent.device)
     else:

@@ -65,6 +65,28 @@ int aia_kv_write_nz(const void* key, int64_t key_token_stride, const void* value
                     const int32_t* slot_mapping, int32_t num_tokens, int32_t row_elems,
                     int32_t block_size, int64_t num_slots, void* stream);
 
+/* KV slot write into 8-bit caches.  No counterpart in the reference (its caches
+ * are bf16).  caches: contiguous (num_slots / block_size, block_size,
+ * num_kv_heads, head_dim) OCP e4m3 values, 16-byte aligned; key_scale /
+ * value_scale: contiguous (num_slots / block_size, num_kv_heads) e8m0 bytes (the
+ * power of two 2^(byte - 127)); a cached value stands for value * scale.
+ * For every block and head that the rows touch, need is the least power of two
+ * >= 2^-100 with amax <= 448 * need over the finite values of those rows.  A
+ * block whose first slot is written starts anew with the scale need: its other
+ * slots' contents are lost until they are written.  Any other block gets
+ * max(old, need), and where that grew its other slots are rescaled (to
+ * nearest even, exact above e4m3's subnormal range).  Values that are not
+ * finite are stored as NaN.  Of tokens with the same slot the last one stays.
+ * key / value: (num_tokens, num_kv_heads * head_dim) bf16 rows with token
+ * strides (value may be NULL, with value_cache and value_scale NULL).  Slots < 0
+ * or >= num_slots are skipped.  head_dim 128 or 64, block_size at most 8192
+ * (AIA_ERR_UNSUPPORTED otherwise). */
+int aia_kv_write_fp8(const void* key, int64_t key_token_stride, const void* value,
+                     int64_t value_token_stride, void* key_cache, void* value_cache,
+                     void* key_scale, void* value_scale, const int32_t* slot_mapping,
+                     int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim,
+                     int32_t block_size, int64_t num_slots, void* stream);
+
 /* Bytes of workspace the attention planner/kernels need for a step of at
  * most `batch` requests and `num_tokens` query rows, planned with
  * `num_waves` key ranges (0 = the default, as in aia_attn_plan).  No
@@ -114,6 +136,19 @@ int aia_attn_plan(const int32_t* cu_seqlens_q, const int32_t* seqlens_kv,
                   int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim_v,
                   int32_t num_waves, void* workspace, int64_t workspace_bytes,
                   void* stream);
+
+/* aia_attn_plan for a step whose requests have a prefix that all their rows
+ * see in both directions (prefix_lens: batch int32 entries on the device, 0 =
+ * none; values past the request's keys mean all of them): row i of request b
+ * attends keys j <= Lk - Lq + i and keys j < prefix_lens[b].  Used with
+ * aia_paged_attention_gqa_ex, given the same prefix_lens.  No counterpart in
+ * the reference.  head_dim_v 128 or 64 (AIA_ERR_UNSUPPORTED otherwise). */
+int aia_attn_plan_prefix(const int32_t* cu_seqlens_q, const int32_t* seqlens_kv,
+                         const int32_t* prefix_lens, const int32_t* block_table,
+                         int32_t block_table_stride, int32_t block_size, int32_t batch,
+                         int32_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                         int32_t head_dim_v, int32_t num_waves, void* workspace,
+                         int64_t workspace_bytes, void* stream);
 
 /* Paged GQA attention over a planned step.  Replaces the FIA call of
  * GqaFIABackend._attn (reference auto_infer/layers/attention/gqa.py:81-94 ->
@@ -167,6 +202,33 @@ int aia_paged_attention_gqa(const void* query, int64_t q_token_stride,
                             int64_t new_value_token_stride, int32_t num_waves,
                             int32_t flags, void* workspace, int64_t workspace_bytes,
                             void* stream);
+
+/* aia_paged_attention_gqa over 8-bit caches and with modified scores.  No
+ * counterpart in the reference.  Arguments and checks as there, and:
+ * key_scale / value_scale: both set, the caches are e4m3 values with e8m0
+ *   scales per (block, KV head) as aia_kv_write_fp8 writes them (key_new /
+ *   value_new and AIA_ATTN_KV_NZ are then rejected); both NULL: bf16 caches.
+ * prefix_lens: NULL, or the array the plan was made with (aia_attn_plan_prefix).
+ * alibi_slopes: NULL, or num_q_heads floats on the device.
+ * softcap: 0 for none.
+ * With query position i and key position j, the score of head h is
+ *   s = scale * q.k;  s = softcap * tanh(s / softcap) if softcap > 0;
+ *   s = s - alibi_slopes[h] * |i - j|.
+ * Rows that see no key give zeros. */
+int aia_paged_attention_gqa_ex(const void* query, int64_t q_token_stride, int64_t q_head_stride,
+                               const void* key_cache, const void* value_cache,
+                               const int32_t* block_table, int32_t block_table_stride,
+                               const int32_t* cu_seqlens_q, const int32_t* seqlens_kv,
+                               int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                               int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                               int32_t num_blocks, float scale, void* out,
+                               int64_t out_token_stride, int64_t out_head_stride,
+                               const void* key_new, const void* value_new,
+                               int64_t new_key_token_stride, int64_t new_value_token_stride,
+                               const void* key_scale, const void* value_scale,
+                               const int32_t* prefix_lens, const float* alibi_slopes,
+                               float softcap, int32_t num_waves, int32_t flags, void* workspace,
+                               int64_t workspace_bytes, void* stream);
 
 /* Allocation-free paged GQA attention: aia_attn_plan + aia_paged_attention_gqa
  * in one call, with the plan and the split partials in a static device array
@@ -308,6 +370,25 @@ int aia_qk_norm_rope(void* qkv, int64_t qkv_token_stride, int32_t num_tokens,
                      const void* cos, int64_t cos_token_stride, const void* sin,
                      int64_t sin_token_stride, const void* q_norm_weight,
                      const void* k_norm_weight, float eps, void* stream);
+
+/* Rotary positions of a packed qkv projection (as aia_qk_norm_rope takes it)
+ * from the positions themselves, with an optional per-head RMSNorm in front.
+ * No counterpart in the reference, which gathers cos/sin tables (those go to
+ * aia_qk_norm_rope).  Pair i < rotary_dim / 2 of a head turns by positions[t]
+ * * turns[i] (turns: int64, a 2^-64 fraction of a turn per position, modulo one
+ * turn; exact at any position, also negative ones), cos and sin times factor:
+ * dims i and i + rotary_dim / 2, or with interleaved dims 2 i and 2 i + 1; dims
+ * from rotary_dim on pass through.  All arithmetic is fp32 with one rounding.
+ * q_out (T, Hq, D) / k_out (T, Hkv, D): rows with token strides; the qkv rows
+ * themselves (q_out = qkv, k_out = qkv + Hq * D) for in place, otherwise not
+ * overlapping them.  head_dim 128 or 64, rotary_dim a multiple of 16
+ * (AIA_ERR_UNSUPPORTED otherwise). */
+int aia_rope_qk(const void* qkv, int64_t qkv_token_stride, int32_t num_tokens,
+                int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                const int64_t* positions, const int64_t* turns, int32_t rotary_dim, float factor,
+                int32_t interleaved, const void* q_norm_weight, const void* k_norm_weight,
+                float eps, void* q_out, int64_t q_out_token_stride, void* k_out,
+                int64_t k_out_token_stride, void* stream);
 
 /* Absorbed-MLA latent KV row, one launch.  Replaces the ckv RMSNorm, the
  * k_pe ds_rope_interleave + NeoX RoPE and the cat of mla_paged_absorbed
