@@ -12,15 +12,21 @@
 //
 // All of a block's rows in the call have to be known before any is stored.
 // The slots may come in any order, so each (block, head) has one work-group:
-// that of the call's first token in the block (its leader, found by scanning
-// the slots), which collects the block's tokens in LDS (the highest token of a
-// slot stays), loads their rows once, reduces amax and stores.
+// that of the call's first token in the block, its leader.
+#include <algorithm>
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kHold = 8;              // row passes kept in registers
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kScan = 16;             // slots a thread reads at once in search of a block's tokens
+// Work-groups of a long step.  More leave fewer runs to each but more of them
+// find none (7,399 ragged tokens, 2 heads of 64, blocks of 16, us: 13.3 at 1024,
+// 11.3 at 2048, 11.9 at 3072; 16,384 prompt tokens, 8 heads of 128, blocks of
+// 128: 34.1, 34.3, 36.5).
+constexpr int kTargetGroups = 2048;
 constexpr int kMaxBlock = 8192;       // slots of a block: its tokens are listed in LDS
 constexpr int kMinExp = -100;
 
@@ -30,9 +36,15 @@ struct Args {
   uint8_t* cache[2];
   uint8_t* scale[2];
   const int32_t* slots;
-  int32_t tokens, hkv, bs, window;
+  int32_t tokens, hkv, bs, sub;
   int64_t num_slots;
 };
+
+// A value that all lanes hold, in scalar registers.
+__device__ __forceinline__ uint64_t uniform64(uint64_t x) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
+         (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32;
+}
 
 // Eight consecutive bf16 values.
 template <bool VEC>
@@ -90,95 +102,216 @@ __device__ __forceinline__ uint32_t rescale4(uint32_t w, int down) {
   return (uint32_t)r;
 }
 
-template <int D, bool VEC>
-__global__ __launch_bounds__(kThreads) void kv_write_fp8_kernel(Args a) {
+// Grid: (sub x windows of kThreads tokens, heads of K and V).  A window's runs
+// (tokens at consecutive slots of one block) are found by two loads per
+// thread, this window's and the next one's slots; work-group s of a window
+// takes its runs s, s + sub, ...  A run's rows and its block's scale are loaded
+// at once, speculating that the run is all the block gets in this call, while
+// all slots are scanned to count the block's tokens: a count equal to the run's
+// length confirms it, and the block is done after one barrier.  Otherwise the
+// general path lists the block's tokens in LDS.
+// K and V of a head share the scan.  Measured, us, for 16 decode rows (8 heads of
+// 128, blocks of 16), 16,384 prompt tokens (8 heads of 128, blocks of 128) and
+// 7,399 ragged tokens (2 heads of 64, blocks of 16): every token listed in LDS
+// and all loads dependent 8.7 / 32.1 / 21.7; speculating, K and V apart 4.0 /
+// 34.4 / 15.9; together 4.2 / 33.3 / 11.3, of which the scan is - / 4.9 / 1.9.  The
+// prompt's bytes move at 3.0 TB/s (a large copy: 5.1): every block's loads are
+// over before its stores begin, and the blocks run side by side.  Four heads per
+// work-group (one scan for all): 8.0 / 32.9 / 11.9.
+template <int D, bool VEC, int kHold, int N>
+__global__ __launch_bounds__(kThreads, 4) void kv_write_fp8_kernel(Args a) {
   constexpr int kLanes = D / 8, kRows = kThreads / kLanes;       // threads per new row, rows per pass
   constexpr int kLanes8 = D / 16, kRows8 = kThreads / kLanes8;   // of 16-byte cached pieces
-  extern __shared__ int last[];          // per slot of the block: its last token, -1 = none
-  __shared__ int span[2];                // first and last slot written
-  __shared__ uint32_t wave_max[kThreads / 64];
-  const int tid = threadIdx.x;
-  const int which = blockIdx.y / a.hkv, h = blockIdx.y - which * a.hkv;
-  const uint16_t* src = a.src[which] + (int64_t)h * D;
-  uint8_t* cache = a.cache[which] + (int64_t)h * D;
-  const int64_t ts = a.ts[which];
+  extern __shared__ int last[];          // general path: a slot's last token, -1 = none
+  __shared__ uint64_t starts[kWaves];    // tokens of the window that start a run
+  __shared__ uint64_t joins[2 * kWaves]; // tokens of the window and the next that continue one
+  __shared__ int slots[kThreads];
+  __shared__ int wave_count[kWaves], wave_lo[kWaves], wave_hi[kWaves];
+  __shared__ uint32_t wave_max[N][kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int h = blockIdx.y;
   const int64_t row = (int64_t)a.hkv * D;
-  const int t0 = blockIdx.x * a.window, t1 = min(a.tokens, t0 + a.window);
-  for (int t = t0; t < t1; ++t) {
-    const int slot = a.slots[t];
-    if (slot < 0 || slot >= a.num_slots) continue;
+  auto src = [&](int x, int64_t t) { return a.src[x] + t * a.ts[x] + h * D + 8 * (tid % kLanes); };
+  // (work-groups of one sub index are neighbours, so those that find no run do
+  // not fall on the same XCDs)
+  const int windows = gridDim.x / a.sub, sub = blockIdx.x / windows, window = blockIdx.x - sub * windows;
+  const int t0 = window * kThreads;
+  auto slot_at = [&](int t) { return t >= 0 && t < a.tokens ? a.slots[t] : -1; };
+  const int own = slot_at(t0 + tid);                        // this thread's token's slot
+  {
+    const int before = slot_at(t0 + tid - 1);
+    const int next = slot_at(t0 + kThreads + tid), before_next = slot_at(t0 + kThreads + tid - 1);
+    // (a slot that follows its predecessor's is in the same block unless it
+    // is a block's first; a predecessor that is skipped is followed by none)
+    auto follows = [&](int s, int b) { return s == b + 1 && b >= 0 && s < a.num_slots && s % a.bs != 0; };
+    const bool join = follows(own, before), join_next = follows(next, before_next);
+    const uint64_t s = __ballot(own >= 0 && own < a.num_slots && !join);
+    const uint64_t j = __ballot(join), k = __ballot(join_next);
+    if (lane == 0) { starts[wid] = s; joins[wid] = j; joins[kWaves + wid] = k; }
+    slots[tid] = own;
+  }
+  __syncthreads();
+  const int r = tid / kLanes;
+  bool again = false;
+  int skip = sub;                        // runs of others before this work-group's next one
+  int w = 0;
+  uint64_t left = uniform64(starts[0]);
+  while (true) {
+    const int here = __popcll(left);
+    if (skip >= here) {
+      if (++w == kWaves) return;
+      skip -= here;
+      left = uniform64(starts[w]);
+      continue;
+    }
+    for (; skip > 0; --skip) left &= left - 1;
+    const int bit = __builtin_ctzll(left);
+    left &= left - 1;
+    skip = a.sub - 1;
+    if (again) __syncthreads();          // the previous block's LDS is read no more
+    again = true;
+    const int t = t0 + 64 * w + bit;
+    const int slot = __builtin_amdgcn_readfirstlane(slots[64 * w + bit]);
     const int blk = slot / a.bs, base = blk * a.bs;
-    // a token behind one of its own block is no leader: no scan for it
-    if (t > 0 && (uint32_t)a.slots[t - 1] - (uint32_t)base < (uint32_t)a.bs) continue;
-    __syncthreads();                     // the previous block's LDS is read no more
-    for (int i = tid; i < a.bs; i += kThreads) last[i] = -1;
-    if (tid == 0) { span[0] = a.bs; span[1] = -1; }
+    int run = 1;                         // tokens of the run, as far as the two windows show
+    for (int v = w, from = bit + 1; v < 2 * kWaves; ++v, from = 0) {
+      if (from == 64) continue;
+      const uint64_t stop = ~uniform64(joins[v]) >> from;
+      if (stop) { run += __builtin_ctzll(stop); break; }
+      run += 64 - from;
+    }
+    uint4 held[N][kHold];
+    int old[N];
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+#pragma unroll
+      for (int p = 0; p < kHold; ++p) {
+        held[x][p] = make_uint4(0, 0, 0, 0);
+        if (p * kRows + r < run) held[x][p] = load8<VEC>(src(x, t + p * kRows + r));
+      }
+    }
+    const int64_t scale_at = (int64_t)blk * a.hkv + h;
+#pragma unroll
+    for (int x = 0; x < N; ++x) old[x] = a.scale[x][scale_at];
+    auto mine = [&](int s) { return (uint32_t)s - (uint32_t)base < (uint32_t)a.bs; };
+    int count = 0;                       // the block's tokens that this wave sees
+    if (a.tokens <= kThreads) {
+      count = __popcll(__ballot(mine(own)));
+    } else {
+      int first = 0;
+      for (; first + kThreads * kScan <= a.tokens; first += kThreads * kScan) {
+        int s[kScan];
+#pragma unroll
+        for (int i = 0; i < kScan; ++i) s[i] = a.slots[first + kThreads * i + tid];
+#pragma unroll
+        for (int i = 0; i < kScan; ++i) count += __popcll(__ballot(mine(s[i])));
+      }
+      int s[kScan];
+#pragma unroll
+      for (int i = 0; i < kScan; ++i) {
+        const int at = first + kThreads * i + tid;
+        s[i] = at < a.tokens ? a.slots[at] : -1;
+      }
+#pragma unroll
+      for (int i = 0; i < kScan; ++i) count += __popcll(__ballot(mine(s[i])));
+    }
+    uint32_t m[N];
+    auto wave_amax = [&](uint32_t v) {
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
+      return v;
+    };
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+      m[x] = 0;
+#pragma unroll
+      for (int p = 0; p < kHold; ++p) m[x] = amax8(held[x][p], m[x]);
+      for (int k = kHold * kRows + r; k < run; k += kRows) m[x] = amax8(load8<VEC>(src(x, t + k)), m[x]);
+      m[x] = wave_amax(m[x]);
+      if (lane == 0) wave_max[x][wid] = m[x];
+    }
+    if (lane == 0) wave_count[wid] = count;
     __syncthreads();
-    int earlier = 0;
-    for (int i = tid; i < a.tokens; i += kThreads) {
-      const uint32_t off = (uint32_t)a.slots[i] - (uint32_t)base;
-      if (off < (uint32_t)a.bs) {
+    count = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      count += wave_count[i];
+#pragma unroll
+      for (int x = 0; x < N; ++x) m[x] = max(m[x], wave_max[x][i]);
+    }
+    const bool whole = count == run;     // the run is all the block gets
+    int lo = slot - base, hi = lo + run - 1;
+    if (!whole) {
+      for (int i = tid; i < a.bs; i += kThreads) last[i] = -1;
+      __syncthreads();
+      int earlier = 0;
+      lo = a.bs;
+      hi = -1;
+      for (int i = tid; i < a.tokens; i += kThreads) {
+        const int s = a.slots[i];
+        if (!mine(s)) continue;
         earlier |= i < t;
-        atomicMax(&last[off], i);
-        atomicMin(&span[0], (int)off);
-        atomicMax(&span[1], (int)off);
+        atomicMax(&last[s - base], i);
+        lo = min(lo, s - base);
+        hi = max(hi, s - base);
       }
-    }
-    if (__syncthreads_or(earlier)) continue;
-    const int lo = span[0], hi = span[1];
-    const int passes = (hi - lo) / kRows + 1;
-    const int r = tid / kLanes, c = tid % kLanes;
-    auto token = [&](int p) {
-      const int off = lo + p * kRows + r;
-      return off <= hi ? last[off] : -1;
-    };
-    uint4 held[kHold];
-    uint32_t m = 0;
+      if (__syncthreads_or(earlier)) continue;     // another token leads the block
 #pragma unroll
-    for (int p = 0; p < kHold; ++p) {
-      held[p] = make_uint4(0, 0, 0, 0);
-      if (p < passes) {
-        const int tok = token(p);
-        if (tok >= 0) held[p] = load8<VEC>(src + tok * ts + 8 * c);
-        m = amax8(held[p], m);
+      for (int d = 1; d < 64; d <<= 1) {
+        lo = min(lo, __shfl_xor(lo, d));
+        hi = max(hi, __shfl_xor(hi, d));
       }
-    }
-    for (int p = kHold; p < passes; ++p) {
-      const int tok = token(p);
-      if (tok >= 0) m = amax8(load8<VEC>(src + tok * ts + 8 * c), m);
-    }
+      if (lane == 0) { wave_lo[wid] = lo; wave_hi[wid] = hi; }
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
-    if ((tid & 63) == 0) wave_max[tid >> 6] = m;
-    uint8_t* scale = a.scale[which] + (int64_t)blk * a.hkv + h;
-    const int old = *scale;
-    __syncthreads();
+      for (int x = 0; x < N; ++x) m[x] = 0;
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kThreads / 64; ++i) m = max(m, wave_max[i]);
+      for (int i = 0; i < kWaves; ++i) { lo = min(lo, wave_lo[i]); hi = max(hi, wave_hi[i]); }
+      for (int off = lo + r; off <= hi; off += kRows) {
+        if (last[off] < 0) continue;
+#pragma unroll
+        for (int x = 0; x < N; ++x) m[x] = amax8(load8<VEC>(src(x, last[off])), m[x]);
+      }
+#pragma unroll
+      for (int x = 0; x < N; ++x) {
+        m[x] = wave_amax(m[x]);
+        if (lane == 0) wave_max[x][wid] = m[x];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < N; ++x)
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) m[x] = max(m[x], wave_max[x][i]);
+    }
     const bool anew = lo == 0;           // the block's first slot is written
-    const int need = needed_byte(m);
-    const int e = anew ? need : max(old, need);
-    const float f = __builtin_ldexpf(1.f, 127 - e);
-    auto store = [&](int p, uint4 v) {
-      const int64_t at = (int64_t)(base + lo + p * kRows + r) * row + 8 * c;
-      *reinterpret_cast<uint2*>(cache + at) = quantise8(v, f);
-    };
 #pragma unroll
-    for (int p = 0; p < kHold; ++p)
-      if (p < passes && token(p) >= 0) store(p, held[p]);
-    for (int p = kHold; p < passes; ++p) {
-      const int tok = token(p);
-      if (tok >= 0) store(p, load8<VEC>(src + tok * ts + 8 * c));
-    }
-    if (e == old && !anew) continue;
-    if (tid == 0) *scale = (uint8_t)e;
-    if (anew) continue;
-    for (int off = tid / kLanes8; off < a.bs; off += kRows8) {
-      if (last[off] >= 0) continue;
-      uint4* p = reinterpret_cast<uint4*>(cache + (int64_t)(base + off) * row) + tid % kLanes8;
-      const uint4 v = *p;
-      *p = make_uint4(rescale4(v.x, e - old), rescale4(v.y, e - old), rescale4(v.z, e - old),
-                      rescale4(v.w, e - old));
+    for (int x = 0; x < N; ++x) {
+      const int need = needed_byte(m[x]);
+      const int e = anew ? need : max(old[x], need);
+      const float f = __builtin_ldexpf(1.f, 127 - e);
+      uint8_t* cache = a.cache[x] + (int64_t)base * row + h * D;
+      auto store = [&](int off, uint4 v) {
+        *reinterpret_cast<uint2*>(cache + off * row + 8 * (tid % kLanes)) = quantise8(v, f);
+      };
+      if (whole) {
+#pragma unroll
+        for (int p = 0; p < kHold; ++p)
+          if (p * kRows + r < run) store(lo + p * kRows + r, held[x][p]);
+        for (int k = kHold * kRows + r; k < run; k += kRows) store(lo + k, load8<VEC>(src(x, t + k)));
+      } else {
+        for (int off = lo + r; off <= hi; off += kRows)
+          if (last[off] >= 0) store(off, load8<VEC>(src(x, last[off])));
+      }
+      if (e == old[x]) continue;
+      if (tid == 0) a.scale[x][scale_at] = (uint8_t)e;
+      if (anew) continue;
+      for (int off = tid / kLanes8; off < a.bs; off += kRows8) {
+        if (whole ? off >= lo && off <= hi : last[off] >= 0) continue;
+        uint4* p = reinterpret_cast<uint4*>(cache + off * row) + tid % kLanes8;
+        const uint4 v = *p;
+        *p = make_uint4(rescale4(v.x, e - old[x]), rescale4(v.y, e - old[x]), rescale4(v.z, e - old[x]),
+                        rescale4(v.w, e - old[x]));
+      }
     }
   }
 }
@@ -199,8 +332,8 @@ extern "C" int aia_kv_write_fp8(const void* key, int64_t key_token_stride, const
     return fail(AIA_ERR_UNSUPPORTED, "aia_kv_write_fp8: head_dim %d (128 or 64)", head_dim);
   if (block_size > kMaxBlock)
     return fail(AIA_ERR_UNSUPPORTED, "aia_kv_write_fp8: block_size %d (at most %d)", block_size, kMaxBlock);
-  if (num_kv_heads > 32767)
-    return fail(AIA_ERR_UNSUPPORTED, "aia_kv_write_fp8: %d KV heads (at most 32767)", num_kv_heads);
+  if (num_kv_heads > 65535)
+    return fail(AIA_ERR_UNSUPPORTED, "aia_kv_write_fp8: %d KV heads (at most 65535)", num_kv_heads);
   if (num_tokens == 0) return AIA_OK;
   const bool has_v = value != nullptr;
   if (!key || !key_cache || !key_scale || !slot_mapping)
@@ -220,17 +353,28 @@ extern "C" int aia_kv_write_fp8(const void* key, int64_t key_token_stride, const
   a.scale[0] = static_cast<uint8_t*>(key_scale); a.scale[1] = static_cast<uint8_t*>(value_scale);
   a.slots = slot_mapping;
   a.tokens = num_tokens; a.hkv = num_kv_heads; a.bs = block_size; a.num_slots = num_slots;
-  // tokens a work-group looks over for leaders: one in short steps (every
-  // decode row leads its block), more where most tokens lead nothing
-  const int heads = num_kv_heads * (has_v ? 2 : 1);
-  a.window = 1;
-  while (a.window < 16 && (int64_t)num_tokens * heads > 8192LL * a.window) a.window *= 2;
-  const dim3 grid((unsigned)((num_tokens + a.window - 1) / a.window), (unsigned)heads);
+  // Work-groups per window and head: one round of them on the chip, so that a
+  // decode step's tokens, a run each, spread over many.
+  const int windows = (num_tokens + kThreads - 1) / kThreads;
+  a.sub = std::max(1, std::min({kThreads, num_tokens, kTargetGroups / std::max(1, windows * num_kv_heads)}));
+  const dim3 grid((unsigned)windows * (unsigned)a.sub, (unsigned)num_kv_heads);
   const bool vec = aligned(key) && key_token_stride % 8 == 0 &&
                    (!has_v || (aligned(value) && value_token_stride % 8 == 0));
   const size_t lds = (size_t)block_size * sizeof(int);
-  auto* kernel = head_dim == 128 ? (vec ? kv_write_fp8_kernel<128, true> : kv_write_fp8_kernel<128, false>)
-                                 : (vec ? kv_write_fp8_kernel<64, true> : kv_write_fp8_kernel<64, false>);
+  // row passes kept in registers: all of a block of up to 128 slots (head_dim
+  // 128); small blocks' few registers let twice as many work-groups run
+  auto pick = [&](auto hold) {
+    constexpr int H = decltype(hold)::value;
+    if (!has_v)
+      return head_dim == 128 ? (vec ? kv_write_fp8_kernel<128, true, H, 1> : kv_write_fp8_kernel<128, false, H, 1>)
+                             : (vec ? kv_write_fp8_kernel<64, true, H, 1> : kv_write_fp8_kernel<64, false, H, 1>);
+    return head_dim == 128 ? (vec ? kv_write_fp8_kernel<128, true, H, 2> : kv_write_fp8_kernel<128, false, H, 2>)
+                           : (vec ? kv_write_fp8_kernel<64, true, H, 2> : kv_write_fp8_kernel<64, false, H, 2>);
+  };
+  const int passes = (block_size * (head_dim / 8) + kThreads - 1) / kThreads;
+  auto* kernel = passes <= 1 ? pick(std::integral_constant<int, 1>{})
+                 : passes <= 4 ? pick(std::integral_constant<int, 4>{})
+                               : pick(std::integral_constant<int, 8>{});
   kernel<<<grid, kThreads, lds, (hipStream_t)stream>>>(a);
   return check_hip(hipGetLastError(), "aia_kv_write_fp8 launch");
 }

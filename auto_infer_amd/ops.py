@@ -29,14 +29,30 @@ def _stream(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def _call_on(device, name, *args):
-    """An entry point's launch with ``device`` current: its stream handle may be
-    the default stream's, which is that of the current device."""
-    if torch.cuda.current_device() == device.index:
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _call_on(dev, name, *args):
+    """An entry point's launch with GPU ``dev`` (an index) current: its stream
+    handle may be the default stream's, which is that of the current device."""
+    if _current_device() == dev:
         _native.call(name, *args)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(dev):
             _native.call(name, *args)
+
+
+def _stream_of(dev):
+    return (torch.cuda.current_stream(dev).cuda_stream if _raw_stream is None
+            else _raw_stream(dev))
+
+
+def _check_on(t, name, dtype, dev):
+    """``t`` is a ``dtype`` tensor on GPU ``dev`` (an index: -1, a CPU tensor's,
+    fails the first check of a call)."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.get_device() != dev or dev < 0:
+        _check_device_tensor(t, name, dtype)
+        raise ValueError(f"{name} must be on cuda:{dev}")
 
 
 def _ptr(t):
@@ -201,38 +217,48 @@ def rope_qk(qkv, num_q_heads, num_kv_heads, positions, rope, q_norm_weight=None,
     Returns the rotated (q, k) and the V view, (T, heads, D) each.  Unlike
     ``qk_norm_rope`` (cos/sin rows, bf16 roundings of the separate ops) it
     computes the angles itself and rounds once."""
-    _check_device_tensor(qkv, "qkv", _BF16)
-    _require(qkv.dim() == 2 and qkv.stride(1) == 1, "qkv must be (T, width) with unit inner stride")
-    T, width = qkv.shape
     _require(isinstance(rope, RotaryEmbedding), "rope must be a RotaryEmbedding")
-    D, device = rope.head_dim, qkv.device
-    if num_q_heads <= 0 or num_kv_heads <= 0 or width != (num_q_heads + 2 * num_kv_heads) * D:
+    _check_device_tensor(qkv, "qkv", _BF16)
+    dev, D = qkv.get_device(), rope.head_dim
+    if qkv.dim() != 2 or qkv.stride(1) != 1:
+        raise ValueError("qkv must be (T, width) with unit inner stride")
+    T, width = qkv.shape
+    nq, nk = num_q_heads * D, num_kv_heads * D
+    if num_q_heads <= 0 or num_kv_heads <= 0 or width != nq + 2 * nk:
         raise ValueError(f"qkv width {width} != (Hq + 2 Hkv) x {D}")
-    _check_device_tensor(positions, "positions", torch.int64)
-    _require(positions.shape == (T,) and positions.is_contiguous(),
-             "positions must hold one contiguous entry per token")
-    _require(positions.device == device and rope.turns.device == device,
-             "qkv, positions and rope must be on the same GPU")
-    _require((q_norm_weight is None) == (k_norm_weight is None), "q and k norm weights go together")
-    for t, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
-        if t is not None:
-            _check_device_tensor(t, name, _BF16)
-            if t.numel() != D or not t.is_contiguous() or t.device != device:
-                raise ValueError(f"{name} must be {D} contiguous values on {device}")
-    q, k, v = qkv.split((num_q_heads * D, num_kv_heads * D, num_kv_heads * D), dim=-1)
-    v = v.view(T, num_kv_heads, D)
+    _check_on(positions, "positions", torch.int64, dev)
+    if positions.shape != (T,) or not positions.is_contiguous():
+        raise ValueError("positions must hold one contiguous entry per token")
+    if rope.turns.get_device() != dev:
+        raise ValueError(f"rope must be on cuda:{dev}")
+    if q_norm_weight is not None or k_norm_weight is not None:
+        _require(q_norm_weight is not None and k_norm_weight is not None,
+                 "q and k norm weights go together")
+        for t, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
+            _check_on(t, name, _BF16, dev)
+            if t.numel() != D or not t.is_contiguous():
+                raise ValueError(f"{name} must be {D} contiguous values")
+    ts = qkv.stride(0) if T > 1 else width
+    # (T, heads, D) views of the packed rows
+    v = qkv.as_strided((T, num_kv_heads, D), (ts, D, 1), qkv.storage_offset() + nq + nk)
     if out is None:
-        q, k = q.view(T, num_q_heads, D), k.view(T, num_kv_heads, D)
+        at = qkv.data_ptr()
+        q = qkv.as_strided((T, num_q_heads, D), (ts, D, 1))
+        k = qkv.as_strided((T, num_kv_heads, D), (ts, D, 1), qkv.storage_offset() + nq)
+        q_at, q_ts, k_at, k_ts = at, ts, at + 2 * nq, ts
     else:
         q, k = out
-        _check_out(q, "q_out", (T, num_q_heads, D), device)
-        _check_out(k, "k_out", (T, num_kv_heads, D), device)
-    _call_on(device, "aia_rope_qk", _ptr(qkv), qkv.stride(0) if T > 1 else width, T, num_q_heads,
-                 num_kv_heads, D, _ptr(positions), _ptr(rope.turns), rope.rotary_dim,
-                 rope.attention_factor, int(rope.interleaved), _ptr(q_norm_weight),
-                 _ptr(k_norm_weight), float(eps), _ptr(q),
-                 _row_stride(q, "q_out") if T > 1 else num_q_heads * D, _ptr(k),
-                 _row_stride(k, "k_out") if T > 1 else num_kv_heads * D, _stream(device))
+        for t, name, heads in ((q, "q_out", num_q_heads), (k, "k_out", num_kv_heads)):
+            _check_on(t, name, _BF16, dev)
+            if t.shape != (T, heads, D):
+                raise ValueError(f"{name} must have shape {(T, heads, D)}, got {tuple(t.shape)}")
+        q_at, k_at = q.data_ptr(), k.data_ptr()
+        q_ts = _row_stride(q, "q_out") if T > 1 else nq
+        k_ts = _row_stride(k, "k_out") if T > 1 else nk
+    _call_on(dev, "aia_rope_qk", qkv.data_ptr(), ts, T, num_q_heads, num_kv_heads, D,
+             positions.data_ptr(), rope.turns.data_ptr(), rope.rotary_dim, rope.attention_factor,
+             rope.interleaved, _ptr(q_norm_weight), _ptr(k_norm_weight), eps, q_at, q_ts, k_at,
+             k_ts, _stream_of(dev))
     return q, k, v
 
 
@@ -437,16 +463,17 @@ def write_kv_nz(key, value, key_cache, value_cache, slot_mapping):
                  _stream(key.device))
 
 
-def _check_fp8_cache(cache, scale, name, device):
-    """An 8-bit cache (NB, bs, Hkv, D) and its scales (NB, Hkv)."""
-    _check_device_tensor(cache, f"{name}_cache", FP8_KV)
-    _check_device_tensor(scale, f"{name}_scale", FP8_KV_SCALE)
-    if cache.dim() != 4 or not cache.is_contiguous():
-        raise ValueError(f"{name}_cache must be a contiguous (num_blocks, block_size, Hkv, D) tensor")
-    if scale.shape != (cache.shape[0], cache.shape[2]) or not scale.is_contiguous():
-        raise ValueError(f"{name}_scale must be a contiguous (num_blocks, Hkv) tensor")
-    if cache.device != device or scale.device != device:
-        raise ValueError(f"{name}_cache and {name}_scale must be on {device}")
+def _check_fp8_cache(cache, scale, cache_name, scale_name, dev):
+    """An 8-bit cache (NB, bs, Hkv, D) and its scales (NB, Hkv); returns the
+    cache's shape."""
+    _check_on(cache, cache_name, FP8_KV, dev)
+    _check_on(scale, scale_name, FP8_KV_SCALE, dev)
+    shape = cache.shape
+    if len(shape) != 4 or not cache.is_contiguous():
+        raise ValueError(f"{cache_name} must be a contiguous (num_blocks, block_size, Hkv, D) tensor")
+    if scale.shape != (shape[0], shape[2]) or not scale.is_contiguous():
+        raise ValueError(f"{scale_name} must be a contiguous (num_blocks, Hkv) tensor")
+    return shape
 
 
 def write_kv_fp8(key, value, key_cache, value_cache, key_scale, value_scale, slot_mapping):
@@ -462,29 +489,32 @@ def write_kv_fp8(key, value, key_cache, value_cache, key_scale, value_scale, slo
     cache and its scale may be None.  Slots outside the cache are skipped; of
     tokens with the same slot the last one stays."""
     _check_device_tensor(key, "key", _BF16)
-    device = key.device
-    _check_fp8_cache(key_cache, key_scale, "key", device)
-    _check_device_tensor(slot_mapping, "slot_mapping", torch.int32)
-    nb, bs, hkv, d = key_cache.shape
-    _require(key.dim() == 3 and key.shape[1:] == (hkv, d),
-             "key rows do not match the key cache's (heads, dim)")
-    T = key.shape[0]
-    _require(slot_mapping.shape == (T,) and slot_mapping.is_contiguous() and
-             slot_mapping.device == device,
-             "slot_mapping must be a contiguous 1-D tensor with one slot per token")
-    kts, vts = _row_stride(key, "key") if T > 1 else hkv * d, 0
+    dev = key.get_device()
+    shape = _check_fp8_cache(key_cache, key_scale, "key_cache", "key_scale", dev)
+    nb, bs, hkv, d = shape
+    rows = key.shape
+    if len(rows) != 3 or rows[1:] != shape[2:]:
+        raise ValueError("key rows do not match the key cache's (heads, dim)")
+    T = rows[0]
+    _check_on(slot_mapping, "slot_mapping", torch.int32, dev)
+    if slot_mapping.shape != (T,) or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be a contiguous 1-D tensor with one slot per token")
+    kts = _row_stride(key, "key") if T > 1 else hkv * d
     if value is not None:
-        _check_device_tensor(value, "value", _BF16)
-        _check_fp8_cache(value_cache, value_scale, "value", device)
-        _require(value_cache.shape == key_cache.shape, "value_cache must match key_cache")
-        _require(value.shape == key.shape and value.device == device, "value must match key")
+        _check_on(value, "value", _BF16, dev)
+        if _check_fp8_cache(value_cache, value_scale, "value_cache", "value_scale", dev) != shape:
+            raise ValueError("value_cache must match key_cache")
+        if value.shape != rows:
+            raise ValueError("value must match key")
         vts = _row_stride(value, "value") if T > 1 else hkv * d
+        v_at, vc_at, vs_at = value.data_ptr(), value_cache.data_ptr(), value_scale.data_ptr()
     else:
         _require(value_cache is None and value_scale is None,
                  "value_cache or value_scale given without value")
-    _call_on(device, "aia_kv_write_fp8", _ptr(key), kts, _ptr(value), vts, _ptr(key_cache),
-                 _ptr(value_cache), _ptr(key_scale), _ptr(value_scale), _ptr(slot_mapping), T, hkv,
-                 d, bs, nb * bs, _stream(device))
+        vts, v_at, vc_at, vs_at = 0, None, None, None
+    _call_on(dev, "aia_kv_write_fp8", key.data_ptr(), kts, v_at, vts, key_cache.data_ptr(), vc_at,
+             key_scale.data_ptr(), vs_at, slot_mapping.data_ptr(), T, hkv, d, bs, nb * bs,
+             _stream_of(dev))
 
 
 KV_LAYOUTS = {"nd": 0, "nz": 1}   # nz: AIA_ATTN_KV_NZ
@@ -586,9 +616,9 @@ class AttentionPlan:
                 self.head_dim_v, self.num_waves, _ptr(self.workspace),
                 self.workspace.numel(), self._on[1])
         if self.prefix_lens is None:
-            _call_on(device, "aia_attn_plan", _ptr(self.cu_seqlens_q), _ptr(self.seqlens_kv), *args)
+            _call_on(device.index, "aia_attn_plan", _ptr(self.cu_seqlens_q), _ptr(self.seqlens_kv), *args)
         else:
-            _call_on(device, "aia_attn_plan_prefix", _ptr(self.cu_seqlens_q), _ptr(self.seqlens_kv),
+            _call_on(device.index, "aia_attn_plan_prefix", _ptr(self.cu_seqlens_q), _ptr(self.seqlens_kv),
                          _ptr(self.prefix_lens), *args)
 
     def _use_on(self, stream):
@@ -699,8 +729,9 @@ def paged_attention_gqa(query, key_cache, value_cache, plan, scale, out=None, fl
     _check_device_tensor(query, "query", _BF16)
     fp8 = key_scale is not None or value_scale is not None
     if fp8:
-        _check_fp8_cache(key_cache, key_scale, "key", query.device)
-        _check_fp8_cache(value_cache, value_scale, "value", query.device)
+        dev = query.get_device()
+        _check_fp8_cache(key_cache, key_scale, "key_cache", "key_scale", dev)
+        _check_fp8_cache(value_cache, value_scale, "value_cache", "value_scale", dev)
         _require(key_new is None and value_new is None,
                  "8-bit caches are written by write_kv_fp8, not by key_new / value_new")
     else:
@@ -741,7 +772,7 @@ def paged_attention_gqa(query, key_cache, value_cache, plan, scale, out=None, fl
     table, ws = plan.block_table, plan.workspace
     if fp8 or scored:
         _require(table.device == device, "plan was made on another GPU")
-        _call_on(device, "aia_paged_attention_gqa_ex", query.data_ptr(), q_ts, q_hs,
+        _call_on(device.index, "aia_paged_attention_gqa_ex", query.data_ptr(), q_ts, q_hs,
                      key_cache.data_ptr(), value_cache.data_ptr(), table.data_ptr(),
                      table.stride(0), plan.cu_seqlens_q.data_ptr(), plan.seqlens_kv.data_ptr(),
                      plan.batch, T, hq, hkv, d, bs, nb, float(scale), out.data_ptr(), o_ts,

@@ -82,6 +82,24 @@ def test_slots_in_any_order(order):
     write_both(k, v, slots, kv, vv)
 
 
+@pytest.mark.parametrize("bs", [16, 128, 1000])
+def test_slots_in_any_order_of_a_long_step(bs):
+    """Blocks whose tokens are spread over a step of several windows, runs that
+    cross windows, and both in one call."""
+    gen = torch.Generator().manual_seed(bs)
+    h, d, nb = 2, 64, -(-4000 // bs)
+    for kind in ("shuffled", "straight", "pieces"):
+        kv, vv = fresh(nb, bs, h, d, gen), fresh(nb, bs, h, d, gen)
+        slots = list(range(5, 5 + 900))
+        if kind == "shuffled":
+            slots = torch.randperm(nb * bs, generator=gen)[:700].tolist()
+        elif kind == "pieces":
+            slots = slots[300:] + [-1] * 7 + slots[:290] + [slots[40], slots[850]] + list(range(2000, 3100))
+        k = (torch.randn(len(slots), h, d, generator=gen) * 9).bfloat16()
+        v = torch.randn(len(slots), h, d, generator=gen).bfloat16()
+        write_both(k, v, slots, kv, vv)
+
+
 def test_values_at_the_borders():
     """Largest values at and next to 448 * 2^e, ties of the rounding, zeros,
     subnormal and huge rows, and values that are not finite."""
