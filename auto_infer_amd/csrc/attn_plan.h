@@ -88,14 +88,11 @@ struct PrefillArgs {
 // Cache formats a GQA kernel is built for.
 constexpr int kKvNd = 0, kKvNz = 1, kKvFp8 = 2;
 
-// The attention launches of one call (without the merge) with modified scores
-// over bf16 caches (kv kKvNd or kKvNz), and over 8-bit caches (scored: with
-// modified scores).
-int launch_gqa_scored(int kv, const AttnArgs& a, const PrefillArgs& pa, const Layout& L,
-                      const Geometry& g, int32_t head_dim, int32_t waves, bool one_block,
-                      hipStream_t s);
-int launch_gqa_fp8(bool scored, const AttnArgs& a, const PrefillArgs& pa, const Layout& L,
-                   const Geometry& g, int32_t head_dim, int32_t waves, bool one_block, hipStream_t s);
+// The attention launches of one call (without the merge) that sources of their
+// own build: modified scores over bf16 caches, and 8-bit caches.
+using LaunchGqa = int(const AttnArgs& a, const PrefillArgs& pa, const Layout& L, const Geometry& g,
+                      int32_t head_dim, int32_t waves, bool one_block, hipStream_t s);
+LaunchGqa launch_gqa_scored_nd, launch_gqa_scored_nz, launch_gqa_fp8, launch_gqa_fp8_scored;
 
 }  // namespace aia
 

@@ -19,8 +19,9 @@ ROOT = os.path.dirname(PKG)
 OUT_DIR = os.path.join(PKG, "_lib")
 LIB = os.path.join(OUT_DIR, "libautoinfer_amd.so")
 PROBES = os.path.join(OUT_DIR, "libaia_probes.so")
-SOURCES = ["core.hip", "kv_write.hip", "kv_write_fp8.hip", "paged_attention.hip", "gqa_scored.hip",
-           "gqa_fp8.hip", "noalloc.hip", "pack.hip", "qk_rope.hip", "rope.hip", "mtp_compact.hip", "mla_pre.hip"]
+SOURCES = ["gqa_fp8_scored.hip", "gqa_scored_nz.hip", "gqa_scored.hip", "paged_attention.hip",
+           "gqa_fp8.hip", "core.hip", "kv_write.hip", "kv_write_fp8.hip", "noalloc.hip",
+           "pack.hip", "qk_rope.hip", "rope.hip", "mtp_compact.hip", "mla_pre.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",

@@ -151,20 +151,29 @@ __device__ __forceinline__ void write_segment(const AttnArgs& a, float4_t (&o)[R
 // caches (gqa.py:163,202-226): each block viewed (Hkv D / 16, block_size,
 // 16), so 16 dims of all of a block's tokens are contiguous.  kv_piece gives
 // the 16-byte index of piece p (8 dims) of head h of (block, offset).
-// Modified score of a raw dot product, in log2 units (see ScoreArgs): far =
-// query position - key position.
+// What is done to a raw dot product: nothing (the scale goes into the
+// exponent), nothing but a prefix to see, a cap, a bias, both, or what the call's
+// ScoreArgs say at run time.  Decode rows wait for memory, so one run-time form
+// serves them all (64 requests of up to 4096 keys, 32/8 heads: 120.5 us with a
+// cap, 119.4 without); prefill units wait for the VALU and have a form each.
+constexpr int kPlain = 0, kPrefixOnly = 1, kCap = 2, kBias = 3, kCapBias = 4, kAnyScore = 5;
+
+// Modified scores in log2 units (see ScoreArgs); far = query position - key
+// position.
+template <int SC>
 struct ScoreMod {
   float scale, cap_in, cap_out;
   bool cap, bias;
   __device__ __forceinline__ ScoreMod(const ScoreArgs& s, float scale_log2)
-      : scale(scale_log2), cap_in(s.cap_in), cap_out(s.cap_out), cap(s.cap_out > 0.f),
-        bias(s.slopes != nullptr) {}
+      : scale(scale_log2), cap_in(s.cap_in), cap_out(s.cap_out),
+        cap(SC == kAnyScore ? s.cap_out > 0.f : SC == kCap || SC == kCapBias),
+        bias(SC == kAnyScore ? s.slopes != nullptr : SC == kBias || SC == kCapBias) {}
+  __device__ __forceinline__ float capped(float x) const {
+    const float t = __builtin_amdgcn_exp2f(x * cap_in);
+    return __builtin_fmaf(-2.f * cap_out, __builtin_amdgcn_rcpf(t + 1.f), cap_out);
+  }
   __device__ __forceinline__ float operator()(float x, float far, float slope) const {
-    float y = x * scale;
-    if (cap) {
-      const float t = __builtin_amdgcn_exp2f(x * cap_in);
-      y = __builtin_fmaf(-2.f * cap_out, __builtin_amdgcn_rcpf(t + 1.f), cap_out);
-    }
+    float y = cap ? capped(x) : x * scale;
     if (bias) y = __builtin_fmaf(-slope, __builtin_fabsf(far), y);
     return y;
   }
@@ -184,7 +193,7 @@ __device__ __forceinline__ int64_t kv_piece(int64_t blk, int off, int bs, int ro
          (((int64_t)(h * (D / 16) + (p >> 1)) * bs + off) << 1) + (p & 1);
 }
 
-template <int RB, int D, int KV, bool MOD>
+template <int RB, int D, int KV, int SC>
 __device__ __forceinline__ void gqa_segment(const AttnArgs& a, const int* rec, int s, int lt0,
                                             int lt1, int w, int tpw, uint16_t* vt, int lane,
                                             int wid, bool use_pre, int pre) {
@@ -207,9 +216,9 @@ __device__ __forceinline__ void gqa_segment(const AttnArgs& a, const int* rec, i
     lim[r] = rv[r] ? lim_base + qi[r] : -1;
   }
   int visible = max(0, lim_base + nq);
-  const ScoreMod mod(a.sc, a.scale_log2);
+  const ScoreMod<SC> mod(a.sc, a.scale_log2);
   float slope[RB];
-  if (MOD) {
+  if (SC != kPlain) {
     const int pre = prefix_keys(a.sc, b);
     visible = max(visible, pre);
 #pragma unroll
@@ -323,12 +332,12 @@ __device__ __forceinline__ void gqa_segment(const AttnArgs& a, const int* rec, i
       float sv[4];
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
-        const float x = MOD ? mod(acc[r][v], (float)(lim_base + qi[r] - tb - v), slope[r]) : acc[r][v];
+        const float x = SC != kPlain ? mod(acc[r][v], (float)(lim_base + qi[r] - tb - v), slope[r]) : acc[r][v];
         sv[v] = (!masked || tb + v <= lim[r]) ? x : -INFINITY;
       }
       float tmax = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
       tmax = aia::group4_max(tmax);
-      const float sl = MOD ? 1.f : a.scale_log2;
+      const float sl = SC != kPlain ? 1.f : a.scale_log2;
       const float mnew = fmaxf(m[r], tmax * sl);
       float p[4];
 #pragma unroll
@@ -418,7 +427,7 @@ __device__ __forceinline__ void fp8_to_bf16(uint4 w, uint32_t e, uint4 (&out)[2]
 // the same order.  Values become bf16 in registers with their block's scale,
 // so the scores need no further factor.  The scales are held like the block
 // ids, one logical block per lane.
-template <int RB, int D, bool MOD>
+template <int RB, int D, int SC>
 __device__ __forceinline__ void gqa_segment_fp8(const AttnArgs& a, const int* rec, int s, int lt0,
                                                 int lt1, int w, int tpw, uint16_t* vt0, uint16_t* vt1,
                                                 int lane, int wid, bool use_pre, int pre_id) {
@@ -434,10 +443,10 @@ __device__ __forceinline__ void gqa_segment_fp8(const AttnArgs& a, const int* re
   const int nblk = (nq + qb - 1) / qb;               // row blocks holding tokens
   const int head = kvh * a.group + hbi * a.hb + hh;
   const int row_bytes = a.hkv * D;
-  const ScoreMod mod(a.sc, a.scale_log2);
+  const ScoreMod<SC> mod(a.sc, a.scale_log2);
   int visible = max(0, lim_base + nq);
   int pre = 0;
-  if (MOD) {
+  if (SC != kPlain) {
     pre = prefix_keys(a.sc, b);
     visible = max(visible, pre);
   }
@@ -451,7 +460,7 @@ __device__ __forceinline__ void gqa_segment_fp8(const AttnArgs& a, const int* re
     rv[r] = nt < qb && qi[r] < nq && hbi * a.hb + hh < a.group;
     lim[r] = rv[r] ? max(lim_base + qi[r], pre - 1) : -1;
     lim_lo = rv[r] ? min(lim_lo, lim[r]) : lim_lo;
-    slope[r] = MOD && mod.bias && rv[r] ? a.sc.slopes[head] * kLog2e : 0.f;
+    slope[r] = SC != kPlain && mod.bias && rv[r] ? a.sc.slopes[head] * kLog2e : 0.f;
   }
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) lim_lo = min(lim_lo, __shfl_xor(lim_lo, d));
@@ -538,12 +547,12 @@ __device__ __forceinline__ void gqa_segment_fp8(const AttnArgs& a, const int* re
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
           const int k = 16 * st + v;
-          const float x = MOD ? mod(acc[r][st][v], (float)(lim_base + qi[r] - tb - k), slope[r]) : acc[r][st][v];
+          const float x = SC != kPlain ? mod(acc[r][st][v], (float)(lim_base + qi[r] - tb - k), slope[r]) : acc[r][st][v];
           sv[st][v] = (!masked || k <= last) ? x : -INFINITY;
           tmax = fmaxf(tmax, sv[st][v]);
         }
       tmax = aia::group4_max(tmax);
-      const float sl = MOD ? 1.f : a.scale_log2;
+      const float sl = SC != kPlain ? 1.f : a.scale_log2;
       const float mnew = fmaxf(m[r], tmax * sl);
       float p[2][4];
       float psum = 0.f;
@@ -609,7 +618,7 @@ __device__ __forceinline__ void gqa_segment_fp8(const AttnArgs& a, const int* re
 
 // One work-group per key range, one wave per kv head of the segment's group.
 // D: head dim, 128 or 64.
-template <int NW, int RB, int D, int KV, bool MOD>
+template <int NW, int RB, int D, int KV, int SC>
 #ifndef AIA_GQA_WAVES_PER_EU
 #define AIA_GQA_WAVES_PER_EU 2
 #endif
@@ -643,10 +652,10 @@ __device__ __forceinline__ void gqa_attn_body(const AttnArgs& a, int bid,
       if ((rec[1] & 0xffff) * NW + wid < a.hkv)
       {
         if constexpr (KV == aia::kKvFp8)
-          gqa_segment_fp8<RB, D, MOD>(a, rec, s, t - rec[5], chunk_end - rec[5], w, tpw, vt, vt_all1[wid],
+          gqa_segment_fp8<RB, D, SC>(a, rec, s, t - rec[5], chunk_end - rec[5], w, tpw, vt, vt_all1[wid],
                                       lane, wid, first, pre);
         else
-          gqa_segment<RB, D, KV, MOD>(a, rec, s, t - rec[5], chunk_end - rec[5], w, tpw, vt, lane, wid,
+          gqa_segment<RB, D, KV, SC>(a, rec, s, t - rec[5], chunk_end - rec[5], w, tpw, vt, lane, wid,
                                       first, pre);
       }
       first = false;
@@ -660,15 +669,15 @@ __device__ __forceinline__ void gqa_attn_body(const AttnArgs& a, int bid,
   }
 }
 
-template <int NW, int RB, int D, int KV, bool MOD>
+template <int NW, int RB, int D, int KV, int SC>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(AIA_GQA_WAVES_PER_EU, AIA_GQA_WAVES_PER_EU)))
 void gqa_attn_kernel(AttnArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t vt_all[NW][kTile * kVStride];
   if constexpr (KV == aia::kKvFp8) {       // a step is two 16-key tiles
     __shared__ __attribute__((aligned(16))) uint16_t vt_all1[NW][kTile * kVStride];
-    gqa_attn_body<NW, RB, D, KV, MOD>(a, blockIdx.x, vt_all, vt_all1);
+    gqa_attn_body<NW, RB, D, KV, SC>(a, blockIdx.x, vt_all, vt_all1);
   } else {
-    gqa_attn_body<NW, RB, D, KV, MOD>(a, blockIdx.x, vt_all, nullptr);
+    gqa_attn_body<NW, RB, D, KV, SC>(a, blockIdx.x, vt_all, nullptr);
   }
 }
 
@@ -714,7 +723,7 @@ constexpr float kLazyLog2 = AIA_PF_LAZY;              // max growth (log2) befor
 #ifndef AIA_PF_WPE
 #define AIA_PF_WPE 2
 #endif
-template <bool ONE_BLOCK, bool FUSED, int D, int KV, bool MOD>
+template <bool ONE_BLOCK, bool FUSED, int D, int KV, int SC>
 __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
                                                  uint16_t* k0, uint16_t* k1,
                                                  uint16_t* v0, uint16_t* v1) {
@@ -761,8 +770,8 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
     }
   }
 
-  const int pre = MOD ? prefix_keys(a.sc, b) : 0;
-  const ScoreMod mod(a.sc, a.scale_log2);
+  const int pre = SC != kPlain ? prefix_keys(a.sc, b) : 0;
+  const ScoreMod<SC> mod(a.sc, a.scale_log2);
   float slope[kPfRt];
   // this wave's rows
   int lim[kPfRt], tokr[kPfRt], headr[kPfRt];
@@ -775,7 +784,9 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
     tokr[rt] = row / G;
     headr[rt] = kvh * G + (row - tokr[rt] * G);
     lim[rt] = rv[rt] ? min(max(ctx0 + tokr[rt], pre - 1), lk - 1) : -1;
-    if (MOD) slope[rt] = mod.bias && rv[rt] ? a.sc.slopes[headr[rt]] * kLog2e : 0.f;
+    // a bias without a cap starts the accumulators, in units of raw products
+    if (SC == kBias || SC == kCapBias)
+      slope[rt] = rv[rt] ? a.sc.slopes[headr[rt]] * (SC == kBias ? kLog2e / a.scale_log2 : kLog2e) : 0.f;
     if (rv[rt]) { wlim_lo = min(wlim_lo, lim[rt]); wlim_hi = max(wlim_hi, lim[rt]); }
   }
 #pragma unroll
@@ -965,6 +976,9 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
     const uint16_t* vt = B ? v1 : v0;
     constexpr int kSt = kPfKeys / 16;      // 16-key sub-tiles
     float4_t acc[kPfRt][kSt];
+    float far[kPfRt];                      // the rows' distances from the lane's first key
+#pragma unroll
+    for (int rt = 0; rt < kPfRt; ++rt) far[rt] = (float)(ctx0 + tokr[rt] - kbase - 4 * g);
     __builtin_amdgcn_sched_barrier(0);     // the block below is scheduled on its own
 #pragma unroll
     for (int st = 0; st < kSt; ++st) {
@@ -976,6 +990,11 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
       for (int rt = 0; rt < kPfRt; ++rt) {
         // (a row tile with no valid row computes rows that are never written)
         acc[rt][st] = float4_t{0.f, 0.f, 0.f, 0.f};
+        if (SC == kBias) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            acc[rt][st][v] = -slope[rt] * __builtin_fabsf(far[rt] - (float)(16 * st + v));
+        }
 #pragma unroll
         for (int j = 0; j < KJ; ++j) acc[rt][st] = qk_step(kf[j], qf[rt][j], acc[rt][st]);
       }
@@ -993,13 +1012,12 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
     for (int rt = 0; rt < kPfRt; ++rt) {
       float sv[kSt][4];
       float tmax = -INFINITY;
-      if (MOD) {
-        const float far = (float)(ctx0 + tokr[rt] - kbase - 4 * g);
+      if (SC == kCap || SC == kCapBias) {
 #pragma unroll
         for (int st = 0; st < kSt; ++st)
 #pragma unroll
           for (int v = 0; v < 4; ++v)
-            acc[rt][st][v] = mod(acc[rt][st][v], far - (float)(16 * st + v), slope[rt]);
+            acc[rt][st][v] = mod(acc[rt][st][v], far[rt] - (float)(16 * st + v), slope[rt]);
       }
       if (MASK) {     // causal diagonal / sequence end: per-key limits
         const int rel = lim[rt] - kbase - 4 * g;
@@ -1022,7 +1040,7 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
       // exceeds it by more than kLazyLog2, so P stays below 2^kLazyLog2 and O
       // and l (which share m) need no rescale on most tiles.  m = -inf until
       // a row sees a key; exp2(-inf) = 0 then.
-      const float sl = MOD ? 1.f : a.scale_log2;
+      const float sl = SC == kCap || SC == kCapBias ? 1.f : a.scale_log2;
       const float tm = tmax * sl;
       const bool grow = __any(tm > m[rt] + kLazyLog2);
       const float mnew = grow ? fmaxf(m[rt], tm) : m[rt];
@@ -1189,14 +1207,14 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
   }
 }
 
-template <bool ONE_BLOCK, bool FUSED, int D, int KV, bool MOD>
+template <bool ONE_BLOCK, bool FUSED, int D, int KV, int SC>
 __global__ __launch_bounds__(kPfWaves * 64) __attribute__((amdgpu_waves_per_eu(AIA_PF_WPE, AIA_PF_WPE)))
 void gqa_prefill_kernel(PrefillArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t k0[kPfKeys * D];
   __shared__ __attribute__((aligned(16))) uint16_t k1[kPfKeys * D];
   __shared__ __attribute__((aligned(16))) uint16_t v0[kPfKeys * D];
   __shared__ __attribute__((aligned(16))) uint16_t v1[kPfKeys * D];
-  gqa_prefill_body<ONE_BLOCK, FUSED, D, KV, MOD>(a, blockIdx.x, k0, k1, v0, v1);
+  gqa_prefill_body<ONE_BLOCK, FUSED, D, KV, SC>(a, blockIdx.x, k0, k1, v0, v1);
 }
 
 // Mixed steps (prefill items beside split-K decode ranges) in one grid, for
@@ -1210,7 +1228,7 @@ void gqa_prefill_kernel(PrefillArgs a) {
 // caches, whose steps are two tiles, in both).
 constexpr int kMixedK0 = kPfWaves * kTile * kVStride > kPfKeys * kKStride
                              ? kPfWaves * kTile * kVStride : kPfKeys * kKStride;
-template <bool ONE_BLOCK, bool FUSED, int KV, bool MOD>
+template <bool ONE_BLOCK, bool FUSED, int KV, int SC>
 __global__ __launch_bounds__(kPfWaves * 64) __attribute__((amdgpu_waves_per_eu(AIA_PF_WPE, AIA_PF_WPE)))
 void gqa_mixed_kernel(AttnArgs a, PrefillArgs pa, int npf) {
   __shared__ __attribute__((aligned(16))) uint16_t k0[kMixedK0];
@@ -1226,62 +1244,85 @@ void gqa_mixed_kernel(AttnArgs a, PrefillArgs pa, int npf) {
   const bool prefill = b < npf;
   const int idx = prefill ? b : b - npf;
   if (prefill)
-    gqa_prefill_body<ONE_BLOCK, FUSED, kHeadDim, KV, MOD>(pa, idx, k0, k1, v0, v1);
+    gqa_prefill_body<ONE_BLOCK, FUSED, kHeadDim, KV, SC>(pa, idx, k0, k1, v0, v1);
   else
-    gqa_attn_body<kPfWaves, 1, kHeadDim, KV, MOD>(a, idx,
+    gqa_attn_body<kPfWaves, 1, kHeadDim, KV, SC == kPlain ? kPlain : kAnyScore>(a, idx,
                                          reinterpret_cast<uint16_t(*)[kTile * kVStride]>(&k0[0]),
                                          reinterpret_cast<uint16_t(*)[kTile * kVStride]>(&k1[0]));
 }
 
-// The attention launches of one call, for one cache format.  MOD: modified
-// scores.  (8-bit caches have no fused write: pa.kn is null.)
-template <int KV, bool MOD>
-int launch_gqa(const AttnArgs& a, const PrefillArgs& pa, const Layout& L, const Geometry& g,
-               int32_t head_dim, int32_t waves, bool one_block, hipStream_t s) {
-  using aia::check_hip;
+// The attention launches of one call, for one cache format.  SC: the prefill
+// units' scores; the split-K ranges take any.  (8-bit caches have no fused
+// write: pa.kn is null.)
+template <int KV, int SC>
+int launch_prefill(const PrefillArgs& pa, const Layout& L, const Geometry& g, int32_t head_dim,
+                   bool one_block, hipStream_t s) {
   constexpr bool FUSE = KV != aia::kKvFp8;
   const bool fused = FUSE && pa.kn;
+  const dim3 grid((unsigned)(L.pf_unit_cap * g.hkv));
+#define AIA_PF_LAUNCH(D)                                                                             \
+  (one_block && fused ? gqa_prefill_kernel<true, FUSE, D, KV, SC><<<grid, kPfWaves * 64, 0, s>>>(pa)    \
+   : one_block        ? gqa_prefill_kernel<true, false, D, KV, SC><<<grid, kPfWaves * 64, 0, s>>>(pa)   \
+   : fused            ? gqa_prefill_kernel<false, FUSE, D, KV, SC><<<grid, kPfWaves * 64, 0, s>>>(pa)   \
+                      : gqa_prefill_kernel<false, false, D, KV, SC><<<grid, kPfWaves * 64, 0, s>>>(pa))
+  if (head_dim == 64) AIA_PF_LAUNCH(64);
+  else AIA_PF_LAUNCH(kHeadDim);
+#undef AIA_PF_LAUNCH
+  return aia::check_hip(hipGetLastError(), "gqa_prefill_kernel launch");
+}
+
+template <int KV, int SC>
+int launch_mixed(const AttnArgs& a, const PrefillArgs& pa, const Layout& L, const Geometry& g,
+                 int32_t waves, bool one_block, hipStream_t s) {
+  constexpr bool FUSE = KV != aia::kKvFp8;
+  const bool fused = FUSE && pa.kn;
+  const int npf = (int)(L.pf_unit_cap * g.hkv);
+  const dim3 grid((unsigned)(npf + waves));
+  if (one_block && fused) gqa_mixed_kernel<true, FUSE, KV, SC><<<grid, kPfWaves * 64, 0, s>>>(a, pa, npf);
+  else if (one_block) gqa_mixed_kernel<true, false, KV, SC><<<grid, kPfWaves * 64, 0, s>>>(a, pa, npf);
+  else if (fused) gqa_mixed_kernel<false, FUSE, KV, SC><<<grid, kPfWaves * 64, 0, s>>>(a, pa, npf);
+  else gqa_mixed_kernel<false, false, KV, SC><<<grid, kPfWaves * 64, 0, s>>>(a, pa, npf);
+  return aia::check_hip(hipGetLastError(), "gqa_mixed_kernel launch");
+}
+
+template <int KV, bool SCORED>
+int launch_gqa(const AttnArgs& a, const PrefillArgs& pa, const Layout& L, const Geometry& g,
+               int32_t head_dim, int32_t waves, bool one_block, hipStream_t s) {
+  constexpr int DEC = SCORED ? kAnyScore : kPlain;
+  const bool cap = a.sc.cap_out > 0.f, bias = a.sc.slopes != nullptr;
   if (mixed_grid(g, head_dim)) {
-    const int npf = (int)(L.pf_unit_cap * g.hkv);
-    const dim3 grid((unsigned)(npf + waves));
-    if (one_block && fused) gqa_mixed_kernel<true, FUSE, KV, MOD><<<grid, kPfWaves * 64, 0, s>>>(a, pa, npf);
-    else if (one_block) gqa_mixed_kernel<true, false, KV, MOD><<<grid, kPfWaves * 64, 0, s>>>(a, pa, npf);
-    else if (fused) gqa_mixed_kernel<false, FUSE, KV, MOD><<<grid, kPfWaves * 64, 0, s>>>(a, pa, npf);
-    else gqa_mixed_kernel<false, false, KV, MOD><<<grid, kPfWaves * 64, 0, s>>>(a, pa, npf);
-    if (int rc = check_hip(hipGetLastError(), "gqa_mixed_kernel launch")) return rc;
-  } else {
+    if constexpr (!SCORED) return launch_mixed<KV, kPlain>(a, pa, L, g, waves, one_block, s);
+    else
+      return cap && bias ? launch_mixed<KV, kCapBias>(a, pa, L, g, waves, one_block, s)
+             : cap       ? launch_mixed<KV, kCap>(a, pa, L, g, waves, one_block, s)
+             : bias      ? launch_mixed<KV, kBias>(a, pa, L, g, waves, one_block, s)
+                         : launch_mixed<KV, kPrefixOnly>(a, pa, L, g, waves, one_block, s);
+  }
 #define AIA_GQA_LAUNCH_D(NW, D)                                                         \
-  (g.rb == 2 ? gqa_attn_kernel<NW, 2, D, KV, MOD><<<waves, 64 * NW, 0, s>>>(a)             \
-             : gqa_attn_kernel<NW, 1, D, KV, MOD><<<waves, 64 * NW, 0, s>>>(a))
+  (g.rb == 2 ? gqa_attn_kernel<NW, 2, D, KV, DEC><<<waves, 64 * NW, 0, s>>>(a)             \
+             : gqa_attn_kernel<NW, 1, D, KV, DEC><<<waves, 64 * NW, 0, s>>>(a))
 #define AIA_GQA_LAUNCH(NW)                                                        \
   (head_dim == 64 ? AIA_GQA_LAUNCH_D(NW, 64) : AIA_GQA_LAUNCH_D(NW, kHeadDim))
-    switch (g.nw) {
-      case 1: AIA_GQA_LAUNCH(1); break;
-      case 2: AIA_GQA_LAUNCH(2); break;
-      case 3: AIA_GQA_LAUNCH(3); break;
-      case 4: AIA_GQA_LAUNCH(4); break;
-      case 5: AIA_GQA_LAUNCH(5); break;
-      case 6: AIA_GQA_LAUNCH(6); break;
-      case 7: AIA_GQA_LAUNCH(7); break;
-      default: AIA_GQA_LAUNCH(8); break;
-    }
+  switch (g.nw) {
+    case 1: AIA_GQA_LAUNCH(1); break;
+    case 2: AIA_GQA_LAUNCH(2); break;
+    case 3: AIA_GQA_LAUNCH(3); break;
+    case 4: AIA_GQA_LAUNCH(4); break;
+    case 5: AIA_GQA_LAUNCH(5); break;
+    case 6: AIA_GQA_LAUNCH(6); break;
+    case 7: AIA_GQA_LAUNCH(7); break;
+    default: AIA_GQA_LAUNCH(8); break;
+  }
 #undef AIA_GQA_LAUNCH
 #undef AIA_GQA_LAUNCH_D
-    if (int rc = check_hip(hipGetLastError(), "gqa_attn_kernel launch")) return rc;
-    if (L.pf_cap > 0) {
-      const dim3 grid((unsigned)(L.pf_unit_cap * g.hkv));
-#define AIA_PF_LAUNCH(D)                                                                             \
-  (one_block && fused ? gqa_prefill_kernel<true, FUSE, D, KV, MOD><<<grid, kPfWaves * 64, 0, s>>>(pa)   \
-   : one_block        ? gqa_prefill_kernel<true, false, D, KV, MOD><<<grid, kPfWaves * 64, 0, s>>>(pa)  \
-   : fused            ? gqa_prefill_kernel<false, FUSE, D, KV, MOD><<<grid, kPfWaves * 64, 0, s>>>(pa)  \
-                      : gqa_prefill_kernel<false, false, D, KV, MOD><<<grid, kPfWaves * 64, 0, s>>>(pa))
-      if (head_dim == 64) AIA_PF_LAUNCH(64);
-      else AIA_PF_LAUNCH(kHeadDim);
-#undef AIA_PF_LAUNCH
-      if (int rc = check_hip(hipGetLastError(), "gqa_prefill_kernel launch")) return rc;
-    }
-  }
-  return AIA_OK;
+  if (int rc = aia::check_hip(hipGetLastError(), "gqa_attn_kernel launch")) return rc;
+  if (L.pf_cap <= 0) return AIA_OK;
+  if constexpr (!SCORED) return launch_prefill<KV, kPlain>(pa, L, g, head_dim, one_block, s);
+  else
+    return cap && bias ? launch_prefill<KV, kCapBias>(pa, L, g, head_dim, one_block, s)
+           : cap       ? launch_prefill<KV, kCap>(pa, L, g, head_dim, one_block, s)
+           : bias      ? launch_prefill<KV, kBias>(pa, L, g, head_dim, one_block, s)
+                       : launch_prefill<KV, kPrefixOnly>(pa, L, g, head_dim, one_block, s);
 }
 
 }  // namespace

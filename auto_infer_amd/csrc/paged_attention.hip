@@ -2699,12 +2699,10 @@ static int attention_gqa(
   const bool one_block = block_size % kPfKeys == 0;
   const bool scored = ex.softcap > 0.f || ex.alibi_slopes || ex.prefix_lens;
   const bool nz = flags & AIA_ATTN_KV_NZ;
-  const int rc =
-      fp8      ? launch_gqa_fp8(scored, a, pa, L, g, head_dim, waves, one_block, s)
-      : scored ? launch_gqa_scored(nz ? kKvNz : kKvNd, a, pa, L, g, head_dim, waves, one_block, s)
-      : nz     ? launch_gqa<kKvNz, false>(a, pa, L, g, head_dim, waves, one_block, s)
-               : launch_gqa<kKvNd, false>(a, pa, L, g, head_dim, waves, one_block, s);
-  if (rc)
+  LaunchGqa* const launch = fp8      ? (scored ? launch_gqa_fp8_scored : launch_gqa_fp8)
+                            : scored ? (nz ? launch_gqa_scored_nz : launch_gqa_scored_nd)
+                                     : (nz ? launch_gqa<kKvNz, false> : launch_gqa<kKvNd, false>);
+  if (const int rc = launch(a, pa, L, g, head_dim, waves, one_block, s))
     return rc;
   return launch_merge(ws, L, g, g.nw, head_dim, batch, num_tokens, waves, (int64_t)block_table_stride * block_size, a.part_o, a.part_ml, a.seg, a.out, a.o_ts, a.o_hs,
                       s);
