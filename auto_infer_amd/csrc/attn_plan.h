@@ -31,6 +31,8 @@ struct ScoreArgs {
   const int32_t* prefix;     // keys of each request that all its rows see, or null
   const int32_t* kvlen;
   float cap_in, cap_out;     // cap_out 0: no cap
+  float cap_small;           // |q.k| up to which cap_poly serves
+  float cap_poly[5];
 };
 
 struct AttnArgs {

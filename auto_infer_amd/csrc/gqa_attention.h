@@ -180,6 +180,17 @@ struct ScoreMod {
 };
 constexpr float kLog2e = 1.4426950408889634f;
 
+// A capped score of at most three quarters of the cap: x times a polynomial in
+// x^2 whose coefficients hold the call's factors (see the host side), within
+// 2^-22 of the cap.
+__device__ __forceinline__ float capped_small(float x, const float (&c)[5]) {
+  const float u = x * x;
+  float y = __builtin_fmaf(u, c[4], c[3]);
+  y = __builtin_fmaf(u, y, c[2]);
+  y = __builtin_fmaf(u, y, c[1]);
+  return x * __builtin_fmaf(u, y, c[0]);
+}
+
 // Keys of request b that all its rows see.
 __device__ __forceinline__ int prefix_keys(const ScoreArgs& s, int b) {
   return s.prefix ? max(0, min(s.prefix[b], s.kvlen[b])) : 0;
@@ -1013,11 +1024,27 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
       float sv[kSt][4];
       float tmax = -INFINITY;
       if (SC == kCap || SC == kCapBias) {
+        // The VALU is what these units wait for, and the cap's exponential and
+        // reciprocal are a quarter as fast as other instructions: tiles whose
+        // scores all stay below three quarters of the cap take a polynomial
+        // (six multiply-adds) instead.
+        float big = 0.f;
 #pragma unroll
         for (int st = 0; st < kSt; ++st)
 #pragma unroll
-          for (int v = 0; v < 4; ++v)
-            acc[rt][st][v] = mod(acc[rt][st][v], far[rt] - (float)(16 * st + v), slope[rt]);
+          for (int v = 0; v < 4; ++v) big = fmaxf(big, __builtin_fabsf(acc[rt][st][v]));
+        auto each = [&](auto f) {
+#pragma unroll
+          for (int st = 0; st < kSt; ++st)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              const float y = f(acc[rt][st][v]);
+              acc[rt][st][v] = SC == kCapBias
+                  ? __builtin_fmaf(-slope[rt], __builtin_fabsf(far[rt] - (float)(16 * st + v)), y) : y;
+            }
+        };
+        if (__any(big > a.sc.cap_small)) each([&](float x) { return mod.capped(x); });
+        else each([&](float x) { return capped_small(x, a.sc.cap_poly); });
       }
       if (MASK) {     // causal diagonal / sequence end: per-key limits
         const int rel = lim[rt] - kbase - 4 * g;

@@ -2650,7 +2650,7 @@ static int attention_gqa(
     return fail(AIA_ERR_CAPACITY, "%s: workspace %lld bytes < %lld needed", fn,
                 (long long)workspace_bytes, (long long)L.total);
   char* ws = static_cast<char*>(workspace);
-  AttnArgs a;
+  AttnArgs a = {};
   a.q = static_cast<const uint16_t*>(query);
   a.q_ts = q_token_stride; a.q_hs = q_head_stride;
   a.kc = static_cast<uint16_t*>(const_cast<void*>(key_cache));
@@ -2678,6 +2678,16 @@ static int attention_gqa(
   a.sc.kvlen = seqlens_kv;
   a.sc.cap_in = ex.softcap > 0.f ? 2.f * a.scale_log2 / ex.softcap : 0.f;
   a.sc.cap_out = ex.softcap * 1.4426950408889634f;
+  if (ex.softcap > 0.f) {
+    // tanh(z) = z (c0 + c1 z^2 + ...) for |z| <= 3/4, z = q.k * scale / cap: the
+    // least largest error of five terms, 2^-22.4 (fitted on Chebyshev nodes)
+    const double c[5] = {0.9999972283263151, -0.33323076500793086, 0.13226091761972558,
+                         -0.049280451090587346, 0.0123188353892593};
+    const double z = (double)scale / ex.softcap;
+    double f = (double)ex.softcap * 1.4426950408889634 * z;
+    for (int i = 0; i < 5; ++i, f *= z * z) a.sc.cap_poly[i] = (float)(c[i] * f);
+    a.sc.cap_small = (float)(0.75 / z);
+  }
   hipStream_t s = (hipStream_t)stream;
   PrefillArgs pa = {};
   if (L.pf_cap > 0) {
