@@ -82,7 +82,7 @@ constexpr int kPipe = AIA_PIPE;
 
 // End of a segment's range: bf16 output where the range covers all of its
 // keys, else an fp16 partial.
-template <int RB, int D>
+template <int RB, int D, bool SCORED>
 __device__ __forceinline__ void write_segment(const AttnArgs& a, float4_t (&o)[RB][D / 16], float (&m)[RB],
                                               float (&lsum)[RB], const bool (&rv)[RB],
                                               const int (&qi)[RB], int n, int g, int qtok0, int head,
@@ -124,7 +124,8 @@ __device__ __forceinline__ void write_segment(const AttnArgs& a, float4_t (&o)[R
         for (int i = 0; i < 4; ++i) cmax = fmaxf(cmax, fabsf(o[r][dt][i]));
       cmax = aia::group4_max(cmax);
       if (!rv[r]) continue;
-      const float c = cmax > 0.f ? cmax : 1.f;
+      // (an infinite output stays one: its row keeps its values)
+      const float c = cmax > 0.f && !(SCORED && cmax == INFINITY) ? cmax : 1.f;
       const float inv = 1.f / c;
       const int64_t prow = ((int64_t)part * a.nw + wid) * seg_rows + r * kRows + n;
       uint16_t* pp = a.part_o + prow * D;
@@ -189,6 +190,43 @@ __device__ __forceinline__ float capped_small(float x, const float (&c)[5]) {
   y = __builtin_fmaf(u, y, c[2]);
   y = __builtin_fmaf(u, y, c[1]);
   return x * __builtin_fmaf(u, y, c[0]);
+}
+
+// Non-finite values.  P is zero where a row does not see a key, but 0 x V is not
+// where V is an infinity or NaN, so the matrix product of a masked tile would
+// carry them into every row of the tile.  The kernels for modified scores and
+// 8-bit caches look through V in masked tiles (the diagonal and the sequence's
+// end) and multiply those that hold such a value key by key, leaving out what
+// a row does not see.
+__device__ __forceinline__ uint32_t not_finite_bf16(uint32_t w, uint32_t acc) {   // bits 15 and 31
+  return ((w & 0x7fff7fffu) + 0x00800080u) | acc;
+}
+__device__ __forceinline__ uint32_t not_finite_bf16(uint4 w, uint32_t acc) {
+  return not_finite_bf16(w.x, not_finite_bf16(w.y, not_finite_bf16(w.z, not_finite_bf16(w.w, acc))));
+}
+__device__ __forceinline__ uint32_t nan_fp8(uint4 w, uint32_t acc) {              // bits 7, 15, ...
+  const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc |= (x[i] & 0x7f7f7f7fu) + 0x01010101u;
+  return acc;
+}
+// Row n's weight of key k, from packed weights: the word of k's pair, held by the
+// lane of group (k % 16) / 4 with row n.
+__device__ __forceinline__ float weight_of(uint32_t word, int n, int k) {
+  const uint32_t w = __shfl(word, n + 16 * ((k & 15) >> 2));
+  return k & 1 ? aia::bf16_hi(w) : aia::bf16_lo(w);
+}
+// o += p * (this lane's 4 dims of each 16 of a V row)
+template <int DT, class At>
+__device__ __forceinline__ void add_key(float4_t (&o)[DT], float p, At at) {
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    const uint2 w = *reinterpret_cast<const uint2*>(at(dt));
+    o[dt][0] = __builtin_fmaf(p, aia::bf16_lo(w.x), o[dt][0]);
+    o[dt][1] = __builtin_fmaf(p, aia::bf16_hi(w.x), o[dt][1]);
+    o[dt][2] = __builtin_fmaf(p, aia::bf16_lo(w.y), o[dt][2]);
+    o[dt][3] = __builtin_fmaf(p, aia::bf16_hi(w.y), o[dt][3]);
+  }
 }
 
 // Keys of request b that all its rows see.
@@ -366,6 +404,24 @@ __device__ __forceinline__ void gqa_segment(const AttnArgs& a, const int* rec, i
       pb[r] = as_s4(aia::pack_bf16x2(p[0], p[1]), aia::pack_bf16x2(p[2], p[3]));
     }
     __builtin_amdgcn_wave_barrier();
+    if (SC != kPlain && masked) {
+      uint32_t odd = 0;
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) odd = not_finite_bf16(vv[j], odd);
+      if (__any(odd & 0x80008000u)) {
+        for (int k = 0; k < kTile; ++k) {
+#pragma unroll
+          for (int r = 0; r < RB; ++r) {
+            const uint2 w = __builtin_bit_cast(uint2, pb[r]);
+            const float p = weight_of(k & 2 ? w.y : w.x, n, k);
+            if (lt * kTile + k <= lim[r])
+              add_key(o[r], p, [&](int dt) { return vt + k * kVStride + 16 * dt + 4 * g; });
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+        return;
+      }
+    }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const short4_t va = vt_frag(vt, n, g, dt);
@@ -405,7 +461,7 @@ __device__ __forceinline__ void gqa_segment(const AttnArgs& a, const int* rec, i
     w0 = w1;
   }
 
-  write_segment<RB, D>(a, o, m, lsum, rv, qi, n, g, qtok0, head, wid, w, tpw, tile_begin, tile_end, part_base);
+  write_segment<RB, D, SC != kPlain>(a, o, m, lsum, rv, qi, n, g, qtok0, head, wid, w, tpw, tile_begin, tile_end, part_base);
 }
 
 // ---- 8-bit caches
@@ -587,6 +643,26 @@ __device__ __forceinline__ void gqa_segment_fp8(const AttnArgs& a, const int* re
                          aia::pack_bf16x2(p[1][0], p[1][1]), aia::pack_bf16x2(p[1][2], p[1][3]));
     }
     __builtin_amdgcn_wave_barrier();
+    if (masked) {
+      uint32_t odd = 0;
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int j = 0; j < CH; ++j) odd = nan_fp8(vv[st][j], odd);
+      if (__any(odd & 0x80808080u)) {
+        for (int k = 0; k < 2 * kTile; ++k) {
+          const uint16_t* vs = (k < kTile ? vt0 : vt1) + (k & 15) * kVStride + 4 * g;
+#pragma unroll
+          for (int r = 0; r < RB; ++r) {
+            const uint32_t lo = k < kTile ? pb[r].x : pb[r].z, hi = k < kTile ? pb[r].y : pb[r].w;
+            const float p = weight_of(k & 2 ? hi : lo, n, k);
+            if (lt * kTile + k <= min(lim[r], past - 1)) add_key(o[r], p, [&](int dt) { return vs + 16 * dt; });
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+        return;
+      }
+    }
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) {
       const bf16x8_t va = __builtin_bit_cast(
@@ -624,7 +700,7 @@ __device__ __forceinline__ void gqa_segment_fp8(const AttnArgs& a, const int* re
     }
     w0 = w1;
   }
-  write_segment<RB, D>(a, o, m, lsum, rv, qi, n, g, qtok0, head, wid, w, tpw, tile_begin, tile_end, part_base);
+  write_segment<RB, D, false>(a, o, m, lsum, rv, qi, n, g, qtok0, head, wid, w, tpw, tile_begin, tile_end, part_base);
 }
 
 // One work-group per key range, one wave per kv head of the segment's group.
@@ -737,7 +813,7 @@ constexpr float kLazyLog2 = AIA_PF_LAZY;              // max growth (log2) befor
 template <bool ONE_BLOCK, bool FUSED, int D, int KV, int SC>
 __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
                                                  uint16_t* k0, uint16_t* k1,
-                                                 uint16_t* v0, uint16_t* v1) {
+                                                 uint16_t* v0, uint16_t* v1, int* odd_tile) {
   constexpr int KJ = D / 32;        // 32-dim MFMA k-steps
   constexpr int DT = D / 16;        // 16-dim output tiles
   constexpr int RC = D / 8;         // 16-byte chunks per K / V row
@@ -974,7 +1050,11 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
   // the load addresses and issue overlap the MFMAs' execution: 0-1% faster
   // than issuing them first.  (A raised wave priority around each MFMA block,
   // 3% faster with register-staged loads, made this order 1-2% slower, and
-  // either order is as fast without it, so no priority is set.)
+  // either order is as fast without it, so no priority is set: but for modified
+  // scores and 8-bit caches, whose waves spend longer between the blocks.
+  // 8-bit, 512 tokens behind 32K, 28/4 heads: 281.9 -> 274.8 us, with a cap 360
+  // -> 354.5; prefix and cap, 3 prompts of 600 to 2000: 106.4 -> 104.7.)
+  constexpr bool PRIO = F8 || SC != kPlain, CARE = PRIO;
   auto compute = [&](int t, auto buf_tag, auto mask_tag, auto issue_next) {
     constexpr bool MASK = decltype(mask_tag)::value;
     constexpr int B = decltype(buf_tag)::value;
@@ -990,6 +1070,7 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
     float far[kPfRt];                      // the rows' distances from the lane's first key
 #pragma unroll
     for (int rt = 0; rt < kPfRt; ++rt) far[rt] = (float)(ctx0 + tokr[rt] - kbase - 4 * g);
+    if (PRIO) __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);     // the block below is scheduled on its own
 #pragma unroll
     for (int st = 0; st < kSt; ++st) {
@@ -1017,6 +1098,7 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
       if (st + kPfQkAhead < kSt) __builtin_amdgcn_sched_group_barrier(kSgDsRead, KJ, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
+    if (PRIO) __builtin_amdgcn_s_setprio(0);
     issue_next();
     uint4 pb[kPfRt][kSt / 2];
 #pragma unroll
@@ -1099,6 +1181,27 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
       }
     }
     __builtin_amdgcn_sched_barrier(0);     // the block below is scheduled on its own
+    if (CARE && MASK && *reinterpret_cast<volatile int*>(odd_tile + B) == t) {
+      for (int k = 0; k < kPfKeys; ++k) {
+        const uint16_t* vs = vt + k * D + 4 * (g & 1);
+        const int sw = 2 * (k & (RC / 2 - 1));
+#pragma unroll
+        for (int rt = 0; rt < kPfRt; ++rt) {
+          uint32_t word = 0;
+#pragma unroll
+          for (int w = 0; w < kSt * 2; ++w) {       // word w: keys 16 (w / 2) + 4 g + 2 (w % 2), + 1
+            const uint4 q = pb[rt][w >> 2];
+            const uint32_t x = (w & 3) == 0 ? q.x : (w & 3) == 1 ? q.y : (w & 3) == 2 ? q.z : q.w;
+            word = w == 2 * (k >> 4) + ((k >> 1) & 1) ? x : word;
+          }
+          const float p = weight_of(word, n, k);
+          if (kbase + k <= lim[rt])
+            add_key(o[rt], p, [&](int dt) { return vs + 8 * ((2 * dt + (g >> 1)) ^ sw); });
+        }
+      }
+      return;
+    }
+    if (PRIO) __builtin_amdgcn_s_setprio(1);
     // PV over V^T fragments f = (32-key pair pp, 16 dims dt), read kPfPvAhead
     // fragments ahead of their MFMAs.  Lane (n, g) reads keys 4 g + n / 4
     // (+ 16), dims 16 dt + 4 (n % 4), at their swizzled place (the
@@ -1124,6 +1227,32 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
       if (f + kPfPvAhead < kSt / 2 * DT) __builtin_amdgcn_sched_group_barrier(kSgDsRead, 2, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
+    if (PRIO) __builtin_amdgcn_s_setprio(0);
+  };
+
+  // Tiles from t_care on are masked for some of the work-group's rows.  As such a
+  // tile's bytes arrive, each thread looks through the V values that it loaded
+  // and names the tile in odd_tile[its buffer] where one is not finite.
+  const int t_care = max(t0, min(t1, (min(max(ctx0 + row0 / G, pre - 1), lk - 1) + 1) / kPfKeys));
+  auto look = [&](int t, auto buf_tag) {
+    constexpr int B = decltype(buf_tag)::value;
+    if (!CARE || t < t_care || t >= t1) return;
+    bool odd;
+    if constexpr (F8) {
+      uint32_t x = 0;
+#pragma unroll
+      for (int i = 0; i < kLdRounds; ++i) x = nan_fp8(vr[i], x);
+      odd = x & 0x80808080u;
+    } else {
+      asm volatile("" ::: "memory");       // after the wait for this wave's direct loads
+      uint32_t x = 0;
+      const uint16_t* vt = (B ? v1 : v0) + (kWaveKeys * wid) * D + 8 * lane;
+#pragma unroll
+      for (int i = 0; i < kLdRounds; ++i)
+        x = not_finite_bf16(*reinterpret_cast<const uint4*>(vt + kLdKeys * i * D), x);
+      odd = x & 0x80008000u;
+    }
+    if (odd) odd_tile[B] = t;
   };
 
   if (t1 > t0) {
@@ -1136,8 +1265,13 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
     fetch_ids(t0);
     load(t0, buf0{});
     fetch_ids(t0 + 1);
+    if constexpr (CARE) {
+      if (tid < 2) odd_tile[tid] = -1;
+      __syncthreads();
+    }
     if constexpr (F8) store_fp8(buf0{});
     else __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+    look(t0, buf0{});
     __syncthreads();
     // Tiles below the wave's smallest row limit need no mask; the two runs
     // together take every tile, so all waves pass the same barriers.  The
@@ -1163,6 +1297,7 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
       } else {
         __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
       }
+      look(t + 1, other{});
       __syncthreads();
     };
     auto run = [&](int t, int t_end, auto mask_tag) {
@@ -1209,7 +1344,7 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
       continue;
     }
     if (!whole) {
-      const float c = cmax > 0.f ? cmax : 1.f, ic = 1.f / c;
+      const float c = cmax > 0.f && !(SC != kPlain && cmax == INFINITY) ? cmax : 1.f, ic = 1.f / c;
       const int64_t blk = (int64_t)unit * a.hkv + kvh, r = (wid * kPfRt + rt) * kRows + n;
       uint16_t* pp = a.part_o + (2 * blk * kPfRows + r) * D;
 #pragma unroll
@@ -1241,7 +1376,12 @@ void gqa_prefill_kernel(PrefillArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t k1[kPfKeys * D];
   __shared__ __attribute__((aligned(16))) uint16_t v0[kPfKeys * D];
   __shared__ __attribute__((aligned(16))) uint16_t v1[kPfKeys * D];
-  gqa_prefill_body<ONE_BLOCK, FUSED, D, KV, SC>(a, blockIdx.x, k0, k1, v0, v1);
+  if constexpr (KV == aia::kKvFp8 || SC != kPlain) {
+    __shared__ int odd_tile[2];
+    gqa_prefill_body<ONE_BLOCK, FUSED, D, KV, SC>(a, blockIdx.x, k0, k1, v0, v1, odd_tile);
+  } else {
+    gqa_prefill_body<ONE_BLOCK, FUSED, D, KV, SC>(a, blockIdx.x, k0, k1, v0, v1, nullptr);
+  }
 }
 
 // Mixed steps (prefill items beside split-K decode ranges) in one grid, for
@@ -1270,8 +1410,13 @@ void gqa_mixed_kernel(AttnArgs a, PrefillArgs pa, int npf) {
   const int b = blockIdx.x;
   const bool prefill = b < npf;
   const int idx = prefill ? b : b - npf;
+  int* odd = nullptr;
+  if constexpr (KV == aia::kKvFp8 || SC != kPlain) {
+    __shared__ int odd_tile[2];
+    odd = odd_tile;
+  }
   if (prefill)
-    gqa_prefill_body<ONE_BLOCK, FUSED, kHeadDim, KV, SC>(pa, idx, k0, k1, v0, v1);
+    gqa_prefill_body<ONE_BLOCK, FUSED, kHeadDim, KV, SC>(pa, idx, k0, k1, v0, v1, odd);
   else
     gqa_attn_body<kPfWaves, 1, kHeadDim, KV, SC == kPlain ? kPlain : kAnyScore>(a, idx,
                                          reinterpret_cast<uint16_t(*)[kTile * kVStride]>(&k0[0]),

@@ -123,6 +123,63 @@ def test_long_requests_are_split(kv):
     run([300], [4000], 14, 2, 64, 16, kv, seed=5, **MODS["all"])
 
 
+@pytest.mark.parametrize("kv", ["nd", "nz", "fp8"])
+@pytest.mark.parametrize("heads", ["28_4_128", "14_2_64", "16_8_128"])
+@pytest.mark.parametrize("mod", ["cap", "bias", "all"])
+def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(kv, heads, mod):
+    """Infinities and NaN in later tokens' keys and values, and in slots past a
+    request's end: rows that do not see them are as if they were not there."""
+    hq, hkv, d = HEADS[heads]
+    lqs, lks = [4, 150, 1, 90, 3], [37, 150, 64, 517, 1500]
+    bs = 16
+    step = workloads.make_gqa_step(lqs=lqs, lks=lks, num_q_heads=hq, num_kv_heads=hkv, head_dim=d,
+                                   block_size=bs, seed=3, extra_blocks=2)
+    m = MODS[mod]
+    gen = torch.Generator().manual_seed(4)
+    slopes = torch.exp2(-8.0 * torch.rand(hq, generator=gen)) if m.get("bias") else None
+    pre = torch.tensor([0, 20, 10, 0, 0], dtype=torch.int32) if m.get("prefix") else None
+    keys, values = step.k_cache, step.v_cache
+    more = {}
+    if kv == "fp8":
+        (kq, ks), (vq, vs) = quantised(keys, 5), quantised(values, 6)
+        keys, values = kq.float(), vq.float()
+
+    def put(cache, request, position, head, dim, x):
+        cache[step.block_table[request, position // bs], position % bs, head, dim] = x
+    inf = float("nan") if kv == "fp8" else float("inf")
+    put(values, 0, 35, 0, 3, inf), put(values, 0, 36, hkv - 1, 5, float("nan"))
+    put(keys, 0, 36, 0, 7, float("nan"))
+    put(values, 1, 149, 0, 0, float("nan")), put(values, 1, 120, hkv - 1, d - 1, inf)
+    put(values, 1, 70, 0, d // 2, -inf), put(keys, 1, 131, hkv - 1, 1, inf)
+    put(values, 3, 500, 0, 9, inf), put(values, 3, 516, hkv - 1, 9, float("nan"))
+    put(values, 4, 1498, 0, 9, inf)
+    for r, lk in enumerate(lks):               # slots past the end
+        for p in range(lk, -(-lk // bs) * bs):
+            put(values, r, p, slice(None), slice(None), float("nan"))
+            put(keys, r, p, slice(None), slice(None), float("nan"))
+    if kv == "fp8":
+        kq, vq = keys.to(torch.float8_e4m3fn), values.to(torch.float8_e4m3fn)
+        keys, values = oracle.dequantised(kq, ks), oracle.dequantised(vq, vs)
+        dk, dv = kq.to(DEV), vq.to(DEV)
+        more = dict(key_scale=ks.to(DEV), value_scale=vs.to(DEV))
+    elif kv == "nz":
+        dk, dv, more = nz_from_nd(keys).to(DEV), nz_from_nd(values).to(DEV), dict(kv_layout="nz")
+    else:
+        dk, dv = keys.to(DEV), values.to(DEV)
+    plan = ops.AttentionPlan.from_lists(step.block_table.to(DEV), step.cu_seqlens_q, step.seqlens_kv, hq,
+                                        hkv, d, bs, prefix_lens=None if pre is None else pre.to(DEV))
+    out = ops.paged_attention_gqa(step.q.to(DEV), dk, dv, plan, step.scale, softcap=m.get("cap", 0.0),
+                                  alibi_slopes=None if slopes is None else slopes.to(DEV), **more)
+    ref, bound = oracle.scored_attention(step.q, keys, values, step.block_table, step.cu_seqlens_q,
+                                         step.seqlens_kv, step.scale, m.get("cap", 0.0), slopes,
+                                         None if pre is None else pre.tolist())
+    got = out.cpu().double()
+    fine = torch.isfinite(ref)
+    assert torch.equal(torch.isfinite(got), fine)
+    assert 0.3 < fine.double().mean() < 1
+    assert bool(((got - ref).abs() <= bound)[fine].all())
+
+
 def test_capped_scores_far_past_the_cap():
     """Scores of +-1000 at a cap of 2: weights within e^4 of each other."""
     hq, hkv, d, bs = 4, 2, 64, 16
