@@ -14,6 +14,13 @@ graph-mode backend (``GraphGqaBackend``, gqa.py:134-226): per layer a (k, v)
 pair of (num_blocks, block_size, n_kv, head_dim) tensors whose memory is the
 16-wide fractal NZ layout (viewed (num_blocks, n_kv * head_dim / 16,
 block_size, 16) by npu_scatter_pa_kv_cache and FIA-v2, gqa.py:202-226).
+
+Beyond the reference: ``kv_dtype="fp8"`` keeps the caches as e4m3 values with a
+power-of-two scale per block and head, ``softcap`` / ``alibi_slopes`` modify the
+scores, ``rope`` (an ``ops.RotaryEmbedding``) turns Q and K from
+``ctx.positions`` instead of ``ctx.cos`` / ``ctx.sin``, and a context with
+``aia_prefix_lens`` (device int32, one per request) lets all rows of a request
+see its first keys.
 """
 import torch
 
@@ -28,7 +35,8 @@ class GqaHipBackend(AttentionBackend):
     def __init__(self, n_q_heads: int, n_kv_heads: int, head_dim: int, scale: float,
                  num_layers: int, device, dtype, w: dict = None, layer_prefix=None,
                  rms_eps=None, fuse_kv_write: bool = True, fuse_pre_attention: bool = True,
-                 kv_layout: str = "nd"):
+                 kv_layout: str = "nd", kv_dtype: str = "bf16", softcap: float = 0.0,
+                 alibi_slopes=None, rope=None):
         self.n_q_heads = n_q_heads
         self.n_kv_heads = n_kv_heads
         self.head_dim = head_dim
@@ -55,9 +63,25 @@ class GqaHipBackend(AttentionBackend):
         if kv_layout not in ops.KV_LAYOUTS:
             raise ValueError(f"kv_layout must be one of {sorted(ops.KV_LAYOUTS)}")
         self.kv_layout = kv_layout
+        if kv_dtype not in ("bf16", "fp8"):
+            raise ValueError(f"kv_dtype must be bf16 or fp8, got {kv_dtype!r}")
+        self.fp8 = kv_dtype == "fp8"
+        if self.fp8 and kv_layout != "nd":
+            raise NotImplementedError("8-bit caches have no NZ layout")
+        self.scores = dict(softcap=softcap, alibi_slopes=alibi_slopes)
+        self.rope = rope
         self._pending = None
 
     def alloc_kv_caches(self, num_blocks: int, block_size: int) -> list:
+        if self.fp8:      # per layer (k, v, k scales, v scales)
+            shape = (num_blocks, block_size, self.n_kv_heads, self.head_dim)
+
+            def zeros(shape, dtype):      # byte 0: value 0, the smallest scale
+                return torch.zeros(shape, device=self.device, dtype=torch.uint8).view(dtype)
+            return [(zeros(shape, ops.FP8_KV), zeros(shape, ops.FP8_KV),
+                     zeros((num_blocks, self.n_kv_heads), ops.FP8_KV_SCALE),
+                     zeros((num_blocks, self.n_kv_heads), ops.FP8_KV_SCALE))
+                    for _ in range(self.num_layers)]
         if self.kv_layout == "nz":      # GraphGqaBackend.alloc_kv_caches (gqa.py:195-204)
             shape = (num_blocks, block_size, self.n_kv_heads, self.head_dim)
             return [(torch.zeros(shape, device=self.device, dtype=self.dtype),
@@ -67,11 +91,13 @@ class GqaHipBackend(AttentionBackend):
         return [torch.zeros(shape, device=self.device, dtype=self.dtype)
                 for _ in range(self.num_layers)]
 
-    def _write(self, k, v, kc, vc, slot_mapping):
-        if self.kv_layout == "nz":
-            ops.write_kv_nz(k, v, kc, vc, slot_mapping)
+    def _write(self, k, v, cache, slot_mapping):
+        if self.fp8:
+            ops.write_kv_fp8(k, v, *cache, slot_mapping)
+        elif self.kv_layout == "nz":
+            ops.write_kv_nz(k, v, cache[0], cache[1], slot_mapping)
         else:
-            ops.write_kv(k, v, kc, vc, slot_mapping)
+            ops.write_kv(k, v, cache[0], cache[1], slot_mapping)
 
     def attention(self, layer_idx: int, x: torch.Tensor, ctx) -> torch.Tensor:
         T = x.shape[0]
@@ -80,7 +106,11 @@ class GqaHipBackend(AttentionBackend):
         p = self.layer_prefix(layer_idx) + "self_attn."
         qkv = lin(x, w[p + "qkv_proj.weight"], w.get(p + "qkv_proj.bias"))
         qn = w.get(p + "q_norm.weight")
-        if self._fusable(qkv, ctx):
+        if self.rope is not None:
+            q, k, v = ops.rope_qk(qkv, n_q, n_kv, ctx.positions, self.rope, qn,
+                                  w.get(p + "k_norm.weight") if qn is not None else None,
+                                  self.rms_eps if self.rms_eps is not None else 1e-6)
+        elif self._fusable(qkv, ctx):
             q, k, v = ops.qk_norm_rope(qkv, n_q, n_kv, ctx.cos, ctx.sin, qn,
                                        w.get(p + "k_norm.weight") if qn is not None else None,
                                        self.rms_eps if self.rms_eps is not None else 1e-6,
@@ -111,11 +141,11 @@ class GqaHipBackend(AttentionBackend):
 
     def _write_kv(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, ctx) -> None:
         cache = ctx.kv_caches[layer_idx]
-        if (self.fuse_kv_write and getattr(ctx, "aia_slots_from_block_table", False)
+        if (self.fuse_kv_write and not self.fp8 and getattr(ctx, "aia_slots_from_block_table", False)
                 and k.shape[0] == ctx.slot_mapping.shape[0]):
             self._pending = (layer_idx, id(ctx), k, v)
             return
-        self._write(k, v, cache[0], cache[1], ctx.slot_mapping)
+        self._write(k, v, cache, ctx.slot_mapping)
 
     def _attn(self, layer_idx: int, q, k, v, ctx) -> torch.Tensor:
         cache = ctx.kv_caches[layer_idx]
@@ -124,10 +154,12 @@ class GqaHipBackend(AttentionBackend):
         if pending is not None and pending[:2] == (layer_idx, id(ctx)):
             return ops.paged_attention_gqa(q, cache[0], cache[1], plan, self.scale,
                                            key_new=pending[2], value_new=pending[3],
-                                           kv_layout=self.kv_layout)
+                                           kv_layout=self.kv_layout, **self.scores)
         if pending is not None:      # a deferred write for another call: do it now
             lay, _, pk, pv = pending
-            c = ctx.kv_caches[lay]
-            self._write(pk, pv, c[0], c[1], ctx.slot_mapping)
+            self._write(pk, pv, ctx.kv_caches[lay], ctx.slot_mapping)
+        if self.fp8:
+            return ops.paged_attention_gqa(q, cache[0], cache[1], plan, self.scale,
+                                           key_scale=cache[2], value_scale=cache[3], **self.scores)
         return ops.paged_attention_gqa(q, cache[0], cache[1], plan, self.scale,
-                                       kv_layout=self.kv_layout)
+                                       kv_layout=self.kv_layout, **self.scores)

@@ -7,7 +7,9 @@ split-K plan; both depend only on the step, so they are built once per
 ``ForwardContext`` (on first use, or by the GPU packer which attaches them
 as ``ctx.aia_cu_seqlens_q`` / ``ctx.aia_seqlens_kv``) and cached on it.
 Every context's plan owns its workspace, so steps in flight on different
-streams do not share scratch memory.
+streams do not share scratch memory.  A context may carry
+``aia_prefix_lens`` (device int32, one per request): the first keys of each
+request that all its rows see.
 
 Device metadata attached by a packer is not checked on the host.  Query
 lengths that do not add up to the step's token count make the planner plan
@@ -54,7 +56,7 @@ def step_plan(ctx, num_q_heads, num_kv_heads, head_dim_v, block_size):
     # plan records every stream it is used on, so the memory is not handed
     # out again while a step on another stream still reads it
     plan = ops.AttentionPlan(bt, cu, kv, T, num_q_heads, num_kv_heads, head_dim_v, block_size,
-                             owned=owned)
+                             owned=owned, prefix_lens=getattr(ctx, "aia_prefix_lens", None))
     if not owned and os.environ.get("AIA_CHECK_PLAN", "0") == "1" and \
             not torch.cuda.is_current_stream_capturing():
         plan.status()

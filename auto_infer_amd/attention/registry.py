@@ -46,6 +46,17 @@ def _paged_only(family, mode):
             f"full-softmax backends")
 
 
+def _gqa_options(model):
+    """What a model may ask for beyond the reference's backends:
+    ``KV_CACHE_DTYPE`` ("bf16" or "fp8"), ``attn_softcap``, ``alibi_slopes`` (device
+    float32, one per local query head) and ``aia_rope`` (an
+    ``ops.RotaryEmbedding``)."""
+    return dict(kv_dtype=getattr(model, "KV_CACHE_DTYPE", "bf16"),
+                softcap=getattr(model, "attn_softcap", 0.0),
+                alibi_slopes=getattr(model, "alibi_slopes", None),
+                rope=getattr(model, "aia_rope", None))
+
+
 def _gqa_hip(model, mode: str, kv_layout: str = "nd", family: str = GQA_FAMILY):
     from auto_infer_amd.attention.gqa import GqaHipBackend
     _paged_only(family, mode)
@@ -54,7 +65,7 @@ def _gqa_hip(model, mode: str, kv_layout: str = "nd", family: str = GQA_FAMILY):
         n_q_heads=model.n_q_local, n_kv_heads=model.n_kv_local, head_dim=cfg.head_dim,
         scale=cfg.head_dim ** -0.5, num_layers=cfg.num_layers, device=model.device,
         dtype=model.dtype, w=model.w, layer_prefix=model.layer_prefix,
-        rms_eps=getattr(cfg, "rms_eps", None), kv_layout=kv_layout)
+        rms_eps=getattr(cfg, "rms_eps", None), kv_layout=kv_layout, **_gqa_options(model))
 
 
 def _gqa_hip_nz(model, mode: str):
@@ -80,7 +91,7 @@ def _gqa_hip_mtp(model, mode: str, prefix: str, kv_layout: str = "nd"):
         n_q_heads=model.n_q_local, n_kv_heads=model.n_kv_local, head_dim=cfg.head_dim,
         scale=cfg.head_dim ** -0.5, num_layers=1, device=model.device, dtype=model.dtype,
         w=model.w, layer_prefix=lambda _: prefix, rms_eps=getattr(cfg, "rms_eps", None),
-        kv_layout=kv_layout)
+        kv_layout=kv_layout, **_gqa_options(model))
 
 
 def _gqa_hip_nz_mtp(model, mode: str, prefix: str):

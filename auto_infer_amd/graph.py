@@ -50,13 +50,20 @@ class DecodeGraph(_GearGraph):
     each layer's attention output.  ``kv_layout="nz"``: the caches are in the
     NZ layout of the reference's graph mode (``GraphGqaBackend``,
     gqa.py:192-226), as ``GqaHipBackend(kv_layout="nz")`` allocates them.
+    Caches of four tensors (k, v, k scales, v scales) are 8-bit ones, as
+    ``GqaHipBackend(kv_dtype="fp8")`` allocates them: the graph then writes the
+    new rows at the stager's slots in a launch of its own.  ``softcap`` /
+    ``alibi_slopes``: as ``ops.paged_attention_gqa`` takes them.
     """
 
     def __init__(self, stager, caches, *, num_q_heads, num_kv_heads, head_dim=128, scale=None,
-                 stream=None, kv_layout="nd"):
+                 stream=None, kv_layout="nd", softcap=0.0, alibi_slopes=None):
         if kv_layout not in ops.KV_LAYOUTS:
             raise ValueError(f"kv_layout must be one of {sorted(ops.KV_LAYOUTS)}")
         self.kv_layout = kv_layout
+        self.scores = dict(softcap=softcap, alibi_slopes=alibi_slopes)
+        if kv_layout != "nd" and any(len(c) == 4 for c in caches):
+            raise NotImplementedError("8-bit caches have no NZ layout")
         self.stager = stager
         self.caches = caches
         dev = stager.block_table.device
@@ -76,10 +83,18 @@ class DecodeGraph(_GearGraph):
 
     def _body(self):
         self.plan.replan()
-        for layer, (kc, vc) in enumerate(self.caches):
+        for layer, cache in enumerate(self.caches):
+            kc, vc, *scales = cache
+            if scales:
+                ops.write_kv_fp8(self.k_new[layer], self.v_new[layer], *cache, self.stager.slots)
+                ops.paged_attention_gqa(self.q[layer], kc, vc, self.plan, self.scale,
+                                        out=self.out[layer], key_scale=scales[0],
+                                        value_scale=scales[1], **self.scores)
+                continue
             ops.paged_attention_gqa(self.q[layer], kc, vc, self.plan, self.scale,
                                     out=self.out[layer], key_new=self.k_new[layer],
-                                    value_new=self.v_new[layer], kv_layout=self.kv_layout)
+                                    value_new=self.v_new[layer], kv_layout=self.kv_layout,
+                                    **self.scores)
 
 
 class LatentDecodeGraph(_GearGraph):
