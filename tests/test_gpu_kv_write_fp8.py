@@ -100,6 +100,26 @@ def test_slots_in_any_order_of_a_long_step(bs):
         write_both(k, v, slots, kv, vv)
 
 
+@pytest.mark.parametrize("bs,d", [(128, 128), (40, 64), (17, 128), (16, 128), (32, 64)])
+def test_many_short_runs(bs, d):
+    """A long step of decode rows and verify runs in blocks of their own, some
+    blocks twice, at offsets where a block starts anew or goes on."""
+    gen = torch.Generator().manual_seed(bs)
+    h, nb = 5, 700
+    kv, vv = fresh(nb, bs, h, d, gen), fresh(nb, bs, h, d, gen)
+    slots = []
+    for b in torch.randperm(nb, generator=gen).tolist():
+        n, off = 1 + b % 3, int(torch.randint(0, bs - 3, (1,), generator=gen)) if b % 5 else 0
+        slots += [b * bs + off + i for i in range(n)]
+        if b % 40 == 7:                  # another run of the same block
+            slots += [b * bs + bs - 1]
+        if b % 40 == 9 and len(slots) > 9:   # of an earlier one
+            slots += [slots[-9]]
+    k = (torch.randn(len(slots), h, d, generator=gen) * 6).bfloat16()
+    v = torch.randn(len(slots), h, d, generator=gen).bfloat16()
+    write_both(k, v, slots, kv, vv)
+
+
 def test_values_at_the_borders():
     """Largest values at and next to 448 * 2^e, ties of the rounding, zeros,
     subnormal and huge rows, and values that are not finite."""
