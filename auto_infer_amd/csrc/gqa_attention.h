@@ -159,31 +159,11 @@ __device__ __forceinline__ void write_segment(const AttnArgs& a, float4_t (&o)[R
 // cap, 119.4 without); prefill units wait for the VALU and have a form each.
 constexpr int kPlain = 0, kPrefixOnly = 1, kCap = 2, kBias = 3, kCapBias = 4, kAnyScore = 5;
 
-// Modified scores in log2 units (see ScoreArgs); far = query position - key
-// position.
-template <int SC>
-struct ScoreMod {
-  float scale, cap_in, cap_out;
-  bool cap, bias;
-  __device__ __forceinline__ ScoreMod(const ScoreArgs& s, float scale_log2)
-      : scale(scale_log2), cap_in(s.cap_in), cap_out(s.cap_out),
-        cap(SC == kAnyScore ? s.cap_out > 0.f : SC == kCap || SC == kCapBias),
-        bias(SC == kAnyScore ? s.slopes != nullptr : SC == kBias || SC == kCapBias) {}
-  __device__ __forceinline__ float capped(float x) const {
-    const float t = __builtin_amdgcn_exp2f(x * cap_in);
-    return __builtin_fmaf(-2.f * cap_out, __builtin_amdgcn_rcpf(t + 1.f), cap_out);
-  }
-  __device__ __forceinline__ float operator()(float x, float far, float slope) const {
-    float y = cap ? capped(x) : x * scale;
-    if (bias) y = __builtin_fmaf(-slope, __builtin_fabsf(far), y);
-    return y;
-  }
-};
-constexpr float kLog2e = 1.4426950408889634f;
-
 // A capped score of at most three quarters of the cap: x times a polynomial in
 // x^2 whose coefficients hold the call's factors (see the host side), within
-// 2^-22 of the cap.
+// 2^-22 of the cap and 2^-18 of the score.  (The exponential's form is within
+// 2^-21 of the cap at any score, which is too far for small scores under a
+// large cap.)
 __device__ __forceinline__ float capped_small(float x, const float (&c)[5]) {
   const float u = x * x;
   float y = __builtin_fmaf(u, c[4], c[3]);
@@ -191,6 +171,30 @@ __device__ __forceinline__ float capped_small(float x, const float (&c)[5]) {
   y = __builtin_fmaf(u, y, c[1]);
   return x * __builtin_fmaf(u, y, c[0]);
 }
+
+// Modified scores in log2 units (see ScoreArgs); far = query position - key
+// position.
+template <int SC>
+struct ScoreMod {
+  const ScoreArgs& args;
+  float scale, cap_in, cap_out;
+  bool cap, bias;
+  __device__ __forceinline__ ScoreMod(const ScoreArgs& s, float scale_log2)
+      : args(s), scale(scale_log2), cap_in(s.cap_in), cap_out(s.cap_out),
+        cap(SC == kAnyScore ? s.cap_out > 0.f : SC == kCap || SC == kCapBias),
+        bias(SC == kAnyScore ? s.slopes != nullptr : SC == kBias || SC == kCapBias) {}
+  __device__ __forceinline__ float capped(float x) const {
+    const float t = __builtin_amdgcn_exp2f(x * cap_in);
+    return __builtin_fmaf(-2.f * cap_out, __builtin_amdgcn_rcpf(t + 1.f), cap_out);
+  }
+  __device__ __forceinline__ float operator()(float x, float far, float slope) const {
+    float y = x * scale;
+    if (cap) y = __builtin_fabsf(x) <= args.cap_small ? capped_small(x, args.cap_poly) : capped(x);
+    if (bias) y = __builtin_fmaf(-slope, __builtin_fabsf(far), y);
+    return y;
+  }
+};
+constexpr float kLog2e = 1.4426950408889634f;
 
 // Non-finite values.  P is zero where a row does not see a key, but 0 x V is not
 // where V is an infinity or NaN, so the matrix product of a masked tile would

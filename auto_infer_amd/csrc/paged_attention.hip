@@ -2626,6 +2626,9 @@ static int attention_gqa(
   if (!(ex.softcap >= 0.f && ex.softcap < INFINITY))
     return fail(AIA_ERR_INVALID, "%s: softcap %g must be finite and not negative (0: none)", fn,
                 (double)ex.softcap);
+  if (ex.softcap > 0.f && !((double)scale / ex.softcap < 1e30))
+    return fail(AIA_ERR_INVALID, "%s: softcap %g is too small for scale %g", fn, (double)ex.softcap,
+                (double)scale);
   if (num_tokens == 0 || batch == 0) return AIA_OK;    // empty step (zero-size tensors)
   if (!query || !key_cache || !value_cache || !block_table || !out || !workspace || !cu_seqlens_q ||
       !seqlens_kv)
@@ -2685,8 +2688,15 @@ static int attention_gqa(
                          -0.049280451090587346, 0.0123188353892593};
     const double z = (double)scale / ex.softcap;
     double f = (double)ex.softcap * 1.4426950408889634 * z;
-    for (int i = 0; i < 5; ++i, f *= z * z) a.sc.cap_poly[i] = (float)(c[i] * f);
     a.sc.cap_small = (float)(0.75 / z);
+    for (int i = 0; i < 5; ++i, f *= z * z) {
+      a.sc.cap_poly[i] = (float)(c[i] * f);
+      // caps so large that the last factors vanish in float: those terms are
+      // below 2^-20 up to a tenth of the cap; so small that factors overflow:
+      // the exponential serves all scores
+      if (fabs(c[i] * f) < 1e-36) a.sc.cap_small = std::min(a.sc.cap_small, (float)(0.1 / z));
+      if (!(fabs(c[i] * f) < 1e30)) a.sc.cap_small = -1.f;
+    }
   }
   hipStream_t s = (hipStream_t)stream;
   PrefillArgs pa = {};

@@ -84,6 +84,13 @@ def _row_stride(t, name):
     return s0
 
 
+def _token_stride(t, name):
+    """``_row_stride``, but the row's length for a single token, whose stride
+    means nothing."""
+    ts = _row_stride(t, name)
+    return ts if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
 # ---------------------------------------------------------------- KV write
 
 def qk_norm_rope(qkv, num_q_heads, num_kv_heads, cos, sin, q_norm_weight=None,
@@ -253,8 +260,7 @@ def rope_qk(qkv, num_q_heads, num_kv_heads, positions, rope, q_norm_weight=None,
             if t.shape != (T, heads, D):
                 raise ValueError(f"{name} must have shape {(T, heads, D)}, got {tuple(t.shape)}")
         q_at, k_at = q.data_ptr(), k.data_ptr()
-        q_ts = _row_stride(q, "q_out") if T > 1 else nq
-        k_ts = _row_stride(k, "k_out") if T > 1 else nk
+        q_ts, k_ts = _token_stride(q, "q_out"), _token_stride(k, "k_out")
     _call_on(dev, "aia_rope_qk", qkv.data_ptr(), ts, T, num_q_heads, num_kv_heads, D,
              positions.data_ptr(), rope.turns.data_ptr(), rope.rotary_dim, rope.attention_factor,
              rope.interleaved, _ptr(q_norm_weight), _ptr(k_norm_weight), eps, q_at, q_ts, k_at,
@@ -499,14 +505,14 @@ def write_kv_fp8(key, value, key_cache, value_cache, key_scale, value_scale, slo
     _check_on(slot_mapping, "slot_mapping", torch.int32, dev)
     if slot_mapping.shape != (T,) or not slot_mapping.is_contiguous():
         raise ValueError("slot_mapping must be a contiguous 1-D tensor with one slot per token")
-    kts = _row_stride(key, "key") if T > 1 else hkv * d
+    kts = _token_stride(key, "key")
     if value is not None:
         _check_on(value, "value", _BF16, dev)
         if _check_fp8_cache(value_cache, value_scale, "value_cache", "value_scale", dev) != shape:
             raise ValueError("value_cache must match key_cache")
         if value.shape != rows:
             raise ValueError("value must match key")
-        vts = _row_stride(value, "value") if T > 1 else hkv * d
+        vts = _token_stride(value, "value")
         v_at, vc_at, vs_at = value.data_ptr(), value_cache.data_ptr(), value_scale.data_ptr()
     else:
         _require(value_cache is None and value_scale is None,
@@ -726,17 +732,14 @@ def paged_attention_gqa(query, key_cache, value_cache, plan, scale, out=None, fl
     if kv_layout not in KV_LAYOUTS:
         raise ValueError(f"kv_layout must be one of {sorted(KV_LAYOUTS)}")
     flags |= KV_LAYOUTS[kv_layout]
+    if (key_scale is not None or value_scale is not None or softcap != 0 or
+            alibi_slopes is not None or plan.prefix_lens is not None):
+        return _paged_attention_gqa_ex(query, key_cache, value_cache, plan, scale, out, flags,
+                                       key_new, value_new, key_scale, value_scale, softcap,
+                                       alibi_slopes)
     _check_device_tensor(query, "query", _BF16)
-    fp8 = key_scale is not None or value_scale is not None
-    if fp8:
-        dev = query.get_device()
-        _check_fp8_cache(key_cache, key_scale, "key_cache", "key_scale", dev)
-        _check_fp8_cache(value_cache, value_scale, "value_cache", "value_scale", dev)
-        _require(key_new is None and value_new is None,
-                 "8-bit caches are written by write_kv_fp8, not by key_new / value_new")
-    else:
-        _check_device_tensor(key_cache, "key_cache", _BF16)
-        _check_device_tensor(value_cache, "value_cache", _BF16)
+    _check_device_tensor(key_cache, "key_cache", _BF16)
+    _check_device_tensor(value_cache, "value_cache", _BF16)
     _require(query.dim() == 3 and query.stride(2) == 1, "query must be (T, Hq, D), D contiguous")
     shape = query.shape
     T, hq, d = shape
@@ -761,31 +764,78 @@ def paged_attention_gqa(query, key_cache, value_cache, plan, scale, out=None, fl
         _require(key_new.shape == rows and value_new.shape == rows,
                  "new K/V rows must be (tokens, Hkv, D)")
         kn_ts, vn_ts = _row_stride(key_new, "key_new"), _row_stride(value_new, "value_new")
-    scored = softcap != 0 or alibi_slopes is not None or plan.prefix_lens is not None
-    if alibi_slopes is not None:
-        _check_device_tensor(alibi_slopes, "alibi_slopes", torch.float32)
-        if alibi_slopes.shape != (hq,) or not alibi_slopes.is_contiguous() or alibi_slopes.device != device:
-            raise ValueError(f"alibi_slopes must hold {hq} contiguous values on {device}")
     stream = _ready(plan, device)
     q_ts, q_hs, _ = query.stride()
     o_ts, o_hs, _ = out.stride()
     table, ws = plan.block_table, plan.workspace
-    if fp8 or scored:
-        _require(table.device == device, "plan was made on another GPU")
-        _call_on(device.index, "aia_paged_attention_gqa_ex", query.data_ptr(), q_ts, q_hs,
-                     key_cache.data_ptr(), value_cache.data_ptr(), table.data_ptr(),
-                     table.stride(0), plan.cu_seqlens_q.data_ptr(), plan.seqlens_kv.data_ptr(),
-                     plan.batch, T, hq, hkv, d, bs, nb, float(scale), out.data_ptr(), o_ts,
-                     o_hs, _ptr(key_new), _ptr(value_new), kn_ts, vn_ts, _ptr(key_scale),
-                     _ptr(value_scale), _ptr(plan.prefix_lens), _ptr(alibi_slopes),
-                     float(softcap), plan.num_waves, flags, ws.data_ptr(), ws.numel(), stream)
-        return out
     _native.call("aia_paged_attention_gqa", query.data_ptr(), q_ts, q_hs,
                  key_cache.data_ptr(), value_cache.data_ptr(), table.data_ptr(),
                  table.stride(0), plan.cu_seqlens_q.data_ptr(), plan.seqlens_kv.data_ptr(),
                  plan.batch, T, hq, hkv, d, bs, nb, float(scale), out.data_ptr(), o_ts,
                  o_hs, _ptr(key_new), _ptr(value_new), kn_ts, vn_ts, plan.num_waves,
                  flags, ws.data_ptr(), ws.numel(), stream)
+    return out
+
+
+def _paged_attention_gqa_ex(query, key_cache, value_cache, plan, scale, out, flags, key_new,
+                            value_new, key_scale, value_scale, softcap, alibi_slopes):
+    """``paged_attention_gqa`` over 8-bit caches or with modified scores."""
+    _check_device_tensor(query, "query", _BF16)
+    dev, shape = query.get_device(), query.shape
+    if len(shape) != 3 or query.stride(2) != 1:
+        raise ValueError("query must be (T, Hq, D), D contiguous")
+    T, hq, d = shape
+    ks_at = vs_at = kn_at = vn_at = None
+    kn_ts = vn_ts = 0
+    if key_scale is not None or value_scale is not None:
+        cshape = _check_fp8_cache(key_cache, key_scale, "key_cache", "key_scale", dev)
+        if _check_fp8_cache(value_cache, value_scale, "value_cache", "value_scale", dev) != cshape:
+            raise ValueError("value cache shape differs from key cache")
+        _require(key_new is None and value_new is None,
+                 "8-bit caches are written by write_kv_fp8, not by key_new / value_new")
+        ks_at, vs_at = key_scale.data_ptr(), value_scale.data_ptr()
+    else:
+        _check_on(key_cache, "key_cache", _BF16, dev)
+        _check_on(value_cache, "value_cache", _BF16, dev)
+        cshape = key_cache.shape
+        if len(cshape) != 4 or not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+            raise ValueError("caches must be contiguous (num_blocks, block_size, Hkv, D)")
+        if value_cache.shape != cshape:
+            raise ValueError("value cache shape differs from key cache")
+    nb, bs, hkv, dk = cshape
+    if dk != d:
+        raise ValueError("query head_dim differs from the cache's")
+    if not (hq == plan.num_q_heads and hkv == plan.num_kv_heads and T == plan.num_tokens
+            and bs == plan.block_size and d == plan.head_dim_v):
+        raise ValueError("plan was made for another shape")
+    if key_new is not None or value_new is not None:
+        _check_on(key_new, "key_new", _BF16, dev)
+        _check_on(value_new, "value_new", _BF16, dev)
+        if key_new.shape != (T, hkv, d) or value_new.shape != (T, hkv, d):
+            raise ValueError("new K/V rows must be (tokens, Hkv, D)")
+        kn_ts, vn_ts = _row_stride(key_new, "key_new"), _row_stride(value_new, "value_new")
+        kn_at, vn_at = key_new.data_ptr(), value_new.data_ptr()
+    if alibi_slopes is not None:
+        _check_on(alibi_slopes, "alibi_slopes", torch.float32, dev)
+        if alibi_slopes.shape != (hq,) or not alibi_slopes.is_contiguous():
+            raise ValueError(f"alibi_slopes must hold {hq} contiguous values")
+    table, ws = plan.block_table, plan.workspace
+    if table.get_device() != dev:
+        raise ValueError("plan was made on another GPU")
+    device = query.device
+    if out is None:
+        out = torch.empty(shape, dtype=_BF16, device=device)
+    else:
+        _check_out(out, "out", shape, device)
+    stream = _ready(plan, device)
+    q_ts, q_hs, _ = query.stride()
+    o_ts, o_hs, _ = out.stride()
+    _call_on(dev, "aia_paged_attention_gqa_ex", query.data_ptr(), q_ts, q_hs,
+             key_cache.data_ptr(), value_cache.data_ptr(), table.data_ptr(), table.stride(0),
+             plan.cu_seqlens_q.data_ptr(), plan.seqlens_kv.data_ptr(), plan.batch, T, hq, hkv, d,
+             bs, nb, scale, out.data_ptr(), o_ts, o_hs, kn_at, vn_at, kn_ts, vn_ts, ks_at, vs_at,
+             _ptr(plan.prefix_lens), _ptr(alibi_slopes), softcap, plan.num_waves, flags,
+             ws.data_ptr(), ws.numel(), stream)
     return out
 
 

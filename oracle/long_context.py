@@ -71,8 +71,8 @@ def scored_attention(query, keys, values, block_table, cu_seqlens_q, seqlens_kv,
     output to bf16:
       (2^-8 + 2 eps) A + 2^-10 max_d A + 2^-8 |out|,
     A = sum_j p_j |v_j|, and eps = the error of a score: D 2^-24 sum_d |q_d k_d|
-    scale for the products, 2^-21 of the cap for the tanh, 2^-22 of the largest
-    score for its scaling, bias and exponent."""
+    scale for the products, 2^-21 of the cap or 2^-18 of the largest score for the
+    tanh (the lesser), 2^-22 of the largest score for scaling, bias and exponent."""
     T, hq, d = query.shape
     bs, hkv = keys.shape[1], keys.shape[2]
     g = hq // hkv
@@ -113,7 +113,7 @@ def scored_attention(query, keys, values, block_table, cu_seqlens_q, seqlens_kv,
                 a = p @ torch.where(bad, 0.0, vh).abs()
                 largest = torch.where(seen, s.abs(), 0.0).amax(-1, keepdim=True)
                 eps = (d * 2.0 ** -24 * torch.where(seen, mag, 0.0).amax(-1, keepdim=True)
-                       + 2.0 ** -21 * softcap + 2.0 ** -22 * largest)
+                       + torch.clamp(2.0 ** -18 * largest, max=2.0 ** -21 * softcap) + 2.0 ** -22 * largest)
                 out[start:end, h] = o
                 bound[start:end, h] = ((2.0 ** -8 + 2 * eps) * a + 2.0 ** -10 * a.amax(-1, keepdim=True)
                                        + 2.0 ** -8 * o.abs())

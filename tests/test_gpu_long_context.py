@@ -277,6 +277,9 @@ def test_refused_calls():
     attn(ValueError, "softcap", q, kb, vb, plan, 1.0, softcap=-1.0)
     attn(ValueError, "softcap", q, kb, vb, plan, 1.0, softcap=float("nan"))
     attn(ValueError, "softcap", q, kb, vb, plan, 1.0, softcap=float("inf"))
+    attn(ValueError, "softcap", q, kb, vb, plan, 1.0, softcap=1e-31)
+    attn(ValueError, "another shape", q[..., :64].contiguous(), kb[..., :64].contiguous(), vb[..., :64].contiguous(),
+         plan, 1.0, softcap=1.0)
     attn(ValueError, "alibi_slopes must hold 16", q, kb, vb, plan, 1.0,
          alibi_slopes=torch.ones(8, device=DEV))
     attn(ValueError, "alibi_slopes must be", q, kb, vb, plan, 1.0,
@@ -303,6 +306,8 @@ def test_refused_calls():
     write("value_cache must match", kn, vn, kc, vc[:-1], ks, vs[:-1], slots)
     write("rows .heads, dim. must be contiguous", kn.transpose(0, 1).contiguous().transpose(0, 1), vn, kc, vc, ks, vs,
           slots)
+    one = torch.zeros(1, 16, 128, dtype=torch.bfloat16, device=DEV)[:, ::2]      # a single token's rows too
+    write("rows .heads, dim. must be contiguous", one, None, kc, None, ks, None, slots[:1])
     write("must be on the GPU", kn.cpu(), vn, kc, vc, ks, vs, slots)
     with pytest.raises(NotImplementedError, match="head_dim"):
         ops.write_kv_fp8(kn[..., :32].contiguous(), None, kc[..., :32].contiguous(), None, ks, None, slots)

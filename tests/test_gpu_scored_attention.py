@@ -200,6 +200,25 @@ def test_capped_scores_far_past_the_cap():
     assert far.max().item() <= (2.0 ** -8 + 2.0 ** -10 + 2.0 ** -8) * vmax * 1.5
 
 
+@pytest.mark.parametrize("cap", [1e-20, 1e-4, 0.01, 1.0, 1e3, 1e6, 1e20])
+@pytest.mark.parametrize("zero", [False, True])
+def test_caps_of_any_size(cap, zero):
+    """Tiny caps (all weights equal in the limit), huge ones (no cap), and
+    queries of zeros, whose scores are zero at any cap."""
+    hq, hkv, d, bs = 4, 2, 128, 16
+    step = workloads.make_gqa_step(lqs=[1, 70], lks=[50, 90], num_q_heads=hq, num_kv_heads=hkv, head_dim=d,
+                                   block_size=bs, seed=8)
+    q = step.q * 0 if zero else step.q
+    plan = ops.AttentionPlan.from_lists(step.block_table.to(DEV), step.cu_seqlens_q, step.seqlens_kv, hq,
+                                        hkv, d, bs)
+    for slopes in (None, torch.full((hq,), 0.25)):
+        out = ops.paged_attention_gqa(q.to(DEV), step.k_cache.to(DEV), step.v_cache.to(DEV), plan, step.scale,
+                                      softcap=cap, alibi_slopes=None if slopes is None else slopes.to(DEV))
+        ref, bound = oracle.scored_attention(q, step.k_cache, step.v_cache, step.block_table, step.cu_seqlens_q,
+                                             step.seqlens_kv, step.scale, cap, slopes)
+        assert bool(((out.cpu().double() - ref).abs() <= bound).all())
+
+
 def test_fp8_pool_past_32_bits():
     """Blocks whose bytes lie past 2^32 (and slots past 2^22)."""
     hq, hkv, d, bs = 16, 8, 128, 128
