@@ -295,6 +295,7 @@ __device__ __forceinline__ void gqa_segment(const AttnArgs& a, const int* rec, i
 
   const int32_t* btrow = a.bt + (int64_t)b * a.bt_stride;
   const int nblk_vis = (visible + a.bs - 1) / a.bs;
+  const int last_key = max(visible - 1, 0);   // (a segment without keys has one masked tile)
   int blk_base = 0, btv = 0, w1 = 0;
   // 16-byte pieces between MFMA k-steps j and j + 1 of a cached key (4 pieces
   // on in ND; two 16-dim chunks of block_size x 16 on in NZ)
@@ -333,7 +334,7 @@ __device__ __forceinline__ void gqa_segment(const AttnArgs& a, const int* rec, i
   // straight-line and the compiler can wait for each tile with an exact count.
   auto load = [&](int lt, uint4 (&kk)[KJ], uint4 (&vv)[KJ], int64_t& wdst) {
     const bool live = lt < w1;
-    const int tok = live ? max(min(lt * kTile + n, visible - 1), 0) : blk_base * a.bs;
+    const int tok = live ? min(lt * kTile + n, last_key) : blk_base * a.bs;
     const int bi = tok / a.bs;
     // block ids outside the pool are clamped so a bad table cannot fault
     const int blk = min(max(__shfl(btv, bi - blk_base), 0), a.nb - 1);
@@ -538,6 +539,7 @@ __device__ __forceinline__ void gqa_segment_fp8(const AttnArgs& a, const int* re
 
   const int32_t* btrow = a.bt + (int64_t)b * a.bt_stride;
   const int nblk_vis = (visible + a.bs - 1) / a.bs;
+  const int last_key = max(visible - 1, 0);   // (a segment without keys has one masked tile)
   const uint8_t* kc = reinterpret_cast<const uint8_t*>(a.kc) + (int64_t)kvh * D + 16 * g;
   const uint8_t* vc = reinterpret_cast<const uint8_t*>(a.vc) + (int64_t)kvh * D + 16 * g;
   int blk_base = 0, btv = 0, w1 = 0;
@@ -567,7 +569,7 @@ __device__ __forceinline__ void gqa_segment_fp8(const AttnArgs& a, const int* re
   // One 16-key tile's loads (tiles past the window re-read its first row, as
   // in gqa_segment); bi = the lane's logical block in the window.
   auto load = [&](int lt, uint4 (&kk)[CH], uint4 (&vv)[CH], int& bi) {
-    const int tok = lt < w1 ? max(min(lt * kTile + n, visible - 1), 0) : blk_base * a.bs;
+    const int tok = lt < w1 ? min(lt * kTile + n, last_key) : blk_base * a.bs;
     const int bl = tok / a.bs;
     bi = bl - blk_base;
     const int blk = min(max(__shfl(btv, bi), 0), a.nb - 1);
@@ -874,7 +876,7 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
     rv[rt] = row < row_end;
     tokr[rt] = row / G;
     headr[rt] = kvh * G + (row - tokr[rt] * G);
-    lim[rt] = rv[rt] ? min(max(ctx0 + tokr[rt], pre - 1), lk - 1) : -1;
+    lim[rt] = rv[rt] ? min(SC == kPlain ? ctx0 + tokr[rt] : max(ctx0 + tokr[rt], pre - 1), lk - 1) : -1;
     // a bias without a cap starts the accumulators, in units of raw products
     if (SC == kBias || SC == kCapBias)
       slope[rt] = rv[rt] ? a.sc.slopes[headr[rt]] * (SC == kBias ? kLog2e / a.scale_log2 : kLog2e) : 0.f;

@@ -1655,6 +1655,7 @@ __device__ __forceinline__ void mla_segment(const MlaArgs& a, const int* rec, in
 
   const int32_t* btrow = a.bt + (int64_t)b * a.bt_stride;
   const int nblk_vis = (visible + a.bs - 1) / a.bs;
+  const int last_key = max(visible - 1, 0);   // (a segment without keys has one masked tile)
   int blk_base = 0, btv = 0, w1 = 0;
 
   uint4 qf[RB][5];
@@ -1683,7 +1684,7 @@ __device__ __forceinline__ void mla_segment(const MlaArgs& a, const int* rec, in
 
   auto load = [&](int lt, uint4 (&kk)[5]) {
     const bool live = lt < w1;
-    const int tok = live ? max(min(lt * kTile + n, visible - 1), 0) : blk_base * a.bs;
+    const int tok = live ? min(lt * kTile + n, last_key) : blk_base * a.bs;
     const int bi = tok / a.bs;
     const int blk = min(max(__shfl(btv, bi - blk_base), 0), a.nb - 1);
     const int off = tok - bi * a.bs;
