@@ -10,7 +10,8 @@
  * may come from several host threads on different streams.
  *
  * Element type of query/key/value/output tensors is bf16 (passed as raw
- * 16-bit words).  Indices are int32.
+ * 16-bit words).  8-bit KV caches hold OCP e4m3 values with
+ * e8m0 scales (raw bytes).  Indices are int32.
  */
 #ifndef AUTO_INFER_AMD_H
 #define AUTO_INFER_AMD_H
