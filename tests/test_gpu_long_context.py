@@ -327,3 +327,64 @@ def test_refused_calls():
                                                  pos, rope), {})):
         with pytest.raises(ValueError, match=match):
             ops.rope_qk(*args, **kw)
+
+
+def test_a_whole_layer_in_a_graph():
+    """Rotary positions, 8-bit write, planner with prefixes and capped attention
+    captured in one graph; every replay, with new inputs, lengths and prefixes
+    and eager work between, equals the eager calls."""
+    hq, hkv, d, bs, nb, T = 28, 4, 128, 16, 90, 150
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    rope = ops.RotaryEmbedding(d, base=1e6, device=DEV)
+    qkv = torch.empty(T, (hq + 2 * hkv) * d, dtype=torch.bfloat16, device=DEV)
+    pos = torch.zeros(T, dtype=torch.int64, device=DEV)
+    slots = torch.full((T,), -1, dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 1, 141, T], dtype=torch.int32, device=DEV)
+    kv = torch.tensor([1, 140, 9], dtype=torch.int32, device=DEV)
+    pre = torch.zeros(3, dtype=torch.int32, device=DEV)
+    table = torch.randperm(nb, generator=torch.Generator().manual_seed(3)).int().view(3, 30).to(DEV)
+    backend = GqaHipBackend(hq, hkv, d, d ** -0.5, 1, DEV, torch.bfloat16, kv_dtype="fp8")
+    cache, twin = backend.alloc_kv_caches(nb, bs)[0], backend.alloc_kv_caches(nb, bs)[0]
+    plan = ops.AttentionPlan(table, cu, kv, T, hq, hkv, d, bs, prefix_lens=pre)
+    outs = [torch.empty(T, hq, d, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    rotated = (torch.empty(T, hq, d, dtype=torch.bfloat16, device=DEV),
+               torch.empty(T, hkv, d, dtype=torch.bfloat16, device=DEV))
+
+    def layer(c, out):
+        q, k, v = ops.rope_qk(qkv, hq, hkv, pos, rope, out=rotated)
+        ops.write_kv_fp8(k, v, *c, slots)
+        plan.replan()
+        ops.paged_attention_gqa(q, c[0], c[1], plan, d ** -0.5, out=out, key_scale=c[2], value_scale=c[3],
+                                softcap=15.0)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        qkv.zero_()
+        layer(twin, outs[1])
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            layer(cache, outs[0])
+    torch.cuda.synchronize()
+    rng = np.random.default_rng(4)
+    for c in twin:
+        c.view(torch.uint8).zero_()
+    for step in range(5):
+        lens = [int(rng.integers(1, 300)), 140 + int(rng.integers(0, 300)), 9 + int(rng.integers(0, 300))]
+        p, s = [], []
+        for r, (n, lk) in enumerate(zip((1, 140, 9), lens)):
+            p += list(range(lk - n, lk))
+            s += [int(table[r, x // bs]) * bs + x % bs for x in range(lk - n, lk)]
+        qkv.copy_(torch.randn(qkv.shape, generator=gen, device=DEV) * 2.0 ** step)
+        pos.copy_(torch.tensor(p)), slots.copy_(torch.tensor(s, dtype=torch.int32))
+        kv.copy_(torch.tensor(lens, dtype=torch.int32))
+        pre.copy_(torch.tensor([int(rng.integers(0, lk + 1)) for lk in lens], dtype=torch.int32))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            layer(twin, outs[1])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[1])
+        for a, b in zip(cache, twin):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
