@@ -141,17 +141,6 @@ __device__ __forceinline__ void write_segment(const AttnArgs& a, float4_t (&o)[R
   }
 }
 
-// Processes key tiles [lt0, lt1) of one segment; rec = the segment record.
-// A segment holds RB blocks of 16 query rows: block r has the segment's
-// query tokens [r qb, r qb + qb), row n being token n / hb, head n % hb
-// (qb = 16 / hb).  Every K/V tile is loaded once and used by all blocks, so a
-// prefill chunk reads its keys 1/RB as often; blocks past the segment's last
-// token are skipped (a uniform branch), so a decode segment costs one block.
-// Cache layouts.  ND: (num_blocks, block_size, Hkv, D), a token slot's heads
-// contiguous.  NZ: the 16-wide fractal layout of the reference's graph-mode
-// caches (gqa.py:163,202-226): each block viewed (Hkv D / 16, block_size,
-// 16), so 16 dims of all of a block's tokens are contiguous.  kv_piece gives
-// the 16-byte index of piece p (8 dims) of head h of (block, offset).
 // What is done to a raw dot product: nothing (the scale goes into the
 // exponent), nothing but a prefix to see, a cap, a bias, both, or what the call's
 // ScoreArgs say at run time.  Decode rows wait for memory, so one run-time form
@@ -238,6 +227,11 @@ __device__ __forceinline__ int prefix_keys(const ScoreArgs& s, int b) {
   return s.prefix ? max(0, min(s.prefix[b], s.kvlen[b])) : 0;
 }
 
+// Cache layouts.  ND: (num_blocks, block_size, Hkv, D), a token slot's heads
+// contiguous.  NZ: the 16-wide fractal layout of the reference's graph-mode
+// caches (gqa.py:163,202-226): each block viewed (Hkv D / 16, block_size,
+// 16), so 16 dims of all of a block's tokens are contiguous.  kv_piece gives
+// the 16-byte index of piece p (8 dims) of head h of (block, offset).
 template <int KV>
 __device__ __forceinline__ int64_t kv_piece(int64_t blk, int off, int bs, int row_elems, int h,
                                             int D, int p) {
@@ -246,6 +240,12 @@ __device__ __forceinline__ int64_t kv_piece(int64_t blk, int off, int bs, int ro
          (((int64_t)(h * (D / 16) + (p >> 1)) * bs + off) << 1) + (p & 1);
 }
 
+// Processes key tiles [lt0, lt1) of one segment; rec = the segment record.
+// A segment holds RB blocks of 16 query rows: block r has the segment's
+// query tokens [r qb, r qb + qb), row n being token n / hb, head n % hb
+// (qb = 16 / hb).  Every K/V tile is loaded once and used by all blocks, so a
+// prefill chunk reads its keys 1/RB as often; blocks past the segment's last
+// token are skipped (a uniform branch), so a decode segment costs one block.
 template <int RB, int D, int KV, int SC>
 __device__ __forceinline__ void gqa_segment(const AttnArgs& a, const int* rec, int s, int lt0,
                                             int lt1, int w, int tpw, uint16_t* vt, int lane,
@@ -498,7 +498,9 @@ __device__ __forceinline__ void fp8_to_bf16(uint4 w, uint32_t e, uint4 (&out)[2]
 // halves are the operands of k-steps 2 (c / 4) and 2 (c / 4) + 1, and Q is read in
 // the same order.  Values become bf16 in registers with their block's scale,
 // so the scores need no further factor.  The scales are held like the block
-// ids, one logical block per lane.
+// ids, one logical block per lane.  Bound by memory: 128 single tokens over 1K to
+// 8K keys, 64/8 heads of 128, blocks of 16: 219 us a call, 5.5 TB/s (a large
+// read: 6.0).
 template <int RB, int D, int SC>
 __device__ __forceinline__ void gqa_segment_fp8(const AttnArgs& a, const int* rec, int s, int lt0,
                                                 int lt1, int w, int tpw, uint16_t* vt0, uint16_t* vt1,

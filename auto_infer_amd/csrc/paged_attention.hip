@@ -2754,8 +2754,8 @@ extern "C" int aia_paged_attention_gqa_ex(
     int32_t num_blocks, float scale, void* out, int64_t out_token_stride, int64_t out_head_stride,
     const void* key_new, const void* value_new, int64_t new_key_token_stride,
     int64_t new_value_token_stride, const void* key_scale, const void* value_scale,
-    const int32_t* prefix_lens, const float* alibi_slopes, float softcap, int32_t num_waves, int32_t flags, void* workspace,
-    int64_t workspace_bytes, void* stream) {
+    const int32_t* prefix_lens, const float* alibi_slopes, float softcap, int32_t num_waves,
+    int32_t flags, void* workspace, int64_t workspace_bytes, void* stream) {
   return attention_gqa("aia_paged_attention_gqa_ex", query, q_token_stride, q_head_stride, key_cache,
                        value_cache, block_table, block_table_stride, cu_seqlens_q, seqlens_kv, batch,
                        num_tokens, num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, scale,

