@@ -288,8 +288,10 @@ __device__ __forceinline__ void gqa_segment(const AttnArgs& a, const int* rec, i
   for (int d = 1; d < 64; d <<= 1) lim_lo = min(lim_lo, __shfl_xor(lim_lo, d));
   const int row_elems = a.hkv * D;
   // this step's new keys sit at positions [new_start, Lk); the request's last
-  // query block (head block 0) owns writing them into the cache
-  const int new_start = a.kn ? lim_base - q0 : 0x7fffffff;
+  // query block (head block 0) owns writing them into the cache.  (A segment
+  // without keys reads slot 0 in their place: the new row of position 0 would
+  // be the one behind the request's rows.)
+  const int new_start = a.kn && visible > 0 ? lim_base - q0 : 0x7fffffff;
   const int q_begin = qtok0 - q0;
   const bool writer = a.kn && ((rec[1] >> 30) & 1) && hbi == 0;
 
