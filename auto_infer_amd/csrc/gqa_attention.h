@@ -80,6 +80,14 @@ __device__ __forceinline__ short4_t vt_frag(const uint16_t* vs, int n, int g, in
 #endif
 constexpr int kPipe = AIA_PIPE;
 
+// A row that saw no key (its sum is zero): its products of masked tiles are 0 x V,
+// which is not zero where V is not finite.
+template <int DT>
+__device__ __forceinline__ void clear_row(float4_t (&o)[DT]) {
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = float4_t{0.f, 0.f, 0.f, 0.f};
+}
+
 // End of a segment's range: bf16 output where the range covers all of its
 // keys, else an fp16 partial.
 template <int RB, int D, bool SCORED>
@@ -92,6 +100,7 @@ __device__ __forceinline__ void write_segment(const AttnArgs& a, float4_t (&o)[R
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
     lsum[r] = aia::group4_sum(lsum[r]);
+    if (lsum[r] == 0.f) clear_row(o[r]);
   }
   const int first_wave = tile_begin / tpw;
   const int nparts = (tile_end - 1) / tpw - first_wave + 1;
@@ -1330,6 +1339,7 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
 #pragma unroll
   for (int rt = 0; rt < kPfRt; ++rt) {
     lsum[rt] = aia::group4_sum(lsum[rt]);
+    if (lsum[rt] == 0.f) clear_row(o[rt]);
     // a unit that does not cover all of its item's keys writes a partial:
     // y = O / c in fp16, c = the row's largest |O| (1 for an all-zero row),
     // with (m + log2 c, l / c) in place of (m, l).  The merge's log-sum-exp

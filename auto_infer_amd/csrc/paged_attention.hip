@@ -1777,7 +1777,10 @@ __device__ __forceinline__ void mla_segment(const MlaArgs& a, const int* rec, in
   }
 
 #pragma unroll
-  for (int r = 0; r < RB; ++r) lsum[r] = aia::group4_sum(lsum[r]);
+  for (int r = 0; r < RB; ++r) {
+    lsum[r] = aia::group4_sum(lsum[r]);
+    if (lsum[r] == 0.f) clear_row(o[r]);
+  }
   // balanced plans give the range's number within the segment and the
   // segment's range count in its record; otherwise ranges are tpw tiles
   const int first_wave = krec > 0 ? w - jrec : tile_begin / tpw;
