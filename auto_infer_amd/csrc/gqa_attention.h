@@ -88,9 +88,15 @@ __device__ __forceinline__ void clear_row(float4_t (&o)[DT]) {
   for (int dt = 0; dt < DT; ++dt) o[dt] = float4_t{0.f, 0.f, 0.f, 0.f};
 }
 
+// |x|, and zero for an infinity or NaN.
+__device__ __forceinline__ float finite_abs(float x) {
+  return __builtin_fabsf(x) < INFINITY ? __builtin_fabsf(x) : 0.f;
+}
+
 // End of a segment's range: bf16 output where the range covers all of its
-// keys, else an fp16 partial.
-template <int RB, int D, bool SCORED>
+// keys, else an fp16 partial.  CARE: infinities stay with their dims; the
+// partial's scale is the largest finite |O|, so the other dims fit fp16.
+template <int RB, int D, bool CARE>
 __device__ __forceinline__ void write_segment(const AttnArgs& a, float4_t (&o)[RB][D / 16], float (&m)[RB],
                                               float (&lsum)[RB], const bool (&rv)[RB],
                                               const int (&qi)[RB], int n, int g, int qtok0, int head,
@@ -130,11 +136,10 @@ __device__ __forceinline__ void write_segment(const AttnArgs& a, float4_t (&o)[R
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) cmax = fmaxf(cmax, fabsf(o[r][dt][i]));
+        for (int i = 0; i < 4; ++i) cmax = fmaxf(cmax, CARE ? finite_abs(o[r][dt][i]) : fabsf(o[r][dt][i]));
       cmax = aia::group4_max(cmax);
       if (!rv[r]) continue;
-      // (an infinite output stays one: its row keeps its values)
-      const float c = cmax > 0.f && !(SCORED && cmax == INFINITY) ? cmax : 1.f;
+      const float c = cmax > 0.f ? cmax : 1.f;
       const float inv = 1.f / c;
       const int64_t prow = ((int64_t)part * a.nw + wid) * seg_rows + r * kRows + n;
       uint16_t* pp = a.part_o + prow * D;
@@ -719,7 +724,7 @@ __device__ __forceinline__ void gqa_segment_fp8(const AttnArgs& a, const int* re
     }
     w0 = w1;
   }
-  write_segment<RB, D, false>(a, o, m, lsum, rv, qi, n, g, qtok0, head, wid, w, tpw, tile_begin, tile_end, part_base);
+  write_segment<RB, D, true>(a, o, m, lsum, rv, qi, n, g, qtok0, head, wid, w, tpw, tile_begin, tile_end, part_base);
 }
 
 // One work-group per key range, one wave per kv head of the segment's group.
@@ -1341,17 +1346,19 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
     lsum[rt] = aia::group4_sum(lsum[rt]);
     if (lsum[rt] == 0.f) clear_row(o[rt]);
     // a unit that does not cover all of its item's keys writes a partial:
-    // y = O / c in fp16, c = the row's largest |O| (1 for an all-zero row),
-    // with (m + log2 c, l / c) in place of (m, l).  The merge's log-sum-exp
-    // rule then folds c back exactly (its weights are exp2(m - M)), and the
-    // partials take half the bytes of fp32 ones.  The first hdr[11] units of
-    // the list keep O and (m, l) as they are, in fp32 (see the planner).
+    // y = O / c in fp16, c = the row's largest |O| (1 for an all-zero row; with
+    // CARE the largest finite one, so that an infinity leaves the other dims in
+    // range), with (m + log2 c, l / c) in place of (m, l).  The merge's
+    // log-sum-exp rule then folds c back exactly (its weights are exp2(m - M)),
+    // and the partials take half the bytes of fp32 ones.  The first hdr[11] units
+    // of the list keep O and (m, l) as they are, in fp32 (see the planner).
     float cmax = 0.f;
     if (!whole && !wide) {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) cmax = fmaxf(cmax, fabsf(o[rt][dt][v]));
+        for (int v = 0; v < 4; ++v)
+          cmax = fmaxf(cmax, CARE ? finite_abs(o[rt][dt][v]) : fabsf(o[rt][dt][v]));
       cmax = aia::group4_max(cmax);
     }
     if (!rv[rt]) continue;
@@ -1364,7 +1371,7 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
       continue;
     }
     if (!whole) {
-      const float c = cmax > 0.f && !(SC != kPlain && cmax == INFINITY) ? cmax : 1.f, ic = 1.f / c;
+      const float c = cmax > 0.f ? cmax : 1.f, ic = 1.f / c;
       const int64_t blk = (int64_t)unit * a.hkv + kvh, r = (wid * kPfRt + rt) * kRows + n;
       uint16_t* pp = a.part_o + (2 * blk * kPfRows + r) * D;
 #pragma unroll
