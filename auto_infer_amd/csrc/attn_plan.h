@@ -31,8 +31,10 @@ struct ScoreArgs {
   const int32_t* prefix;     // keys of each request that all its rows see, or null
   const int32_t* kvlen;
   float cap_in, cap_out;     // cap_out 0: no cap
+  float cap_unit;            // scale / cap
   float cap_small;           // |q.k| up to which cap_poly serves
-  float cap_poly[5];
+  float cap_poly[5];         // in (q.k cap_unit)^2, times q.k
+  float cap_raw[5];          // the same in (q.k)^2; all 0 where that leaves float32's range
 };
 
 struct AttnArgs {

@@ -163,16 +163,18 @@ __device__ __forceinline__ void write_segment(const AttnArgs& a, float4_t (&o)[R
 constexpr int kPlain = 0, kPrefixOnly = 1, kCap = 2, kBias = 3, kCapBias = 4, kAnyScore = 5;
 
 // A capped score of at most three quarters of the cap: x times a polynomial in
-// x^2 whose coefficients hold the call's factors (see the host side), within
-// 2^-22 of the cap and 2^-18 of the score.  (The exponential's form is within
-// 2^-21 of the cap at any score, which is too far for small scores under a
-// large cap.)
-__device__ __forceinline__ float capped_small(float x, const float (&c)[5]) {
-  const float u = x * x;
+// (x scale / cap)^2, within 2^-22 of the cap and 2^-18 of the score, under caps
+// of any size.  (The exponential's form is within 2^-21 of the cap at any score,
+// which is too far for small scores under a large cap.)
+__device__ __forceinline__ float cap_poly(float x, float u, const float (&c)[5]) {
   float y = __builtin_fmaf(u, c[4], c[3]);
   y = __builtin_fmaf(u, y, c[2]);
   y = __builtin_fmaf(u, y, c[1]);
   return x * __builtin_fmaf(u, y, c[0]);
+}
+__device__ __forceinline__ float capped_small(float x, const ScoreArgs& s) {
+  const float z = x * s.cap_unit;
+  return cap_poly(x, z * z, s.cap_poly);
 }
 
 // Modified scores in log2 units (see ScoreArgs); far = query position - key
@@ -192,7 +194,7 @@ struct ScoreMod {
   }
   __device__ __forceinline__ float operator()(float x, float far, float slope) const {
     float y = x * scale;
-    if (cap) y = __builtin_fabsf(x) <= args.cap_small ? capped_small(x, args.cap_poly) : capped(x);
+    if (cap) y = __builtin_fabsf(x) <= args.cap_small ? capped_small(x, args) : capped(x);
     if (bias) y = __builtin_fmaf(-slope, __builtin_fabsf(far), y);
     return y;
   }
@@ -1133,7 +1135,9 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
         // The VALU is what these units wait for, and the cap's exponential and
         // reciprocal are a quarter as fast as other instructions: tiles whose
         // scores all stay below three quarters of the cap take a polynomial
-        // (six multiply-adds) instead.
+        // (six multiply-adds) instead, of the raw products where its factors fit
+        // float32 (scaled ones, a multiplication more, cost prefix and cap, 3
+        // prompts of 600 to 2000, 2 of 98 us).
         float big = 0.f;
 #pragma unroll
         for (int st = 0; st < kSt; ++st)
@@ -1150,7 +1154,8 @@ __device__ __forceinline__ void gqa_prefill_body(const PrefillArgs& a, int wg,
             }
         };
         if (__any(big > a.sc.cap_small)) each([&](float x) { return mod.capped(x); });
-        else each([&](float x) { return capped_small(x, a.sc.cap_poly); });
+        else if (a.sc.cap_raw[0] != 0.f) each([&](float x) { return cap_poly(x, x * x, a.sc.cap_raw); });
+        else each([&](float x) { return capped_small(x, a.sc); });
       }
       if (MASK) {     // causal diagonal / sequence end: per-key limits
         const int rel = lim[rt] - kbase - 4 * g;

@@ -2627,8 +2627,8 @@ static int attention_gqa(
   if (fp8 && (key_new || value_new))
     return fail(AIA_ERR_INVALID, "%s: 8-bit caches are written by aia_kv_write_fp8 (no key_new / "
                 "value_new)", fn);
-  if (!(ex.softcap >= 0.f && ex.softcap < INFINITY))
-    return fail(AIA_ERR_INVALID, "%s: softcap %g must be finite and not negative (0: none)", fn,
+  if (!(ex.softcap >= 0.f && ex.softcap < 1e38f))
+    return fail(AIA_ERR_INVALID, "%s: softcap %g must be below 1e38 and not negative (0: none)", fn,
                 (double)ex.softcap);
   if (ex.softcap > 0.f && !((double)scale / ex.softcap < 1e30))
     return fail(AIA_ERR_INVALID, "%s: softcap %g is too small for scale %g", fn, (double)ex.softcap,
@@ -2691,16 +2691,13 @@ static int attention_gqa(
     const double c[5] = {0.9999972283263151, -0.33323076500793086, 0.13226091761972558,
                          -0.049280451090587346, 0.0123188353892593};
     const double z = (double)scale / ex.softcap;
-    double f = (double)ex.softcap * 1.4426950408889634 * z;
-    a.sc.cap_small = (float)(0.75 / z);
-    for (int i = 0; i < 5; ++i, f *= z * z) {
-      a.sc.cap_poly[i] = (float)(c[i] * f);
-      // caps so large that the last factors vanish in float: those terms are
-      // below 2^-20 up to a tenth of the cap; so small that factors overflow:
-      // the exponential serves all scores
-      if (fabs(c[i] * f) < 1e-36) a.sc.cap_small = std::min(a.sc.cap_small, (float)(0.1 / z));
-      if (!(fabs(c[i] * f) < 1e30)) a.sc.cap_small = -1.f;
-    }
+    a.sc.cap_unit = (float)z;
+    a.sc.cap_small = (float)std::min(0.75 / z, 3.4e38);   // (an infinite product: the exponential)
+    double f = (double)scale * 1.4426950408889634;
+    for (int i = 0; i < 5; ++i) a.sc.cap_poly[i] = (float)(c[i] * f);
+    // (all factors between 1e-37 and 1e26, and products of at most 7500)
+    if (z > 1e-4 && z < 1e3 && scale > 1e-3f && scale < 1e3f)
+      for (int i = 0; i < 5; ++i, f *= z * z) a.sc.cap_raw[i] = (float)(c[i] * f);
   }
   hipStream_t s = (hipStream_t)stream;
   PrefillArgs pa = {};

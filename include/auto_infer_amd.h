@@ -211,7 +211,8 @@ int aia_paged_attention_gqa(const void* query, int64_t q_token_stride,
  *   value_new and AIA_ATTN_KV_NZ are then rejected); both NULL: bf16 caches.
  * prefix_lens: NULL, or the array the plan was made with (aia_attn_plan_prefix).
  * alibi_slopes: NULL, or num_q_heads floats on the device.
- * softcap: 0 for none; scale / softcap below 1e30 (AIA_ERR_INVALID otherwise).
+ * softcap: 0 for none; below 1e38 and scale / softcap below 1e30
+ *   (AIA_ERR_INVALID otherwise).
  * With query position i and key position j, the score of head h is
  *   s = scale * q.k;  s = softcap * tanh(s / softcap) if softcap > 0;
  *   s = s - alibi_slopes[h] * |i - j|.
