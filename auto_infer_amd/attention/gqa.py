@@ -18,7 +18,8 @@ block_size, 16) by npu_scatter_pa_kv_cache and FIA-v2, gqa.py:202-226).
 Beyond the reference: ``kv_dtype="fp8"`` keeps the caches as e4m3 values with a
 power-of-two scale per block and head, ``softcap`` / ``alibi_slopes`` modify the
 scores, ``rope`` (an ``ops.RotaryEmbedding``) turns Q and K from
-``ctx.positions`` instead of ``ctx.cos`` / ``ctx.sin``, and a context with
+``ctx.positions`` instead of ``ctx.cos`` / ``ctx.sin`` (``rope=False``: a model
+without rotary positions, Q and K stay as they are), and a context with
 ``aia_prefix_lens`` (device int32, one per request) lets all rows of a request
 see its first keys.
 """
@@ -69,6 +70,9 @@ class GqaHipBackend(AttentionBackend):
         if self.fp8 and kv_layout != "nd":
             raise NotImplementedError("8-bit caches have no NZ layout")
         self.scores = dict(softcap=softcap, alibi_slopes=alibi_slopes)
+        if rope is not None and rope is not False and not isinstance(rope, ops.RotaryEmbedding):
+            raise ValueError("rope must be an ops.RotaryEmbedding, False (no rotary positions) or None "
+                             "(ctx.cos / ctx.sin)")
         self.rope = rope
         self._pending = None
 
@@ -106,11 +110,14 @@ class GqaHipBackend(AttentionBackend):
         p = self.layer_prefix(layer_idx) + "self_attn."
         qkv = lin(x, w[p + "qkv_proj.weight"], w.get(p + "qkv_proj.bias"))
         qn = w.get(p + "q_norm.weight")
-        if self.rope is not None:
+        if self.rope is None and (ctx.cos is None or ctx.sin is None):
+            raise ValueError("the context has no cos / sin: give the backend a rope, or rope=False "
+                             "for a model without rotary positions")
+        if self.rope is not None and self.rope is not False:
             q, k, v = ops.rope_qk(qkv, n_q, n_kv, ctx.positions, self.rope, qn,
                                   w.get(p + "k_norm.weight") if qn is not None else None,
                                   self.rms_eps if self.rms_eps is not None else 1e-6)
-        elif self._fusable(qkv, ctx):
+        elif self.rope is None and self._fusable(qkv, ctx):
             q, k, v = ops.qk_norm_rope(qkv, n_q, n_kv, ctx.cos, ctx.sin, qn,
                                        w.get(p + "k_norm.weight") if qn is not None else None,
                                        self.rms_eps if self.rms_eps is not None else 1e-6,
@@ -123,8 +130,9 @@ class GqaHipBackend(AttentionBackend):
             if qn is not None:
                 q = rms_norm(q, qn, self.rms_eps)
                 k = rms_norm(k, w[p + "k_norm.weight"], self.rms_eps)
-            q = q * ctx.cos + rotate_half(q) * ctx.sin
-            k = k * ctx.cos + rotate_half(k) * ctx.sin
+            if self.rope is None:
+                q = q * ctx.cos + rotate_half(q) * ctx.sin
+                k = k * ctx.cos + rotate_half(k) * ctx.sin
         self._write_kv(layer_idx, k, v, ctx)
         o = self._attn(layer_idx, q, k, v, ctx).reshape(T, n_q * hd)
         return lin(o, w[p + "o_proj.weight"])

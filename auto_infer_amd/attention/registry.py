@@ -50,7 +50,7 @@ def _gqa_options(model):
     """What a model may ask for beyond the reference's backends:
     ``KV_CACHE_DTYPE`` ("bf16" or "fp8"), ``attn_softcap``, ``alibi_slopes`` (device
     float32, one per local query head) and ``aia_rope`` (an
-    ``ops.RotaryEmbedding``)."""
+    ``ops.RotaryEmbedding``; False for a model without rotary positions)."""
     return dict(kv_dtype=getattr(model, "KV_CACHE_DTYPE", "bf16"),
                 softcap=getattr(model, "attn_softcap", 0.0),
                 alibi_slopes=getattr(model, "alibi_slopes", None),
