@@ -48,10 +48,12 @@ def _paged_only(family, mode):
 
 def _gqa_options(model):
     """What a model may ask for beyond the reference's backends:
-    ``KV_CACHE_DTYPE`` ("bf16" or "fp8"), ``attn_softcap``, ``alibi_slopes`` (device
-    float32, one per local query head) and ``aia_rope`` (an
-    ``ops.RotaryEmbedding``; False for a model without rotary positions)."""
-    return dict(kv_dtype=getattr(model, "KV_CACHE_DTYPE", "bf16"),
+    ``KV_CACHE_DTYPE`` ("bf16" or "fp8"), ``attn_scale`` (of the scores; default
+    head_dim ** -0.5), ``attn_softcap``, ``alibi_slopes`` (device float32, one per
+    local query head) and ``aia_rope`` (an ``ops.RotaryEmbedding``; False for a model
+    without rotary positions)."""
+    return dict(scale=getattr(model, "attn_scale", model.cfg.head_dim ** -0.5),
+                kv_dtype=getattr(model, "KV_CACHE_DTYPE", "bf16"),
                 softcap=getattr(model, "attn_softcap", 0.0),
                 alibi_slopes=getattr(model, "alibi_slopes", None),
                 rope=getattr(model, "aia_rope", None))
@@ -63,7 +65,7 @@ def _gqa_hip(model, mode: str, kv_layout: str = "nd", family: str = GQA_FAMILY):
     cfg = model.cfg
     return GqaHipBackend(
         n_q_heads=model.n_q_local, n_kv_heads=model.n_kv_local, head_dim=cfg.head_dim,
-        scale=cfg.head_dim ** -0.5, num_layers=cfg.num_layers, device=model.device,
+        num_layers=cfg.num_layers, device=model.device,
         dtype=model.dtype, w=model.w, layer_prefix=model.layer_prefix,
         rms_eps=getattr(cfg, "rms_eps", None), kv_layout=kv_layout, **_gqa_options(model))
 
@@ -89,7 +91,7 @@ def _gqa_hip_mtp(model, mode: str, prefix: str, kv_layout: str = "nd"):
     cfg = model.cfg
     return GqaHipBackend(
         n_q_heads=model.n_q_local, n_kv_heads=model.n_kv_local, head_dim=cfg.head_dim,
-        scale=cfg.head_dim ** -0.5, num_layers=1, device=model.device, dtype=model.dtype,
+        num_layers=1, device=model.device, dtype=model.dtype,
         w=model.w, layer_prefix=lambda _: prefix, rms_eps=getattr(cfg, "rms_eps", None),
         kv_layout=kv_layout, **_gqa_options(model))
 

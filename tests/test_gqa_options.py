@@ -63,3 +63,14 @@ def test_missing_rotary_rows_are_named():
         GqaHipBackend(HQ, HKV, D, 1.0, 1, torch.device("cpu"), torch.float32, rope=True)
     rope = ops.RotaryEmbedding(D, device="cpu")
     assert GqaHipBackend(HQ, HKV, D, 1.0, 1, torch.device("cpu"), torch.float32, rope=rope).rope is rope
+
+
+@pytest.mark.parametrize("family", ["gqa_hip", "gqa_hip_nz"])
+def test_a_query_scale_of_the_models_own(family):
+    for options, scale in (({}, D ** -0.5), ({"attn_scale": 144 ** -0.5, "attn_softcap": 50.0}, 144 ** -0.5)):
+        m = model(**options)
+        m.ATTENTION_FAMILY = family
+        backend, _ = registry.build_attention_backend(m, "paged", 2, 16)
+        mtp, _ = registry.build_mtp_attention_backend(m, "paged", "mtp.", 2, 16)
+        for b in (backend, mtp):
+            assert b.scale == scale and b.scores["softcap"] == options.get("attn_softcap", 0.0)
