@@ -7,9 +7,15 @@ split-K plan; both depend only on the step, so they are built once per
 ``ForwardContext`` (on first use, or by the GPU packer which attaches them
 as ``ctx.aia_cu_seqlens_q`` / ``ctx.aia_seqlens_kv``) and cached on it.
 Every context's plan owns its workspace, so steps in flight on different
-streams do not share scratch memory.  A context may carry
-``aia_prefix_lens`` (device int32, one per request): the first keys of each
-request that all its rows see.
+streams do not share scratch memory.
+
+A context may carry ``aia_prefix_lens``, one per request: the first keys of each
+request that all its rows see.  From the second layer on, keys and values of the
+prefix depend on all of it, so a prefix has to be computed within one step
+(cached blocks of the same prefix in front), and its blocks are shared only
+between requests of the same prefix (``block_allocator.prefix_seed``).  A host list
+is checked for the first and uploaded; a device int32 tensor is taken as it is
+(checked with ``AIA_CHECK_PLAN=1``).
 
 Device metadata attached by a packer is not checked on the host.  Query
 lengths that do not add up to the step's token count make the planner plan
@@ -24,6 +30,11 @@ import os
 import torch
 
 from auto_infer_amd import ops
+
+
+def _checking():
+    return (os.environ.get("AIA_CHECK_PLAN", "0") == "1"
+            and not torch.cuda.is_current_stream_capturing())
 
 
 def step_plan(ctx, num_q_heads, num_kv_heads, head_dim_v, block_size):
@@ -44,9 +55,16 @@ def step_plan(ctx, num_q_heads, num_kv_heads, head_dim_v, block_size):
         cu = torch.tensor([0, *ctx.cu_seqlens_q], dtype=torch.int32).to(dev)
         kv = torch.tensor(list(ctx.seqlens_kv), dtype=torch.int32).to(dev)
         ctx.aia_cu_seqlens_q, ctx.aia_seqlens_kv = cu, kv
-        owned = [cu, kv]
+        owned, packed = [cu, kv], False
     else:
-        owned = []
+        owned, packed = [], True
+    pre = getattr(ctx, "aia_prefix_lens", None)
+    if pre is not None and not isinstance(pre, torch.Tensor):
+        ops.check_prefixes(pre, ctx.cu_seqlens_q, ctx.seqlens_kv)
+        pre = ctx.aia_prefix_lens = torch.tensor(list(pre), dtype=torch.int32).to(bt.device)
+        owned.append(pre)
+    elif pre is not None and _checking():
+        ops.check_prefixes(pre.tolist(), ctx.cu_seqlens_q, ctx.seqlens_kv)
     T = int(ctx.cu_seqlens_q[-1]) if len(ctx.cu_seqlens_q) else 0
     if bt.dtype != torch.int32:
         bt = bt.to(torch.int32)
@@ -56,9 +74,8 @@ def step_plan(ctx, num_q_heads, num_kv_heads, head_dim_v, block_size):
     # plan records every stream it is used on, so the memory is not handed
     # out again while a step on another stream still reads it
     plan = ops.AttentionPlan(bt, cu, kv, T, num_q_heads, num_kv_heads, head_dim_v, block_size,
-                             owned=owned, prefix_lens=getattr(ctx, "aia_prefix_lens", None))
-    if not owned and os.environ.get("AIA_CHECK_PLAN", "0") == "1" and \
-            not torch.cuda.is_current_stream_capturing():
+                             owned=owned, prefix_lens=pre)
+    if packed and _checking():
         plan.status()
     plans[key] = plan
     return plan

@@ -14,6 +14,11 @@ hands out the same block ids:
 * a full block's hash chains its predecessor's, ``hash((prev, chunk))``,
   and a match also compares the stored token chunk (:78-111).
 
+Beyond the reference, the chain may start from a seed.  Below a prefix that sees
+itself in both directions (``aia_prefix_lens``) a block's keys and values depend
+on the whole prefix from the second layer on, not only on the tokens up to the
+block, so such requests match and register with ``prefix_seed``.
+
 The state lives in flat per-block arrays instead of dictionaries: a state
 code and refcount per block, a stack of unused ids, and an intrusive
 doubly linked list (``_prev``/``_next``, sentinel ``N``) that keeps the
@@ -23,6 +28,16 @@ no per-operation rehashing.
 """
 
 _UNUSED, _ACTIVE, _CACHED = 0, 1, 2
+
+
+def prefix_seed(token_ids: list, prefix_len: int) -> int:
+    """The seed of ``match_prefix`` / ``register_prefix`` for a request whose
+    first ``prefix_len`` tokens are seen by all its rows: its blocks are shared
+    only with requests of the same prefix.  (0, the plain chain's start, up to one
+    token, which causal rows see too.)"""
+    if prefix_len <= 1:
+        return 0
+    return hash(("prefix", prefix_len, tuple(token_ids[:prefix_len])))
 
 
 class KVCacheManager:
@@ -135,13 +150,14 @@ class KVCacheManager:
 
     # ----------------------------------------------------- prefix caching
 
-    def match_prefix(self, token_ids: list) -> list:
+    def match_prefix(self, token_ids: list, seed: int = 0) -> list:
         """Blocks holding the longest registered full-block prefix of
         ``token_ids``; each gains a reference (revivable ones come back into
-        use)."""
+        use).  ``seed``: what the chain starts from, as in ``register_prefix``
+        (see ``prefix_seed``)."""
         bs = self.block_size
         state, refs = self._state, self._refs
-        hits, prev = [], 0
+        hits, prev = [], seed
         for start in range(0, len(token_ids) - bs + 1, bs):
             chunk = tuple(token_ids[start:start + bs])
             h = hash((prev, chunk))
@@ -160,12 +176,13 @@ class KVCacheManager:
             prev = h
         return hits
 
-    def register_prefix(self, token_ids: list, block_ids: list) -> None:
+    def register_prefix(self, token_ids: list, block_ids: list, seed: int = 0) -> None:
         """Make the full blocks of ``token_ids`` (held in ``block_ids``)
-        findable by ``match_prefix``.  A hash keeps its first block and a
-        block its first hash; the stored chunk is always the latest."""
+        findable by ``match_prefix`` with the same ``seed``.  A hash keeps its
+        first block and a block its first hash; the stored chunk is always the
+        latest."""
         bs = self.block_size
-        prev = 0
+        prev = seed
         for i in range(len(token_ids) // bs):
             chunk = tuple(token_ids[i * bs:(i + 1) * bs])
             h = hash((prev, chunk))

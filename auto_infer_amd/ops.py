@@ -673,6 +673,20 @@ def check_lists(cu_seqlens_q, seqlens_kv, max_context):
         prev = end
 
 
+def check_prefixes(prefix_lens, cu_seqlens_q, seqlens_kv):
+    """Host check of prefixes that all rows of a request see, against the step's
+    lists: a prefix lies within what the request has after this step.  Its rows
+    see all of it, so a chunk that ends inside it would leave them (and, layers
+    on, their keys and values) without what follows."""
+    _require(len(prefix_lens) == len(seqlens_kv), "prefix_lens must have one entry per request")
+    prev = 0
+    for i, (n, end, lk) in enumerate(zip(prefix_lens, cu_seqlens_q, seqlens_kv)):
+        _require(end == prev or n <= lk,
+                 f"request {i}: its prefix of {n} tokens ends behind the step's {lk}; a prefix must "
+                 f"lie in the request's first chunk")
+        prev = end
+
+
 def _ready(plan, device):
     """Order the attention launch after the planner: on another stream, make
     the current stream wait for the plan's stream (not allowed while
