@@ -18,6 +18,8 @@
 // Bound by memory: each row is read and written once.  8,192 tokens of 28/4
 // heads of 128, half of each head turned, into other tensors: 28.1 us on the
 // GPU, 4.8 TB/s (a large copy: 5.1).  16 tokens: 3.2 us, a launch and one memory round trip.
+#include <algorithm>
+
 #include "common.h"
 
 namespace {
@@ -109,6 +111,24 @@ __global__ __launch_bounds__(kThreads) void rope_qk_kernel(Args a) {
   }
 }
 
+// Rows of a token (16-bit elements) in memory.
+struct Rows {
+  const void* at;
+  int64_t len, stride;
+};
+
+// Whether the rows of n tokens share memory.  Rows of one stride may interleave
+// (columns of one wider tensor): with d the distance modulo the stride, [0, len)
+// and [d, d + other len) must not meet.  Rows of different strides whose spans
+// meet count as sharing.
+bool share_memory(const Rows& a, const Rows& b, int64_t n) {
+  const int64_t a0 = (int64_t)((uintptr_t)a.at / 2), b0 = (int64_t)((uintptr_t)b.at / 2);
+  if (a0 >= b0 + (n - 1) * b.stride + b.len || b0 >= a0 + (n - 1) * a.stride + a.len) return false;
+  if (n == 1 || a.stride != b.stride) return true;
+  const int64_t d = ((b0 - a0) % a.stride + a.stride) % a.stride;
+  return d < a.len || d + b.len > a.stride;
+}
+
 }  // namespace
 
 extern "C" int aia_rope_qk(const void* qkv, int64_t qkv_token_stride, int32_t num_tokens,
@@ -141,6 +161,18 @@ extern "C" int aia_rope_qk(const void* qkv, int64_t qkv_token_stride, int32_t nu
       ((uintptr_t)k_norm_weight & 15))
     return fail(AIA_ERR_INVALID, "aia_rope_qk: tensors must be 16-byte aligned with token strides a "
                 "multiple of 8 that hold a token's heads");
+  // A row is read and written by the same lanes, so the qkv rows themselves may
+  // be the outputs; any other overlap would be read after it was written.
+  const int64_t nq = (int64_t)num_q_heads * head_dim, nk = (int64_t)num_kv_heads * head_dim;
+  const Rows in{qkv, num_tokens > 1 ? std::min(qkv_token_stride, nq + 2 * nk) : nq + 2 * nk, qkv_token_stride};
+  const Rows qo{q_out, nq, q_out_token_stride}, ko{k_out, nk, k_out_token_stride};
+  auto in_place = [&](const Rows& o, int64_t col) {
+    return o.at == static_cast<const uint16_t*>(qkv) + col && (num_tokens == 1 || o.stride == qkv_token_stride);
+  };
+  if ((!in_place(qo, 0) && share_memory(qo, in, num_tokens)) ||
+      (!in_place(ko, nq) && share_memory(ko, in, num_tokens)) || share_memory(qo, ko, num_tokens))
+    return fail(AIA_ERR_INVALID, "aia_rope_qk: the outputs overlap the qkv rows or each other (in place: q_out = "
+                "qkv, k_out = qkv + Hq * D, with its token stride)");
   Args a;
   a.qkv = static_cast<const uint16_t*>(qkv); a.ts = qkv_token_stride;
   a.hq = num_q_heads; a.hkv = num_kv_heads; a.rot = rotary_dim;

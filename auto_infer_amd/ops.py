@@ -220,7 +220,8 @@ def rope_qk(qkv, num_q_heads, num_kv_heads, positions, rope, q_norm_weight=None,
 
     ``positions`` (T,) int64, any values; ``rope`` a ``RotaryEmbedding`` of the
     same head_dim.  In place by default; ``out`` = (q_out, k_out), tensors (T,
-    Hq, D) and (T, Hkv, D) that do not overlap ``qkv``, leaves ``qkv`` as it is.
+    Hq, D) and (T, Hkv, D) that do not overlap ``qkv`` or each other (refused), leaves
+    ``qkv`` as it is.
     Returns the rotated (q, k) and the V view, (T, heads, D) each.  Unlike
     ``qk_norm_rope`` (cos/sin rows, bf16 roundings of the separate ops) it
     computes the angles itself and rounds once."""
@@ -246,6 +247,8 @@ def rope_qk(qkv, num_q_heads, num_kv_heads, positions, rope, q_norm_weight=None,
             if t.numel() != D or not t.is_contiguous():
                 raise ValueError(f"{name} must be {D} contiguous values")
     ts = qkv.stride(0) if T > 1 else width
+    if ts < width:
+        raise ValueError("qkv rows overlap")
     # (T, heads, D) views of the packed rows
     v = qkv.as_strided((T, num_kv_heads, D), (ts, D, 1), qkv.storage_offset() + nq + nk)
     if out is None:

@@ -382,8 +382,9 @@ int aia_qk_norm_rope(void* qkv, int64_t qkv_token_stride, int32_t num_tokens,
  * dims i and i + rotary_dim / 2, or with interleaved dims 2 i and 2 i + 1; dims
  * from rotary_dim on pass through.  All arithmetic is fp32 with one rounding.
  * q_out (T, Hq, D) / k_out (T, Hkv, D): rows with token strides; the qkv rows
- * themselves (q_out = qkv, k_out = qkv + Hq * D) for in place, otherwise not
- * overlapping them.  head_dim 128 or 64, rotary_dim a multiple of 16
+ * themselves (q_out = qkv, k_out = qkv + Hq * D) for in place; any other overlap
+ * with them or of the two is refused (AIA_ERR_INVALID; rows of one token stride
+ * may interleave).  head_dim 128 or 64, rotary_dim a multiple of 16
  * (AIA_ERR_UNSUPPORTED otherwise). */
 int aia_rope_qk(const void* qkv, int64_t qkv_token_stride, int32_t num_tokens,
                 int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
