@@ -1779,7 +1779,7 @@ __device__ __forceinline__ void mla_segment(const MlaArgs& a, const int* rec, in
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
     lsum[r] = aia::group4_sum(lsum[r]);
-    if (lsum[r] == 0.f) clear_row(o[r]);
+    if (lim_base < 0 && lim[r] < 0) clear_row(o[r]);
   }
   // balanced plans give the range's number within the segment and the
   // segment's range count in its record; otherwise ranges are tpw tiles
