@@ -494,7 +494,10 @@ def write_kv_fp8(key, value, key_cache, value_cache, key_scale, value_scale, slo
     first slot is written starts anew (its other slots' contents are lost
     until they are written, which a paged cache does in order); in any other
     block the scale grows where the new rows need it and the block's other
-    rows are rescaled.  Values that are not finite become NaN.  ``value``, its
+    rows are rescaled; it stays grown when those rows are overwritten (rejected
+    drafts), which costs the block's small values precision until it starts anew.
+    Values that are not finite become NaN, magnitudes from 1.9375 * 2^127 on are
+    read as infinities.  ``value``, its
     cache and its scale may be None.  Slots outside the cache are skipped; of
     tokens with the same slot the last one stays."""
     _check_device_tensor(key, "key", _BF16)
@@ -742,7 +745,7 @@ def paged_attention_gqa(query, key_cache, value_cache, plan, scale, out=None, fl
     ``value_scale`` (see ``write_kv_fp8``, which also writes new rows: ``key_new``
     and the NZ layout are for bf16 caches).
     Modified scores, with query position i and key position j: ``softcap`` > 0
-    makes them ``softcap * tanh(scale * q.k / softcap)``; ``alibi_slopes`` (Hq,)
+    (below 1e38) makes them ``softcap * tanh(scale * q.k / softcap)``; ``alibi_slopes`` (Hq,)
     float32 subtracts ``slope * |i - j|``; a plan with ``prefix_lens`` lets all
     rows of a request see its first keys.  Rows that see no key give zeros.
     """

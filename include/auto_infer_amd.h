@@ -76,8 +76,11 @@ int aia_kv_write_nz(const void* key, int64_t key_token_stride, const void* value
  * block whose first slot is written starts anew with the scale need: its other
  * slots' contents are lost until they are written.  Any other block gets
  * max(old, need), and where that grew its other slots are rescaled (to
- * nearest even, exact above e4m3's subnormal range).  Values that are not
- * finite are stored as NaN.  Of tokens with the same slot the last one stays.
+ * nearest even, exact above e4m3's subnormal range).  A scale never shrinks but
+ * by writing the first slot: one that grew for rows which are overwritten later
+ * (rejected drafts) stays.  Values that are not finite are stored as NaN;
+ * magnitudes from 1.9375 * 2^127 on round to 2^128 and are read as infinities.
+ * Of tokens with the same slot the last one stays.
  * key / value: (num_tokens, num_kv_heads * head_dim) bf16 rows with token
  * strides (value may be NULL, with value_cache and value_scale NULL).  Slots < 0
  * or >= num_slots are skipped.  head_dim 128 or 64, block_size at most 8192
