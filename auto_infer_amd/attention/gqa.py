@@ -20,7 +20,7 @@ power-of-two scale per block and head, ``softcap`` / ``alibi_slopes`` modify the
 scores, ``rope`` (an ``ops.RotaryEmbedding``) turns Q and K from
 ``ctx.positions`` instead of ``ctx.cos`` / ``ctx.sin`` (``rope=False``: a model
 without rotary positions, Q and K stay as they are), and a context with
-``aia_prefix_lens`` (device int32, one per request) lets all rows of a request
+``aia_prefix_lens`` (one per request; a host list or device int32) lets all rows of a request
 see its first keys.
 """
 import torch
