@@ -115,8 +115,10 @@ def draw(rng):
         groups = rng.choice([1, 1, 2, max(1, rows // 7)])
         shi = min(shi, 100000 // groups)
         lo = min(_log_int(rng, 1, 1000), 60000 // rows)
-        kw.update(rows=rows, width=rng.choice([1, 1, 1, 2, 4]), lo=lo, hi=_log_int(rng, lo, 2 * lo + 1),
-                  groups=groups, shared_hi=shi, shared_lo=max(1, shi // rng.choice([1, 1, 3])))
+        width = rng.choice([1, 1, 1, 2, 4])
+        shi = min(shi, int(1.3e11 / (rows * width * hq * d * 4)))
+        kw.update(rows=rows, width=width, lo=lo, hi=_log_int(rng, lo, 2 * lo + 1), groups=groups,
+                  shared_hi=shi, shared_lo=max(1, shi // rng.choice([1, 1, 3])))
     else:
         kw.update(select=rng.choice([4, 16, 32, 64, 64, 100]), sink=rng.choice([0, 1, 1]),
                   local=rng.choice([1, 2, 2]))
