@@ -1,0 +1,864 @@
+// Sparse attention over cache blocks that a cheap score selects for each query
+// token and KV head: the step's plan, 8-bit bounds of each block's keys, the
+// selection, and the attention over what was selected.
+//
+// Bounds.  For a block and KV head, hi[d] and lo[d] are the largest and the smallest
+// k[d] of the keys that it holds, so q.k <= sum_d max(q[d] hi[d], q[d] lo[d])
+// = sum_d q+[d] hi[d] + q-[d] nlo[d] with q+ = max(q, 0), q- = max(-q, 0), nlo = -lo.
+// Both are kept as whole numbers times a power of two 2^e of their block and head,
+// rounded up, e the least >= -100 with |k| <= 127 * 2^e: half the bytes of one bf16
+// key per block.  The query is rounded to whole numbers -127 .. 127 times a power of
+// two of its token and KV head, so a score, summed over the group's heads, is a
+// whole number times two powers of two: the same bits in any order of summation, and
+// a selection that does not depend on how the work is cut.
+#include <algorithm>
+
+#include "wave_attention.h"
+
+namespace {
+
+constexpr int kMinExp = -100;
+constexpr int kSparseThreads = 256;
+constexpr int kMaxSelected = 1024;
+constexpr int kHdrInts = 64;
+constexpr int64_t kScoreFloats = 1ll << 26;   // scores held at once
+
+struct SparseLayout {
+  int64_t hdr, tok, touched, scores, part_o, part_ml, total;
+  int32_t touched_cap, score_tokens, splits, hblocks;
+};
+
+// Work-groups that share a (token, KV head)'s keys: about four per compute unit in
+// all, each of 256 keys or more.
+int sparse_splits(int64_t items, int64_t keys) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(1024 / std::max<int64_t>(1, items), keys / 256));
+}
+
+SparseLayout sparse_layout(int32_t batch, int32_t tokens, int32_t hq, int32_t hkv, int32_t d, int32_t bs,
+                           int32_t width, int32_t selected) {
+  SparseLayout L;
+  auto up = [](int64_t x) { return (x + 255) & ~255ll; };
+  const int32_t group = hq / hkv;
+  L.hblocks = (group + kRows - 1) / kRows;
+  L.touched_cap = (int32_t)std::min<int64_t>(tokens, tokens / bs + 2ll * batch);
+  L.score_tokens = (int32_t)std::max<int64_t>(1, std::min<int64_t>(tokens, kScoreFloats / ((int64_t)hkv * std::max(1, width))));
+  L.splits = sparse_splits((int64_t)tokens * hkv * L.hblocks, (int64_t)std::min(selected, width) * bs);
+  L.hdr = 0;
+  L.tok = up(kHdrInts * 4);
+  L.touched = L.tok + up(16ll * tokens);
+  L.scores = L.touched + up(16ll * L.touched_cap);
+  L.part_o = L.scores + up(4ll * L.score_tokens * hkv * width);
+  const int64_t rows = L.splits > 1 ? (int64_t)L.splits * tokens * hkv * L.hblocks * kRows : 0;
+  L.part_ml = L.part_o + up(4 * rows * d);
+  L.total = L.part_ml + up(8 * rows);
+  return L;
+}
+
+// ------------------------------------------------------------------ plan
+
+struct PlanArgs {
+  const int32_t* cu;
+  const int32_t* lk;
+  const int32_t* bt;
+  int64_t bt_stride;
+  int32_t batch, tokens, bs, width;
+  int32_t* hdr;              // {blocks written to by the step}
+  int4* tok;                 // {request or -1, position, visible blocks, 0}
+  int4* touched;             // {block id, keys that it holds, 0, 0}
+  int32_t touched_cap;
+};
+
+constexpr int kPlanT = 1024;
+
+// Every work-group counts the blocks that each request's new tokens fall into (and
+// those of the requests before it), then places its own kPlanT tokens.
+__global__ __launch_bounds__(kPlanT) void sparse_plan_kernel(PlanArgs a) {
+  extern __shared__ int lds[];               // cu (batch + 1), first touched entry (batch)
+  int* cu = lds;
+  int* first = lds + a.batch + 1;
+  __shared__ int wave_sum[kPlanT / 64], carry;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  if (tid == 0) carry = 0;
+  for (int b = tid; b <= a.batch; b += kPlanT) cu[b] = a.cu[b];
+  __syncthreads();
+  for (int b0 = 0; b0 < a.batch; b0 += kPlanT) {
+    const int b = b0 + tid;
+    int n = 0;
+    if (b < a.batch) {
+      const int lq = cu[b + 1] - cu[b], lk = a.lk[b];
+      const int from = max(0, lk - lq);
+      if (lq > 0 && lk > 0) n = (lk - 1) / a.bs - from / a.bs + 1;
+    }
+    int sum = n;                             // inclusive scan of the wave
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int x = __shfl_up(sum, d);
+      if (lane >= d) sum += x;
+    }
+    if (lane == 63) wave_sum[wid] = sum;
+    __syncthreads();
+    int before = carry;
+    for (int w = 0; w < wid; ++w) before += wave_sum[w];
+    if (b < a.batch) first[b] = before + sum - n;
+    __syncthreads();
+    if (tid == kPlanT - 1) carry = before + sum;
+    __syncthreads();
+  }
+  if (blockIdx.x == 0 && tid == 0) a.hdr[0] = min(carry, a.touched_cap);
+  const int t = blockIdx.x * kPlanT + tid;
+  if (t >= a.tokens) return;
+  int lo = 0, hi = a.batch;                  // the last request that begins at or before t
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= t) lo = mid; else hi = mid;
+  }
+  const int b = lo;
+  int4 r = make_int4(-1, -1, 0, 0);
+  if (a.batch > 0 && t >= cu[b] && t < cu[b + 1]) {
+    const int lk = a.lk[b], from = lk - (cu[b + 1] - cu[b]), pos = from + t - cu[b];
+    r.x = b;
+    r.y = pos;
+    if (pos >= 0) {
+      const int blk = pos / a.bs;
+      r.z = min(blk + 1, a.width);
+      const int at = first[b] + blk - max(0, from) / a.bs;
+      if ((pos == max(0, from) || pos % a.bs == 0) && blk < a.width && at >= 0 && at < a.touched_cap)
+        a.touched[at] = make_int4(a.bt[(int64_t)b * a.bt_stride + blk], min(a.bs, lk - blk * a.bs), 0, 0);
+      else if ((pos == max(0, from) || pos % a.bs == 0) && at >= 0 && at < a.touched_cap)
+        a.touched[at] = make_int4(-1, 0, 0, 0);     // (behind the table)
+    }
+  }
+  a.tok[t] = r;
+}
+
+// ------------------------------------------------------------------ bounds
+
+struct SummaryArgs {
+  const uint16_t* kc;
+  const uint8_t* ks;
+  int32_t hkv, bs, nb;
+  const int32_t* hdr;
+  const int4* touched;
+  int8_t* bounds;            // (num_blocks, hkv, 2, D): hi, nlo
+  uint8_t* scale;            // (num_blocks, hkv)
+};
+
+__device__ __forceinline__ int bound_of(float x, float f) {      // rounded up; a positive one is not lost
+  const float y = __builtin_ceilf(x * f);
+  return (int)(x > 0.f ? fmaxf(y, 1.f) : y);
+}
+
+// The least e >= -100 with amax <= 127 * 2^e, for a bf16 value's bits: 127 = 1.984375
+// * 2^6, and bf16 has one significand above it.
+__device__ __forceinline__ int bound_exp(uint32_t amax) {
+  const int e = (int)(amax >> 7) - 127 - 6 + ((amax & 0x7fu) > 0x7eu ? 1 : 0);
+  return max(amax < 0x80u ? kMinExp : e, kMinExp);
+}
+
+// WPB waves take a (block, KV head): 64 / (D / 8) rows a pass, a lane 8 dims of one.
+// Blocks of 64 keys and more are cut over the work-group's four waves: a decode step
+// has few blocks, and the rows of one are loaded at once.
+template <int D, bool F8, int WPB>
+__global__ __launch_bounds__(kSparseThreads) void summarize_kernel(SummaryArgs a) {
+  constexpr int CH = D / 8, RPW = 64 / CH, DEEP = 8;
+  __shared__ float part[WPB > 1 ? 4 : 1][2][D];
+  __shared__ uint32_t part_bad[WPB > 1 ? 4 : 1][CH];
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int c = lane % CH, r = lane / CH;
+  constexpr int HPW = 4 / WPB;               // heads of a work-group
+  const int h = blockIdx.y * HPW + wid / WPB, sub = wid % WPB;
+  if ((int)blockIdx.x >= a.hdr[0]) return;
+  const int4 t = a.touched[blockIdx.x];
+  if (t.x < 0 || t.x >= a.nb) return;
+  const int held = min(max(t.y, 0), a.bs);
+  const bool live = h < a.hkv;
+  if (WPB == 1 && !live) return;
+  const int64_t row = (int64_t)a.hkv * D;
+  const int64_t at = (int64_t)t.x * a.bs * row + (int64_t)h * D + 8 * c;
+  float hi[8], nlo[8];
+  uint32_t bad = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) hi[i] = nlo[i] = -INFINITY;
+  const float f8 = F8 && live ? __uint_as_float((uint32_t)a.ks[(int64_t)t.x * a.hkv + h] << 23) : 0.f;
+  const int rows = live ? held : 0;
+  for (int j0 = sub * RPW + r; j0 < rows; j0 += DEEP * WPB * RPW) {
+    uint4 w[DEEP];
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u) {
+      const int j = min(j0 + u * WPB * RPW, rows - 1);         // (the last row again)
+      if constexpr (F8) {
+        const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(a.kc) + at + j * row);
+        const uint2 lo = fp8x4_to_bf16(x.x, f8), up = fp8x4_to_bf16(x.y, f8);
+        w[u] = make_uint4(lo.x, lo.y, up.x, up.y);
+      } else {
+        w[u] = *reinterpret_cast<const uint4*>(a.kc + at + j * row);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < DEEP; ++u) {
+      const uint32_t p[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = i & 1 ? aia::bf16_hi(p[i >> 1]) : aia::bf16_lo(p[i >> 1]);
+        const bool ok = __builtin_fabsf(x) < INFINITY;
+        if (!ok) bad |= 1u << i;
+        hi[i] = fmaxf(hi[i], ok ? x : -INFINITY);
+        nlo[i] = fmaxf(nlo[i], ok ? -x : -INFINITY);
+      }
+    }
+  }
+#pragma unroll
+  for (int d = CH; d < 64; d <<= 1) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], d));
+      nlo[i] = fmaxf(nlo[i], __shfl_xor(nlo[i], d));
+    }
+    bad |= (uint32_t)__shfl_xor((int)bad, d);
+  }
+  if constexpr (WPB > 1) {
+    if (r == 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { part[wid][0][8 * c + i] = hi[i]; part[wid][1][8 * c + i] = nlo[i]; }
+      part_bad[wid][c] = bad;
+    }
+    __syncthreads();
+    if (sub != 0 || !live) return;
+#pragma unroll
+    for (int w = 1; w < WPB; ++w) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        hi[i] = fmaxf(hi[i], part[wid + w][0][8 * c + i]);
+        nlo[i] = fmaxf(nlo[i], part[wid + w][1][8 * c + i]);
+      }
+      bad |= part_bad[wid + w][c];
+    }
+  }
+  float most = 0.f;                          // (a dim without a finite value has -inf in both)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = fmaxf(most, fmaxf(hi[i], nlo[i]));
+#pragma unroll
+  for (int d = 1; d < CH; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+  const int e = bound_exp(__float_as_uint(most) >> 16);
+  const float f = __builtin_ldexpf(1.f, -e);
+  if (r < 2) {
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int x = bad >> i & 1 ? 127 : bound_of(r ? nlo[i] : hi[i], f);
+      w[i >> 2] |= (uint32_t)(x & 0xff) << (8 * (i & 3));
+    }
+    *reinterpret_cast<uint2*>(a.bounds + (((int64_t)t.x * a.hkv + h) * 2 + r) * D + 8 * c) = make_uint2(w[0], w[1]);
+    if (lane == 0) a.scale[(int64_t)t.x * a.hkv + h] = (uint8_t)(e + 127);
+  }
+}
+
+// ------------------------------------------------------------------ scores
+
+typedef int int4v_t __attribute__((ext_vector_type(4)));
+
+struct ScoreKernelArgs {
+  const uint16_t* q;
+  int64_t q_ts, q_hs;
+  const int8_t* bounds;
+  const uint8_t* scale;
+  const int32_t* bt;
+  int64_t bt_stride;
+  const int4* tok;
+  float* scores;             // (tokens of this launch, hkv, width)
+  int32_t t0, t1, hkv, group, nb, width, chunk, per;   // tokens [t0, t1), blocks per work-group, tokens per tile
+};
+
+// One work-group: the 16 query rows of up to `per` tokens of one KV head (per token
+// `lanes` rows, the group's heads padded to a power of two; groups of more than 16
+// heads take 16 at a time) against `chunk` blocks.  S = Q B^T on v_mfma_i32_16x16x64_i8:
+// lane (row or block n, group g) holds bytes 64 j + 16 g .. of [q+ (D), q- (D)] and of
+// [hi, nlo]; the four accumulators are rows 4 g .. 4 g + 3 of block n.  Tokens of
+// several requests in one tile are taken one request at a time.
+template <int D>
+__global__ __launch_bounds__(kSparseThreads) void score_kernel(ScoreKernelArgs a) {
+  constexpr int KS = 2 * D / 64;             // MFMA steps
+  extern __shared__ uint4 qfrag[];           // [head block][step][lane]
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int n = lane & 15, g = lane >> 4;
+  const int kvh = blockIdx.y;
+  int lanes = 1;
+  while (lanes < a.group && lanes < 16) lanes <<= 1;
+  const int hblocks = (a.group + 15) / 16;
+  const int tb = a.t0 + blockIdx.x * a.per;
+  const int tokens = min(a.per, a.t1 - tb);
+  // rows of the first head block: token n / lanes, head n % lanes
+  const int tn = n / lanes, hn = n - tn * lanes;
+  int done = 0;
+  while (done < tokens) {
+    const int4 lead = a.tok[tb + done];
+    int same = done + 1, vis = lead.z;       // tokens [done, same) of one request
+    while (same < tokens) {
+      const int4 x = a.tok[tb + same];
+      if (x.x != lead.x) break;
+      vis = max(vis, x.z);
+      ++same;
+    }
+    const int from = done;
+    done = same;
+    const int c0 = blockIdx.z * a.chunk, c1 = min(vis, c0 + a.chunk);
+    if (lead.x < 0 || c0 >= c1) continue;
+    __syncthreads();
+    // largest finite |q| of each token's heads
+    uint32_t amax = 0;
+    for (int hb = 0; hb < hblocks; ++hb) {
+      const int head = hn + 16 * hb;
+      if (tn >= from && tn < same && head < a.group) {
+        const uint16_t* qp = a.q + (int64_t)(tb + tn) * a.q_ts + (int64_t)(kvh * a.group + head) * a.q_hs;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          const uint4 w = reinterpret_cast<const uint4*>(qp)[4 * j + g];
+          const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t lo = p[i] & 0x7fffu, up = (p[i] >> 16) & 0x7fffu;
+            amax = max(amax, lo < 0x7f80u ? lo : 0u);
+            amax = max(amax, up < 0x7f80u ? up : 0u);
+          }
+        }
+      }
+    }
+    for (int d = 1; d < lanes; d <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, d));
+    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
+    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
+    const float f = __builtin_ldexpf(1.f, -bound_exp(amax));
+    for (int hb = wid; hb < hblocks; hb += kSparseThreads / 64) {
+      const int head = hn + 16 * hb;
+      const bool live = tn >= from && tn < same && head < a.group;
+      const uint16_t* qp = a.q + (int64_t)(tb + tn) * a.q_ts + (int64_t)(kvh * a.group + head) * a.q_hs;
+#pragma unroll
+      for (int j = 0; j < KS / 2; ++j) {
+        uint32_t pos[4] = {0, 0, 0, 0}, neg[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (live) w = reinterpret_cast<const uint4*>(qp + 64 * j + 16 * g)[half];
+          const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float x = i & 1 ? aia::bf16_hi(p[i >> 1]) : aia::bf16_lo(p[i >> 1]);
+            const int v = __builtin_fabsf(x) < INFINITY ? (int)__builtin_rintf(x * f) : 0;
+            pos[2 * half + (i >> 2)] |= (uint32_t)max(v, 0) << (8 * (i & 3));
+            neg[2 * half + (i >> 2)] |= (uint32_t)max(-v, 0) << (8 * (i & 3));
+          }
+        }
+        qfrag[(hb * KS + j) * 64 + lane] = make_uint4(pos[0], pos[1], pos[2], pos[3]);
+        qfrag[(hb * KS + KS / 2 + j) * 64 + lane] = make_uint4(neg[0], neg[1], neg[2], neg[3]);
+      }
+    }
+    __syncthreads();
+    const int32_t* btrow = a.bt + (int64_t)lead.x * a.bt_stride;
+    auto step = [&](int hb, int j) { return __builtin_bit_cast(int4v_t, as_u4(qfrag[(hb * KS + j) * 64 + lane])); };
+    int4v_t qf[KS];
+#pragma unroll
+    for (int j = 0; j < KS; ++j) qf[j] = step(0, j);
+    for (int b0 = c0 + 64 * wid; b0 < c1; b0 += kSparseThreads) {
+      const int id = b0 + lane < c1 ? min(max(btrow[b0 + lane], 0), a.nb - 1) : 0;
+      const int ebyte = a.scale[(int64_t)id * a.hkv + kvh];
+      uint4 bf[4][KS];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int blk = __shfl(id, 16 * s + n);
+        const uint4* bp = reinterpret_cast<const uint4*>(a.bounds + ((int64_t)blk * a.hkv + kvh) * 2 * D) + g;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) bf[s][j] = bp[4 * j];
+      }
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        int4v_t acc = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < KS; ++j)
+          acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf[j], __builtin_bit_cast(int4v_t, as_u4(bf[s][j])), acc, 0, 0, 0);
+        for (int hb = 1; hb < hblocks; ++hb)
+#pragma unroll
+          for (int j = 0; j < KS; ++j)
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(step(hb, j), __builtin_bit_cast(int4v_t, as_u4(bf[s][j])), acc, 0, 0, 0);
+        // sums over a token's rows: `lanes` of the rows 4 g + v
+        if (lanes > 1) { acc[0] += acc[1]; acc[2] += acc[3]; }
+        if (lanes > 2) acc[0] += acc[2];
+        if (lanes > 4) acc[0] += __shfl_xor(acc[0], 16);
+        if (lanes > 8) acc[0] += __shfl_xor(acc[0], 32);
+        const int blk = b0 + 16 * s + n;
+        const int eb = __shfl(ebyte, 16 * s + n) - 127;
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int row = 4 * g + v;
+          if (row % lanes) continue;
+          const int t = row / lanes;
+          if (t < from || t >= same || blk >= c1) continue;
+          const int sum = v == 0 ? acc[0] : v == 1 ? acc[1] : v == 2 ? acc[2] : acc[3];
+          a.scores[((int64_t)(tb + t - a.t0) * a.hkv + kvh) * a.width + blk] = __builtin_ldexpf((float)sum, eb);
+        }
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ selection
+
+struct SelectArgs {
+  const float* scores;
+  const int4* tok;
+  int32_t* out;
+  int64_t out_ts, out_hs;
+  int32_t t0, hkv, width, selected, sink, local;
+};
+
+constexpr int kSelThreads = 512, kSelWaves = kSelThreads / 64;
+constexpr int kDigits = 2048;
+
+// A score's order as an unsigned key, 0xffffffff for blocks that are always kept.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// One work-group per (token, KV head): the key of the `selected`-th largest score,
+// 11 bits at a time by counting, then the blocks above it and the first of those at it,
+// in order.
+__global__ __launch_bounds__(kSelThreads) void select_kernel(SelectArgs a) {
+  __shared__ int hist[kDigits];
+  __shared__ int wave_a[kSelWaves], wave_b[kSelWaves], found[2];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int t = a.t0 + blockIdx.x, kvh = blockIdx.y;
+  const int n = a.tok[t].z;
+  int32_t* out = a.out + (int64_t)t * a.out_ts + (int64_t)kvh * a.out_hs;
+  if (n <= a.selected) {
+    for (int i = tid; i < a.selected; i += kSelThreads) out[i] = i < n ? i : -1;
+    return;
+  }
+  const float* sc = a.scores + ((int64_t)blockIdx.x * a.hkv + kvh) * a.width;
+  auto key_at = [&](int i) -> uint32_t {
+    if (i < a.sink || i >= n - a.local) return 0xffffffffu;
+    return min(order_key(sc[i]), 0xfffffffeu);
+  };
+  uint32_t prefix = 0;                       // the digits found so far
+  int need = a.selected;                     // blocks to take among those of the prefix
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    for (int i = tid; i < kDigits; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kSelThreads) {
+      const uint32_t k = key_at(i);
+      if (pass == 0 || k >> (shift + bits) == prefix) atomicAdd(&hist[k >> shift & ((1 << bits) - 1)], 1);
+    }
+    __syncthreads();
+    // digits from the largest down: thread tid has kDigits / kSelThreads of them
+    constexpr int PER = kDigits / kSelThreads;
+    const int top = kDigits - 1 - PER * tid;
+    int c[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) { c[i] = hist[top - i]; sum += c[i]; }
+    int upto = sum;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int x = __shfl_up(upto, d);
+      if (lane >= d) upto += x;
+    }
+    if (lane == 63) wave_a[wid] = upto;
+    __syncthreads();
+    for (int w = 0; w < wid; ++w) upto += wave_a[w];
+    int above = upto - sum;
+    if (above < need && upto >= need) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        if (above < need && above + c[i] >= need) { found[0] = top - i; found[1] = need - above; }
+        above += c[i];
+      }
+    }
+    __syncthreads();
+    prefix = prefix << bits | (uint32_t)found[0];
+    need = found[1];
+    __syncthreads();
+  }
+  // blocks in order: a wave takes a run of them
+  const int per = (n + kSelWaves - 1) / kSelWaves, i0 = wid * per, i1 = min(n, i0 + per);
+  int more = 0, ties = 0;
+  for (int i = i0; i < i1; i += 64) {
+    const uint32_t k = i + lane < i1 ? key_at(i + lane) : 0;
+    more += __popcll(__ballot(i + lane < i1 && k > prefix));
+    ties += __popcll(__ballot(i + lane < i1 && k == prefix));
+  }
+  if (lane == 0) { wave_a[wid] = more; wave_b[wid] = ties; }
+  __syncthreads();
+  int at = 0, tied = 0;                      // taken above and equals before this wave's run
+  for (int w = 0; w < wid; ++w) { at += wave_a[w]; tied += wave_b[w]; }
+  const uint64_t below = (1ull << lane) - 1;
+  for (int i = i0; i < i1; i += 64) {
+    const bool in = i + lane < i1;
+    const uint32_t k = in ? key_at(i + lane) : 0;
+    const bool up = in && k > prefix, eq = in && k == prefix;
+    const uint64_t mu = __ballot(up), me = __ballot(eq);
+    const int ub = at + __popcll(mu & below), eb = tied + __popcll(me & below);
+    if (up || (eq && eb < need)) out[ub + min(eb, need)] = i + lane;
+    at += __popcll(mu);
+    tied += __popcll(me);
+  }
+}
+
+// ------------------------------------------------------------------ attention
+
+struct SparseArgs {
+  CacheArgs c;
+  const uint16_t* q;
+  int64_t q_ts, q_hs;
+  const int32_t* bt;
+  int64_t bt_stride;
+  const int4* tok;
+  const int32_t* sel;
+  int64_t sel_ts, sel_hs;
+  int32_t selected, splits, tokens;
+  uint16_t* out;
+  int64_t o_ts, o_hs;
+  float* part_o;             // (token, KV head, head block, split): 16 rows of D
+  float2* part_ml;
+};
+
+constexpr int kSpWaves = 4;
+
+// One work-group: a token, a KV head, up to 16 of its query heads and one of the
+// splits of the selected keys, four waves with a run of tiles each.  The list is
+// compacted first: entries that do not exceed all before them or that the token does
+// not see drop out, so all keys but the own block's behind the token's position are
+// seen, and only the last tile needs a limit.
+template <int D, bool F8>
+__global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a) {
+  constexpr int DT = D / 16;
+  constexpr int kStage = (F8 ? 2 : 1) * kTile * kVStride;      // a wave's V tiles
+  constexpr int kJoinBytes = kSpWaves * DT * 64 * 16, kStageBytes = kSpWaves * kStage * 2;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kJoinBytes > kStageBytes ? kJoinBytes : kStageBytes];
+  __shared__ int list[kMaxSelected];
+  __shared__ float wave_m[kSpWaves][kRows], wave_l[kSpWaves][kRows];
+  auto* join = reinterpret_cast<float4_t(*)[DT][64]>(lds);     // the waves' results, after their last V tile
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int item = blockIdx.x / a.splits, split = blockIdx.x - item * a.splits;
+  const int hblocks = (a.c.group + kRows - 1) / kRows;
+  const int hb = item % hblocks, kvh = item / hblocks % a.c.hkv, t = item / hblocks / a.c.hkv;
+  const int4 tk = a.tok[t];
+  const int head = hb * kRows + n;
+  const bool rv = head < a.c.group;
+  const uint16_t* qp = rv ? a.q + (int64_t)t * a.q_ts + (int64_t)(kvh * a.c.group + head) * a.q_hs : nullptr;
+  uint4 qf[1][D / 32];
+  load_q<D, F8>(qp, g, qf[0]);
+  // every wave builds the same list
+  const int32_t* sel = a.sel + (int64_t)t * a.sel_ts + (int64_t)kvh * a.sel_hs;
+  const int32_t* btrow = a.bt + (int64_t)max(tk.x, 0) * a.bt_stride;
+  int count = 0, most = -1;
+  bool own = false;                          // the token's own block is among them: the last one then
+  for (int i = 0; i < a.selected; i += 64) {
+    const int e = i + lane < a.selected ? sel[i + lane] : -1;
+    int upto = e;                            // the largest entry up to this lane's
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int x = __shfl_up(upto, d);
+      if (lane >= d) upto = max(upto, x);
+    }
+    const int prev = __shfl_up(upto, 1);
+    const int before = lane ? max(most, prev) : most;
+    const bool ok = e >= 0 && e < tk.z && e > before;
+    const uint64_t m = __ballot(ok);
+    if (ok) list[count + __popcll(m & ((1ull << lane) - 1))] = btrow[e];
+    count += __popcll(m);
+    own |= __any(ok && e == tk.y / a.c.bs) != 0;
+    most = max(most, __shfl(upto, 63));
+  }
+  __syncthreads();
+  const int keys = count * a.c.bs - (own ? a.c.bs - 1 - tk.y % a.c.bs : 0);
+  const int tiles = (keys + kTile - 1) / kTile;
+  const int parts = a.splits * kSpWaves, p = split * kSpWaves + wid;
+  const int t0 = (int)((int64_t)tiles * p / parts), t1 = (int)((int64_t)tiles * (p + 1) / parts);
+  RowState<1, D> s;
+  s.clear();
+  const int p1 = min(keys, t1 * kTile);
+  const int lim[1] = {keys - 1};
+  attend<1, D, F8, false>(a.c, kvh, qf, lim, keys - 1, t0 * kTile, p1, count, [&](int i) { return list[i]; },
+                          reinterpret_cast<uint16_t*>(lds) + wid * kStage, lane, s);
+  s.finish();
+  __syncthreads();
+  if (g == 0) { wave_m[wid][n] = s.m[0]; wave_l[wid][n] = s.l[0]; }
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) join[wid][dt][lane] = s.o[0][dt];
+  __syncthreads();
+  float m = -INFINITY, l = 0.f, w[kSpWaves];
+#pragma unroll
+  for (int i = 0; i < kSpWaves; ++i) m = fmaxf(m, wave_m[i][n]);
+#pragma unroll
+  for (int i = 0; i < kSpWaves; ++i) {
+    // (a wave that saw no key; one that saw NaN alone has -inf and NaN)
+    w[i] = wave_m[i][n] == -INFINITY && wave_l[i][n] == 0.f ? 0.f : __builtin_amdgcn_exp2f(wave_m[i][n] - m);
+    l += w[i] * wave_l[i][n];
+  }
+  if (!rv) return;
+  const int64_t prow = (((int64_t)item * a.splits) + split) * kRows + n;
+  if (a.splits > 1 && wid == 0 && g == 0) a.part_ml[prow] = make_float2(m, l);
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : __builtin_nanf("");
+  uint16_t* op = a.out + (int64_t)t * a.o_ts + (int64_t)(kvh * a.c.group + head) * a.o_hs;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    if (dt % kSpWaves != wid) continue;      // a wave takes its share of the dims
+    float4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kSpWaves; ++i) o += join[i][dt][lane] * w[i];
+    if (a.splits > 1) {
+      *reinterpret_cast<float4_t*>(a.part_o + prow * D + 16 * dt + 4 * g) = o;
+    } else {
+      *reinterpret_cast<uint2*>(op + 16 * dt + 4 * g) =
+          make_uint2(aia::pack_bf16x2(o[0] * inv, o[1] * inv), aia::pack_bf16x2(o[2] * inv, o[3] * inv));
+    }
+  }
+}
+
+// The splits of each row, joined.
+template <int D>
+__global__ __launch_bounds__(kSparseThreads) void sparse_join_kernel(SparseArgs a) {
+  constexpr int LANES = D / 4;               // threads per row
+  const int hblocks = (a.c.group + kRows - 1) / kRows;
+  const int64_t row = (int64_t)blockIdx.x * (kSparseThreads / LANES) + threadIdx.x / LANES;
+  const int c = threadIdx.x % LANES;
+  const int hq = a.c.group * a.c.hkv;
+  if (row >= (int64_t)a.tokens * hq) return;
+  const int t = (int)(row / hq), head = (int)(row - (int64_t)t * hq);
+  const int kvh = head / a.c.group, hh = head - kvh * a.c.group;
+  const int64_t item = ((int64_t)t * a.c.hkv + kvh) * hblocks + hh / kRows;
+  const int64_t first = item * a.splits * kRows + hh % kRows;
+  float m = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[first + s * kRows].x);
+  float l = 0.f;
+  float4_t o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 ml = a.part_ml[first + s * kRows];
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;
+    const float w = __builtin_amdgcn_exp2f(ml.x - m);
+    l += w * ml.y;
+    o += *reinterpret_cast<const float4_t*>(a.part_o + (first + s * kRows) * D + 4 * c) * w;
+  }
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : __builtin_nanf("");
+  *reinterpret_cast<uint2*>(a.out + (int64_t)t * a.o_ts + (int64_t)head * a.o_hs + 4 * c) =
+      make_uint2(aia::pack_bf16x2(o[0] * inv, o[1] * inv), aia::pack_bf16x2(o[2] * inv, o[3] * inv));
+}
+
+// ------------------------------------------------------------------ checks
+
+int check_step(const char* what, int32_t batch, int32_t tokens, int32_t hq, int32_t hkv, int32_t d, int32_t bs,
+               int32_t width, int32_t selected) {
+  using namespace aia;
+  if (batch < 0 || tokens < 0 || hq <= 0 || hkv <= 0 || bs <= 0 || width <= 0 || hq % hkv)
+    return fail(AIA_ERR_INVALID, "%s: bad sizes (batch %d, tokens %d, heads %d / %d, block %d, table width %d)",
+                what, batch, tokens, hq, hkv, bs, width);
+  if (d != 128 && d != 64) return fail(AIA_ERR_UNSUPPORTED, "%s: head_dim %d (128 or 64)", what, d);
+  if (batch > kMaxBatch) return fail(AIA_ERR_UNSUPPORTED, "%s: %d requests (at most %d)", what, batch, kMaxBatch);
+  if (hkv > 65535) return fail(AIA_ERR_UNSUPPORTED, "%s: %d KV heads (at most 65535)", what, hkv);
+  if (hq / hkv > 256) return fail(AIA_ERR_UNSUPPORTED, "%s: %d query heads per KV head (at most 256)", what, hq / hkv);
+  if ((int64_t)bs * width > INT32_MAX)
+    return fail(AIA_ERR_UNSUPPORTED, "%s: contexts of 2^31 tokens and more", what);
+  if (selected <= 0 || selected > kMaxSelected)
+    return fail(AIA_ERR_UNSUPPORTED, "%s: %d selected blocks (1 to %d)", what, selected, kMaxSelected);
+  return AIA_OK;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+
+}  // namespace
+
+extern "C" int aia_sparse_workspace_bytes(int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                                          int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                          int32_t table_width, int32_t num_selected, int64_t* bytes) {
+  using namespace aia;
+  if (!bytes) return fail(AIA_ERR_INVALID, "aia_sparse_workspace_bytes: null pointer argument");
+  if (int rc = check_step("aia_sparse_workspace_bytes", batch, num_tokens, num_q_heads, num_kv_heads, head_dim,
+                          block_size, table_width, num_selected))
+    return rc;
+  *bytes = sparse_layout(batch, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size, table_width, num_selected).total;
+  return AIA_OK;
+}
+
+// What the entry points check of a step and its workspace; fills L.
+static int sparse_step(const char* what, int32_t batch, int32_t tokens, int32_t hq, int32_t hkv, int32_t d,
+                       int32_t bs, int32_t width, int32_t selected, const void* ws, int64_t ws_bytes,
+                       SparseLayout& L) {
+  using namespace aia;
+  if (int rc = check_step(what, batch, tokens, hq, hkv, d, bs, width, selected)) return rc;
+  if (!ws || ((uintptr_t)ws & 255u)) return fail(AIA_ERR_INVALID, "%s: workspace must be 256-byte aligned", what);
+  L = sparse_layout(batch, tokens, hq, hkv, d, bs, width, selected);
+  if (ws_bytes < L.total)
+    return fail(AIA_ERR_CAPACITY, "%s: workspace of %lld bytes, %lld needed", what, (long long)ws_bytes, (long long)L.total);
+  return AIA_OK;
+}
+
+extern "C" int aia_sparse_plan(const int32_t* cu_seqlens_q, const int32_t* seqlens_kv, const int32_t* block_table,
+                               int32_t block_table_stride, int32_t table_width, int32_t block_size, int32_t batch,
+                               int32_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                               int32_t num_selected, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace aia;
+  SparseLayout L;
+  if (int rc = sparse_step("aia_sparse_plan", batch, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size,
+                           table_width, num_selected, workspace, workspace_bytes, L))
+    return rc;
+  if (!cu_seqlens_q || (batch > 0 && (!seqlens_kv || !block_table)))
+    return fail(AIA_ERR_INVALID, "aia_sparse_plan: null pointer argument");
+  if (batch > 1 && block_table_stride < table_width)
+    return fail(AIA_ERR_INVALID, "aia_sparse_plan: table rows overlap");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  PlanArgs a;
+  a.cu = cu_seqlens_q; a.lk = seqlens_kv; a.bt = block_table; a.bt_stride = block_table_stride;
+  a.batch = batch; a.tokens = num_tokens; a.bs = block_size; a.width = table_width;
+  a.hdr = reinterpret_cast<int32_t*>(ws + L.hdr);
+  a.tok = reinterpret_cast<int4*>(ws + L.tok);
+  a.touched = reinterpret_cast<int4*>(ws + L.touched);
+  a.touched_cap = L.touched_cap;
+  const unsigned grid = std::max(1, (num_tokens + kPlanT - 1) / kPlanT);
+  const size_t lds = (size_t)(2 * batch + 1) * sizeof(int);
+  if (lds > 48 * 1024) {
+    if (int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(sparse_plan_kernel),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds),
+                           "aia_sparse_plan"))
+      return rc;
+  }
+  sparse_plan_kernel<<<grid, kPlanT, lds, (hipStream_t)stream>>>(a);
+  return check_hip(hipGetLastError(), "aia_sparse_plan launch");
+}
+
+extern "C" int aia_summarize_blocks(const void* key_cache, const void* key_scale, int32_t num_blocks,
+                                    void* bounds, void* bounds_scale, int32_t block_size, int32_t table_width,
+                                    int32_t batch, int32_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                                    int32_t head_dim, int32_t num_selected, const void* workspace,
+                                    int64_t workspace_bytes, void* stream) {
+  using namespace aia;
+  SparseLayout L;
+  if (int rc = sparse_step("aia_summarize_blocks", batch, num_tokens, num_q_heads, num_kv_heads, head_dim,
+                           block_size, table_width, num_selected, workspace, workspace_bytes, L))
+    return rc;
+  if (num_tokens == 0) return AIA_OK;
+  if (!key_cache || !bounds || !bounds_scale || num_blocks <= 0)
+    return fail(AIA_ERR_INVALID, "aia_summarize_blocks: null pointer argument or no blocks");
+  if (!aligned16(key_cache) || !aligned16(bounds))
+    return fail(AIA_ERR_INVALID, "aia_summarize_blocks: tensors must be 16-byte aligned");
+  const uint8_t* ws = static_cast<const uint8_t*>(workspace);
+  SummaryArgs a;
+  a.kc = static_cast<const uint16_t*>(key_cache); a.ks = static_cast<const uint8_t*>(key_scale);
+  a.hkv = num_kv_heads; a.bs = block_size; a.nb = num_blocks;
+  a.hdr = reinterpret_cast<const int32_t*>(ws + L.hdr);
+  a.touched = reinterpret_cast<const int4*>(ws + L.touched);
+  a.bounds = static_cast<int8_t*>(bounds); a.scale = static_cast<uint8_t*>(bounds_scale);
+  const bool cut = block_size >= 64;
+  const dim3 grid((unsigned)L.touched_cap, (unsigned)(cut ? num_kv_heads : (num_kv_heads + 3) / 4));
+  auto pick = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    return key_scale ? (cut ? summarize_kernel<D, true, 4> : summarize_kernel<D, true, 1>)
+                     : (cut ? summarize_kernel<D, false, 4> : summarize_kernel<D, false, 1>);
+  };
+  auto* kernel = head_dim == 128 ? pick(std::integral_constant<int, 128>{}) : pick(std::integral_constant<int, 64>{});
+  kernel<<<grid, kSparseThreads, 0, (hipStream_t)stream>>>(a);
+  return check_hip(hipGetLastError(), "aia_summarize_blocks launch");
+}
+
+extern "C" int aia_select_blocks(const void* query, int64_t q_token_stride, int64_t q_head_stride,
+                                 const void* bounds, const void* bounds_scale, int32_t num_blocks,
+                                 const int32_t* block_table, int32_t block_table_stride, int32_t table_width,
+                                 int32_t block_size, int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                                 int32_t num_kv_heads, int32_t head_dim, int32_t num_selected, int32_t sink,
+                                 int32_t local, int32_t* selected, int64_t sel_token_stride,
+                                 int64_t sel_head_stride, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace aia;
+  SparseLayout L;
+  if (int rc = sparse_step("aia_select_blocks", batch, num_tokens, num_q_heads, num_kv_heads, head_dim, block_size,
+                           table_width, num_selected, workspace, workspace_bytes, L))
+    return rc;
+  if (sink < 0 || local < 1 || (int64_t)sink + local > num_selected)
+    return fail(AIA_ERR_INVALID, "aia_select_blocks: sink %d and local %d do not fit %d selected blocks (local at least 1)",
+                sink, local, num_selected);
+  if (num_tokens == 0) return AIA_OK;
+  if (!query || !bounds || !bounds_scale || !block_table || !selected || num_blocks <= 0)
+    return fail(AIA_ERR_INVALID, "aia_select_blocks: null pointer argument or no blocks");
+  if (!aligned16(query) || !aligned16(bounds) || q_token_stride % 8 || q_head_stride % 8)
+    return fail(AIA_ERR_INVALID, "aia_select_blocks: tensors must be 16-byte aligned with strides a multiple of 8");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int group = num_q_heads / num_kv_heads;
+  int lanes = 1;
+  while (lanes < group && lanes < 16) lanes <<= 1;
+  ScoreKernelArgs a;
+  a.q = static_cast<const uint16_t*>(query); a.q_ts = q_token_stride; a.q_hs = q_head_stride;
+  a.bounds = static_cast<const int8_t*>(bounds); a.scale = static_cast<const uint8_t*>(bounds_scale);
+  a.bt = block_table; a.bt_stride = block_table_stride;
+  a.tok = reinterpret_cast<const int4*>(ws + L.tok);
+  a.scores = reinterpret_cast<float*>(ws + L.scores);
+  a.hkv = num_kv_heads; a.group = group; a.nb = num_blocks; a.width = table_width;
+  // tokens of a tile share their request's bounds: worth it where requests have several
+  a.per = num_tokens >= 4 * batch ? 16 / lanes : 1;
+  SelectArgs s;
+  s.scores = a.scores; s.tok = a.tok; s.out = selected; s.out_ts = sel_token_stride; s.out_hs = sel_head_stride;
+  s.hkv = num_kv_heads; s.width = table_width; s.selected = num_selected; s.sink = sink; s.local = local;
+  const size_t lds = (size_t)((group + 15) / 16) * (2 * head_dim / 64) * 64 * 16;
+  for (int t0 = 0; t0 < num_tokens; t0 += L.score_tokens) {
+    const int t1 = std::min(num_tokens, t0 + L.score_tokens);
+    a.t0 = t0; a.t1 = t1; s.t0 = t0;
+    const int tiles = (t1 - t0 + a.per - 1) / a.per;
+    // work-groups: about eight per compute unit, each of 256 blocks or more
+    const int64_t cuts = std::max<int64_t>(1, std::min<int64_t>(2048 / std::max<int64_t>(1, (int64_t)tiles * num_kv_heads), (table_width + 255) / 256));
+    a.chunk = (int)(((table_width + cuts - 1) / cuts + 255) / 256 * 256);
+    const dim3 grid((unsigned)tiles, (unsigned)num_kv_heads, (unsigned)((table_width + a.chunk - 1) / a.chunk));
+    (head_dim == 128 ? score_kernel<128> : score_kernel<64>)<<<grid, kSparseThreads, lds, (hipStream_t)stream>>>(a);
+    if (int rc = check_hip(hipGetLastError(), "aia_select_blocks: score launch")) return rc;
+    select_kernel<<<dim3((unsigned)(t1 - t0), (unsigned)num_kv_heads), kSelThreads, 0, (hipStream_t)stream>>>(s);
+    if (int rc = check_hip(hipGetLastError(), "aia_select_blocks: select launch")) return rc;
+  }
+  return AIA_OK;
+}
+
+extern "C" int aia_paged_attention_sparse(const void* query, int64_t q_token_stride, int64_t q_head_stride,
+                                          const void* key_cache, const void* value_cache, const void* key_scale,
+                                          const void* value_scale, int32_t num_blocks, const int32_t* block_table,
+                                          int32_t block_table_stride, int32_t table_width, int32_t block_size,
+                                          int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                                          int32_t num_kv_heads, int32_t head_dim, float scale,
+                                          const int32_t* selected, int64_t sel_token_stride, int64_t sel_head_stride,
+                                          int32_t num_selected, void* out, int64_t out_token_stride,
+                                          int64_t out_head_stride, void* workspace, int64_t workspace_bytes,
+                                          void* stream) {
+  using namespace aia;
+  SparseLayout L;
+  if (int rc = sparse_step("aia_paged_attention_sparse", batch, num_tokens, num_q_heads, num_kv_heads, head_dim,
+                           block_size, table_width, num_selected, workspace, workspace_bytes, L))
+    return rc;
+  if (!(scale > 0.f) || !(scale < 1e30f))
+    return fail(AIA_ERR_INVALID, "aia_paged_attention_sparse: scale must be positive");
+  if (num_tokens == 0) return AIA_OK;
+  if (!query || !key_cache || !value_cache || !block_table || !selected || !out || num_blocks <= 0)
+    return fail(AIA_ERR_INVALID, "aia_paged_attention_sparse: null pointer argument or no blocks");
+  if ((key_scale == nullptr) != (value_scale == nullptr))
+    return fail(AIA_ERR_INVALID, "aia_paged_attention_sparse: key_scale and value_scale go together");
+  if (!aligned16(query) || !aligned16(key_cache) || !aligned16(value_cache) || q_token_stride % 8 ||
+      q_head_stride % 8 || ((uintptr_t)out & 7u) || out_token_stride % 4 || out_head_stride % 4)
+    return fail(AIA_ERR_INVALID, "aia_paged_attention_sparse: query and caches must be 16-byte aligned with strides "
+                "a multiple of 8, out 8-byte aligned with strides a multiple of 4");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  SparseArgs a;
+  a.c.kc = static_cast<const uint16_t*>(key_cache); a.c.vc = static_cast<const uint16_t*>(value_cache);
+  a.c.ks = static_cast<const uint8_t*>(key_scale); a.c.vs = static_cast<const uint8_t*>(value_scale);
+  a.c.hkv = num_kv_heads; a.c.group = num_q_heads / num_kv_heads; a.c.bs = block_size; a.c.nb = num_blocks;
+  a.c.scale_log2 = scale * kLog2e;
+  a.q = static_cast<const uint16_t*>(query); a.q_ts = q_token_stride; a.q_hs = q_head_stride;
+  a.bt = block_table; a.bt_stride = block_table_stride;
+  a.tok = reinterpret_cast<const int4*>(ws + L.tok);
+  a.sel = selected; a.sel_ts = sel_token_stride; a.sel_hs = sel_head_stride; a.selected = num_selected;
+  a.splits = L.splits; a.tokens = num_tokens;
+  a.out = static_cast<uint16_t*>(out); a.o_ts = out_token_stride; a.o_hs = out_head_stride;
+  a.part_o = reinterpret_cast<float*>(ws + L.part_o); a.part_ml = reinterpret_cast<float2*>(ws + L.part_ml);
+  const int64_t groups = (int64_t)num_tokens * num_kv_heads * L.hblocks * a.splits;
+  if (groups > INT32_MAX) return fail(AIA_ERR_UNSUPPORTED, "aia_paged_attention_sparse: too many rows in one call");
+  auto* kernel = head_dim == 128 ? (key_scale ? sparse_attn_kernel<128, true> : sparse_attn_kernel<128, false>)
+                                 : (key_scale ? sparse_attn_kernel<64, true> : sparse_attn_kernel<64, false>);
+  kernel<<<(unsigned)groups, 64 * kSpWaves, 0, (hipStream_t)stream>>>(a);
+  if (int rc = check_hip(hipGetLastError(), "aia_paged_attention_sparse launch")) return rc;
+  if (a.splits == 1) return AIA_OK;
+  const int64_t rows = (int64_t)num_tokens * num_q_heads, per = kSparseThreads / (head_dim / 4);
+  (head_dim == 128 ? sparse_join_kernel<128> : sparse_join_kernel<64>)<<<(unsigned)((rows + per - 1) / per), kSparseThreads, 0, (hipStream_t)stream>>>(a);
+  return check_hip(hipGetLastError(), "aia_paged_attention_sparse: join launch");
+}

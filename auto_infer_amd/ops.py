@@ -859,6 +859,222 @@ def _paged_attention_gqa_ex(query, key_cache, value_cache, plan, scale, out, fla
     return out
 
 
+class _StepPlan:
+    """What the plans of the operators below share: a step's metadata on one GPU,
+    a workspace that its calls use, and the streams that they run on."""
+
+    def _take(self, block_table, cu_seqlens_q, seqlens_kv, num_tokens, num_q_heads, num_kv_heads,
+              head_dim, block_size):
+        _check_device_tensor(block_table, "block_table", torch.int32)
+        dev = block_table.get_device()
+        _check_on(cu_seqlens_q, "cu_seqlens_q", torch.int32, dev)
+        _check_on(seqlens_kv, "seqlens_kv", torch.int32, dev)
+        _require(block_table.dim() == 2 and block_table.shape[1] > 0 and block_table.stride(1) == 1,
+                 "block_table must be (batch, max_blocks) with unit column stride")
+        _require(seqlens_kv.dim() == 1 and cu_seqlens_q.shape == (seqlens_kv.shape[0] + 1,),
+                 "cu_seqlens_q must have batch + 1 entries")
+        self.batch = seqlens_kv.shape[0]
+        _require(block_table.shape[0] >= self.batch, "block_table has fewer rows than requests")
+        _require(cu_seqlens_q.is_contiguous() and seqlens_kv.is_contiguous(),
+                 "metadata tensors must be contiguous")
+        self.block_table, self.cu_seqlens_q, self.seqlens_kv = block_table, cu_seqlens_q, seqlens_kv
+        self.num_tokens, self.block_size = int(num_tokens), int(block_size)
+        self.num_q_heads, self.num_kv_heads = int(num_q_heads), int(num_kv_heads)
+        self.head_dim, self.device = int(head_dim), block_table.device
+        # (a single row's stride means nothing)
+        self._table_stride = block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1]
+
+    def _make(self, nbytes, workspace):
+        if workspace is None:
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        _check_on(workspace, "workspace", torch.uint8, self.device.index)
+        _require(workspace.is_contiguous() and workspace.numel() >= nbytes, "workspace too small")
+        self.workspace = workspace
+        self._streams = {torch.cuda.current_stream(self.device)}
+        self.replan()
+
+    def replan(self):
+        """Plan again from the (possibly updated in place) metadata tensors;
+        graph-capturable.  The plan is then valid on the current stream."""
+        self.stream = torch.cuda.current_stream(self.device)
+        self._on = (self.device, self.stream.cuda_stream)
+        self._use_on(self.stream)
+        self._plan(self._on[1])
+
+    def _use_on(self, stream):
+        if stream not in self._streams:
+            self._streams.add(stream)
+            self.workspace.record_stream(stream)
+
+
+def _attention_inputs(what, query, key_cache, value_cache, plan, key_scale, value_scale, out):
+    """The checks of an attention call over a ``_StepPlan``; returns (device index,
+    number of blocks, out)."""
+    _check_device_tensor(query, "query", _BF16)
+    dev, shape = query.get_device(), query.shape
+    if shape != (plan.num_tokens, plan.num_q_heads, plan.head_dim) or query.stride(2) != 1:
+        raise ValueError(f"{what}: query must be (T, Hq, D) of the plan's sizes, D contiguous")
+    if plan.device.index != dev:
+        raise ValueError("plan was made on another GPU")
+    if key_scale is not None or value_scale is not None:
+        cshape = _check_fp8_cache(key_cache, key_scale, "key_cache", "key_scale", dev)
+        if _check_fp8_cache(value_cache, value_scale, "value_cache", "value_scale", dev) != cshape:
+            raise ValueError("value cache shape differs from key cache")
+    else:
+        _check_on(key_cache, "key_cache", _BF16, dev)
+        _check_on(value_cache, "value_cache", _BF16, dev)
+        cshape = key_cache.shape
+        if len(cshape) != 4 or not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+            raise ValueError("caches must be contiguous (num_blocks, block_size, Hkv, D)")
+        if value_cache.shape != cshape:
+            raise ValueError("value cache shape differs from key cache")
+    if cshape[1:] != (plan.block_size, plan.num_kv_heads, plan.head_dim):
+        raise ValueError("plan was made for another cache shape")
+    if out is None:
+        out = torch.empty(shape, dtype=_BF16, device=query.device)
+    else:
+        _check_out(out, "out", shape, query.device)
+    return dev, cshape[0], out
+
+
+class BlockSparsePlan(_StepPlan):
+    """A step of block-sparse attention, made once for all its layers.
+
+    Metadata as ``AttentionPlan`` takes it.  Every query token and KV head attends
+    at most ``num_selected`` (up to 1024) cache blocks: always the first ``sink``
+    and the last ``local`` (at least 1) that it sees, and those of the highest
+    score.  ``summarize_blocks``, ``select_blocks`` and ``paged_attention_sparse``
+    take the plan; it holds their scratch space, so the plan's calls run on one
+    stream at a time.
+    """
+
+    def __init__(self, block_table, cu_seqlens_q, seqlens_kv, num_tokens, num_q_heads, num_kv_heads,
+                 head_dim, block_size, num_selected, sink=1, local=1, workspace=None):
+        self._take(block_table, cu_seqlens_q, seqlens_kv, num_tokens, num_q_heads, num_kv_heads,
+                   head_dim, block_size)
+        self.num_selected, self.sink, self.local = int(num_selected), int(sink), int(local)
+        _require(self.sink >= 0 and self.local >= 1 and self.sink + self.local <= self.num_selected,
+                 f"sink {sink} and local {local} do not fit {num_selected} selected blocks (local at "
+                 f"least 1)")
+        self._sizes = (block_table.shape[1], self.block_size, self.batch, self.num_tokens,
+                       self.num_q_heads, self.num_kv_heads, self.head_dim)
+        nbytes = ctypes.c_int64(0)
+        _native.call("aia_sparse_workspace_bytes", self.batch, self.num_tokens, self.num_q_heads,
+                     self.num_kv_heads, self.head_dim, self.block_size, block_table.shape[1],
+                     self.num_selected, ctypes.byref(nbytes))
+        self._make(nbytes.value, workspace)
+
+    def _plan(self, stream):
+        width, bs, batch, *rest = self._sizes
+        _call_on(self.device.index, "aia_sparse_plan", self.cu_seqlens_q.data_ptr(),
+                 self.seqlens_kv.data_ptr(), self.block_table.data_ptr(), self._table_stride, width, bs,
+                 batch, *rest, self.num_selected, self.workspace.data_ptr(), self.workspace.numel(),
+                 stream)
+
+
+def _check_bounds(bounds, bounds_scale, plan, dev):
+    _check_on(bounds, "bounds", torch.int8, dev)
+    _check_on(bounds_scale, "bounds_scale", FP8_KV_SCALE, dev)
+    shape = bounds.shape
+    if shape[1:] != (plan.num_kv_heads, 2, plan.head_dim) or not bounds.is_contiguous():
+        raise ValueError("bounds must be a contiguous (num_blocks, Hkv, 2, D) tensor")
+    if bounds_scale.shape != shape[:2] or not bounds_scale.is_contiguous():
+        raise ValueError("bounds_scale must be a contiguous (num_blocks, Hkv) tensor")
+
+
+def summarize_blocks(key_cache, plan, bounds, bounds_scale, key_scale=None):
+    """8-bit bounds of the keys in every cache block that the step's new tokens lie
+    in, for ``select_blocks``; call it after the step's keys are written.
+
+    ``key_cache`` (NB, bs, Hkv, D) bf16, or ``torch.float8_e4m3fn`` with its
+    ``key_scale``; ``plan`` a ``BlockSparsePlan``.  ``bounds`` (NB, Hkv, 2, D) int8
+    receives the largest and the negated smallest key value per dim, as whole
+    numbers times the power of two ``bounds_scale`` (NB, Hkv)
+    ``torch.float8_e8m0fnu``, rounded up.  A block's bounds follow from what it holds
+    of its request now, so rejected drafts leave no trace."""
+    dev = plan.device.index
+    if key_scale is not None:
+        shape = _check_fp8_cache(key_cache, key_scale, "key_cache", "key_scale", dev)
+    else:
+        _check_on(key_cache, "key_cache", _BF16, dev)
+        shape = key_cache.shape
+        if len(shape) != 4 or not key_cache.is_contiguous():
+            raise ValueError("key_cache must be a contiguous (num_blocks, block_size, Hkv, D) tensor")
+    if shape[1:] != (plan.block_size, plan.num_kv_heads, plan.head_dim):
+        raise ValueError("plan was made for another cache shape")
+    _check_bounds(bounds, bounds_scale, plan, dev)
+    if bounds.shape[0] != shape[0]:
+        raise ValueError("bounds must have an entry per cache block")
+    stream = _ready(plan, plan.device)
+    width, bs, *rest = plan._sizes
+    _call_on(dev, "aia_summarize_blocks", key_cache.data_ptr(), _ptr(key_scale), shape[0],
+             bounds.data_ptr(), bounds_scale.data_ptr(), bs, width, *rest, plan.num_selected,
+             plan.workspace.data_ptr(), plan.workspace.numel(), stream)
+
+
+def select_blocks(query, plan, bounds, bounds_scale, out=None):
+    """The cache blocks that each query token and KV head attends: (T, Hkv,
+    num_selected) int32 block numbers within the request, ascending, -1 behind them.
+
+    ``query`` (T, Hq, D) bf16 (rotated, as attention takes it); ``plan`` a
+    ``BlockSparsePlan``; ``bounds`` / ``bounds_scale`` of ``summarize_blocks``.  A
+    block's score is an upper bound of the sum of the group's products with its keys,
+    in whole numbers (8-bit query values and bounds), so the selection does not
+    depend on any order of summation; of equal scores the lowest block wins."""
+    _check_device_tensor(query, "query", _BF16)
+    dev = query.get_device()
+    if query.shape != (plan.num_tokens, plan.num_q_heads, plan.head_dim) or query.stride(2) != 1:
+        raise ValueError("query must be (T, Hq, D) of the plan's sizes, D contiguous")
+    if plan.device.index != dev:
+        raise ValueError("plan was made on another GPU")
+    _check_bounds(bounds, bounds_scale, plan, dev)
+    shape = (plan.num_tokens, plan.num_kv_heads, plan.num_selected)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.int32, device=query.device)
+    else:
+        _check_on(out, "out", torch.int32, dev)
+        if out.shape != shape or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {shape} tensor")
+    stream = _ready(plan, query.device)
+    q_ts, q_hs, _ = query.stride()
+    width, bs, *rest = plan._sizes
+    _call_on(dev, "aia_select_blocks", query.data_ptr(), q_ts, q_hs, bounds.data_ptr(),
+             bounds_scale.data_ptr(), bounds.shape[0], plan.block_table.data_ptr(), plan._table_stride,
+             width, bs, *rest, plan.num_selected, plan.sink, plan.local, out.data_ptr(),
+             shape[1] * shape[2], shape[2], plan.workspace.data_ptr(), plan.workspace.numel(), stream)
+    return out
+
+
+def paged_attention_sparse(query, key_cache, value_cache, plan, selected, scale, out=None,
+                           key_scale=None, value_scale=None):
+    """Paged attention over selected blocks alone: query head h of token t attends
+    the keys of blocks ``selected[t, h // (Hq // Hkv)]`` up to its own position.
+
+    query (T, Hq, D) bf16, D 128 or 64; caches (NB, bs, Hkv, D) bf16 or 8-bit with
+    their scales; ``plan`` a ``BlockSparsePlan``; ``selected`` (T, Hkv,
+    num_selected) int32 as ``select_blocks`` returns it: ascending block numbers
+    within the request (an entry that is negative, past the token's own block or not
+    above all before it is left out).  Returns (T, Hq, D) bf16; rows without a key
+    give zeros."""
+    dev, nb, out = _attention_inputs("paged_attention_sparse", query, key_cache, value_cache, plan,
+                                     key_scale, value_scale, out)
+    _check_on(selected, "selected", torch.int32, dev)
+    if (selected.shape != (plan.num_tokens, plan.num_kv_heads, plan.num_selected)
+            or selected.stride(2) != 1):
+        raise ValueError("selected must be (T, Hkv, num_selected) with unit inner stride")
+    stream = _ready(plan, query.device)
+    q_ts, q_hs, _ = query.stride()
+    o_ts, o_hs, _ = out.stride()
+    s_ts, s_hs, _ = selected.stride()
+    width, bs, *rest = plan._sizes
+    _call_on(dev, "aia_paged_attention_sparse", query.data_ptr(), q_ts, q_hs, key_cache.data_ptr(),
+             value_cache.data_ptr(), _ptr(key_scale), _ptr(value_scale), nb,
+             plan.block_table.data_ptr(), plan._table_stride, width, bs, *rest, scale,
+             selected.data_ptr(), s_ts, s_hs, plan.num_selected, out.data_ptr(), o_ts, o_hs,
+             plan.workspace.data_ptr(), plan.workspace.numel(), stream)
+    return out
+
+
 MLA_LATENT, MLA_ROPE = 512, 64
 
 

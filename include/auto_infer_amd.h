@@ -235,6 +235,77 @@ int aia_paged_attention_gqa_ex(const void* query, int64_t q_token_stride, int64_
                                float softcap, int32_t num_waves, int32_t flags, void* workspace,
                                int64_t workspace_bytes, void* stream);
 
+/* Block-sparse attention: every query token attends only the cache blocks that are
+ * selected for it and a KV head.  No counterpart in the reference.  Four calls share
+ * a step's plan in a caller workspace (aia_sparse_workspace_bytes long, 256-byte
+ * aligned, the same sizes in every call): aia_sparse_plan once per step, then per
+ * layer aia_summarize_blocks (after the step's keys are in the cache),
+ * aia_select_blocks and aia_paged_attention_sparse, in the plan's stream order.  The
+ * workspace also holds scores and partials, so a workspace serves one stream at a
+ * time.  table_width: columns of block_table (batch rows, block_table_stride apart);
+ * block_size * table_width below 2^31.  head_dim 128 or 64, at most 8192 requests, 256
+ * query heads per KV head and 1024 selected blocks (AIA_ERR_UNSUPPORTED otherwise).
+ * Query token i of request b stands at position Lk - Lq + i; tokens that no request
+ * covers (cu_seqlens_q ends before num_tokens) select nothing and give zeros. */
+int aia_sparse_workspace_bytes(int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                               int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                               int32_t table_width, int32_t num_selected, int64_t* bytes);
+
+/* The step's plan from its metadata (as aia_attn_plan takes it). */
+int aia_sparse_plan(const int32_t* cu_seqlens_q, const int32_t* seqlens_kv,
+                    const int32_t* block_table, int32_t block_table_stride, int32_t table_width,
+                    int32_t block_size, int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                    int32_t num_kv_heads, int32_t head_dim, int32_t num_selected, void* workspace,
+                    int64_t workspace_bytes, void* stream);
+
+/* Bounds of the keys of every block that the step's new tokens lie in, from the
+ * cache as it is: bounds (num_blocks, num_kv_heads, 2, head_dim) int8 holds hi and -lo,
+ * the largest and the smallest k[d] of the keys that the block holds of its request,
+ * as whole numbers times 2^e, rounded up; bounds_scale (num_blocks, num_kv_heads) the
+ * e8m0 byte e + 127, e the least >= -100 with |k| <= 127 * 2^e over the finite values.
+ * A dim with a value that is not finite gets 127 in both.  key_scale: NULL for bf16
+ * caches, else the e8m0 scales of an 8-bit one (aia_kv_write_fp8). */
+int aia_summarize_blocks(const void* key_cache, const void* key_scale, int32_t num_blocks,
+                         void* bounds, void* bounds_scale, int32_t block_size, int32_t table_width,
+                         int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                         int32_t num_kv_heads, int32_t head_dim, int32_t num_selected,
+                         const void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The blocks that each token and KV head attends: selected (num_tokens, num_kv_heads,
+ * num_selected) int32 with strides, ascending, -1 behind them.  Of the token's visible
+ * blocks (those up to its own) the first `sink` and the last `local` are always taken,
+ * the rest by the score
+ *   float32(sum over heads and dims of max(q, 0) hi + max(-q, 0) nlo) * 2^e,
+ * q the group's query values as whole numbers: rounded to nearest even after division
+ * by the least power of two >= 2^-100 that leaves the token's and KV head's |q| <= 127
+ * (values that are not finite count as 0); of equal scores the lowest block wins.
+ * sink >= 0, local >= 1, sink + local <= num_selected. */
+int aia_select_blocks(const void* query, int64_t q_token_stride, int64_t q_head_stride,
+                      const void* bounds, const void* bounds_scale, int32_t num_blocks,
+                      const int32_t* block_table, int32_t block_table_stride, int32_t table_width,
+                      int32_t block_size, int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                      int32_t num_kv_heads, int32_t head_dim, int32_t num_selected, int32_t sink,
+                      int32_t local, int32_t* selected, int64_t sel_token_stride,
+                      int64_t sel_head_stride, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+
+/* Attention over the selected blocks: query head h of token t attends the keys of the
+ * blocks selected[t][h / (Hq / Hkv)] up to the token's position.  Entries that are
+ * negative, past the token's own block or not above all entries before them are left
+ * out; a row without a key gives zeros.  Tensors as in aia_paged_attention_gqa_ex
+ * (standard layout; key_scale / value_scale both or neither). */
+int aia_paged_attention_sparse(const void* query, int64_t q_token_stride, int64_t q_head_stride,
+                               const void* key_cache, const void* value_cache,
+                               const void* key_scale, const void* value_scale, int32_t num_blocks,
+                               const int32_t* block_table, int32_t block_table_stride,
+                               int32_t table_width, int32_t block_size, int32_t batch,
+                               int32_t num_tokens, int32_t num_q_heads, int32_t num_kv_heads,
+                               int32_t head_dim, float scale, const int32_t* selected,
+                               int64_t sel_token_stride, int64_t sel_head_stride,
+                               int32_t num_selected, void* out, int64_t out_token_stride,
+                               int64_t out_head_stride, void* workspace, int64_t workspace_bytes,
+                               void* stream);
+
 /* Allocation-free paged GQA attention: aia_attn_plan + aia_paged_attention_gqa
  * in one call, with the plan and the split partials in a static device array
  * of the library (aia_noalloc_scratch_bytes: 96 MiB; one per GPU, held until
