@@ -74,6 +74,9 @@ SIGNATURES = {
                          c_vp, c_vp, c_f32, c_vp],
     "aia_rope_qk": [c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_i32, c_f32, c_i32, c_vp,
                     c_vp, c_f32, c_vp, c_i64, c_vp, c_i64, c_vp],
+    "aia_rope_append": [c_vp, c_i64, c_i32, c_i32, c_i32, c_i32, c_vp, c_vp, c_i32, c_f32, c_i32,
+                        c_vp, c_vp, c_f32, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i64,
+                        c_i32, c_vp],
     "aia_mla_kv_latent": [c_vp, c_i64, c_i32, c_vp, c_f32, c_vp, c_i64, c_vp, c_i64, c_vp, c_i64,
                           c_vp],
     "aia_mla_q_latent": [c_vp, c_i64, c_i64, c_i32, c_i32, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp,

@@ -213,18 +213,9 @@ class RotaryEmbedding:
         return out, float(att)
 
 
-def rope_qk(qkv, num_q_heads, num_kv_heads, positions, rope, q_norm_weight=None,
-            k_norm_weight=None, eps=1e-6, out=None):
-    """Rotary positions of the Q and K heads of a packed qkv projection (T, (Hq
-    + 2 Hkv) D), with an optional per-head RMSNorm in front, one launch.
-
-    ``positions`` (T,) int64, any values; ``rope`` a ``RotaryEmbedding`` of the
-    same head_dim.  In place by default; ``out`` = (q_out, k_out), tensors (T,
-    Hq, D) and (T, Hkv, D) that do not overlap ``qkv`` or each other (refused), leaves
-    ``qkv`` as it is.
-    Returns the rotated (q, k) and the V view, (T, heads, D) each.  Unlike
-    ``qk_norm_rope`` (cos/sin rows, bf16 roundings of the separate ops) it
-    computes the angles itself and rounds once."""
+def _rope_inputs(qkv, num_q_heads, num_kv_heads, positions, rope, q_norm_weight, k_norm_weight):
+    """The checks of a packed qkv projection whose heads turn by positions; returns
+    (device index, tokens, head_dim, width of Q, width of K, token stride)."""
     _require(isinstance(rope, RotaryEmbedding), "rope must be a RotaryEmbedding")
     _check_device_tensor(qkv, "qkv", _BF16)
     dev, D = qkv.get_device(), rope.head_dim
@@ -249,6 +240,23 @@ def rope_qk(qkv, num_q_heads, num_kv_heads, positions, rope, q_norm_weight=None,
     ts = qkv.stride(0) if T > 1 else width
     if ts < width:
         raise ValueError("qkv rows overlap")
+    return dev, T, D, nq, nk, ts
+
+
+def rope_qk(qkv, num_q_heads, num_kv_heads, positions, rope, q_norm_weight=None,
+            k_norm_weight=None, eps=1e-6, out=None):
+    """Rotary positions of the Q and K heads of a packed qkv projection (T, (Hq
+    + 2 Hkv) D), with an optional per-head RMSNorm in front, one launch.
+
+    ``positions`` (T,) int64, any values; ``rope`` a ``RotaryEmbedding`` of the
+    same head_dim.  In place by default; ``out`` = (q_out, k_out), tensors (T,
+    Hq, D) and (T, Hkv, D) that do not overlap ``qkv`` or each other (refused), leaves
+    ``qkv`` as it is.
+    Returns the rotated (q, k) and the V view, (T, heads, D) each.  Unlike
+    ``qk_norm_rope`` (cos/sin rows, bf16 roundings of the separate ops) it
+    computes the angles itself and rounds once."""
+    dev, T, D, nq, nk, ts = _rope_inputs(qkv, num_q_heads, num_kv_heads, positions, rope,
+                                         q_norm_weight, k_norm_weight)
     # (T, heads, D) views of the packed rows
     v = qkv.as_strided((T, num_kv_heads, D), (ts, D, 1), qkv.storage_offset() + nq + nk)
     if out is None:
@@ -269,6 +277,62 @@ def rope_qk(qkv, num_q_heads, num_kv_heads, positions, rope, q_norm_weight=None,
              rope.interleaved, _ptr(q_norm_weight), _ptr(k_norm_weight), eps, q_at, q_ts, k_at,
              k_ts, _stream_of(dev))
     return q, k, v
+
+
+def rope_append(qkv, num_q_heads, num_kv_heads, positions, rope, key_cache, value_cache,
+                slot_mapping, q_norm_weight=None, k_norm_weight=None, eps=1e-6, q_out=None,
+                key_scale=None, value_scale=None, kv_layout="nd"):
+    """``rope_qk`` and the cache write in one launch: the Q and K heads of a packed
+    qkv projection (T, (Hq + 2 Hkv) D) are normed (with weights) and turned by their
+    positions, K and V go to ``slot_mapping`` of the caches, turned Q is returned.
+
+    ``positions`` / ``rope`` / norm weights as ``rope_qk`` takes them, with the same
+    bits; caches (NB, bs, Hkv, D) bf16 (``kv_layout`` as in ``paged_attention_gqa``)
+    or ``torch.float8_e4m3fn`` with ``key_scale`` / ``value_scale`` (as
+    ``write_kv_fp8`` writes them).  Q is turned in place, or into ``q_out`` (T, Hq,
+    D), which does not overlap ``qkv`` (refused); the K and V parts of ``qkv`` stay as
+    they are.  ``slot_mapping`` (T,) int32: slots outside the cache are skipped; the
+    slots of a call differ from each other (8-bit caches keep the last token of a
+    slot, bf16 ones any)."""
+    dev, T, D, nq, nk, ts = _rope_inputs(qkv, num_q_heads, num_kv_heads, positions, rope,
+                                         q_norm_weight, k_norm_weight)
+    if kv_layout not in KV_LAYOUTS:
+        raise ValueError(f"kv_layout must be one of {sorted(KV_LAYOUTS)}")
+    ks_at = vs_at = None
+    if key_scale is not None or value_scale is not None:
+        shape = _check_fp8_cache(key_cache, key_scale, "key_cache", "key_scale", dev)
+        if _check_fp8_cache(value_cache, value_scale, "value_cache", "value_scale", dev) != shape:
+            raise ValueError("value_cache must match key_cache")
+        ks_at, vs_at = key_scale.data_ptr(), value_scale.data_ptr()
+    else:
+        _check_on(key_cache, "key_cache", _BF16, dev)
+        _check_on(value_cache, "value_cache", _BF16, dev)
+        shape = key_cache.shape
+        if len(shape) != 4 or not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+            raise ValueError("caches must be contiguous (num_blocks, block_size, Hkv, D)")
+        if value_cache.shape != shape:
+            raise ValueError("value_cache must match key_cache")
+    nb, bs, hkv, d = shape
+    if hkv != num_kv_heads or d != D:
+        raise ValueError(f"caches of {hkv} heads of {d}, not {num_kv_heads} of {D}")
+    _check_on(slot_mapping, "slot_mapping", torch.int32, dev)
+    if slot_mapping.shape != (T,) or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be a contiguous 1-D tensor with one slot per token")
+    if q_out is None:
+        q = qkv.as_strided((T, num_q_heads, D), (ts, D, 1))
+        q_ts = ts
+    else:
+        q = q_out
+        _check_on(q, "q_out", _BF16, dev)
+        if q.shape != (T, num_q_heads, D):
+            raise ValueError(f"q_out must have shape {(T, num_q_heads, D)}, got {tuple(q.shape)}")
+        q_ts = _token_stride(q, "q_out")
+    _call_on(dev, "aia_rope_append", qkv.data_ptr(), ts, T, num_q_heads, num_kv_heads, D,
+             positions.data_ptr(), rope.turns.data_ptr(), rope.rotary_dim, rope.attention_factor,
+             rope.interleaved, _ptr(q_norm_weight), _ptr(k_norm_weight), eps, q.data_ptr(), q_ts,
+             key_cache.data_ptr(), value_cache.data_ptr(), ks_at, vs_at, slot_mapping.data_ptr(), bs,
+             nb * bs, KV_LAYOUTS[kv_layout], _stream_of(dev))
+    return q
 
 
 def _rope_rows(t, name, T, width):

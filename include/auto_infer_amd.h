@@ -467,6 +467,26 @@ int aia_rope_qk(const void* qkv, int64_t qkv_token_stride, int32_t num_tokens,
                 float eps, void* q_out, int64_t q_out_token_stride, void* k_out,
                 int64_t k_out_token_stride, void* stream);
 
+/* Appending to paged caches with the position rotation on the way, one launch: the Q
+ * and K heads of a packed qkv projection are normed and turned as aia_rope_qk does it
+ * (same arguments, same bits); Q goes to q_out (T, Hq, D) with its token stride (the
+ * qkv rows themselves for in place, else no overlap with them), K and V to
+ * slot_mapping[t] of the caches as aia_kv_write, aia_kv_write_nz (flags:
+ * AIA_ATTN_KV_NZ) or aia_kv_write_fp8 (key_scale and value_scale set) store them.
+ * Only the Q part of qkv may be written.  No counterpart in the reference.
+ * num_slots: block_size times the caches' blocks; slots outside are skipped (their
+ * tokens' Q rows are turned all the same).  bf16 caches: the slots of a call differ
+ * from each other (of equal ones it is open which row's pieces stay); 8-bit ones: the
+ * last token of a slot stays.  Caches, 16-byte aligned, overlap nothing else. */
+int aia_rope_append(const void* qkv, int64_t qkv_token_stride, int32_t num_tokens,
+                    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                    const int64_t* positions, const int64_t* turns, int32_t rotary_dim,
+                    float factor, int32_t interleaved, const void* q_norm_weight,
+                    const void* k_norm_weight, float eps, void* q_out, int64_t q_out_token_stride,
+                    void* key_cache, void* value_cache, void* key_scale, void* value_scale,
+                    const int32_t* slot_mapping, int32_t block_size, int64_t num_slots,
+                    int32_t flags, void* stream);
+
 /* Absorbed-MLA latent KV row, one launch.  Replaces the ckv RMSNorm, the
  * k_pe ds_rope_interleave + NeoX RoPE and the cat of mla_paged_absorbed
  * (auto_infer/layers/attention/mla.py:97-111; rotary_embedding/__init__.py:
