@@ -48,6 +48,10 @@ SIGNATURES = {
                                    c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_f32,
                                    c_vp, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_vp, c_vp,
                                    c_vp, c_vp, c_f32, c_i32, c_i32, c_vp, c_i64, c_vp],
+    "aia_shared_workspace_bytes": [c_i32] * 7 + [ctypes.POINTER(c_i64)],
+    "aia_shared_plan": [c_vp, c_vp, c_vp, c_vp] + [c_i32] * 8 + [c_vp, c_i64, c_vp],
+    "aia_paged_attention_shared": [c_vp, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp] +
+                                  [c_i32] * 8 + [c_f32, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp],
     "aia_sparse_workspace_bytes": [c_i32] * 8 + [ctypes.POINTER(c_i64)],
     "aia_sparse_plan": [c_vp, c_vp, c_vp] + [c_i32] * 9 + [c_vp, c_i64, c_vp],
     "aia_summarize_blocks": [c_vp, c_vp, c_i32, c_vp, c_vp] + [c_i32] * 8 + [c_vp, c_i64, c_vp],

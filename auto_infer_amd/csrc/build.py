@@ -21,8 +21,8 @@ LIB = os.path.join(OUT_DIR, "libautoinfer_amd.so")
 PROBES = os.path.join(OUT_DIR, "libaia_probes.so")
 SOURCES = ["gqa_fp8_scored.hip", "gqa_scored_nz.hip", "gqa_scored.hip", "paged_attention.hip",
            "gqa_fp8.hip", "block_sparse.hip", "core.hip", "kv_write.hip", "kv_write_fp8.hip", "noalloc.hip",
-           "pack.hip", "qk_rope.hip", "rope.hip", "rope_append.hip", "mtp_compact.hip",
-           "mla_pre.hip"]
+           "pack.hip", "qk_rope.hip", "rope.hip", "rope_append.hip", "shared_prefix.hip",
+           "mtp_compact.hip", "mla_pre.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",

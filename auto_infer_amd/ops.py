@@ -1001,6 +1001,69 @@ def _attention_inputs(what, query, key_cache, value_cache, plan, key_scale, valu
     return dev, cshape[0], out
 
 
+class SharedPrefixPlan(_StepPlan):
+    """A step of attention whose requests share prefixes, made once for all its
+    layers, for ``paged_attention_shared``.
+
+    Metadata as ``AttentionPlan`` takes it.  ``group_ids`` (B,) int32 on the device
+    names each request's group (negative: alone); without it, requests with the same
+    first block form a group.  What a group shares is found on the GPU: the leading
+    keys, in front of the new tokens, for which the block table rows agree, from 128
+    keys on.  A wrong group costs speed, never the result.  The plan holds scratch
+    space, so its calls run on one stream at a time.
+    """
+
+    def __init__(self, block_table, cu_seqlens_q, seqlens_kv, num_tokens, num_q_heads, num_kv_heads,
+                 head_dim, block_size, group_ids=None, workspace=None):
+        self._take(block_table, cu_seqlens_q, seqlens_kv, num_tokens, num_q_heads, num_kv_heads,
+                   head_dim, block_size)
+        if group_ids is not None:
+            _check_on(group_ids, "group_ids", torch.int32, self.device.index)
+            _require(group_ids.shape == (self.batch,) and group_ids.is_contiguous(),
+                     "group_ids must hold one contiguous entry per request")
+        self.group_ids = group_ids
+        self._sizes = (self._table_stride, block_table.shape[1], self.block_size, self.batch,
+                       self.num_tokens, self.num_q_heads, self.num_kv_heads, self.head_dim)
+        nbytes = ctypes.c_int64(0)
+        _native.call("aia_shared_workspace_bytes", self.batch, self.num_tokens, self.num_q_heads,
+                     self.num_kv_heads, self.head_dim, self.block_size, block_table.shape[1],
+                     ctypes.byref(nbytes))
+        self._make(nbytes.value, workspace)
+
+    def _plan(self, stream):
+        _call_on(self.device.index, "aia_shared_plan", self.cu_seqlens_q.data_ptr(),
+                 self.seqlens_kv.data_ptr(), _ptr(self.group_ids), self.block_table.data_ptr(),
+                 *self._sizes, self.workspace.data_ptr(), self.workspace.numel(), stream)
+
+    def status(self):
+        """Synchronising check of the last plan, as ``AttentionPlan.status``."""
+        code = int(self.workspace[4:8].view(torch.int32).item())
+        if code != 0:
+            raise ValueError(f"shared-prefix planner (status {code}): cu_seqlens_q does not describe "
+                             f"{self.num_tokens} query tokens")
+
+
+def paged_attention_shared(query, key_cache, value_cache, plan, scale, out=None, key_scale=None,
+                           value_scale=None):
+    """Paged GQA attention of a step whose requests share prefixes: the results of
+    ``paged_attention_gqa`` (but for roundings), with shared keys read once for all
+    the requests of a group.
+
+    query (T, Hq, D) bf16, D 128 or 64; caches (NB, bs, Hkv, D) bf16 or 8-bit with
+    their scales (new rows written before, see ``rope_append``); ``plan`` a
+    ``SharedPrefixPlan``.  Returns (T, Hq, D) bf16."""
+    dev, nb, out = _attention_inputs("paged_attention_shared", query, key_cache, value_cache, plan,
+                                     key_scale, value_scale, out)
+    stream = _ready(plan, query.device)
+    q_ts, q_hs, _ = query.stride()
+    o_ts, o_hs, _ = out.stride()
+    _call_on(dev, "aia_paged_attention_shared", query.data_ptr(), q_ts, q_hs, key_cache.data_ptr(),
+             value_cache.data_ptr(), _ptr(key_scale), _ptr(value_scale), nb,
+             plan.cu_seqlens_q.data_ptr(), plan.block_table.data_ptr(), *plan._sizes, scale,
+             out.data_ptr(), o_ts, o_hs, plan.workspace.data_ptr(), plan.workspace.numel(), stream)
+    return out
+
+
 class BlockSparsePlan(_StepPlan):
     """A step of block-sparse attention, made once for all its layers.
 

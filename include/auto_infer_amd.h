@@ -235,6 +235,41 @@ int aia_paged_attention_gqa_ex(const void* query, int64_t q_token_stride, int64_
                                float softcap, int32_t num_waves, int32_t flags, void* workspace,
                                int64_t workspace_bytes, void* stream);
 
+/* Attention for a batch that shares prefixes: aia_paged_attention_gqa_ex's plain form
+ * (standard layout, bf16 or 8-bit caches, no modified scores), with the keys that
+ * requests have in common read once for all of them.  No counterpart in the reference.
+ * Same results as one request at a time, but for roundings.
+ * aia_shared_plan, once per step, finds what is shared: requests of one group_ids entry
+ * (negative: alone; NULL: of one first block id) share the leading keys, in front of
+ * their new tokens, for which their block table rows hold the same block ids as the
+ * group's first request, at least 128 keys.  A wrong group costs speed, never the
+ * result.  Requests of 128 query rows (tokens x heads per KV head) and more, which use
+ * every key that often anyway, do not share.
+ * Workspace: aia_shared_workspace_bytes long, 256-byte aligned, the same sizes in every
+ * call; it holds the plan and the partials, so it serves one stream at a time.  The
+ * int32 at byte offset 4 is the status: 0, or -1 where cu_seqlens_q does not describe
+ * num_tokens query tokens (the outputs are then NaN).
+ * head_dim 128 or 64, at most 4096 requests (AIA_ERR_UNSUPPORTED otherwise). */
+int aia_shared_workspace_bytes(int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                               int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                               int32_t table_width, int64_t* bytes);
+int aia_shared_plan(const int32_t* cu_seqlens_q, const int32_t* seqlens_kv,
+                    const int32_t* group_ids, const int32_t* block_table,
+                    int32_t block_table_stride, int32_t table_width, int32_t block_size,
+                    int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                    int32_t num_kv_heads, int32_t head_dim, void* workspace,
+                    int64_t workspace_bytes, void* stream);
+int aia_paged_attention_shared(const void* query, int64_t q_token_stride, int64_t q_head_stride,
+                               const void* key_cache, const void* value_cache,
+                               const void* key_scale, const void* value_scale, int32_t num_blocks,
+                               const int32_t* cu_seqlens_q, const int32_t* block_table,
+                               int32_t block_table_stride, int32_t table_width,
+                               int32_t block_size, int32_t batch, int32_t num_tokens,
+                               int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                               float scale, void* out, int64_t out_token_stride,
+                               int64_t out_head_stride, void* workspace, int64_t workspace_bytes,
+                               void* stream);
+
 /* Block-sparse attention: every query token attends only the cache blocks that are
  * selected for it and a KV head.  No counterpart in the reference.  Four calls share
  * a step's plan in a caller workspace (aia_sparse_workspace_bytes long, 256-byte
