@@ -545,8 +545,8 @@ __global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a
   const int head = hb * kRows + n;
   const bool rv = head < a.c.group;
   const uint16_t* qp = rv ? a.q + (int64_t)t * a.q_ts + (int64_t)(kvh * a.c.group + head) * a.q_hs : nullptr;
-  uint4 qf[1][D / 32];
-  load_q<D, F8>(qp, g, qf[0]);
+  uint4 qf[D / 32];
+  load_q<D, F8>(qp, g, qf);
   // every wave builds the same list
   const int32_t* sel = a.sel + (int64_t)t * a.sel_ts + (int64_t)kvh * a.sel_hs;
   const int32_t* btrow = a.bt + (int64_t)max(tk.x, 0) * a.bt_stride;
@@ -574,17 +574,16 @@ __global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a
   const int tiles = (keys + kTile - 1) / kTile;
   const int parts = a.splits * kSpWaves, p = split * kSpWaves + wid;
   const int t0 = (int)((int64_t)tiles * p / parts), t1 = (int)((int64_t)tiles * (p + 1) / parts);
-  RowState<1, D> s;
+  RowState<D> s;
   s.clear();
   const int p1 = min(keys, t1 * kTile);
-  const int lim[1] = {keys - 1};
-  attend<1, D, F8, false>(a.c, kvh, qf, lim, keys - 1, t0 * kTile, p1, count, [&](int i) { return list[i]; },
-                          reinterpret_cast<uint16_t*>(lds) + wid * kStage, lane, s);
+  attend<D, F8, false>(a.c, kvh, qf, keys - 1, keys - 1, t0 * kTile, p1, count, [&](int i) { return list[i]; },
+                       reinterpret_cast<uint16_t*>(lds) + wid * kStage, lane, s);
   s.finish();
   __syncthreads();
-  if (g == 0) { wave_m[wid][n] = s.m[0]; wave_l[wid][n] = s.l[0]; }
+  if (g == 0) { wave_m[wid][n] = s.m; wave_l[wid][n] = s.l; }
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) join[wid][dt][lane] = s.o[0][dt];
+  for (int dt = 0; dt < DT; ++dt) join[wid][dt][lane] = s.o[dt];
   __syncthreads();
   float m = -INFINITY, l = 0.f, w[kSpWaves];
 #pragma unroll

@@ -10,48 +10,53 @@
 // is bound by memory, beyond by the matrix cores.
 //
 // The planner finds what is shared by comparing block tables, so a wrong group only
-// costs speed.  It cuts the work into work-groups of two kinds:
-//   wide:   up to 128 rows of one KV head, 64-key tiles of K and V staged in LDS by
-//           direct loads, two buffers;
-//   narrow: up to 32 rows, a wave per KV head (or a share of the keys where there are
-//           fewer than four), each streaming on its own (wave_attention.h).
+// costs speed.  It cuts the work into units of up to 128 rows of one KV head and a run of
+// keys; a work-group takes one, with 64-key tiles of K and V staged in LDS.
 #include <algorithm>
 
-#include "wave_attention.h"
+#include "gqa_attention.h"
 
 namespace {
 
 constexpr int kShWaves = 4, kShThreads = 64 * kShWaves;
-constexpr int kWideRows = 128, kNarrowRows = 32;
-constexpr int kWideRt = kWideRows / (16 * kShWaves);      // 16-row tiles per wave
+constexpr int kUnitRows = 128;
+constexpr int kRt = kUnitRows / (16 * kShWaves);          // 16-row tiles per wave
+constexpr int kLightRows = 64;                            // up to here a unit waits for memory
 constexpr int kKeys = 64;                                 // keys of a tile
 constexpr int kMaxShared = 4096;                          // requests: the planner's LDS arrays
 constexpr int kShPlanT = 1024;
-constexpr int kTargetGroups = 512;                        // work-groups: two per compute unit
-constexpr int kMinWide = 8, kMinNarrow = 2;               // tiles of a cut
+#ifndef SH_TARGET
+#define SH_TARGET 512
+#endif
+#ifndef SH_MINW
+#define SH_MINW 8
+#endif
+#ifndef SH_TURN
+#define SH_TURN 256
+#endif
+constexpr int kTargetGroups = SH_TARGET;                  // units to aim at: two per compute unit
+constexpr int kMinCut = SH_MINW;                          // tiles of a cut
+constexpr int kTurn = SH_TURN;
 constexpr int kMinShare = 128;                            // keys worth a part of their own
+constexpr int kFewRows = 1024;                            // rows that are joined by four waves each
 constexpr int kRecord = 12, kHdr = 64;
 
-// Sizes of a step that host and device compute alike.
-struct ShGeom {
-  int32_t hkv, group, heads_wg, ksplit, hchunks;          // narrow: KV heads per work-group, waves per head
+// What the attention kernels need of a layer's caches.
+struct CacheArgs {
+  const uint16_t* kc;        // (num_blocks, bs, hkv, D) bf16, or e4m3 bytes
+  const uint16_t* vc;
+  const uint8_t* ks;         // e8m0 scales (num_blocks, hkv) of 8-bit caches
+  const uint8_t* vs;
+  int32_t group, bs, nb;
+  float scale_log2;          // score factor times log2(e)
 };
-__host__ __device__ inline ShGeom sh_geom(int32_t hq, int32_t hkv) {
-  ShGeom g;
-  g.hkv = hkv;
-  g.group = hq / hkv;
-  g.heads_wg = hkv < kShWaves ? hkv : kShWaves;
-  g.ksplit = kShWaves / g.heads_wg;
-  g.hchunks = (hkv + g.heads_wg - 1) / g.heads_wg;
-  return g;
-}
 
 // A row set against a run of keys: the rows of a group against what it shares, or of
 // a request against its own keys.  Rows [0, rows) of one KV head, token-major, in
-// tiles of 128; a last tile of up to 32 is narrow.
+// tiles of 128; the keys in `cuts` runs.
 struct Entity {
-  int32_t first_wg, part_base, rows, k0;                  // part_base -1: straight to the output
-  int32_t k1, token_base, wide_cuts, narrow_cuts;
+  int32_t part_base, rows, k0, k1;                        // part_base -1: straight to the output
+  int32_t token_base, cuts, pad0, pad1;
 };
 
 struct ShLayout {
@@ -60,20 +65,18 @@ struct ShLayout {
   int64_t part_cap;
 };
 ShLayout sh_layout(int32_t batch, int32_t tokens, int32_t hq, int32_t hkv, int32_t d) {
-  const ShGeom g = sh_geom(hq, hkv);
   auto up = [](int64_t x) { return (x + 255) & ~255ll; };
   ShLayout L;
-  // every entity's cuts: its share of kTargetGroups (wide and narrow ones each), and
-  // one more for each tile
-  const int64_t tiles = 2 * ((int64_t)tokens * g.group / kWideRows) + 2ll * batch;
-  L.wg_cap = (int32_t)std::min<int64_t>(INT32_MAX / 2, 2 * kTargetGroups + tiles * hkv);
-  L.part_cap = 2ll * tokens * hq * g.ksplit + 2ll * kTargetGroups * kWideRows;
+  // every entity's cuts: its share of kTargetGroups, and one more for each tile
+  const int64_t tiles = 2 * ((int64_t)tokens * (hq / hkv) / kUnitRows) + 2ll * batch;
+  L.wg_cap = (int32_t)std::min<int64_t>(INT32_MAX / 2, kTargetGroups + tiles * hkv);
+  L.part_cap = 2ll * tokens * hq + (int64_t)kTargetGroups * kUnitRows;
   L.hdr = 0;
   L.lead = up(kHdr * 4);
   L.common = L.lead + up(4ll * batch);
   L.place = L.common + up(4ll * batch);
   L.tokreq = L.place + up(4ll * batch);
-  L.order = L.tokreq + up(4ll * tokens);
+  L.order = L.tokreq + up(16ll * tokens);
   L.ent = L.order + up(4ll * tokens);
   L.rec = L.ent + up((int64_t)sizeof(Entity) * 2 * batch);
   L.part_ml = L.rec + up(4ll * kRecord * L.wg_cap);
@@ -94,17 +97,17 @@ struct ShPlanArgs {
   int32_t* lead;             // first request of each request's group
   int32_t* common;           // keys that it has in common with that one, in front of its new tokens
   int32_t* place;            // tokens of the group's requests before it
-  int32_t* tokreq;
+  int4* tokreq;              // {request, token of it, group's first request (-1: alone), place}
   int32_t* order;            // tokens of the sharing groups, group by group
   Entity* ent;               // [0, batch) groups by first request, [batch, 2 batch) requests
   int32_t* rec;
 };
 
-// Requests with fewer query rows than a wide tile share; longer ones use each tile of
+// Requests with fewer query rows than a unit share; longer ones use each tile of
 // keys 128 times as it is.
 __device__ __forceinline__ bool shares(const ShPlanArgs& a, int b) {
   const int lq = a.cu[b + 1] - a.cu[b];
-  return lq > 0 && lq * a.group < kWideRows && a.lk[b] > lq;
+  return lq > 0 && lq * a.group < kUnitRows && a.lk[b] > lq;
 }
 
 // ------------------------------------------------------------------ plan
@@ -142,21 +145,10 @@ __global__ __launch_bounds__(256) void shared_find_kernel(ShPlanArgs a) {
     a.common[b] = (int)min((int64_t)cached, (int64_t)differ * a.bs);
   }
   for (int i = tid; i < lq; i += 256)
-    if (q0 + i >= 0 && q0 + i < a.tokens) a.tokreq[q0 + i] = b;
+    if (q0 + i >= 0 && q0 + i < a.tokens) a.tokreq[q0 + i] = make_int4(b, i, mine ? first : -1, before);
 }
-
-struct Cuts {
-  int wide, narrow;          // tiles per cut
-};
 
 __device__ __forceinline__ int tiles_of(int keys) { return (keys + kKeys - 1) / kKeys; }
-
-// Full tiles of a row set, and rows of its last one (0: none).
-__device__ __forceinline__ void split_rows(int rows, int& full, int& rest, bool& narrow) {
-  full = rows / kWideRows;
-  rest = rows - full * kWideRows;
-  narrow = rest > 0 && rest <= kNarrowRows;
-}
 
 __device__ __forceinline__ int64_t block_sum(int64_t x, int64_t* lds) {
   const int tid = threadIdx.x;
@@ -196,11 +188,11 @@ __global__ __launch_bounds__(kShPlanT) void shared_plan_kernel(ShPlanArgs a) {
   int* tok = lds;                            // per group (first request): tokens,
   int* keys = tok + a.batch;                 // shared keys,
   int* members = keys + a.batch;             // requests
-  int* first_wg = members + a.batch;         // per entity (2 batch + 1)
+  int* first_heavy = members + a.batch;      // per entity (2 batch): its first heavy unit
+  int* first_light = first_heavy + 2 * a.batch;       // and light one (kLightRows) among those
   __shared__ int64_t scratch[kShPlanT / 64];
   __shared__ int bad;
   const int tid = threadIdx.x, B = a.batch;
-  const ShGeom g = sh_geom(a.hq, a.hkv);
   if (tid == 0) bad = a.cu[0] != 0 || a.cu[B] != a.tokens;
   for (int b = tid; b < B; b += kShPlanT) { tok[b] = 0; keys[b] = INT32_MAX; members[b] = 0; }
   __syncthreads();
@@ -238,67 +230,57 @@ __global__ __launch_bounds__(kShPlanT) void shared_plan_kernel(ShPlanArgs a) {
   };
   int64_t work = 0;
   for (int e = tid; e < 2 * B; e += kShPlanT) {
-    int rows, k0, k1, full, rest;
-    bool narrow;
+    int rows, k0, k1;
     extent(e, rows, k0, k1);
-    split_rows(rows, full, rest, narrow);
-    work += (int64_t)(full + (rest > 0)) * tiles_of(k1 - k0);
+    work += (int64_t)((rows + kUnitRows - 1) / kUnitRows) * tiles_of(k1 - k0);
   }
-  work = block_sum(work, scratch) * g.hkv;
-  Cuts cut;
-  cut.wide = (int)max((int64_t)kMinWide, (work + kTargetGroups - 1) / kTargetGroups);
-  cut.narrow = (int)max((int64_t)kMinNarrow, (work + (int64_t)kTargetGroups * g.heads_wg - 1) / ((int64_t)kTargetGroups * g.heads_wg));
-  // entities: work-groups, partial rows and (groups) places in the token order
-  int64_t wg_at = 0, part_at = 0, order_at = 0;
+  work = block_sum(work, scratch) * a.hkv;
+  const int per_cut = (int)max((int64_t)kMinCut, (work + kTargetGroups - 1) / kTargetGroups);
+  // entities: units, partial rows and (groups) places in the token order
+  int64_t heavy_at = 0, light_at = 0, part_at = 0, order_at = 0;
   for (int e0 = 0; e0 < 2 * B; e0 += kShPlanT) {
     const int e = e0 + tid;
     Entity x = {};
-    int full = 0, rest = 0, cw = 0, cn = 0;
-    bool narrow = false;
-    int64_t wgs = 0, parts = 0;
+    int64_t heavies = 0, lights = 0, parts = 0;
     if (e < 2 * B) {
       extent(e, x.rows, x.k0, x.k1);
-      split_rows(x.rows, full, rest, narrow);
-      const int tiles = tiles_of(x.k1 - x.k0);
       // (rows without keys still have one cut, which gives zeros)
-      cw = max(1, (tiles + cut.wide - 1) / cut.wide);
-      cn = max(1, (tiles + cut.narrow - 1) / cut.narrow);
-      const int wide = full + (rest > 0 && !narrow);
-      wgs = (int64_t)wide * cw * g.hkv + (narrow ? cn * g.hchunks : 0);
-      parts = ((int64_t)full * kWideRows * cw + (int64_t)rest * (narrow ? cn * g.ksplit : cw)) * g.hkv;
+      x.cuts = max(1, (tiles_of(x.k1 - x.k0) + per_cut - 1) / per_cut);
+      const int rest = x.rows % kUnitRows;
+      heavies = (int64_t)(x.rows / kUnitRows + (rest > kLightRows)) * x.cuts * a.hkv;
+      lights = rest > 0 && rest <= kLightRows ? (int64_t)x.cuts * a.hkv : 0;
+      parts = (int64_t)x.rows * x.cuts * a.hkv;
       if (e >= B) {
         const int l = a.lead[e - B];
-        const bool alone = l < 0 || keys[l] == 0;
-        const bool one = (wide == 0 || cw == 1) && (!narrow || cn * g.ksplit == 1);
-        if (alone && one) { parts = 0; x.part_base = -1; }
+        if ((l < 0 || keys[l] == 0) && x.cuts == 1) { parts = 0; x.part_base = -1; }
         x.token_base = a.cu[e - B];
       }
-      x.wide_cuts = cw;
-      x.narrow_cuts = cn;
     }
     int64_t total;
-    const int64_t wg = wg_at + block_scan(wgs, total, scratch);
-    wg_at += total;
+    const int64_t heavy = heavy_at + block_scan(heavies, total, scratch);
+    heavy_at += total;
+    const int64_t light = light_at + block_scan(lights, total, scratch);
+    light_at += total;
     const int64_t part = part_at + block_scan(parts, total, scratch);
     part_at += total;
     const int64_t at = order_at + block_scan(e < B ? tok[e] : 0, total, scratch);
     order_at += total;
     if (e < 2 * B) {
       if (e < B) x.token_base = (int)at;
-      x.first_wg = (int)min(wg, (int64_t)a.wg_cap);
       if (x.part_base >= 0) x.part_base = (int)min(part, (int64_t)INT32_MAX);
       a.ent[e] = x;
-      first_wg[e] = x.first_wg;
+      first_heavy[e] = (int)min(heavy, (int64_t)a.wg_cap);
+      first_light[e] = (int)min(light, (int64_t)a.wg_cap);
     }
   }
   // (the workspace is sized for any step of these sizes; a plan that would not fit is
   // not used)
-  if (wg_at > a.wg_cap || part_at > a.part_cap) {
+  if (heavy_at + light_at > a.wg_cap || part_at > a.part_cap) {
     if (tid == 0) { a.hdr[0] = 0; a.hdr[1] = -1; }
     return;
   }
-  const int count = (int)wg_at;
-  if (tid == 0) { first_wg[2 * B] = count; a.hdr[0] = count; a.hdr[1] = 0; }
+  const int heavies = (int)heavy_at, count = heavies + (int)light_at;
+  if (tid == 0) { a.hdr[0] = count; a.hdr[1] = 0; }
   __syncthreads();
   __threadfence_block();
   for (int b = tid; b < B; b += kShPlanT) {
@@ -308,50 +290,37 @@ __global__ __launch_bounds__(kShPlanT) void shared_plan_kernel(ShPlanArgs a) {
     for (int i = 0; i < n; ++i)
       if (at + i < a.tokens) a.order[at + i] = a.cu[b] + i;
   }
-  // the work-groups' records
+  // the units' records, heavy and light ones in turns of kTurn, so that a compute unit
+  // has one that waits for the matrix cores beside one that waits for memory
   for (int w = tid; w < count; w += kShPlanT) {
-    int lo = 0, hi = 2 * B;                  // the entity with first_wg[lo] <= w < first_wg[lo + 1]
+    const bool heavy = w < heavies;
+    const int* first = heavy ? first_heavy : first_light;
+    const int j = heavy ? w : w - heavies;   // its number among its kind
+    int lo = 0, hi = 2 * B;                  // the last entity with first[lo] <= j
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (first_wg[mid] <= w) lo = mid; else hi = mid;
+      if (first[mid] <= j) lo = mid; else hi = mid;
     }
     const int e = lo;
     const Entity x = a.ent[e];
-    int full, rest;
-    bool narrow;
-    split_rows(x.rows, full, rest, narrow);
-    const int wide = full + (rest > 0 && !narrow);
-    int i = w - x.first_wg;
-    const int nwide = wide * x.wide_cuts * g.hkv;
-    const bool is_wide = i < nwide;
-    int tile, c, h, cuts, per;
-    if (is_wide) {
-      // Work-groups of one run of keys and KV head (they differ in the row tile) are
-      // eight apart, so that they fall on one XCD and share its L2.
-      const int pairs = x.wide_cuts * g.hkv, block = i / (8 * wide), in = i - block * 8 * wide;
-      const int here = min(8, pairs - 8 * block);
-      tile = in / here;
-      const int pair = 8 * block + in - tile * here;
-      h = pair % g.hkv;
-      c = pair / g.hkv;
-      cuts = x.wide_cuts;
-      per = 1;
-    } else {
-      i -= nwide;
-      tile = full;
-      h = i % g.hchunks;
-      c = i / g.hchunks;
-      cuts = x.narrow_cuts;
-      per = g.ksplit;
-    }
-    const int rows = min(kWideRows, x.rows - tile * kWideRows);
+    const int slot = heavy ? j + min(count - heavies, j / kTurn * kTurn) : j + min(heavies, (j / kTurn + 1) * kTurn);
+    const int rest = x.rows % kUnitRows, full = x.rows / kUnitRows;
+    const int row_tiles = heavy ? full + (rest > kLightRows) : 1;
+    // Units of one run of keys and KV head (they differ in the row tile) are eight
+    // apart, so that they fall on one XCD and share its L2.
+    const int i = j - first[e], pairs = x.cuts * a.hkv;
+    const int block = i / (8 * row_tiles), in = i - block * 8 * row_tiles, here = min(8, pairs - 8 * block);
+    const int tile = heavy ? in / here : full;
+    const int pair = 8 * block + in % here;
+    const int h = pair % a.hkv, c = pair / a.hkv;
+    const int rows = min(kUnitRows, x.rows - tile * kUnitRows);
     const int tiles = tiles_of(x.k1 - x.k0);
-    const int t0 = (int)((int64_t)tiles * c / cuts), t1 = (int)((int64_t)tiles * (c + 1) / cuts);
+    const int t0 = (int)((int64_t)tiles * c / x.cuts), t1 = (int)((int64_t)tiles * (c + 1) / x.cuts);
     const int b = e < B ? e : e - B;
-    int32_t* r = a.rec + (int64_t)w * kRecord;
-    r[0] = (e < B ? 1 : 0) | (is_wide ? 2 : 0);
+    int32_t* r = a.rec + (int64_t)slot * kRecord;
+    r[0] = e < B ? 1 : 0;
     r[1] = b;
-    r[2] = tile * kWideRows;
+    r[2] = tile * kUnitRows;
     r[3] = rows;
     r[4] = x.token_base;
     r[5] = x.k0 + t0 * kKeys;
@@ -359,7 +328,7 @@ __global__ __launch_bounds__(kShPlanT) void shared_plan_kernel(ShPlanArgs a) {
     r[7] = h;
     r[8] = e < B ? INT32_MAX / 2 : a.lk[b] - (a.cu[b + 1] - a.cu[b]);
     // a tile's partial rows follow those of the tiles before it: (cut, KV head, row)
-    r[9] = x.part_base < 0 ? -1 : x.part_base + (tile * kWideRows * x.wide_cuts + c * per * rows) * g.hkv;
+    r[9] = x.part_base < 0 ? -1 : x.part_base + (tile * kUnitRows * x.cuts + c * rows) * a.hkv;
     r[10] = r[11] = 0;
   }
 }
@@ -383,10 +352,7 @@ struct ShArgs {
   int64_t part_cap;
   // for the join
   const Entity* ent;
-  const int32_t* lead;
-  const int32_t* place;
-  const int32_t* tokreq;
-  const int32_t* cu;
+  const int4* tokreq;
   int32_t hq, hkv;
 };
 
@@ -395,14 +361,13 @@ struct Unit {
   int b, row0, rows, token_base, k0, k1, h, ctx0, part;
 };
 
-__device__ __forceinline__ bool load_unit(const ShArgs& a, int w, Unit& u, bool& wide) {
+__device__ __forceinline__ bool load_unit(const ShArgs& a, int w, Unit& u) {
   if (w >= a.hdr[0]) return false;
   const int32_t* r = a.rec + (int64_t)w * kRecord;
   u.shared = r[0] & 1;
-  wide = r[0] & 2;
   u.b = r[1]; u.row0 = r[2]; u.rows = r[3]; u.token_base = r[4];
   u.k0 = r[5]; u.k1 = r[6]; u.h = r[7]; u.ctx0 = r[8]; u.part = r[9];
-  return u.b >= 0 && u.b < a.batch && u.rows > 0 && u.rows <= kWideRows;
+  return u.b >= 0 && u.b < a.batch && u.rows > 0 && u.rows <= kUnitRows;
 }
 
 // Row r of a unit: its token and its token's index among the unit's.
@@ -411,6 +376,16 @@ __device__ __forceinline__ int token_of(const ShArgs& a, const Unit& u, int row,
   const int t = u.token_base + index;
   const int tok = u.shared ? a.order[min(t, a.tokens - 1)] : t;
   return min(max(tok, 0), a.tokens - 1);
+}
+
+// Q operands of a 16-row MFMA tile: row n from qp (null: zeros).
+template <int D>
+__device__ __forceinline__ void load_q(const uint16_t* qp, int g, uint4 (&qf)[D / 32]) {
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) {
+    qf[j] = make_uint4(0, 0, 0, 0);
+    if (qp) qf[j] = reinterpret_cast<const uint4*>(qp)[4 * j + g];
+  }
 }
 
 // End of a 16-row tile: the output where the unit has all of the rows' keys, else a
@@ -447,93 +422,66 @@ __device__ __forceinline__ void write_rows(const ShArgs& a, float4_t (&o)[D / 16
   if (g == 0) a.part_ml[prow] = make_float2(m + __log2f(c), l * ic);
 }
 
-template <int RB, int D, bool F8>
-__device__ __forceinline__ void narrow_rows(const ShArgs& a, const Unit& u, uint16_t* vt) {
-  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n = lane & 15, g = lane >> 4;
-  const ShGeom geo = sh_geom(a.hq, a.hkv);
-  const int ks = wid / geo.heads_wg, kvh = u.h * geo.heads_wg + wid - ks * geo.heads_wg;
-  if (ks >= geo.ksplit || kvh >= a.hkv) return;
-  // this wave's keys
-  const int tiles = (u.k1 - u.k0 + kTile - 1) / kTile;
-  const int t0 = (int)((int64_t)tiles * ks / geo.ksplit), t1 = (int)((int64_t)tiles * (ks + 1) / geo.ksplit);
-  const int k0 = u.k0 + t0 * kTile, k1 = min(u.k1, u.k0 + t1 * kTile);
-  uint4 qf[RB][D / 32];
-  int lim[RB], tok[RB], head[RB], lim_lo = 0x7fffffff;
-  bool live[RB];
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    const int row = 16 * r + n;
-    live[r] = row < u.rows;
-    int index;
-    tok[r] = token_of(a, u, u.row0 + min(row, u.rows - 1), index);
-    head[r] = kvh * a.c.group + (u.row0 + row) % a.c.group;
-    lim[r] = live[r] ? min(u.ctx0 + index, k1 - 1) : -1;
-    lim_lo = live[r] ? min(lim_lo, lim[r]) : lim_lo;
-    load_q<D, F8>(live[r] ? a.q + (int64_t)tok[r] * a.q_ts + (int64_t)head[r] * a.q_hs : nullptr, g, qf[r]);
-  }
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) lim_lo = min(lim_lo, __shfl_xor(lim_lo, d));
-  lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
-  const int32_t* btrow = a.bt + (int64_t)u.b * a.bt_stride;
-  RowState<RB, D> s;
-  s.clear();
-  attend<RB, D, F8, true>(a.c, kvh, qf, lim, lim_lo, k0, k1, (k1 + a.c.bs - 1) / a.c.bs,
-                          [&](int i) { return btrow[i]; }, vt, lane, s);
-  s.finish();
-#pragma unroll
-  for (int r = 0; r < RB; ++r) {
-    const int64_t prow = u.part < 0 ? -1 : u.part + ((int64_t)ks * a.hkv + kvh) * u.rows + 16 * r + n;
-    write_rows<D>(a, s.o[r], s.m[r], s.l[r], live[r], prow,
-                  a.out + (int64_t)tok[r] * a.o_ts + (int64_t)head[r] * a.o_hs, g);
-  }
+// Row `row` of the unit, with its token and head found again rather than held through
+// the loop, which needs every register.
+template <int D>
+__device__ __forceinline__ void finish_row(const ShArgs& a, const Unit& u, int kvh, int row, float4_t (&o)[D / 16],
+                                           float m, float l, int g) {
+  int index;
+  const int tok = token_of(a, u, u.row0 + min(row, u.rows - 1), index);
+  const int head = kvh * a.c.group + (u.row0 + row) % a.c.group;
+  const int64_t prow = u.part < 0 ? -1 : u.part + (int64_t)kvh * u.rows + row;
+  write_rows<D>(a, o, m, l, row < u.rows, prow, a.out + (int64_t)tok * a.o_ts + (int64_t)head * a.o_hs, g);
 }
 
-// Wide unit: each of the four waves owns 32 rows (two 16-row MFMA tiles) and walks the
-// unit's keys in tiles of 64, staged once for all in one of two LDS buffers:
+// A unit: K and V in tiles of 64 keys, staged once for the four waves in one of two
+// LDS buffers:
 //   S^T = K Q^T    K fragments from LDS, Q^T in registers for the whole unit;
-//   O^T += V^T P^T over pairs of 16-key sub-tiles, V^T by transposing LDS reads, P from
-//                  where the S^T accumulators leave it.
-// One barrier a tile; the next tile's direct loads are issued behind QK^T and land
-// during the softmax and PV.  K chunk c of key r sits at c ^ (r % RC), V chunk c at
-// c ^ 2 (r % (RC / 2)) (RC = D / 8 chunks a row), which spreads the fragment reads over
-// the banks.  8-bit caches: a thread's chunks wait in registers and become bf16 on
-// their way to the same places, once per work-group.
-template <int D, bool F8, bool ONE_BLOCK>
-__device__ __forceinline__ void wide_rows(const ShArgs& a, const Unit& u, uint16_t* k0b, uint16_t* k1b,
-                                          uint16_t* v0b, uint16_t* v1b, int* odd_tile) {
-  constexpr int KJ = D / 32, DT = D / 16, RC = D / 8, ST = kKeys / 16;
+//   O^T += V^T P^T V^T by transposing LDS reads, P from where the S^T accumulators
+//                  leave it.
+// WK waves share 32 rows (two 16-row MFMA tiles) and take a share of each tile's keys:
+// 1 where the rows fill the waves, 4 where there are up to 32, whose shares are joined
+// in LDS at the end.  One barrier a tile; the next tile's direct loads are issued behind
+// QK^T and land during the softmax and PV.  K chunk c of key r sits at c ^ (r % RC), V
+// chunk c at c ^ 2 (r % (RC / 2)) (RC = D / 8 chunks a row), which spreads the fragment
+// reads over the banks.  8-bit caches: a thread's chunks wait in registers and become
+// bf16 on their way to the same places, once per work-group.
+template <int D, bool F8, bool ONE_BLOCK, int WK>
+__device__ __forceinline__ void unit_rows(const ShArgs& a, const Unit& u, uint16_t* k0b, uint16_t* k1b,
+                                          uint16_t* v0b, uint16_t* v1b, int* odd_tile, float2 (*share)[16 * kRt]) {
+  constexpr int KJ = D / 32, DT = D / 16, RC = D / 8;
+  constexpr int ST = kKeys / 16 / WK;        // 16-key sub-tiles of this wave, from s0 on
   const int tid = threadIdx.x, lane = tid & 63;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int kvh = u.h, G = a.c.group;
+  const int rw = wid / WK, ws = wid % WK, s0 = ws * ST;
   const int row_elems = a.hkv * D;
   const int32_t* btrow = a.bt + (int64_t)u.b * a.bt_stride;
   const int kend = u.k1;
   const int t0 = u.k0 / kKeys, t1 = (u.k1 + kKeys - 1) / kKeys;
 
-  int lim[kWideRt], tok[kWideRt], head[kWideRt];
-  bool live[kWideRt];
-  uint4 qf[kWideRt][KJ];
+  int lim[kRt];
+  uint4 qf[kRt][KJ];
   int wlo = 0x7fffffff, whi = -1;
 #pragma unroll
-  for (int rt = 0; rt < kWideRt; ++rt) {
-    const int row = (wid * kWideRt + rt) * 16 + n;
-    live[rt] = row < u.rows;
+  for (int rt = 0; rt < kRt; ++rt) {
+    const int row = (rw * kRt + rt) * 16 + n;
+    const bool live = row < u.rows;
     int index;
-    tok[rt] = token_of(a, u, u.row0 + min(row, u.rows - 1), index);
-    head[rt] = kvh * G + (u.row0 + row) % G;
-    lim[rt] = live[rt] ? min(u.ctx0 + index, kend - 1) : -1;
-    if (live[rt]) { wlo = min(wlo, lim[rt]); whi = max(whi, lim[rt]); }
-    load_q<D, false>(live[rt] ? a.q + (int64_t)tok[rt] * a.q_ts + (int64_t)head[rt] * a.q_hs : nullptr, g, qf[rt]);
+    const int tok = token_of(a, u, u.row0 + min(row, u.rows - 1), index);
+    const int head = kvh * G + (u.row0 + row) % G;
+    lim[rt] = live ? min(u.ctx0 + index, kend - 1) : -1;
+    if (live) { wlo = min(wlo, lim[rt]); whi = max(whi, lim[rt]); }
+    load_q<D>(live ? a.q + (int64_t)tok * a.q_ts + (int64_t)head * a.q_hs : nullptr, g, qf[rt]);
   }
 #pragma unroll
   for (int d = 1; d < 16; d <<= 1) {
     wlo = min(wlo, __shfl_xor(wlo, d));
     whi = max(whi, __shfl_xor(whi, d));
   }
-  wlo = __builtin_amdgcn_readfirstlane(wlo);
-  whi = __builtin_amdgcn_readfirstlane(whi);
+  // (All lanes hold the same limits; told so, the compiler joins the masked and the
+  // unmasked run of the loop below and spills up to 380 bytes a lane.)
 
   // loader: thread tid moves 16-byte chunk tid % RCL of keys kLdKeys i + tid / RCL
   constexpr int RCL = F8 ? D / 16 : RC;
@@ -608,10 +556,10 @@ __device__ __forceinline__ void wide_rows(const ShArgs& a, const Unit& u, uint16
     }
   };
 
-  float4_t o[kWideRt][DT];
-  float m[kWideRt], l[kWideRt];
+  float4_t o[kRt][DT];
+  float m[kRt], l[kRt];
 #pragma unroll
-  for (int rt = 0; rt < kWideRt; ++rt) {
+  for (int rt = 0; rt < kRt; ++rt) {
     clear_row(o[rt]);
     m[rt] = -INFINITY;
     l[rt] = 0.f;
@@ -626,7 +574,7 @@ __device__ __forceinline__ void wide_rows(const ShArgs& a, const Unit& u, uint16
     }
     const uint16_t* kt = Bf ? k1b : k0b;
     const uint16_t* vt = Bf ? v1b : v0b;
-    float4_t acc[kWideRt][ST];
+    float4_t acc[kRt][ST];
     if (F8) __builtin_amdgcn_s_setprio(1);
     __builtin_amdgcn_sched_barrier(0);       // the block below is scheduled on its own
 #pragma unroll
@@ -634,28 +582,28 @@ __device__ __forceinline__ void wide_rows(const ShArgs& a, const Unit& u, uint16
       uint4 kf[KJ];
 #pragma unroll
       for (int j = 0; j < KJ; ++j)
-        kf[j] = *reinterpret_cast<const uint4*>(kt + (16 * st + n) * D + 8 * ((4 * j + g) ^ (n & (RC - 1))));
+        kf[j] = *reinterpret_cast<const uint4*>(kt + (16 * (s0 + st) + n) * D + 8 * ((4 * j + g) ^ (n & (RC - 1))));
 #pragma unroll
-      for (int rt = 0; rt < kWideRt; ++rt) {
+      for (int rt = 0; rt < kRt; ++rt) {
         acc[rt][st] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < KJ; ++j) acc[rt][st] = qk_step(kf[j], qf[rt][j], acc[rt][st]);
       }
     }
-    __builtin_amdgcn_sched_group_barrier(kSgDsRead, KJ * kPfQkAhead, 0);
+    __builtin_amdgcn_sched_group_barrier(kSgDsRead, KJ * (ST < kPfQkAhead ? ST : kPfQkAhead), 0);
 #pragma unroll
     for (int st = 0; st < ST; ++st) {
-      __builtin_amdgcn_sched_group_barrier(kSgMfma, KJ * kWideRt, 0);
+      __builtin_amdgcn_sched_group_barrier(kSgMfma, KJ * kRt, 0);
       if (st + kPfQkAhead < ST) __builtin_amdgcn_sched_group_barrier(kSgDsRead, KJ, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
     if (F8) __builtin_amdgcn_s_setprio(0);
     issue_next();
-    uint4 pb[kWideRt][ST / 2];
+    uint4 pb[kRt][(ST + 1) / 2];
 #pragma unroll
-    for (int rt = 0; rt < kWideRt; ++rt) {
+    for (int rt = 0; rt < kRt; ++rt) {
       float x[ST][4];
-      const int rel = lim[rt] - kbase - 4 * g;
+      const int rel = lim[rt] - kbase - 16 * s0 - 4 * g;
       float top = -INFINITY;
 #pragma unroll
       for (int st = 0; st < ST; ++st)
@@ -688,25 +636,27 @@ __device__ __forceinline__ void wide_rows(const ShArgs& a, const Unit& u, uint16
       }
       m[rt] = mnew;
 #pragma unroll
-      for (int p = 0; p < ST / 2; ++p)
-        pb[rt][p] = make_uint4(aia::pack_bf16x2(x[2 * p][0], x[2 * p][1]), aia::pack_bf16x2(x[2 * p][2], x[2 * p][3]),
-                               aia::pack_bf16x2(x[2 * p + 1][0], x[2 * p + 1][1]),
-                               aia::pack_bf16x2(x[2 * p + 1][2], x[2 * p + 1][3]));
+      for (int p = 0; p < (ST + 1) / 2; ++p)
+        if (ST == 1) pb[rt][p] = make_uint4(aia::pack_bf16x2(x[0][0], x[0][1]), aia::pack_bf16x2(x[0][2], x[0][3]), 0, 0);
+        else pb[rt][p] = make_uint4(aia::pack_bf16x2(x[2 * p][0], x[2 * p][1]), aia::pack_bf16x2(x[2 * p][2], x[2 * p][3]),
+                               aia::pack_bf16x2(x[(2 * p + 1) % ST][0], x[(2 * p + 1) % ST][1]),
+                               aia::pack_bf16x2(x[(2 * p + 1) % ST][2], x[(2 * p + 1) % ST][3]));
     }
     __builtin_amdgcn_sched_barrier(0);
     if (MASK && *reinterpret_cast<volatile int*>(odd_tile + Bf) == t) {
       // a masked tile with a value that is not finite: key by key (see attend())
-      for (int k = 0; k < kKeys; ++k) {
+      for (int kk = 0; kk < 16 * ST; ++kk) {
+        const int k = 16 * s0 + kk;
         const uint16_t* vs = vt + k * D + 4 * (g & 1);
         const int sw = 2 * (k & (RC / 2 - 1));
 #pragma unroll
-        for (int rt = 0; rt < kWideRt; ++rt) {
+        for (int rt = 0; rt < kRt; ++rt) {
           uint32_t word = 0;
 #pragma unroll
           for (int w = 0; w < ST * 2; ++w) {      // word w: keys 16 (w / 2) + 4 g + 2 (w % 2), + 1
             const uint4 q = pb[rt][w >> 2];
             const uint32_t y = (w & 3) == 0 ? q.x : (w & 3) == 1 ? q.y : (w & 3) == 2 ? q.z : q.w;
-            word = w == 2 * (k >> 4) + ((k >> 1) & 1) ? y : word;
+            word = w == 2 * (kk >> 4) + ((kk >> 1) & 1) ? y : word;
           }
           const float p = weight_of(word, n, k);
           if (kbase + k <= lim[rt])
@@ -717,24 +667,35 @@ __device__ __forceinline__ void wide_rows(const ShArgs& a, const Unit& u, uint16
     }
     if (F8) __builtin_amdgcn_s_setprio(1);
     const int vrow = 4 * g + (n >> 2);
+    if constexpr (ST == 1) {
 #pragma unroll
-    for (int f = 0; f < ST / 2 * DT; ++f) {
-      const int pp = f / DT, dt = f % DT;
-      const int vsw = 16 * (dt ^ (vrow & (RC / 2 - 1)));
-      const short4_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (lds_short4_t*)(vt + (32 * pp + vrow) * D + vsw + 4 * (n & 3)));
-      const short4_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (lds_short4_t*)(vt + (32 * pp + 16 + vrow) * D + vsw + 4 * (n & 3)));
-      const bf16x8_t va = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+      for (int dt = 0; dt < DT; ++dt) {
+        const short4_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_short4_t*)(vt + (16 * s0 + vrow) * D + 16 * (dt ^ (vrow & (RC / 2 - 1))) + 4 * (n & 3)));
 #pragma unroll
-      for (int rt = 0; rt < kWideRt; ++rt)
-        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, as_b8(pb[rt][pp]), o[rt][dt], 0, 0, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(kSgDsRead, 2 * kPfPvAhead, 0);
+        for (int rt = 0; rt < kRt; ++rt)
+          o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(x0, as_s4(pb[rt][0].x, pb[rt][0].y), o[rt][dt], 0, 0, 0);
+      }
+    } else {
 #pragma unroll
-    for (int f = 0; f < ST / 2 * DT; ++f) {
-      __builtin_amdgcn_sched_group_barrier(kSgMfma, kWideRt, 0);
-      if (f + kPfPvAhead < ST / 2 * DT) __builtin_amdgcn_sched_group_barrier(kSgDsRead, 2, 0);
+      for (int f = 0; f < ST / 2 * DT; ++f) {
+        const int pp = f / DT, dt = f % DT;
+        const int vsw = 16 * (dt ^ (vrow & (RC / 2 - 1)));
+        const short4_t x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_short4_t*)(vt + (16 * s0 + 32 * pp + vrow) * D + vsw + 4 * (n & 3)));
+        const short4_t x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (lds_short4_t*)(vt + (16 * s0 + 32 * pp + 16 + vrow) * D + vsw + 4 * (n & 3)));
+        const bf16x8_t va = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x0, x1, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+        for (int rt = 0; rt < kRt; ++rt)
+          o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, as_b8(pb[rt][pp]), o[rt][dt], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(kSgDsRead, 2 * kPfPvAhead, 0);
+#pragma unroll
+      for (int f = 0; f < ST / 2 * DT; ++f) {
+        __builtin_amdgcn_sched_group_barrier(kSgMfma, kRt, 0);
+        if (f + kPfPvAhead < ST / 2 * DT) __builtin_amdgcn_sched_group_barrier(kSgDsRead, 2, 0);
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
     if (F8) __builtin_amdgcn_s_setprio(0);
@@ -817,104 +778,166 @@ __device__ __forceinline__ void wide_rows(const ShArgs& a, const Unit& u, uint16
     run(t0, t_um, std::false_type{});
     run(t_um, t1, std::true_type{});
   }
+  if constexpr (WK > 1) {
+    // The waves' shares of the keys, joined: wave ws takes row tile ws.  (The last tile's
+    // barrier is behind every wave; a wave's O fills one of the four buffers.)
+    static_assert(kRt * DT * 64 * 16 <= kKeys * D * 2 && kRt <= WK, "a buffer per wave, a wave per row tile");
+    auto buffer = [&](int w) { return reinterpret_cast<float4_t*>(w == 0 ? k0b : w == 1 ? k1b : w == 2 ? v0b : v1b); };
 #pragma unroll
-  for (int rt = 0; rt < kWideRt; ++rt) {
-    const int row = (wid * kWideRt + rt) * 16 + n;
-    const int64_t prow = u.part < 0 ? -1 : u.part + (int64_t)kvh * u.rows + row;
-    write_rows<D>(a, o[rt], m[rt], aia::group4_sum(l[rt]), live[rt], prow,
-                  a.out + (int64_t)tok[rt] * a.o_ts + (int64_t)head[rt] * a.o_hs, g);
+    for (int rt = 0; rt < kRt; ++rt) {
+      l[rt] = aia::group4_sum(l[rt]);
+      if (g == 0) share[wid][16 * rt + n] = make_float2(m[rt], l[rt]);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) buffer(wid)[(rt * DT + dt) * 64 + lane] = o[rt][dt];
+    }
+    __syncthreads();
+    if (ws >= kRt) return;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) top = fmaxf(top, share[rw * WK + w][16 * ws + n].x);
+    float4_t y[DT];
+    clear_row(y);
+#pragma unroll
+    for (int w = 0; w < WK; ++w) {
+      const float2 ml = share[rw * WK + w][16 * ws + n];
+      // (a share without keys has -inf and 0; one that saw NaN alone -inf and NaN)
+      const float f = ml.x == -INFINITY && ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
+      sum += f * ml.y;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) y[dt] += buffer(rw * WK + w)[(ws * DT + dt) * 64 + lane] * f;
+    }
+    finish_row<D>(a, u, kvh, (rw * kRt + ws) * 16 + n, y, top, sum, g);
+    return;
   }
+#pragma unroll
+  for (int rt = 0; rt < kRt; ++rt)
+    finish_row<D>(a, u, kvh, (rw * kRt + rt) * 16 + n, o[rt], m[rt], aia::group4_sum(l[rt]), g);
 }
 
 template <int D, bool F8, bool ONE_BLOCK>
 __global__ __launch_bounds__(kShThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void shared_attn_kernel(ShArgs a) {
-  // (narrow units stage their V tiles in the K buffers: 8-bit caches' pairs of tiles
-  // two waves each)
-  constexpr int kStage = (F8 ? 2 : 1) * kTile * kVStride;      // of a wave
-  constexpr int kPerBuf = F8 ? 2 : kShWaves;
-  constexpr int kBuf0 = kKeys * D > kPerBuf * kStage ? kKeys * D : kPerBuf * kStage;
-  __shared__ __attribute__((aligned(16))) uint16_t k0[kBuf0];
-  __shared__ __attribute__((aligned(16))) uint16_t k1[F8 ? kBuf0 : kKeys * D];
+  __shared__ __attribute__((aligned(16))) uint16_t k0[kKeys * D];
+  __shared__ __attribute__((aligned(16))) uint16_t k1[kKeys * D];
   __shared__ __attribute__((aligned(16))) uint16_t v0[kKeys * D];
   __shared__ __attribute__((aligned(16))) uint16_t v1[kKeys * D];
+  __shared__ float2 share[kShWaves][16 * kRt];
   __shared__ int odd_tile[2];
   Unit u;
-  bool wide;
-  if (!load_unit(a, blockIdx.x, u, wide)) return;
-  if (wide) {
-    wide_rows<D, F8, ONE_BLOCK>(a, u, k0, k1, v0, v1, odd_tile);
-    return;
-  }
-  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  uint16_t* vt = (wid < kPerBuf ? k0 : k1) + wid % kPerBuf * kStage;
-  if (u.rows <= 16) narrow_rows<1, D, F8>(a, u, vt);
-  else narrow_rows<2, D, F8>(a, u, vt);
+  if (!load_unit(a, blockIdx.x, u)) return;
+  if (u.rows <= 32) unit_rows<D, F8, ONE_BLOCK, 4>(a, u, k0, k1, v0, v1, odd_tile, share);
+  else if (u.rows <= 64) unit_rows<D, F8, ONE_BLOCK, 2>(a, u, k0, k1, v0, v1, odd_tile, share);
+  else unit_rows<D, F8, ONE_BLOCK, 1>(a, u, k0, k1, v0, v1, odd_tile, share);
 }
 
 // ------------------------------------------------------------------ join
 
 // Row r's parts of an entity: the first one's index, their distance and number.
-__device__ __forceinline__ void parts_of(const Entity& x, int r, int kvh, const ShGeom& g, int64_t& at,
+__device__ __forceinline__ void parts_of(const Entity& x, int r, int kvh, int hkv, int64_t& at,
                                          int64_t& step, int& count) {
-  const int tile = r / kWideRows;
-  const int rows = min(kWideRows, x.rows - tile * kWideRows);
-  const bool narrow = rows <= kNarrowRows;
-  count = narrow ? x.narrow_cuts * g.ksplit : x.wide_cuts;
-  step = (int64_t)g.hkv * rows;
-  at = x.part_base + (int64_t)tile * kWideRows * x.wide_cuts * g.hkv + (int64_t)kvh * rows + (r - tile * kWideRows);
+  const int tile = r / kUnitRows;
+  const int rows = min(kUnitRows, x.rows - tile * kUnitRows);
+  count = x.cuts;
+  step = (int64_t)hkv * rows;
+  at = x.part_base + (int64_t)tile * kUnitRows * x.cuts * hkv + (int64_t)kvh * rows + (r - tile * kUnitRows);
 }
 
-// D / 8 threads per row: the weights exp2(m - M) of its parts, and their sums.
-template <int D>
+// W waves per row (token and query head): a wave's lanes weigh up to 64 parts at once,
+// then take the parts' values 64 / (D / 8) at a time, 8 dims each.  (One thread per 8
+// dims walking the parts one after another: 36 us for 256 rows of 36 parts, a memory
+// round trip each.)  Four waves where the rows are few, and their parts many.
+template <int D, int W>
 __global__ __launch_bounds__(256) void shared_join_kernel(ShArgs a) {
-  constexpr int LANES = D / 8;
-  const int t = blockIdx.x, head = blockIdx.y * (256 / LANES) + threadIdx.x / LANES, c = threadIdx.x % LANES;
+  constexpr int LANES = D / 8, GROUPS = 64 / LANES;
+  __shared__ float part[W > 1 ? W : 1][LANES][8];
+  __shared__ float part_m[W > 1 ? W : 1], part_l[W > 1 ? W : 1];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = blockIdx.x, head = W > 1 ? blockIdx.y : blockIdx.y * 4 + wid, c = lane % LANES, sub = lane / LANES;
   if (head >= a.hq) return;
   uint16_t* op = a.out + (int64_t)t * a.o_ts + (int64_t)head * a.o_hs + 8 * c;
+  const int4 tk = a.tokreq[t];
   if (a.hdr[1] != 0) {                       // the lengths do not describe the step
-    const uint32_t w = 0x7fc07fc0u;
-    *reinterpret_cast<uint2*>(op) = make_uint2(w, w);
-    *reinterpret_cast<uint2*>(op + 4) = make_uint2(w, w);
+    const uint2 w = make_uint2(0x7fc07fc0u, 0x7fc07fc0u);
+    if (sub == 0) { *reinterpret_cast<uint2*>(op) = w; *reinterpret_cast<uint2*>(op + 4) = w; }
     return;
   }
-  const int b = a.tokreq[t];
+  const int b = tk.x;
   if (b < 0 || b >= a.batch) return;
-  const ShGeom g = sh_geom(a.hq, a.hkv);
-  const int kvh = head / g.group, hh = head - kvh * g.group, index = t - a.cu[b];
+  const int kvh = head / a.c.group, hh = head - kvh * a.c.group;
   const Entity own = a.ent[a.batch + b];
-  if (own.part_base < 0) return;
-  const int l = a.lead[b];
   Entity sh = {};
-  if (l >= 0) sh = a.ent[l];
-  int64_t at[2], step[2];
-  int count[2] = {0, 0};
-  parts_of(own, index * g.group + hh, kvh, g, at[0], step[0], count[0]);
-  if (sh.rows > 0) parts_of(sh, (a.place[b] + index) * g.group + hh, kvh, g, at[1], step[1], count[1]);
-  float m = -INFINITY;
-#pragma unroll
-  for (int s = 0; s < 2; ++s)
-    for (int i = 0; i < count[s]; ++i) m = fmaxf(m, a.part_ml[at[s] + i * step[s]].x);
-  float sum = 0.f, o[8];
+  if (tk.z >= 0) sh = a.ent[tk.z];
+  if (own.part_base < 0) return;
+  int64_t at0, at1 = 0, step0, step1 = 0;
+  int n0, n1 = 0;
+  parts_of(own, tk.y * a.c.group + hh, kvh, a.hkv, at0, step0, n0);
+  if (sh.rows > 0) parts_of(sh, (tk.w + tk.y) * a.c.group + hh, kvh, a.hkv, at1, step1, n1);
+  float m = -INFINITY, sum = 0.f, o[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) o[i] = 0.f;
+  // this wave's parts
+  const int first = W > 1 ? (int)((int64_t)(n0 + n1) * wid / W) : 0;
+  const int last = W > 1 ? (int)((int64_t)(n0 + n1) * (wid + 1) / W) : n0 + n1;
+  for (int p0 = first; p0 < last; p0 += 64) {
+    const int n = min(64, last - p0), p = p0 + lane;
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < n) ml = a.part_ml[p < n0 ? at0 + p * step0 : at1 + (p - n0) * step1];
+    float top = ml.x;
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
-    for (int i = 0; i < count[s]; ++i) {
-      const int64_t p = at[s] + i * step[s];
-      const float2 ml = a.part_ml[p];
-      const uint4 y = *reinterpret_cast<const uint4*>(a.part_o + p * D + 8 * c);
-      if (ml.x == -INFINITY && ml.y == 0.f) continue;      // a part without keys
-      const float w = __builtin_amdgcn_exp2f(ml.x - m);
-      sum += w * ml.y;
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float mnew = fmaxf(m, top);
+    // (a part without keys has -inf and 0; one that saw NaN alone -inf and NaN)
+    const float w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - mnew);
+    const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mnew);   // (nothing but NaN to scale then)
+    sum = sum * alpha + w * ml.y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] *= alpha;
+    m = mnew;
+#pragma unroll 4
+    for (int i0 = 0; i0 < n; i0 += GROUPS) {
+      const int i = i0 + sub;
+      const float wi = __shfl(w, min(i, 63));          // (of all lanes: the last round has idle ones)
+      if (i >= n) continue;
+      const int q = p0 + i;
+      const uint4 y = *reinterpret_cast<const uint4*>(a.part_o + (q < n0 ? at0 + q * step0 : at1 + (q - n0) * step1) * D + 8 * c);
       const uint32_t v[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const half2_t h = __builtin_bit_cast(half2_t, v[k]);
-        o[2 * k] += w * (float)h[0];
-        o[2 * k + 1] += w * (float)h[1];
+        o[2 * k] += wi * (float)h[0];
+        o[2 * k + 1] += wi * (float)h[1];
       }
     }
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+#pragma unroll
+  for (int d = LANES; d < 64; d <<= 1)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] += __shfl_xor(o[i], d);
+  if (W > 1) {
+    if (sub == 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) part[wid][c][i] = o[i];
+      if (c == 0) { part_m[wid] = m; part_l[wid] = sum; }
+    }
+    __syncthreads();
+    if (wid != 0) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = fmaxf(top, part_m[w]);
+    sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float x = part_m[w] == -INFINITY && part_l[w] == 0.f ? 0.f : __builtin_amdgcn_exp2f(part_m[w] - top);
+      sum += x * part_l[w];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] += x * part[w][c][i];
+    }
+  }
+  if (sub != 0) return;
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : __builtin_nanf("");
   *reinterpret_cast<uint2*>(op) = make_uint2(aia::pack_bf16x2(o[0] * inv, o[1] * inv), aia::pack_bf16x2(o[2] * inv, o[3] * inv));
   *reinterpret_cast<uint2*>(op + 4) = make_uint2(aia::pack_bf16x2(o[4] * inv, o[5] * inv), aia::pack_bf16x2(o[6] * inv, o[7] * inv));
@@ -931,7 +954,7 @@ int sh_check(const char* what, int32_t batch, int32_t tokens, int32_t hq, int32_
   if ((int64_t)bs * width > INT32_MAX - 128 * kKeys)
     return fail(AIA_ERR_UNSUPPORTED, "%s: contexts of 2^31 tokens and more", what);
   // partial rows are numbered in 32 bits
-  if (2ll * tokens * hq * kShWaves + 2ll * kTargetGroups * kWideRows > INT32_MAX / 2)
+  if (2ll * tokens * hq * kShWaves + 2ll * kTargetGroups * kUnitRows > INT32_MAX / 2)
     return fail(AIA_ERR_UNSUPPORTED, "%s: %d tokens of %d heads in one step", what, tokens, hq);
   return AIA_OK;
 }
@@ -983,14 +1006,14 @@ extern "C" int aia_shared_plan(const int32_t* cu_seqlens_q, const int32_t* seqle
   a.wg_cap = L.wg_cap; a.part_cap = L.part_cap;
   auto ints = [&](int64_t at) { return reinterpret_cast<int32_t*>(ws + at); };
   a.hdr = ints(L.hdr); a.lead = ints(L.lead); a.common = ints(L.common); a.place = ints(L.place);
-  a.tokreq = ints(L.tokreq); a.order = ints(L.order); a.rec = ints(L.rec);
+  a.tokreq = reinterpret_cast<int4*>(ws + L.tokreq); a.order = ints(L.order); a.rec = ints(L.rec);
   a.ent = reinterpret_cast<Entity*>(ws + L.ent);
   hipStream_t s = (hipStream_t)stream;
   if (batch > 0) {
     shared_find_kernel<<<(unsigned)batch, 256, 0, s>>>(a);
     if (int rc = check_hip(hipGetLastError(), "aia_shared_plan launch")) return rc;
   }
-  const size_t lds = (size_t)(5 * batch + 1) * sizeof(int);
+  const size_t lds = (size_t)(7 * batch) * sizeof(int);
   if (lds > 48 * 1024) {
     if (int rc = check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(shared_plan_kernel),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds),
@@ -1034,7 +1057,7 @@ extern "C" int aia_paged_attention_shared(const void* query, int64_t q_token_str
   ShArgs a;
   a.c.kc = static_cast<const uint16_t*>(key_cache); a.c.vc = static_cast<const uint16_t*>(value_cache);
   a.c.ks = static_cast<const uint8_t*>(key_scale); a.c.vs = static_cast<const uint8_t*>(value_scale);
-  a.c.hkv = num_kv_heads; a.c.group = num_q_heads / num_kv_heads; a.c.bs = block_size; a.c.nb = num_blocks;
+  a.c.group = num_q_heads / num_kv_heads; a.c.bs = block_size; a.c.nb = num_blocks;
   a.c.scale_log2 = scale * kLog2e;
   a.q = static_cast<const uint16_t*>(query); a.q_ts = q_token_stride; a.q_hs = q_head_stride;
   a.bt = block_table; a.bt_stride = block_table_stride; a.batch = batch; a.tokens = num_tokens; a.width = table_width;
@@ -1042,8 +1065,8 @@ extern "C" int aia_paged_attention_shared(const void* query, int64_t q_token_str
   a.out = static_cast<uint16_t*>(out); a.o_ts = out_token_stride; a.o_hs = out_head_stride;
   a.part_o = reinterpret_cast<uint16_t*>(ws + L.part_o); a.part_ml = reinterpret_cast<float2*>(ws + L.part_ml);
   a.part_cap = L.part_cap;
-  a.ent = reinterpret_cast<const Entity*>(ws + L.ent); a.lead = ints(L.lead); a.place = ints(L.place);
-  a.tokreq = ints(L.tokreq); a.cu = cu_seqlens_q; a.hq = num_q_heads; a.hkv = num_kv_heads;
+  a.ent = reinterpret_cast<const Entity*>(ws + L.ent);
+  a.tokreq = reinterpret_cast<const int4*>(ws + L.tokreq); a.hq = num_q_heads; a.hkv = num_kv_heads;
   const bool one = block_size % kKeys == 0;
   auto pick = [&](auto d) {
     constexpr int D = decltype(d)::value;
@@ -1054,7 +1077,9 @@ extern "C" int aia_paged_attention_shared(const void* query, int64_t q_token_str
   hipStream_t s = (hipStream_t)stream;
   kernel<<<(unsigned)L.wg_cap, kShThreads, 0, s>>>(a);
   if (int rc = check_hip(hipGetLastError(), "aia_paged_attention_shared launch")) return rc;
-  const unsigned rows = 256 / (head_dim / 8);
-  (head_dim == 128 ? shared_join_kernel<128> : shared_join_kernel<64>)<<<dim3((unsigned)num_tokens, (num_q_heads + rows - 1) / rows), 256, 0, s>>>(a);
+  const bool few = (int64_t)num_tokens * num_q_heads < kFewRows;
+  auto* join = head_dim == 128 ? (few ? shared_join_kernel<128, 4> : shared_join_kernel<128, 1>)
+                               : (few ? shared_join_kernel<64, 4> : shared_join_kernel<64, 1>);
+  join<<<dim3((unsigned)num_tokens, (unsigned)(few ? num_q_heads : (num_q_heads + 3) / 4)), 256, 0, s>>>(a);
   return check_hip(hipGetLastError(), "aia_paged_attention_shared: join launch");
 }

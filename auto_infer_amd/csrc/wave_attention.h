@@ -1,6 +1,7 @@
-// One wave's attention of up to RB x 16 query rows to a run of listed cache
-// blocks: the inner loop of the block-sparse kernel and of the shared-prefix
-// kernel's narrow units.
+// One wave's attention of up to 16 query rows to a run of listed cache blocks: the inner loop of the block-sparse kernel and of the shared-prefix
+// kernel's narrow units.  (Two row blocks per wave took 250 registers against 124, and
+// 28 us against 24 for 16 requests behind 4096 shared keys: two waves that share a
+// tile's bytes through the caches are the better use of a tile for 32 rows.)
 //
 // Keys are numbered by their place in the list (place p: block p / bs of the list,
 // offset p % bs).  A wave takes them in tiles of 16: S^T = K Q^T with K straight
@@ -24,28 +25,21 @@ struct CacheArgs {
   float scale_log2;          // score factor times log2(e)
 };
 
-// What a wave keeps of its rows: lane (n, g) holds row n's dims 16 dt + 4 g + (0..3)
-// of each 16-row block; m in log2 units (-inf: no key seen), l this lane's share of
-// the sum until finish().
-template <int RB, int D>
+// What a wave keeps of its rows: lane (n, g) holds row n's dims 16 dt + 4 g + (0..3);
+// m in log2 units (-inf: no key seen), l this lane's share of the sum until finish().
+template <int D>
 struct RowState {
-  float4_t o[RB][D / 16];
-  float m[RB], l[RB];
+  float4_t o[D / 16];
+  float m, l;
   __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      clear_row(o[r]);
-      m[r] = -INFINITY;
-      l[r] = 0.f;
-    }
+    clear_row(o);
+    m = -INFINITY;
+    l = 0.f;
   }
-  __device__ __forceinline__ void finish() {
-#pragma unroll
-    for (int r = 0; r < RB; ++r) l[r] = aia::group4_sum(l[r]);
-  }
+  __device__ __forceinline__ void finish() { l = aia::group4_sum(l); }
 };
 
-// Q operands of one 16-row block: row n from qp (null: zeros), in the order that
+// Q operands: row n from qp (null: zeros), in the order that
 // attend() reads keys of the cache format in.
 template <int D, bool F8>
 __device__ __forceinline__ void load_q(const uint16_t* qp, int g, uint4 (&qf)[D / 32]) {
@@ -87,20 +81,20 @@ __device__ __forceinline__ void soften(float (&x)[NT][4], float scale_log2, floa
   m = mnew;
 }
 
-// Attends places [p0, p1) (p0 a multiple of 16) with rows qf; row n of block r sees
-// places up to lim[r] (lim_lo: the smallest of the valid rows', wave-uniform; places
-// from p1 on are seen by none).  id(i): the block id of list entry i, called with
-// different i per lane, 0 <= i < entries.  vt: kTile * kVStride values of the wave's
-// own LDS (8-bit caches: twice that).
+// Attends places [p0, p1) (p0 a multiple of 16) with rows qf; row n sees places up to
+// lim (lim_lo: the smallest of the valid rows', wave-uniform; places from p1 on are
+// seen by none).  id(i): the block id of list entry i, called with different i per
+// lane, 0 <= i < entries.  vt: kTile * kVStride values of the wave's own LDS (8-bit
+// caches: twice that).
 //
 // Values that are not finite: weights of masked keys are zero, but 0 x V is not
 // where V is an infinity or NaN.  Places from p1 on are replaced by zeros, and with
 // CARE (rows of different limits) a masked tile that holds such a value is
 // multiplied key by key.
-template <int RB, int D, bool F8, bool CARE, class Id>
-__device__ __forceinline__ void attend(const CacheArgs& a, int kvh, const uint4 (&qf)[RB][D / 32],
-                                       const int (&lim)[RB], int lim_lo, int p0, int p1, int entries,
-                                       Id id, uint16_t* vt, int lane, RowState<RB, D>& s) {
+template <int D, bool F8, bool CARE, class Id>
+__device__ __forceinline__ void attend(const CacheArgs& a, int kvh, const uint4 (&qf)[D / 32], int lim,
+                                       int lim_lo, int p0, int p1, int entries, Id id, uint16_t* vt,
+                                       int lane, RowState<D>& s) {
   constexpr int KJ = D / 32, DT = D / 16, CH = D / 64;
   constexpr int NT = F8 ? 2 : 1;             // 16-key tiles per step
   constexpr int LD = F8 ? CH : KJ;           // 16-byte loads per key row and lane
@@ -147,7 +141,7 @@ __device__ __forceinline__ void attend(const CacheArgs& a, int kvh, const uint4 
         }
       odd &= F8 ? 0x80808080u : 0x80008000u;
     }
-    float4_t acc[RB][NT];
+    float4_t acc[NT];
 #pragma unroll
     for (int st = 0; st < NT; ++st) {
       uint4 kf[KJ];
@@ -169,37 +163,28 @@ __device__ __forceinline__ void attend(const CacheArgs& a, int kvh, const uint4 
         for (int j = 0; j < KJ; ++j) kf[j] = kk[st][j];
         stage_v(vt + st * kTile * kVStride, n, g, vv[st]);
       }
+      acc[st] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        acc[r][st] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < KJ; ++j) acc[r][st] = qk_step(kf[j], qf[r][j], acc[r][st]);
-      }
+      for (int j = 0; j < KJ; ++j) acc[st] = qk_step(kf[j], qf[j], acc[st]);
     }
-    uint2 pb[RB][NT];
+    uint2 pb[NT];
+    float x[NT][4];
+    const int last = min(lim, end - 1) - tb - 4 * g;
 #pragma unroll
-    for (int r = 0; r < RB; ++r) {
-      float x[NT][4];
-      const int last = min(lim[r], end - 1) - tb - 4 * g;
+    for (int st = 0; st < NT; ++st)
 #pragma unroll
-      for (int st = 0; st < NT; ++st)
+      for (int v = 0; v < 4; ++v) x[st][v] = !masked || kTile * st + v <= last ? acc[st][v] : -INFINITY;
+    soften<NT, DT>(x, a.scale_log2, s.m, s.l, s.o);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) x[st][v] = !masked || kTile * st + v <= last ? acc[r][st][v] : -INFINITY;
-      soften<NT, DT>(x, a.scale_log2, s.m[r], s.l[r], s.o[r]);
-#pragma unroll
-      for (int st = 0; st < NT; ++st)
-        pb[r][st] = make_uint2(aia::pack_bf16x2(x[st][0], x[st][1]), aia::pack_bf16x2(x[st][2], x[st][3]));
-    }
+    for (int st = 0; st < NT; ++st)
+      pb[st] = make_uint2(aia::pack_bf16x2(x[st][0], x[st][1]), aia::pack_bf16x2(x[st][2], x[st][3]));
     __builtin_amdgcn_wave_barrier();
     if (CARE && masked && __any(odd)) {
       for (int k = 0; k < NT * kTile; ++k) {
-#pragma unroll
-        for (int r = 0; r < RB; ++r) {
-          const uint2 w = NT == 1 || k < kTile ? pb[r][0] : pb[r][NT - 1];
-          const float p = weight_of(k & 2 ? w.y : w.x, n, k);
-          if (tb + k <= lim[r] && tb + k < end)
-            add_key(s.o[r], p, [&](int dt) { return vt + k * kVStride + 16 * dt + 4 * g; });
-        }
+        const uint2 w = NT == 1 || k < kTile ? pb[0] : pb[NT - 1];
+        const float p = weight_of(k & 2 ? w.y : w.x, n, k);
+        if (tb + k <= lim && tb + k < end)
+          add_key(s.o, p, [&](int dt) { return vt + k * kVStride + 16 * dt + 4 * g; });
       }
       __builtin_amdgcn_wave_barrier();
       return;
@@ -210,14 +195,10 @@ __device__ __forceinline__ void attend(const CacheArgs& a, int kvh, const uint4 
       if constexpr (F8) {
         const short4_t v1 = vt_frag(vt + kTile * kVStride, n, g, dt);
         const bf16x8_t va = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-        for (int r = 0; r < RB; ++r)
-          s.o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              va, as_b8(make_uint4(pb[r][0].x, pb[r][0].y, pb[r][1].x, pb[r][1].y)), s.o[r][dt], 0, 0, 0);
+        s.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            va, as_b8(make_uint4(pb[0].x, pb[0].y, pb[1].x, pb[1].y)), s.o[dt], 0, 0, 0);
       } else {
-#pragma unroll
-        for (int r = 0; r < RB; ++r)
-          s.o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v0, as_s4(pb[r][0].x, pb[r][0].y), s.o[r][dt], 0, 0, 0);
+        s.o[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v0, as_s4(pb[0].x, pb[0].y), s.o[dt], 0, 0, 0);
       }
     }
     __builtin_amdgcn_wave_barrier();

@@ -103,10 +103,14 @@ def test_attention(step, hq, hkv, d, fp8, bs):
     check(s, out)
 
 
-def test_long_prefix_in_many_cuts():
-    s = make([(6000, [(1, 100 + i) for i in range(40)]), (3000, [(2, 50 + i) for i in range(9)])], 16, 2, 128, 16, seed=1)
-    out, plan = run(s)
-    check(s, out)
+@pytest.mark.parametrize("hq,hkv,d", [(16, 2, 128), (32, 1, 128), (14, 2, 64), (28, 4, 64)])
+def test_long_prefix_in_many_cuts(hq, hkv, d):
+    """Rows of many parts, few rows (joined by four waves each) and many."""
+    groups = [(6000, [(1, 100 + i) for i in range(40)]), (3000, [(2, 50 + i) for i in range(9)])]
+    for g in (groups, groups[1:]):
+        s = make(g, hq, hkv, d, 16, seed=1)
+        out, _ = run(s)
+        check(s, out)
 
 
 def test_groups_by_first_block_or_wrong_groups_give_the_same():
