@@ -22,18 +22,50 @@ constexpr int kSparseThreads = 256;
 constexpr int kMaxSelected = 1024;
 constexpr int kHdrInts = 64;
 constexpr int64_t kScoreFloats = 1ll << 26;   // scores held at once
+constexpr int64_t kPartRows = 1ll << 20;      // and partial rows
+
+// How the attention of a step is cut.  Few tokens: `parts` work-groups share a (token,
+// KV head)'s selected keys, about four per compute unit in all, each of 256 keys or
+// more.  Many tokens of a request: their selections overlap in a context that no L2
+// holds, so the context (as long as the longest that a token sees, which the plan
+// knows) is cut into `parts` equal ranges, a multiple of the eight XCDs, so many that a
+// range's K and V fit an XCD's L2 in the longest context, and all tokens and KV heads
+// take a range there together.  (All KV heads: the rows of one of four lie in a quarter
+// of the L2's channels.)  512 tokens behind 32K, 28/4 heads of 128, 32 of 513 blocks of 64
+// each, chosen by chance: 180 us in 16 ranges, 186 in 8, 199 in 24, 226 in 32, 345
+// without: a wave's start, four dependent round trips, costs as much as the ranges' L2
+// hits save.
+struct SparseCut {
+  int32_t parts, tokens;     // tokens per launch
+  bool ranges;
+};
+constexpr int64_t kRangeBytes = 9ll << 19;    // 4.5 MB: a little over an XCD's L2
+constexpr int kRangeBlocks = 256, kMaxRanges = 64;           // blocks of a range at most
+SparseCut sparse_cut(int32_t batch, int32_t tokens, int32_t hkv, int32_t hblocks, int32_t d, int32_t bs,
+                     int32_t width, int32_t selected) {
+  SparseCut c{1, tokens, false};
+  const int64_t items = std::max<int64_t>(1, (int64_t)tokens * hkv * hblocks);
+  if (tokens >= 64 && tokens >= 16 * (int64_t)batch) {
+    // (sized for bf16; 8-bit caches' ranges take half the bytes)
+    const int64_t bytes = 4ll * d * bs * hkv * width;
+    const int64_t ranges = std::min<int64_t>(kMaxRanges, (bytes + 8 * kRangeBytes - 1) / (8 * kRangeBytes) * 8);
+    if (bytes > kRangeBytes && (width + ranges - 1) / ranges <= kRangeBlocks) {
+      c.ranges = true;
+      c.parts = (int32_t)ranges;
+      c.tokens = (int32_t)std::min<int64_t>(tokens, std::max<int64_t>(64, kPartRows / ((int64_t)hkv * hblocks * ranges * kRows)));
+      return c;
+    }
+  }
+  const int64_t keys = (int64_t)std::min(selected, width) * bs;
+  c.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>(1024 / items, keys / 256));
+  return c;
+}
 
 struct SparseLayout {
   int64_t hdr, tok, touched, scores, part_o, part_ml, total;
-  int32_t touched_cap, score_tokens, splits, hblocks;
+  int32_t touched_cap, score_tokens, hblocks;
+  SparseCut cut;
 };
-
-// Work-groups that share a (token, KV head)'s keys: about four per compute unit in
-// all, each of 256 keys or more.
-int sparse_splits(int64_t items, int64_t keys) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>(1024 / std::max<int64_t>(1, items), keys / 256));
-}
-
 SparseLayout sparse_layout(int32_t batch, int32_t tokens, int32_t hq, int32_t hkv, int32_t d, int32_t bs,
                            int32_t width, int32_t selected) {
   SparseLayout L;
@@ -42,14 +74,14 @@ SparseLayout sparse_layout(int32_t batch, int32_t tokens, int32_t hq, int32_t hk
   L.hblocks = (group + kRows - 1) / kRows;
   L.touched_cap = (int32_t)std::min<int64_t>(tokens, tokens / bs + 2ll * batch);
   L.score_tokens = (int32_t)std::max<int64_t>(1, std::min<int64_t>(tokens, kScoreFloats / ((int64_t)hkv * std::max(1, width))));
-  L.splits = sparse_splits((int64_t)tokens * hkv * L.hblocks, (int64_t)std::min(selected, width) * bs);
+  L.cut = sparse_cut(batch, tokens, hkv, L.hblocks, d, bs, width, selected);
   L.hdr = 0;
   L.tok = up(kHdrInts * 4);
   L.touched = L.tok + up(16ll * tokens);
   L.scores = L.touched + up(16ll * L.touched_cap);
   L.part_o = L.scores + up(4ll * L.score_tokens * hkv * width);
-  const int64_t rows = L.splits > 1 ? (int64_t)L.splits * tokens * hkv * L.hblocks * kRows : 0;
-  L.part_ml = L.part_o + up(4 * rows * d);
+  const int64_t rows = L.cut.parts > 1 ? (int64_t)L.cut.parts * L.cut.tokens * hkv * L.hblocks * kRows : 0;
+  L.part_ml = L.part_o + up(2 * rows * d);
   L.total = L.part_ml + up(8 * rows);
   return L;
 }
@@ -62,7 +94,7 @@ struct PlanArgs {
   const int32_t* bt;
   int64_t bt_stride;
   int32_t batch, tokens, bs, width;
-  int32_t* hdr;              // {blocks written to by the step}
+  int32_t* hdr;              // {blocks written to by the step, most blocks that a token sees}
   int4* tok;                 // {request or -1, position, visible blocks, 0}
   int4* touched;             // {block id, keys that it holds, 0, 0}
   int32_t touched_cap;
@@ -76,9 +108,9 @@ __global__ __launch_bounds__(kPlanT) void sparse_plan_kernel(PlanArgs a) {
   extern __shared__ int lds[];               // cu (batch + 1), first touched entry (batch)
   int* cu = lds;
   int* first = lds + a.batch + 1;
-  __shared__ int wave_sum[kPlanT / 64], carry;
+  __shared__ int wave_sum[kPlanT / 64], carry, most;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  if (tid == 0) carry = 0;
+  if (tid == 0) { carry = 0; most = 0; }
   for (int b = tid; b <= a.batch; b += kPlanT) cu[b] = a.cu[b];
   __syncthreads();
   for (int b0 = 0; b0 < a.batch; b0 += kPlanT) {
@@ -87,7 +119,10 @@ __global__ __launch_bounds__(kPlanT) void sparse_plan_kernel(PlanArgs a) {
     if (b < a.batch) {
       const int lq = cu[b + 1] - cu[b], lk = a.lk[b];
       const int from = max(0, lk - lq);
-      if (lq > 0 && lk > 0) n = (lk - 1) / a.bs - from / a.bs + 1;
+      if (lq > 0 && lk > 0) {
+        n = (lk - 1) / a.bs - from / a.bs + 1;
+        atomicMax(&most, min((lk - 1) / a.bs + 1, a.width));
+      }
     }
     int sum = n;                             // inclusive scan of the wave
 #pragma unroll
@@ -104,7 +139,7 @@ __global__ __launch_bounds__(kPlanT) void sparse_plan_kernel(PlanArgs a) {
     if (tid == kPlanT - 1) carry = before + sum;
     __syncthreads();
   }
-  if (blockIdx.x == 0 && tid == 0) a.hdr[0] = min(carry, a.touched_cap);
+  if (blockIdx.x == 0 && tid == 0) { a.hdr[0] = min(carry, a.touched_cap); a.hdr[1] = most; }
   const int t = blockIdx.x * kPlanT + tid;
   if (t >= a.tokens) return;
   int lo = 0, hi = a.batch;                  // the last request that begins at or before t
@@ -513,134 +548,160 @@ struct SparseArgs {
   const int4* tok;
   const int32_t* sel;
   int64_t sel_ts, sel_hs;
-  int32_t selected, splits, tokens;
+  int32_t selected, parts, t0, t1;                    // tokens [t0, t1) of this launch
+  const int32_t* hdr;
   uint16_t* out;
   int64_t o_ts, o_hs;
-  float* part_o;             // (token, KV head, head block, split): 16 rows of D
+  uint16_t* part_o;          // (token, KV head, head block, part): 16 rows of D
   float2* part_ml;
 };
 
 constexpr int kSpWaves = 4;
 
-// One work-group: a token, a KV head, up to 16 of its query heads and one of the
-// splits of the selected keys, four waves with a run of tiles each.  The list is
-// compacted first: entries that do not exceed all before them or that the token does
-// not see drop out, so all keys but the own block's behind the token's position are
-// seen, and only the last tile needs a limit.
-template <int D, bool F8>
-__global__ __launch_bounds__(64 * kSpWaves) void sparse_attn_kernel(SparseArgs a) {
+// A wave's row of 16 query heads: token t, KV head kvh, head block hb.
+struct SparseRow {
+  int t, kvh, hb;
+  int4 tk;                   // {request, position, visible blocks}
+  const int32_t* sel;
+  const int32_t* btrow;
+  __device__ __forceinline__ SparseRow(const SparseArgs& a, int t, int kvh, int hb)
+      : t(t), kvh(kvh), hb(hb), tk(a.tok[t]), sel(a.sel + (int64_t)t * a.sel_ts + (int64_t)kvh * a.sel_hs),
+        btrow(a.bt + (int64_t)max(tk.x, 0) * a.bt_stride) {}
+  // The block ids of the selected blocks in [b0, b1) that the token sees, in order, into
+  // list; returns their number and the keys that they hold for it.  Entries that do not
+  // exceed all before them drop out, so only the last block, the token's own, can be
+  // cut short.
+  __device__ __forceinline__ int blocks(const SparseArgs& a, int b0, int b1, int* list, int lane, int& keys) const {
+    int count = 0, most = -1;
+    bool own = false;
+    for (int i = 0; i < a.selected; i += 64) {
+      const int e = i + lane < a.selected ? sel[i + lane] : -1;
+      int upto = e;                          // the largest entry up to this lane's
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int x = __shfl_up(upto, d);
+        if (lane >= d) upto = max(upto, x);
+      }
+      const int prev = __shfl_up(upto, 1);
+      const int before = lane ? max(most, prev) : most;
+      const bool ok = e >= b0 && e < min(b1, tk.z) && e > before;
+      const uint64_t m = __ballot(ok);
+      if (ok) list[count + __popcll(m & ((1ull << lane) - 1))] = btrow[e];
+      count += __popcll(m);
+      own |= __any(ok && e == tk.y / a.c.bs) != 0;
+      most = max(most, __shfl(upto, 63));
+      if (most >= b1) break;                 // (the rest is behind the range)
+    }
+    keys = count * a.c.bs - (own ? a.c.bs - 1 - tk.y % a.c.bs : 0);
+    return count;
+  }
+  // row n's query head within the KV head's group
+  __device__ __forceinline__ int head(int n) const { return hb * kRows + n; }
+  __device__ __forceinline__ const uint16_t* query(const SparseArgs& a, int n) const {
+    return head(n) < a.c.group ? a.q + (int64_t)t * a.q_ts + (int64_t)(kvh * a.c.group + head(n)) * a.q_hs : nullptr;
+  }
+  __device__ __forceinline__ uint16_t* output(const SparseArgs& a, int n) const {
+    return a.out + (int64_t)t * a.o_ts + (int64_t)(kvh * a.c.group + head(n)) * a.o_hs;
+  }
+};
+__device__ __forceinline__ int head_blocks(const SparseArgs& a) { return (a.c.group + kRows - 1) / kRows; }
+__device__ __forceinline__ int64_t part_row(const SparseArgs& a, int t, int kvh, int hb, int part) {
+  return ((((int64_t)(t - a.t0) * a.c.hkv + kvh) * head_blocks(a) + hb) * a.parts + part) * kRows;
+}
+
+// One work-group: 16 query heads of a token and KV head and one of the parts of its
+// selected keys, four waves with a run of tiles each, joined in LDS.
+template <int D, bool F8, bool WHOLE>
+__global__ __launch_bounds__(64 * kSpWaves) __attribute__((amdgpu_waves_per_eu(3, 3))) void sparse_attn_kernel(SparseArgs a) {
   constexpr int DT = D / 16;
-  constexpr int kStage = (F8 ? 2 : 1) * kTile * kVStride;      // a wave's V tiles
-  constexpr int kJoinBytes = kSpWaves * DT * 64 * 16, kStageBytes = kSpWaves * kStage * 2;
+  constexpr int kJoinBytes = kSpWaves * DT * 64 * 16, kStageBytes = kSpWaves * kStep * 2;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kJoinBytes > kStageBytes ? kJoinBytes : kStageBytes];
   __shared__ int list[kMaxSelected];
   __shared__ float wave_m[kSpWaves][kRows], wave_l[kSpWaves][kRows];
   auto* join = reinterpret_cast<float4_t(*)[DT][64]>(lds);     // the waves' results, after their last V tile
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int item = blockIdx.x / a.splits, split = blockIdx.x - item * a.splits;
-  const int hblocks = (a.c.group + kRows - 1) / kRows;
-  const int hb = item % hblocks, kvh = item / hblocks % a.c.hkv, t = item / hblocks / a.c.hkv;
-  const int4 tk = a.tok[t];
-  const int head = hb * kRows + n;
-  const bool rv = head < a.c.group;
-  const uint16_t* qp = rv ? a.q + (int64_t)t * a.q_ts + (int64_t)(kvh * a.c.group + head) * a.q_hs : nullptr;
+  const int item = blockIdx.x / a.parts, part = blockIdx.x - item * a.parts, hblocks = head_blocks(a);
+  const SparseRow r(a, a.t0 + item / hblocks / a.c.hkv, item / hblocks % a.c.hkv, item % hblocks);
   uint4 qf[D / 32];
-  load_q<D, F8>(qp, g, qf);
-  // every wave builds the same list
-  const int32_t* sel = a.sel + (int64_t)t * a.sel_ts + (int64_t)kvh * a.sel_hs;
-  const int32_t* btrow = a.bt + (int64_t)max(tk.x, 0) * a.bt_stride;
-  int count = 0, most = -1;
-  bool own = false;                          // the token's own block is among them: the last one then
-  for (int i = 0; i < a.selected; i += 64) {
-    const int e = i + lane < a.selected ? sel[i + lane] : -1;
-    int upto = e;                            // the largest entry up to this lane's
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int x = __shfl_up(upto, d);
-      if (lane >= d) upto = max(upto, x);
-    }
-    const int prev = __shfl_up(upto, 1);
-    const int before = lane ? max(most, prev) : most;
-    const bool ok = e >= 0 && e < tk.z && e > before;
-    const uint64_t m = __ballot(ok);
-    if (ok) list[count + __popcll(m & ((1ull << lane) - 1))] = btrow[e];
-    count += __popcll(m);
-    own |= __any(ok && e == tk.y / a.c.bs) != 0;
-    most = max(most, __shfl(upto, 63));
-  }
+  load_q<D>(r.query(a, n), g, qf);
+  int keys;
+  const int count = r.blocks(a, 0, INT32_MAX, list, lane, keys);   // (every wave builds the same list)
   __syncthreads();
-  const int keys = count * a.c.bs - (own ? a.c.bs - 1 - tk.y % a.c.bs : 0);
-  const int tiles = (keys + kTile - 1) / kTile;
-  const int parts = a.splits * kSpWaves, p = split * kSpWaves + wid;
-  const int t0 = (int)((int64_t)tiles * p / parts), t1 = (int)((int64_t)tiles * (p + 1) / parts);
+  const int tiles = (keys + kTile - 1) / kTile, cuts = a.parts * kSpWaves, p = part * kSpWaves + wid;
+  const int t0 = (int)((int64_t)tiles * p / cuts), t1 = (int)((int64_t)tiles * (p + 1) / cuts);
   RowState<D> s;
   s.clear();
-  const int p1 = min(keys, t1 * kTile);
-  attend<D, F8, false>(a.c, kvh, qf, keys - 1, keys - 1, t0 * kTile, p1, count, [&](int i) { return list[i]; },
-                       reinterpret_cast<uint16_t*>(lds) + wid * kStage, lane, s);
+  attend<D, F8, WHOLE>(a.c, r.kvh, qf, t0 * kTile, min(keys, t1 * kTile), count, [&](int i) { return list[i]; },
+                reinterpret_cast<uint16_t*>(lds) + wid * kStep, lane, s);
   s.finish();
   __syncthreads();
   if (g == 0) { wave_m[wid][n] = s.m; wave_l[wid][n] = s.l; }
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) join[wid][dt][lane] = s.o[dt];
   __syncthreads();
-  float m = -INFINITY, l = 0.f, w[kSpWaves];
+  if (wid != 0) return;
+  float m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int i = 0; i < kSpWaves; ++i) m = fmaxf(m, wave_m[i][n]);
+  float4_t o[DT];
+  clear_row(o);
 #pragma unroll
   for (int i = 0; i < kSpWaves; ++i) {
     // (a wave that saw no key; one that saw NaN alone has -inf and NaN)
-    w[i] = wave_m[i][n] == -INFINITY && wave_l[i][n] == 0.f ? 0.f : __builtin_amdgcn_exp2f(wave_m[i][n] - m);
-    l += w[i] * wave_l[i][n];
-  }
-  if (!rv) return;
-  const int64_t prow = (((int64_t)item * a.splits) + split) * kRows + n;
-  if (a.splits > 1 && wid == 0 && g == 0) a.part_ml[prow] = make_float2(m, l);
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : __builtin_nanf("");
-  uint16_t* op = a.out + (int64_t)t * a.o_ts + (int64_t)(kvh * a.c.group + head) * a.o_hs;
+    const float w = wave_m[i][n] == -INFINITY && wave_l[i][n] == 0.f ? 0.f : __builtin_amdgcn_exp2f(wave_m[i][n] - m);
+    l += w * wave_l[i][n];
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) {
-    if (dt % kSpWaves != wid) continue;      // a wave takes its share of the dims
-    float4_t o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < kSpWaves; ++i) o += join[i][dt][lane] * w[i];
-    if (a.splits > 1) {
-      *reinterpret_cast<float4_t*>(a.part_o + prow * D + 16 * dt + 4 * g) = o;
-    } else {
-      *reinterpret_cast<uint2*>(op + 16 * dt + 4 * g) =
-          make_uint2(aia::pack_bf16x2(o[0] * inv, o[1] * inv), aia::pack_bf16x2(o[2] * inv, o[3] * inv));
-    }
+    for (int dt = 0; dt < DT; ++dt) o[dt] += join[i][dt][lane] * w;
   }
+  const bool live = r.head(n) < a.c.group;
+  if (a.parts > 1) write_part<D>(a.part_o, a.part_ml, part_row(a, r.t, r.kvh, r.hb, part) + n, o, m, l, live, g);
+  else if (live) write_out<D>(r.output(a, n), o, l, g);
 }
 
-// The splits of each row, joined.
-template <int D>
-__global__ __launch_bounds__(kSparseThreads) void sparse_join_kernel(SparseArgs a) {
-  constexpr int LANES = D / 4;               // threads per row
-  const int hblocks = (a.c.group + kRows - 1) / kRows;
-  const int64_t row = (int64_t)blockIdx.x * (kSparseThreads / LANES) + threadIdx.x / LANES;
-  const int c = threadIdx.x % LANES;
-  const int hq = a.c.group * a.c.hkv;
-  if (row >= (int64_t)a.tokens * hq) return;
-  const int t = (int)(row / hq), head = (int)(row - (int64_t)t * hq);
-  const int kvh = head / a.c.group, hh = head - kvh * a.c.group;
-  const int64_t item = ((int64_t)t * a.c.hkv + kvh) * hblocks + hh / kRows;
-  const int64_t first = item * a.splits * kRows + hh % kRows;
-  float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[first + s * kRows].x);
-  float l = 0.f;
-  float4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = a.part_ml[first + s * kRows];
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;
-    const float w = __builtin_amdgcn_exp2f(ml.x - m);
-    l += w * ml.y;
-    o += *reinterpret_cast<const float4_t*>(a.part_o + (first + s * kRows) * D + 4 * c) * w;
+// One wave: 16 query heads of a token and KV head and the selected blocks in one range
+// of the context.  A range is taken on one XCD (block ids are dealt to the eight in
+// turn).
+template <int D, bool F8, bool WHOLE>
+__global__ __launch_bounds__(64 * kSpWaves) __attribute__((amdgpu_waves_per_eu(3, 3))) void sparse_range_kernel(SparseArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t vt[kSpWaves][kStep];
+  __shared__ int list[kSpWaves][kRangeBlocks];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4, hblocks = head_blocks(a);
+  const int per = ((a.t1 - a.t0) * a.c.hkv * hblocks + kSpWaves - 1) / kSpWaves;      // work-groups of a range
+  const int k = blockIdx.x / 8, part = k / per * 8 + blockIdx.x % 8, i = k % per * kSpWaves + wid;
+  const int t = a.t0 + i / hblocks / a.c.hkv, kvh = i / hblocks % a.c.hkv;
+  if (t >= a.t1) return;
+  const SparseRow r(a, t, kvh, i % hblocks);
+  int keys;
+  const int blocks = min(kRangeBlocks, (a.hdr[1] + a.parts - 1) / a.parts), b0 = part * blocks;
+  const int count = r.blocks(a, b0, b0 + blocks, list[wid], lane, keys);
+  const int64_t row = part_row(a, t, kvh, r.hb, part) + n;
+  const bool live = r.head(n) < a.c.group;
+  if (count == 0) {
+    if (live && g == 0) a.part_ml[row] = make_float2(-INFINITY, 0.f);
+    return;
   }
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : __builtin_nanf("");
-  *reinterpret_cast<uint2*>(a.out + (int64_t)t * a.o_ts + (int64_t)head * a.o_hs + 4 * c) =
-      make_uint2(aia::pack_bf16x2(o[0] * inv, o[1] * inv), aia::pack_bf16x2(o[2] * inv, o[3] * inv));
+  uint4 qf[D / 32];
+  load_q<D>(r.query(a, n), g, qf);
+  RowState<D> s;
+  s.clear();
+  __builtin_amdgcn_wave_barrier();           // the list is the wave's own
+  attend<D, F8, WHOLE>(a.c, kvh, qf, 0, keys, count, [&](int j) { return list[wid][j]; }, vt[wid], lane, s);
+  s.finish();
+  write_part<D>(a.part_o, a.part_ml, row, s.o, s.m, s.l, live, g);
+}
+
+// The parts of each row, joined.
+template <int D, int W>
+__global__ __launch_bounds__(256) void sparse_join_kernel(SparseArgs a) {
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hq = a.c.group * a.c.hkv, t = a.t0 + blockIdx.x, head = W > 1 ? blockIdx.y : blockIdx.y * 4 + wid;
+  if (head >= hq) return;
+  const int kvh = head / a.c.group, hh = head - kvh * a.c.group;
+  const int64_t first = part_row(a, t, kvh, hh / kRows, 0) + hh % kRows;
+  join_row<D, W>(a.part_o, a.part_ml, a.parts, [&](int i) { return first + i * kRows; },
+                 a.out + (int64_t)t * a.o_ts + (int64_t)head * a.o_hs);
 }
 
 // ------------------------------------------------------------------ checks
@@ -847,17 +908,35 @@ extern "C" int aia_paged_attention_sparse(const void* query, int64_t q_token_str
   a.bt = block_table; a.bt_stride = block_table_stride;
   a.tok = reinterpret_cast<const int4*>(ws + L.tok);
   a.sel = selected; a.sel_ts = sel_token_stride; a.sel_hs = sel_head_stride; a.selected = num_selected;
-  a.splits = L.splits; a.tokens = num_tokens;
+  a.parts = L.cut.parts; a.hdr = reinterpret_cast<const int32_t*>(ws + L.hdr);
   a.out = static_cast<uint16_t*>(out); a.o_ts = out_token_stride; a.o_hs = out_head_stride;
-  a.part_o = reinterpret_cast<float*>(ws + L.part_o); a.part_ml = reinterpret_cast<float2*>(ws + L.part_ml);
-  const int64_t groups = (int64_t)num_tokens * num_kv_heads * L.hblocks * a.splits;
-  if (groups > INT32_MAX) return fail(AIA_ERR_UNSUPPORTED, "aia_paged_attention_sparse: too many rows in one call");
-  auto* kernel = head_dim == 128 ? (key_scale ? sparse_attn_kernel<128, true> : sparse_attn_kernel<128, false>)
-                                 : (key_scale ? sparse_attn_kernel<64, true> : sparse_attn_kernel<64, false>);
-  kernel<<<(unsigned)groups, 64 * kSpWaves, 0, (hipStream_t)stream>>>(a);
-  if (int rc = check_hip(hipGetLastError(), "aia_paged_attention_sparse launch")) return rc;
-  if (a.splits == 1) return AIA_OK;
-  const int64_t rows = (int64_t)num_tokens * num_q_heads, per = kSparseThreads / (head_dim / 4);
-  (head_dim == 128 ? sparse_join_kernel<128> : sparse_join_kernel<64>)<<<(unsigned)((rows + per - 1) / per), kSparseThreads, 0, (hipStream_t)stream>>>(a);
-  return check_hip(hipGetLastError(), "aia_paged_attention_sparse: join launch");
+  a.part_o = reinterpret_cast<uint16_t*>(ws + L.part_o); a.part_ml = reinterpret_cast<float2*>(ws + L.part_ml);
+  hipStream_t s = (hipStream_t)stream;
+  for (int t0 = 0; t0 < num_tokens; t0 += L.cut.tokens) {
+    a.t0 = t0;
+    a.t1 = std::min(num_tokens, t0 + L.cut.tokens);
+    const int64_t items = (int64_t)(a.t1 - a.t0) * num_kv_heads * L.hblocks;
+    const int64_t groups = a.parts * (L.cut.ranges ? (items + kSpWaves - 1) / kSpWaves : items);
+    if (groups > INT32_MAX) return fail(AIA_ERR_UNSUPPORTED, "aia_paged_attention_sparse: too many rows in one call");
+    auto pick = [&](auto d, auto f8) {
+      constexpr int D = decltype(d)::value;
+      constexpr bool F8 = decltype(f8)::value, T = true, F = false;
+      const bool whole = block_size % kTile == 0;
+      return L.cut.ranges ? (whole ? sparse_range_kernel<D, F8, T> : sparse_range_kernel<D, F8, F>)
+                            : (whole ? sparse_attn_kernel<D, F8, T> : sparse_attn_kernel<D, F8, F>);
+    };
+    using d128 = std::integral_constant<int, 128>;
+    using d64 = std::integral_constant<int, 64>;
+    auto* kernel = head_dim == 128 ? (key_scale ? pick(d128{}, std::true_type{}) : pick(d128{}, std::false_type{}))
+                                   : (key_scale ? pick(d64{}, std::true_type{}) : pick(d64{}, std::false_type{}));
+    kernel<<<(unsigned)groups, 64 * kSpWaves, 0, s>>>(a);
+    if (int rc = check_hip(hipGetLastError(), "aia_paged_attention_sparse launch")) return rc;
+    if (a.parts == 1) continue;
+    const bool few = (int64_t)(a.t1 - t0) * num_q_heads < kFewRows;
+    auto* join = head_dim == 128 ? (few ? sparse_join_kernel<128, 4> : sparse_join_kernel<128, 1>)
+                                 : (few ? sparse_join_kernel<64, 4> : sparse_join_kernel<64, 1>);
+    join<<<dim3((unsigned)(a.t1 - t0), (unsigned)(few ? num_q_heads : (num_q_heads + 3) / 4)), 256, 0, s>>>(a);
+    if (int rc = check_hip(hipGetLastError(), "aia_paged_attention_sparse: join launch")) return rc;
+  }
+  return AIA_OK;
 }

@@ -14,7 +14,7 @@
 // keys; a work-group takes one, with 64-key tiles of K and V staged in LDS.
 #include <algorithm>
 
-#include "gqa_attention.h"
+#include "row_parts.h"
 
 namespace {
 
@@ -38,7 +38,6 @@ constexpr int kTargetGroups = SH_TARGET;                  // units to aim at: tw
 constexpr int kMinCut = SH_MINW;                          // tiles of a cut
 constexpr int kTurn = SH_TURN;
 constexpr int kMinShare = 128;                            // keys worth a part of their own
-constexpr int kFewRows = 1024;                            // rows that are joined by four waves each
 constexpr int kRecord = 12, kHdr = 64;
 
 // What the attention kernels need of a layer's caches.
@@ -388,40 +387,6 @@ __device__ __forceinline__ void load_q(const uint16_t* qp, int g, uint4 (&qf)[D 
   }
 }
 
-// End of a 16-row tile: the output where the unit has all of the rows' keys, else a
-// partial: y = O / c in fp16, c the row's largest finite |O|, with (m + log2 c, l / c)
-// for (m, l), as the split rows of the other attention kernels have them: half the
-// bytes of float32, 2^-11 of a value at most.
-template <int D>
-__device__ __forceinline__ void write_rows(const ShArgs& a, float4_t (&o)[D / 16], float m, float l, bool live,
-                                           int64_t prow, uint16_t* op, int g) {
-  constexpr int DT = D / 16;
-  if (prow < 0) {
-    if (!live) return;
-    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : __builtin_nanf("");
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-      *reinterpret_cast<uint2*>(op + 16 * dt + 4 * g) =
-          make_uint2(aia::pack_bf16x2(o[dt][0] * inv, o[dt][1] * inv), aia::pack_bf16x2(o[dt][2] * inv, o[dt][3] * inv));
-    return;
-  }
-  float c = 0.f;
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int v = 0; v < 4; ++v) c = fmaxf(c, finite_abs(o[dt][v]));
-  c = aia::group4_max(c);
-  if (!live || prow >= a.part_cap) return;
-  c = c > 0.f ? c : 1.f;
-  const float ic = 1.f / c;
-  uint16_t* pp = a.part_o + prow * D;
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-    *reinterpret_cast<uint2*>(pp + 16 * dt + 4 * g) =
-        make_uint2(pack_f16x2(o[dt][0] * ic, o[dt][1] * ic), pack_f16x2(o[dt][2] * ic, o[dt][3] * ic));
-  if (g == 0) a.part_ml[prow] = make_float2(m + __log2f(c), l * ic);
-}
-
 // Row `row` of the unit, with its token and head found again rather than held through
 // the loop, which needs every register.
 template <int D>
@@ -430,8 +395,13 @@ __device__ __forceinline__ void finish_row(const ShArgs& a, const Unit& u, int k
   int index;
   const int tok = token_of(a, u, u.row0 + min(row, u.rows - 1), index);
   const int head = kvh * a.c.group + (u.row0 + row) % a.c.group;
-  const int64_t prow = u.part < 0 ? -1 : u.part + (int64_t)kvh * u.rows + row;
-  write_rows<D>(a, o, m, l, row < u.rows, prow, a.out + (int64_t)tok * a.o_ts + (int64_t)head * a.o_hs, g);
+  const bool live = row < u.rows;
+  if (u.part < 0) {              // the unit has all of the rows' keys
+    if (live) write_out<D>(a.out + (int64_t)tok * a.o_ts + (int64_t)head * a.o_hs, o, l, g);
+    return;
+  }
+  const int64_t prow = u.part + (int64_t)kvh * u.rows + row;
+  write_part<D>(a.part_o, a.part_ml, prow, o, m, l, live && prow < a.part_cap, g);
 }
 
 // A unit: K and V in tiles of 64 keys, staged once for the four waves in one of two
@@ -842,23 +812,20 @@ __device__ __forceinline__ void parts_of(const Entity& x, int r, int kvh, int hk
   at = x.part_base + (int64_t)tile * kUnitRows * x.cuts * hkv + (int64_t)kvh * rows + (r - tile * kUnitRows);
 }
 
-// W waves per row (token and query head): a wave's lanes weigh up to 64 parts at once,
-// then take the parts' values 64 / (D / 8) at a time, 8 dims each.  (One thread per 8
-// dims walking the parts one after another: 36 us for 256 rows of 36 parts, a memory
-// round trip each.)  Four waves where the rows are few, and their parts many.
+// W waves per row (token and query head).
 template <int D, int W>
 __global__ __launch_bounds__(256) void shared_join_kernel(ShArgs a) {
-  constexpr int LANES = D / 8, GROUPS = 64 / LANES;
-  __shared__ float part[W > 1 ? W : 1][LANES][8];
-  __shared__ float part_m[W > 1 ? W : 1], part_l[W > 1 ? W : 1];
-  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = blockIdx.x, head = W > 1 ? blockIdx.y : blockIdx.y * 4 + wid, c = lane % LANES, sub = lane / LANES;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = blockIdx.x, head = W > 1 ? blockIdx.y : blockIdx.y * 4 + wid;
   if (head >= a.hq) return;
-  uint16_t* op = a.out + (int64_t)t * a.o_ts + (int64_t)head * a.o_hs + 8 * c;
+  uint16_t* op = a.out + (int64_t)t * a.o_ts + (int64_t)head * a.o_hs;
   const int4 tk = a.tokreq[t];
   if (a.hdr[1] != 0) {                       // the lengths do not describe the step
-    const uint2 w = make_uint2(0x7fc07fc0u, 0x7fc07fc0u);
-    if (sub == 0) { *reinterpret_cast<uint2*>(op) = w; *reinterpret_cast<uint2*>(op + 4) = w; }
+    const int i = 8 * (threadIdx.x & 63);
+    if (i < D) {
+      *reinterpret_cast<uint2*>(op + i) = make_uint2(0x7fc07fc0u, 0x7fc07fc0u);
+      *reinterpret_cast<uint2*>(op + i + 4) = make_uint2(0x7fc07fc0u, 0x7fc07fc0u);
+    }
     return;
   }
   const int b = tk.x;
@@ -872,75 +839,7 @@ __global__ __launch_bounds__(256) void shared_join_kernel(ShArgs a) {
   int n0, n1 = 0;
   parts_of(own, tk.y * a.c.group + hh, kvh, a.hkv, at0, step0, n0);
   if (sh.rows > 0) parts_of(sh, (tk.w + tk.y) * a.c.group + hh, kvh, a.hkv, at1, step1, n1);
-  float m = -INFINITY, sum = 0.f, o[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) o[i] = 0.f;
-  // this wave's parts
-  const int first = W > 1 ? (int)((int64_t)(n0 + n1) * wid / W) : 0;
-  const int last = W > 1 ? (int)((int64_t)(n0 + n1) * (wid + 1) / W) : n0 + n1;
-  for (int p0 = first; p0 < last; p0 += 64) {
-    const int n = min(64, last - p0), p = p0 + lane;
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (lane < n) ml = a.part_ml[p < n0 ? at0 + p * step0 : at1 + (p - n0) * step1];
-    float top = ml.x;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    const float mnew = fmaxf(m, top);
-    // (a part without keys has -inf and 0; one that saw NaN alone -inf and NaN)
-    const float w = ml.x == -INFINITY && ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - mnew);
-    const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mnew);   // (nothing but NaN to scale then)
-    sum = sum * alpha + w * ml.y;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] *= alpha;
-    m = mnew;
-#pragma unroll 4
-    for (int i0 = 0; i0 < n; i0 += GROUPS) {
-      const int i = i0 + sub;
-      const float wi = __shfl(w, min(i, 63));          // (of all lanes: the last round has idle ones)
-      if (i >= n) continue;
-      const int q = p0 + i;
-      const uint4 y = *reinterpret_cast<const uint4*>(a.part_o + (q < n0 ? at0 + q * step0 : at1 + (q - n0) * step1) * D + 8 * c);
-      const uint32_t v[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const half2_t h = __builtin_bit_cast(half2_t, v[k]);
-        o[2 * k] += wi * (float)h[0];
-        o[2 * k + 1] += wi * (float)h[1];
-      }
-    }
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-#pragma unroll
-  for (int d = LANES; d < 64; d <<= 1)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] += __shfl_xor(o[i], d);
-  if (W > 1) {
-    if (sub == 0) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) part[wid][c][i] = o[i];
-      if (c == 0) { part_m[wid] = m; part_l[wid] = sum; }
-    }
-    __syncthreads();
-    if (wid != 0) return;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < W; ++w) top = fmaxf(top, part_m[w]);
-    sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float x = part_m[w] == -INFINITY && part_l[w] == 0.f ? 0.f : __builtin_amdgcn_exp2f(part_m[w] - top);
-      sum += x * part_l[w];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] += x * part[w][c][i];
-    }
-  }
-  if (sub != 0) return;
-  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : __builtin_nanf("");
-  *reinterpret_cast<uint2*>(op) = make_uint2(aia::pack_bf16x2(o[0] * inv, o[1] * inv), aia::pack_bf16x2(o[2] * inv, o[3] * inv));
-  *reinterpret_cast<uint2*>(op + 4) = make_uint2(aia::pack_bf16x2(o[4] * inv, o[5] * inv), aia::pack_bf16x2(o[6] * inv, o[7] * inv));
+  join_row<D, W>(a.part_o, a.part_ml, n0 + n1, [&](int i) { return i < n0 ? at0 + i * step0 : at1 + (i - n0) * step1; }, op);
 }
 
 int sh_check(const char* what, int32_t batch, int32_t tokens, int32_t hq, int32_t hkv, int32_t d, int32_t bs,

@@ -1,17 +1,24 @@
-// One wave's attention of up to 16 query rows to a run of listed cache blocks: the inner loop of the block-sparse kernel and of the shared-prefix
-// kernel's narrow units.  (Two row blocks per wave took 250 registers against 124, and
-// 28 us against 24 for 16 requests behind 4096 shared keys: two waves that share a
-// tile's bytes through the caches are the better use of a tile for 32 rows.)
+// One wave's attention of up to 16 query rows to a run of listed cache blocks: the
+// inner loop of the block-sparse kernels.
 //
 // Keys are numbered by their place in the list (place p: block p / bs of the list,
-// offset p % bs).  A wave takes them in tiles of 16: S^T = K Q^T with K straight
-// from memory to the MFMA's operand registers, an online softmax per row, and
-// O^T += V^T P^T with V staged in the wave's own LDS for the transposing reads.
-// No barriers: waves drift, so some load while others compute.  The next tile's
-// loads are in flight during a tile's math.
+// offset p % bs).  A wave takes them in steps of NT tiles of 16: S^T = K Q^T, an online
+// softmax per row, O^T += V^T P^T.  No barriers: waves drift, so some load while others
+// compute.  K of the next step is loaded behind the staging of this one's, V likewise,
+// so a step's bytes are in flight during the math of the one before.
+//
+// Rows come in whole (neighbouring lanes take neighbouring 16-byte pieces) and pass
+// through the wave's own LDS, K and V after each other in the same place, to where the
+// MFMA wants them.  Loaded straight into K's operand registers, neighbouring lanes have
+// different keys, and the L1 takes each lane's 16 bytes for an access of its own: it
+// then delivers 16 bytes a clock, 9 TB/s on the chip, which caps what the L2 holds.
+//
+// What a step costs beyond its bytes is the softmax's bookkeeping and addresses, so it
+// takes several tiles, and blocks of whole tiles (bs a multiple of 16) have their
+// addresses in scalar registers.
 #pragma once
 
-#include "gqa_attention.h"
+#include "row_parts.h"
 
 namespace {
 
@@ -39,14 +46,13 @@ struct RowState {
   __device__ __forceinline__ void finish() { l = aia::group4_sum(l); }
 };
 
-// Q operands: row n from qp (null: zeros), in the order that
-// attend() reads keys of the cache format in.
-template <int D, bool F8>
+// Q operands: row n from qp (null: zeros).
+template <int D>
 __device__ __forceinline__ void load_q(const uint16_t* qp, int g, uint4 (&qf)[D / 32]) {
 #pragma unroll
   for (int j = 0; j < D / 32; ++j) {
     qf[j] = make_uint4(0, 0, 0, 0);
-    if (qp) qf[j] = reinterpret_cast<const uint4*>(qp)[F8 ? 8 * (j >> 1) + 2 * g + (j & 1) : 4 * j + g];
+    if (qp) qf[j] = reinterpret_cast<const uint4*>(qp)[4 * j + g];
   }
 }
 
@@ -81,151 +87,155 @@ __device__ __forceinline__ void soften(float (&x)[NT][4], float scale_log2, floa
   m = mnew;
 }
 
-// Attends places [p0, p1) (p0 a multiple of 16) with rows qf; row n sees places up to
-// lim (lim_lo: the smallest of the valid rows', wave-uniform; places from p1 on are
-// seen by none).  id(i): the block id of list entry i, called with different i per
-// lane, 0 <= i < entries.  vt: kTile * kVStride values of the wave's own LDS (8-bit
-// caches: twice that).
-//
-// Values that are not finite: weights of masked keys are zero, but 0 x V is not
-// where V is an infinity or NaN.  Places from p1 on are replaced by zeros, and with
-// CARE (rows of different limits) a masked tile that holds such a value is
-// multiplied key by key.
-template <int D, bool F8, bool CARE, class Id>
-__device__ __forceinline__ void attend(const CacheArgs& a, int kvh, const uint4 (&qf)[D / 32], int lim,
-                                       int lim_lo, int p0, int p1, int entries, Id id, uint16_t* vt,
-                                       int lane, RowState<D>& s) {
-  constexpr int KJ = D / 32, DT = D / 16, CH = D / 64;
-  constexpr int NT = F8 ? 2 : 1;             // 16-key tiles per step
-  constexpr int LD = F8 ? CH : KJ;           // 16-byte loads per key row and lane
+// Attends places [p0, p1) (p0 a multiple of 16) with rows qf, which all see them all.
+// id(i): the block id of list entry i, called with different i per lane, 0 <= i <
+// entries.  vt: kStep values of the wave's own LDS.  V behind p1 counts as zeros: a
+// weight of zero times an infinity or NaN there would not be zero.
+constexpr int kNt = 2;                           // tiles per step
+constexpr int kStep = kNt * kTile * kVStride;        // K or V values of a step in LDS
+
+template <int D, bool F8, bool WHOLE, class Id>
+__device__ __forceinline__ void attend(const CacheArgs& a, int kvh, const uint4 (&qf)[D / 32], int p0, int p1,
+                                       int entries, Id id, uint16_t* lds, int lane, RowState<D>& s) {
+  constexpr int KJ = D / 32, DT = D / 16, CELL = F8 ? 1 : 2;
+  constexpr int CPR = D * CELL / 16;         // 16-byte pieces of a key
+  constexpr int RPL = 64 / CPR, LD = kTile / RPL;      // keys per load of the wave, loads per tile
   const int n = lane & 15, g = lane >> 4;
+  const int lr = lane / CPR, lc = lane % CPR;          // this lane's key and piece of a load
+  p0 = __builtin_amdgcn_readfirstlane(p0);
+  p1 = __builtin_amdgcn_readfirstlane(p1);
+  entries = __builtin_amdgcn_readfirstlane(entries);
   if (p0 >= p1) return;
-  const int64_t row_elems = (int64_t)a.hkv * D;
+  const int row_bytes = a.hkv * D * CELL, head_bytes = kvh * D * CELL;
+  const uint8_t* kc = reinterpret_cast<const uint8_t*>(a.kc) + head_bytes + 16 * lc;
+  const uint8_t* vc = reinterpret_cast<const uint8_t*>(a.vc) + head_bytes + 16 * lc;
   int base = 0, bend = 0, ids = 0, sev = 0;  // list entries held by the lanes: [base, bend)
+  int end = 0;                               // places of the window
 
-  auto load = [&](int tile, uint4 (&kk)[LD], uint4 (&vv)[LD], int& at) {
-    // (tiles past the window read its first row again: an L1 hit)
-    const int place = tile * kTile < p1 && tile * kTile < bend * a.bs ? min(tile * kTile + n, p1 - 1) : base * a.bs;
-    const int e = place / a.bs;
-    at = e - base;
-    const int blk = __shfl(ids, at);
-    const int64_t row = ((int64_t)blk * a.bs + (place - e * a.bs)) * row_elems + (int64_t)kvh * D;
-    if constexpr (F8) {
-      const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.kc) + row + 16 * g;
-      const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.vc) + row + 16 * g;
+  uint4 kk[kNt][LD], vv[kNt][LD];
+  int64_t at[kNt][WHOLE ? 1 : LD];           // byte offsets of the rows being loaded
+  int off[kNt][WHOLE ? LD : 1];
+  int ek[kNt][WHOLE ? 1 : LD], ev[kNt][WHOLE ? 1 : LD];      // 8-bit caches: scales of the keys in kk, vv
+  // Tiles behind the window read its first row again (an L1 hit); keys behind the end
+  // the last one (never a slot that may hold stale bytes).
+  auto load_k = [&](int t) {
 #pragma unroll
-      for (int j = 0; j < LD; ++j) kk[j] = *reinterpret_cast<const uint4*>(kp + 64 * j);
+    for (int st = 0; st < kNt; ++st) {
+      const int first = (t + st) * kTile;
+      const bool in = first < end;
+      if (WHOLE) {
+        const int p = in ? first : base * a.bs, e = p / a.bs;
+        const int blk = __builtin_amdgcn_readlane(ids, e - base);
+        if (F8) ek[st][0] = __builtin_amdgcn_readlane(sev, e - base);
+        at[st][0] = ((int64_t)blk * a.bs + (p - e * a.bs)) * row_bytes;
+        const int last = in ? end - 1 - first : 0;
 #pragma unroll
-      for (int j = 0; j < LD; ++j) vv[j] = *reinterpret_cast<const uint4*>(vp + 64 * j);
-    } else {
-      const uint4* kp = reinterpret_cast<const uint4*>(a.kc + row) + g;
-      const uint4* vp = reinterpret_cast<const uint4*>(a.vc + row) + g;
-#pragma unroll
-      for (int j = 0; j < LD; ++j) kk[j] = kp[4 * j];
-#pragma unroll
-      for (int j = 0; j < LD; ++j) vv[j] = vp[4 * j];
-    }
-  };
-
-  auto compute = [&](int tile, const uint4 (&kk)[NT][LD], uint4 (&vv)[NT][LD], const int (&at)[NT], int end) {
-    const int tb = tile * kTile;
-    const bool masked = tb + NT * kTile - 1 > lim_lo || tb + NT * kTile > end;
-    uint32_t odd = 0;
-    if (masked) {
-#pragma unroll
-      for (int st = 0; st < NT; ++st)
-#pragma unroll
-        for (int j = 0; j < LD; ++j) {
-          if (tb + kTile * st + n >= end) vv[st][j] = make_uint4(0, 0, 0, 0);
-          if (CARE) odd = F8 ? nan_fp8(vv[st][j], odd) : not_finite_bf16(vv[st][j], odd);
-        }
-      odd &= F8 ? 0x80808080u : 0x80008000u;
-    }
-    float4_t acc[NT];
-#pragma unroll
-    for (int st = 0; st < NT; ++st) {
-      uint4 kf[KJ];
-      if constexpr (F8) {
-        const int e = __shfl(sev, at[st]);
-#pragma unroll
-        for (int j = 0; j < CH; ++j) {
-          uint4 x[2];
-          fp8_to_bf16(kk[st][j], e & 0xff, x);
-          kf[2 * j] = x[0];
-          kf[2 * j + 1] = x[1];
-          fp8_to_bf16(vv[st][j], (e >> 8) & 0xff, x);
-          uint16_t* to = vt + (st * kTile + n) * kVStride + 64 * j + 16 * g;
-          *reinterpret_cast<u32x4_t*>(to) = as_u4(x[0]);
-          *reinterpret_cast<u32x4_t*>(to + 8) = as_u4(x[1]);
+        for (int i = 0; i < LD; ++i) {
+          off[st][i] = min(i * RPL + lr, last) * row_bytes;
+          kk[st][i] = *reinterpret_cast<const uint4*>(kc + at[st][0] + off[st][i]);
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < KJ; ++j) kf[j] = kk[st][j];
-        stage_v(vt + st * kTile * kVStride, n, g, vv[st]);
+        for (int i = 0; i < LD; ++i) {
+          const int p = in ? min(first + i * RPL + lr, end - 1) : base * a.bs, e = p / a.bs;
+          const int blk = __shfl(ids, e - base);
+          if (F8) ek[st][i] = __shfl(sev, e - base);
+          at[st][i] = ((int64_t)blk * a.bs + (p - e * a.bs)) * row_bytes;
+          kk[st][i] = *reinterpret_cast<const uint4*>(kc + at[st][i]);
+        }
       }
-      acc[st] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < KJ; ++j) acc[st] = qk_step(kf[j], qf[j], acc[st]);
     }
-    uint2 pb[NT];
-    float x[NT][4];
-    const int last = min(lim, end - 1) - tb - 4 * g;
+  };
+  auto load_v = [&]() {
 #pragma unroll
-    for (int st = 0; st < NT; ++st)
+    for (int st = 0; st < kNt; ++st)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) x[st][v] = !masked || kTile * st + v <= last ? acc[st][v] : -INFINITY;
-    soften<NT, DT>(x, a.scale_log2, s.m, s.l, s.o);
-#pragma unroll
-    for (int st = 0; st < NT; ++st)
-      pb[st] = make_uint2(aia::pack_bf16x2(x[st][0], x[st][1]), aia::pack_bf16x2(x[st][2], x[st][3]));
-    __builtin_amdgcn_wave_barrier();
-    if (CARE && masked && __any(odd)) {
-      for (int k = 0; k < NT * kTile; ++k) {
-        const uint2 w = NT == 1 || k < kTile ? pb[0] : pb[NT - 1];
-        const float p = weight_of(k & 2 ? w.y : w.x, n, k);
-        if (tb + k <= lim && tb + k < end)
-          add_key(s.o, p, [&](int dt) { return vt + k * kVStride + 16 * dt + 4 * g; });
+      for (int i = 0; i < LD; ++i) {
+        if (F8) ev[st][WHOLE ? 0 : i] = ek[st][WHOLE ? 0 : i];
+        vv[st][i] = *reinterpret_cast<const uint4*>(vc + at[st][WHOLE ? 0 : i] + (WHOLE ? off[st][i] : 0));
       }
-      __builtin_amdgcn_wave_barrier();
-      return;
-    }
+  };
+  // rows of a tile into LDS, as bf16
+  auto stage = [&](int st, const uint4 (&w)[LD], const int (&e8)[WHOLE ? 1 : LD], int shift) {
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) {
-      const short4_t v0 = vt_frag(vt, n, g, dt);
+    for (int i = 0; i < LD; ++i) {
+      uint16_t* to = lds + (st * kTile + i * RPL + lr) * kVStride;
       if constexpr (F8) {
-        const short4_t v1 = vt_frag(vt + kTile * kVStride, n, g, dt);
-        const bf16x8_t va = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-        s.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            va, as_b8(make_uint4(pb[0].x, pb[0].y, pb[1].x, pb[1].y)), s.o[dt], 0, 0, 0);
+        uint4 x[2];
+        fp8_to_bf16(w[i], (e8[WHOLE ? 0 : i] >> shift) & 0xff, x);
+        *reinterpret_cast<u32x4_t*>(to + 16 * lc) = as_u4(x[0]);
+        *reinterpret_cast<u32x4_t*>(to + 16 * lc + 8) = as_u4(x[1]);
       } else {
-        s.o[dt] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v0, as_s4(pb[0].x, pb[0].y), s.o[dt], 0, 0, 0);
+        *reinterpret_cast<u32x4_t*>(to + 8 * lc) = as_u4(w[i]);
       }
     }
-    __builtin_amdgcn_wave_barrier();
   };
 
-  uint4 kbuf[NT][LD], vbuf[NT][LD];
-  int at[NT];
   for (int t0 = p0 / kTile, t_end = (p1 + kTile - 1) / kTile; t0 < t_end;) {
     base = t0 * kTile / a.bs;
     bend = min(base + 64, entries);
     // tiles whose places all fall into the window (the last: up to p1)
-    const int t1 = bend >= entries ? t_end : min(t_end, bend * a.bs / kTile);
-    const int end = min(p1, t1 * kTile);
+    const int t1 = bend >= entries ? t_end : min(t_end, (int)((int64_t)bend * a.bs / kTile));
+    end = min(p1, t1 * kTile);
     // ids outside the pool are clamped, so that a bad table cannot fault
     ids = base + lane < bend ? min(max(id(base + lane), 0), a.nb - 1) : 0;
-    if constexpr (F8) {
+    if (F8) {
       const int64_t se = (int64_t)ids * a.hkv + kvh;
       sev = a.ks[se] | a.vs[se] << 8;
     }
+    load_k(t0);
+    load_v();
+    for (int t = t0; t < t1; t += kNt) {
+      const int tb = t * kTile;
+      const bool masked = tb + kNt * kTile > end;
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int st = 0; st < NT; ++st) load(t0 + st, kbuf[st], vbuf[st], at[st]);
-    __builtin_amdgcn_sched_barrier(0);
-    for (int t = t0; t < t1; t += NT) {
-      compute(t, kbuf, vbuf, at, end);
+      for (int st = 0; st < kNt; ++st) stage(st, kk[st], ek[st], 0);
+      const bool more = t + kNt < t1;
+      if (more) load_k(t + kNt);
+      __builtin_amdgcn_wave_barrier();
+      float4_t acc[kNt];
 #pragma unroll
-      for (int st = 0; st < NT; ++st) load(t + NT + st, kbuf[st], vbuf[st], at[st]);
+      for (int st = 0; st < kNt; ++st) {
+        acc[st] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < KJ; ++j)
+          acc[st] = qk_step(*reinterpret_cast<const uint4*>(lds + (st * kTile + n) * kVStride + 32 * j + 8 * g), qf[j], acc[st]);
+      }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int st = 0; st < kNt; ++st) {
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < LD; ++i)
+            if (tb + kTile * st + i * RPL + lr >= end) vv[st][i] = make_uint4(0, 0, 0, 0);
+        }
+        stage(st, vv[st], ev[st], 8);
+      }
+      if (more) load_v();
       __builtin_amdgcn_sched_barrier(0);
+      float x[kNt][4];
+      const int last = end - 1 - tb - 4 * g;
+#pragma unroll
+      for (int st = 0; st < kNt; ++st)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) x[st][v] = !masked || kTile * st + v <= last ? acc[st][v] : -INFINITY;
+      soften<kNt, DT>(x, a.scale_log2, s.m, s.l, s.o);
+      uint4 pb[kNt / 2];
+#pragma unroll
+      for (int p = 0; p < kNt / 2; ++p)
+        pb[p] = make_uint4(aia::pack_bf16x2(x[2 * p][0], x[2 * p][1]), aia::pack_bf16x2(x[2 * p][2], x[2 * p][3]),
+                           aia::pack_bf16x2(x[2 * p + 1][0], x[2 * p + 1][1]), aia::pack_bf16x2(x[2 * p + 1][2], x[2 * p + 1][3]));
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int p = 0; p < kNt / 2; ++p)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          const short4_t v0 = vt_frag(lds + 2 * p * kTile * kVStride, n, g, dt);
+          const short4_t v1 = vt_frag(lds + (2 * p + 1) * kTile * kVStride, n, g, dt);
+          const bf16x8_t va = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+          s.o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, as_b8(pb[p]), s.o[dt], 0, 0, 0);
+        }
     }
     t0 = t1;
   }

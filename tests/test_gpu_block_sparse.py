@@ -192,12 +192,15 @@ def random_selection(s, selected, seed):
     return out
 
 
-def check_attention(s, sel, out, scale):
+def check_attention(s, sel, out, scale, tokens=None):
     """Within the roundings: weights and the output are rounded to bf16 (2^-8 relative
-    each), so |error| <= 2^-8 sum p |v| + 2^-8 |out|; the float32 sums and exponentials
-    are allowed as much again."""
+    each), parts of a row to fp16 (2^-11 of the part's largest value, at most the
+    largest |v|), so |error| <= 2^-8 sum p |v| + 2^-8 |out| + 2^-11 max |v|; the float32
+    sums and exponentials are allowed as much again."""
     hq, hkv, bs = s["hq"], s["hkv"], s["bs"]
     for t, r, pos in tokens_of(s):
+        if tokens is not None and t not in tokens:
+            continue
         rows = s["table"][r].long()
         n = max(0, pos + 1)
         nblk = -(-n // bs)
@@ -213,7 +216,8 @@ def check_attention(s, sel, out, scale):
                 head = h * (hq // hkv) + j
                 want = ref.attention(s["q"][t, head], k[:, h], v[:, h], seen, scale)
                 size = ref.attention(s["q"][t, head], k[:, h], v[:, h].abs(), seen, scale)
-                bound = 2.0 ** -7 * (size + want.abs()) + 1e-30
+                most = float(v[seen, h].abs().max()) if bool(seen.any()) else 0.0
+                bound = 2.0 ** -7 * (size + want.abs()) + 2.0 ** -10 * most + 1e-30
                 assert bool(((out[t, head].double() - want).abs() <= bound).all()), (t, head)
 
 
@@ -277,6 +281,32 @@ def test_split_rows_equal_long_lists():
     sel[0, 0] = torch.arange(250, dtype=torch.int32) + 31
     out = ops.paged_attention_sparse(g["q"], g["kc"], g["vc"], make_plan(g, 250), sel.to(DEV), 128 ** -0.5)
     check_attention(s, sel, out.cpu(), 128 ** -0.5)
+
+
+@pytest.mark.parametrize("hq,hkv,d,bs,fp8", [(4, 2, 128, 16, False), (7, 1, 128, 64, True), (40, 2, 64, 32, False),
+                                             (6, 3, 64, 128, True), (2, 2, 128, 24, False)])
+def test_long_chunks_take_the_context_in_ranges(hq, hkv, d, bs, fp8):
+    from auto_infer_amd import ops
+    s = make([(90, 13000), (3, 9001), (40, 40)], hq, hkv, d, bs, fp8, seed=11, spread=False)
+    g = on_gpu(s)
+    selected = 1500 // bs
+    sel = random_selection(s, selected, 9)
+    sel[5] = -1                                       # a token without a block
+    sel[6, :, 1:] = -1                                # and with one
+    out = ops.paged_attention_sparse(g["q"], g["kc"], g["vc"], make_plan(g, selected), sel.to(DEV), d ** -0.5,
+                                     key_scale=g["ks"], value_scale=g["vs"]).cpu()
+    assert bool((out[5] == 0).all())
+    check_attention(s, sel, out, d ** -0.5, tokens=set(range(0, 95, 7)) | {5, 6, 89, 90, 92, 93, 132})
+
+
+def test_chunks_of_several_launches():
+    from auto_infer_amd import ops
+    s = make([(1700, 7000)], 16, 16, 64, 16, seed=12, spread=False)
+    g = on_gpu(s)
+    gen = torch.Generator().manual_seed(1)
+    sel = torch.rand(1700, 16, 270, generator=gen).topk(20, dim=-1).indices.sort(-1).values.int()
+    out = ops.paged_attention_sparse(g["q"], g["kc"], g["vc"], make_plan(g, 20), sel.to(DEV), 0.125).cpu()
+    check_attention(s, sel, out, 0.125, tokens={0, 1, 511, 512, 900, 1023, 1024, 1400, 1699})
 
 
 def test_tokens_that_no_request_covers():
