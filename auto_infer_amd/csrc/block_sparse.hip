@@ -301,60 +301,53 @@ struct ScoreKernelArgs {
   int64_t bt_stride;
   const int4* tok;
   float* scores;             // (tokens of this launch, hkv, width)
-  int32_t t0, t1, hkv, group, nb, width, chunk, per;   // tokens [t0, t1), blocks per work-group, tokens per tile
+  int32_t t0, t1, hkv, group, nb, width;               // tokens [t0, t1)
+  int32_t lanes, per, tiles, heads, chunk;             // see score_kernel
 };
 
-// One work-group: the 16 query rows of up to `per` tokens of one KV head (per token
-// `lanes` rows, the group's heads padded to a power of two; groups of more than 16
-// heads take 16 at a time) against `chunk` blocks.  S = Q B^T on v_mfma_i32_16x16x64_i8:
-// lane (row or block n, group g) holds bytes 64 j + 16 g .. of [q+ (D), q- (D)] and of
-// [hi, nlo]; the four accumulators are rows 4 g .. 4 g + 3 of block n.  Tokens of
-// several requests in one tile are taken one request at a time.
+// One work-group: `tiles` tiles of 16 query rows, each of `per` tokens (per token `lanes`
+// rows, the group's heads padded to a power of two; groups of more than 16 heads take 16
+// at a time, a token per tile), for `heads` KV heads, against `chunk` blocks.  Its four
+// waves are dealt to the KV heads and, where there are fewer, to 64 blocks each.
+//   The queries become whole numbers in LDS first, in MFMA order; then each wave holds 64
+// blocks' bounds in registers and goes over the tiles: S = Q B^T on
+// v_mfma_i32_16x16x64_i8, lane (row or block n, group g) with bytes 64 j + 16 g .. of
+// [q+ (D), q- (D)] and of [hi, nlo]; the four accumulators are rows 4 g .. 4 g + 3 of
+// block n.  Tokens of several requests are taken one request at a time.
+//   Few tokens: one tile, several KV heads, whose bounds of a block are neighbours in
+// memory; many tokens: many tiles of one KV head, so the bounds are read once for them.
 template <int D>
 __global__ __launch_bounds__(kSparseThreads) void score_kernel(ScoreKernelArgs a) {
   constexpr int KS = 2 * D / 64;             // MFMA steps
-  extern __shared__ uint4 qfrag[];           // [head block][step][lane]
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  extern __shared__ uint4 qfrag[];           // [KV head][tile][head block][step][lane]
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int kvh = blockIdx.y;
-  int lanes = 1;
-  while (lanes < a.group && lanes < 16) lanes <<= 1;
-  const int hblocks = (a.group + 15) / 16;
-  const int tb = a.t0 + blockIdx.x * a.per;
-  const int tokens = min(a.per, a.t1 - tb);
-  // rows of the first head block: token n / lanes, head n % lanes
-  const int tn = n / lanes, hn = n - tn * lanes;
-  int done = 0;
-  while (done < tokens) {
-    const int4 lead = a.tok[tb + done];
-    int same = done + 1, vis = lead.z;       // tokens [done, same) of one request
-    while (same < tokens) {
-      const int4 x = a.tok[tb + same];
-      if (x.x != lead.x) break;
-      vis = max(vis, x.z);
-      ++same;
-    }
-    const int from = done;
-    done = same;
-    const int c0 = blockIdx.z * a.chunk, c1 = min(vis, c0 + a.chunk);
-    if (lead.x < 0 || c0 >= c1) continue;
-    __syncthreads();
-    // largest finite |q| of each token's heads
-    uint32_t amax = 0;
+  const int lanes = a.lanes, hblocks = (a.group + 15) / 16;
+  const int tb = a.t0 + blockIdx.x * a.per * a.tiles;
+  const int tokens = min(a.per * a.tiles, a.t1 - tb);
+  const int c0 = blockIdx.z * a.chunk;
+  // (nothing to do where no token sees the chunk's blocks)
+  int see = 0;
+  for (int i = lane; i < tokens; i += 64) see = max(see, a.tok[tb + i].z);
+  if (__ballot(see > c0) == 0) return;
+  const int tn = n / lanes, hn = n - tn * lanes;       // this lane's row: token of the tile, head
+  for (int u = wid; u < a.heads * a.tiles; u += kSparseThreads / 64) {
+    const int kvh = blockIdx.y * a.heads + u / a.tiles, ti = u % a.tiles * a.per + tn;
+    const bool row = ti < tokens && kvh < a.hkv && tn < a.per;
+    const uint16_t* qt = a.q + (int64_t)(tb + ti) * a.q_ts + (int64_t)kvh * a.group * a.q_hs;
+    uint32_t amax = 0;                       // largest finite |q| of the token's heads
     for (int hb = 0; hb < hblocks; ++hb) {
-      const int head = hn + 16 * hb;
-      if (tn >= from && tn < same && head < a.group) {
-        const uint16_t* qp = a.q + (int64_t)(tb + tn) * a.q_ts + (int64_t)(kvh * a.group + head) * a.q_hs;
+      if (!row || hn + 16 * hb >= a.group) continue;
+      const uint4* qp = reinterpret_cast<const uint4*>(qt + (int64_t)(hn + 16 * hb) * a.q_hs);
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          const uint4 w = reinterpret_cast<const uint4*>(qp)[4 * j + g];
-          const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+      for (int j = 0; j < D / 32; ++j) {
+        const uint4 w = qp[4 * j + g];
+        const uint32_t p[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t lo = p[i] & 0x7fffu, up = (p[i] >> 16) & 0x7fffu;
-            amax = max(amax, lo < 0x7f80u ? lo : 0u);
-            amax = max(amax, up < 0x7f80u ? up : 0u);
-          }
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t lo = p[i] & 0x7fffu, up = (p[i] >> 16) & 0x7fffu;
+          amax = max(amax, lo < 0x7f80u ? lo : 0u);
+          amax = max(amax, up < 0x7f80u ? up : 0u);
         }
       }
     }
@@ -362,10 +355,9 @@ __global__ __launch_bounds__(kSparseThreads) void score_kernel(ScoreKernelArgs a
     amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
     amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
     const float f = __builtin_ldexpf(1.f, -bound_exp(amax));
-    for (int hb = wid; hb < hblocks; hb += kSparseThreads / 64) {
-      const int head = hn + 16 * hb;
-      const bool live = tn >= from && tn < same && head < a.group;
-      const uint16_t* qp = a.q + (int64_t)(tb + tn) * a.q_ts + (int64_t)(kvh * a.group + head) * a.q_hs;
+    for (int hb = 0; hb < hblocks; ++hb) {
+      const bool live = row && hn + 16 * hb < a.group;
+      const uint16_t* qp = qt + (int64_t)(hn + 16 * hb) * a.q_hs;
 #pragma unroll
       for (int j = 0; j < KS / 2; ++j) {
         uint32_t pos[4] = {0, 0, 0, 0}, neg[4] = {0, 0, 0, 0};
@@ -382,52 +374,72 @@ __global__ __launch_bounds__(kSparseThreads) void score_kernel(ScoreKernelArgs a
             neg[2 * half + (i >> 2)] |= (uint32_t)max(-v, 0) << (8 * (i & 3));
           }
         }
-        qfrag[(hb * KS + j) * 64 + lane] = make_uint4(pos[0], pos[1], pos[2], pos[3]);
-        qfrag[(hb * KS + KS / 2 + j) * 64 + lane] = make_uint4(neg[0], neg[1], neg[2], neg[3]);
+        uint4* to = qfrag + (int64_t)((u * hblocks + hb) * KS) * 64 + lane;
+        to[j * 64] = make_uint4(pos[0], pos[1], pos[2], pos[3]);
+        to[(KS / 2 + j) * 64] = make_uint4(neg[0], neg[1], neg[2], neg[3]);
       }
     }
-    __syncthreads();
+  }
+  __syncthreads();
+  const int hw = wid % a.heads, kvh = blockIdx.y * a.heads + hw;
+  if (wid >= kSparseThreads / 64 / a.heads * a.heads || kvh >= a.hkv) return;
+  const int stride = 64 * (kSparseThreads / 64 / a.heads), own = 64 * (wid / a.heads);
+  auto frag = [&](int m, int hb, int j) {
+    return __builtin_bit_cast(int4v_t, as_u4(qfrag[(((hw * a.tiles + m) * hblocks + hb) * KS + j) * 64 + lane]));
+  };
+  for (int done = 0; done < tokens;) {
+    const int4 lead = a.tok[tb + done];
+    const int from = done;
+    int vis = 0;                             // tokens [from, done) of one request
+    while (done < tokens) {
+      const int4 x = a.tok[tb + done];
+      if (x.x != lead.x) break;
+      vis = max(vis, x.z);
+      ++done;
+    }
+    const int c1 = min(vis, c0 + a.chunk);
+    if (lead.x < 0) continue;
     const int32_t* btrow = a.bt + (int64_t)lead.x * a.bt_stride;
-    auto step = [&](int hb, int j) { return __builtin_bit_cast(int4v_t, as_u4(qfrag[(hb * KS + j) * 64 + lane])); };
-    int4v_t qf[KS];
-#pragma unroll
-    for (int j = 0; j < KS; ++j) qf[j] = step(0, j);
-    for (int b0 = c0 + 64 * wid; b0 < c1; b0 += kSparseThreads) {
+    for (int b0 = c0 + own; b0 < c1; b0 += stride) {
       const int id = b0 + lane < c1 ? min(max(btrow[b0 + lane], 0), a.nb - 1) : 0;
       const int ebyte = a.scale[(int64_t)id * a.hkv + kvh];
-      uint4 bf[4][KS];
+      int4v_t bf[4][KS];
+      int eb[4];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         const int blk = __shfl(id, 16 * s + n);
+        eb[s] = __shfl(ebyte, 16 * s + n) - 127;
         const uint4* bp = reinterpret_cast<const uint4*>(a.bounds + ((int64_t)blk * a.hkv + kvh) * 2 * D) + g;
 #pragma unroll
-        for (int j = 0; j < KS; ++j) bf[s][j] = bp[4 * j];
+        for (int j = 0; j < KS; ++j) bf[s][j] = __builtin_bit_cast(int4v_t, as_u4(bp[4 * j]));
       }
+      for (int m = from / a.per; m * a.per < done; ++m) {
+        int4v_t acc[4];
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        int4v_t acc = {0, 0, 0, 0};
+        for (int s = 0; s < 4; ++s) acc[s] = int4v_t{0, 0, 0, 0};
+        for (int hb = 0; hb < hblocks; ++hb) {
 #pragma unroll
-        for (int j = 0; j < KS; ++j)
-          acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf[j], __builtin_bit_cast(int4v_t, as_u4(bf[s][j])), acc, 0, 0, 0);
-        for (int hb = 1; hb < hblocks; ++hb)
+          for (int j = 0; j < KS; ++j) {
+            const int4v_t qf = frag(m, hb, j);
 #pragma unroll
-          for (int j = 0; j < KS; ++j)
-            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(step(hb, j), __builtin_bit_cast(int4v_t, as_u4(bf[s][j])), acc, 0, 0, 0);
-        // sums over a token's rows: `lanes` of the rows 4 g + v
-        if (lanes > 1) { acc[0] += acc[1]; acc[2] += acc[3]; }
-        if (lanes > 2) acc[0] += acc[2];
-        if (lanes > 4) acc[0] += __shfl_xor(acc[0], 16);
-        if (lanes > 8) acc[0] += __shfl_xor(acc[0], 32);
-        const int blk = b0 + 16 * s + n;
-        const int eb = __shfl(ebyte, 16 * s + n) - 127;
+            for (int s = 0; s < 4; ++s) acc[s] = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf, bf[s][j], acc[s], 0, 0, 0);
+          }
+        }
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const int row = 4 * g + v;
-          if (row % lanes) continue;
-          const int t = row / lanes;
-          if (t < from || t >= same || blk >= c1) continue;
-          const int sum = v == 0 ? acc[0] : v == 1 ? acc[1] : v == 2 ? acc[2] : acc[3];
-          a.scores[((int64_t)(tb + t - a.t0) * a.hkv + kvh) * a.width + blk] = __builtin_ldexpf((float)sum, eb);
+        for (int s = 0; s < 4; ++s) {
+          // sums over a token's rows: `lanes` of the rows 4 g + v
+          int sum[4] = {acc[s][0], acc[s][1], acc[s][2], acc[s][3]};
+          if (lanes > 1) { sum[0] += sum[1]; sum[2] += sum[3]; }
+          if (lanes > 2) sum[0] += sum[2];
+          if (lanes > 4) sum[0] += __shfl_xor(sum[0], 16);
+          if (lanes > 8) sum[0] += __shfl_xor(sum[0], 32);
+          const int blk = b0 + 16 * s + n;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int r = 4 * g + v, t = m * a.per + r / lanes;
+            if (r % lanes || t < from || t >= done || r / lanes >= a.per || blk >= c1) continue;
+            a.scores[((int64_t)(tb + t - a.t0) * a.hkv + kvh) * a.width + blk] = __builtin_ldexpf((float)sum[v], eb[s]);
+          }
         }
       }
     }
@@ -441,48 +453,111 @@ struct SelectArgs {
   const int4* tok;
   int32_t* out;
   int64_t out_ts, out_hs;
-  int32_t t0, hkv, width, selected, sink, local;
+  int32_t t0, rows, hkv, width, selected, sink, local;         // rows (token, KV head) from t0 on
 };
+
+// A score's order as an unsigned key; 0xffffffff: blocks that are always kept.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return min(u & 0x80000000u ? ~u : u | 0x80000000u, 0xfffffffeu);
+}
+__device__ __forceinline__ uint32_t key_at(const SelectArgs& a, const float* sc, int i, int n) {
+  if (i >= n) return 0;
+  return i < a.sink || i >= n - a.local ? 0xffffffffu : order_key(sc[i]);
+}
+
+// A wave per row, for tables of up to 64 NK blocks: the key of the `selected`-th largest
+// score bit by bit from the top, counting by ballots, until a bound has exactly so many
+// above it; then the blocks above it and the first of those at it, in order.  No
+// barriers, no LDS.  (A work-group per row that counts digits in LDS: 17.0 us for 2048
+// rows of 513 blocks.)
+template <int NK>
+__global__ __launch_bounds__(256) void select_wave_kernel(SelectArgs a) {
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = blockIdx.x * 4 + wid;
+  if (row >= a.rows) return;
+  const int t = row / a.hkv, kvh = row - t * a.hkv;
+  const int n = __builtin_amdgcn_readfirstlane(a.tok[a.t0 + t].z);
+  int32_t* out = a.out + (int64_t)(a.t0 + t) * a.out_ts + (int64_t)kvh * a.out_hs;
+  if (n <= a.selected) {
+    for (int i = lane; i < a.selected; i += 64) out[i] = i < n ? i : -1;
+    return;
+  }
+  const float* sc = a.scores + (int64_t)row * a.width;
+  uint32_t k[NK];
+#pragma unroll
+  for (int j = 0; j < NK; ++j) k[j] = key_at(a, sc, 64 * j + lane, n);
+  // (keys behind the row's end are 0, below every bound that is tried)
+  uint32_t p = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t bound = p | 1u << bit;
+    int count = 0;
+#pragma unroll
+    for (int j = 0; j < NK; ++j) count += __popcll(__ballot(k[j] >= bound));
+    if (count >= a.selected) p = bound;
+    if (count == a.selected) break;
+  }
+  int above = 0;
+#pragma unroll
+  for (int j = 0; j < NK; ++j) above += __popcll(__ballot(k[j] > p));
+  const int need = a.selected - above;       // of the blocks at the bound
+  const uint64_t below = (1ull << lane) - 1;
+  int at = 0, tied = 0;
+#pragma unroll
+  for (int j = 0; j < NK; ++j) {
+    const bool up = k[j] > p, eq = k[j] == p && 64 * j + lane < n;
+    const uint64_t mu = __ballot(up), me = __ballot(eq);
+    const int ub = at + __popcll(mu & below), eb = tied + __popcll(me & below);
+    if (up || (eq && eb < need)) out[ub + min(eb, need)] = 64 * j + lane;
+    at += __popcll(mu);
+    tied += __popcll(me);
+  }
+}
 
 constexpr int kSelThreads = 512, kSelWaves = kSelThreads / 64;
 constexpr int kDigits = 2048;
 
-// A score's order as an unsigned key, 0xffffffff for blocks that are always kept.
-__device__ __forceinline__ uint32_t order_key(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-
-// One work-group per (token, KV head): the key of the `selected`-th largest score,
-// 11 bits at a time by counting, then the blocks above it and the first of those at it,
-// in order.
+// A work-group per row, for longer tables: the same key by 11 bits at a time, counted in
+// LDS.  A wave has a run of the row's blocks, up to 64 NK of them in registers (NK 0:
+// any number, read again in every pass).
+template <int NK>
 __global__ __launch_bounds__(kSelThreads) void select_kernel(SelectArgs a) {
   __shared__ int hist[kDigits];
-  __shared__ int wave_a[kSelWaves], wave_b[kSelWaves], found[2];
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const int t = a.t0 + blockIdx.x, kvh = blockIdx.y;
-  const int n = a.tok[t].z;
-  int32_t* out = a.out + (int64_t)t * a.out_ts + (int64_t)kvh * a.out_hs;
+  __shared__ int wave_a[kSelWaves], wave_b[kSelWaves], found[3];
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int t = blockIdx.x / a.hkv, kvh = blockIdx.x - t * a.hkv;
+  const int n = __builtin_amdgcn_readfirstlane(a.tok[a.t0 + t].z);
+  int32_t* out = a.out + (int64_t)(a.t0 + t) * a.out_ts + (int64_t)kvh * a.out_hs;
   if (n <= a.selected) {
     for (int i = tid; i < a.selected; i += kSelThreads) out[i] = i < n ? i : -1;
     return;
   }
-  const float* sc = a.scores + ((int64_t)blockIdx.x * a.hkv + kvh) * a.width;
-  auto key_at = [&](int i) -> uint32_t {
-    if (i < a.sink || i >= n - a.local) return 0xffffffffu;
-    return min(order_key(sc[i]), 0xfffffffeu);
+  const float* sc = a.scores + (int64_t)blockIdx.x * a.width;
+  const int rounds = (n + kSelThreads - 1) / kSelThreads, first = wid * 64 * rounds + lane;
+  uint32_t held[NK > 0 ? NK : 1];
+#pragma unroll
+  for (int j = 0; j < NK; ++j) held[j] = j < rounds ? key_at(a, sc, first + 64 * j, n) : 0;
+  auto each = [&](auto f) {
+    if constexpr (NK > 0) {
+#pragma unroll
+      for (int j = 0; j < NK; ++j)
+        if (j < rounds) f(first + 64 * j, held[j]);
+    } else {
+      for (int j = 0; j < rounds; ++j) f(first + 64 * j, key_at(a, sc, first + 64 * j, n));
+    }
   };
   uint32_t prefix = 0;                       // the digits found so far
-  int need = a.selected;                     // blocks to take among those of the prefix
+  int need = a.selected, shift = 32;         // blocks to take among those of the prefix
 #pragma unroll 1
   for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    const int bits = pass == 2 ? 10 : 11;
+    shift -= bits;
     for (int i = tid; i < kDigits; i += kSelThreads) hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += kSelThreads) {
-      const uint32_t k = key_at(i);
-      if (pass == 0 || k >> (shift + bits) == prefix) atomicAdd(&hist[k >> shift & ((1 << bits) - 1)], 1);
-    }
+    each([&](int i, uint32_t k) {
+      if (i < n && (pass == 0 || k >> (shift + bits) == prefix)) atomicAdd(&hist[k >> shift & ((1 << bits) - 1)], 1);
+    });
     __syncthreads();
     // digits from the largest down: thread tid has kDigits / kSelThreads of them
     constexpr int PER = kDigits / kSelThreads;
@@ -503,38 +578,35 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(SelectArgs a) {
     if (above < need && upto >= need) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        if (above < need && above + c[i] >= need) { found[0] = top - i; found[1] = need - above; }
+        if (above < need && above + c[i] >= need) { found[0] = top - i; found[1] = need - above; found[2] = c[i]; }
         above += c[i];
       }
     }
     __syncthreads();
     prefix = prefix << bits | (uint32_t)found[0];
     need = found[1];
-    __syncthreads();
+    if (found[2] == need) break;             // all of the digit's blocks are taken
   }
-  // blocks in order: a wave takes a run of them
-  const int per = (n + kSelWaves - 1) / kSelWaves, i0 = wid * per, i1 = min(n, i0 + per);
+  // blocks above the prefix, and the first `need` of those of it
   int more = 0, ties = 0;
-  for (int i = i0; i < i1; i += 64) {
-    const uint32_t k = i + lane < i1 ? key_at(i + lane) : 0;
-    more += __popcll(__ballot(i + lane < i1 && k > prefix));
-    ties += __popcll(__ballot(i + lane < i1 && k == prefix));
-  }
+  each([&](int i, uint32_t k) {
+    more += __popcll(__ballot(i < n && k >> shift > prefix));
+    ties += __popcll(__ballot(i < n && k >> shift == prefix));
+  });
+  __syncthreads();
   if (lane == 0) { wave_a[wid] = more; wave_b[wid] = ties; }
   __syncthreads();
   int at = 0, tied = 0;                      // taken above and equals before this wave's run
   for (int w = 0; w < wid; ++w) { at += wave_a[w]; tied += wave_b[w]; }
   const uint64_t below = (1ull << lane) - 1;
-  for (int i = i0; i < i1; i += 64) {
-    const bool in = i + lane < i1;
-    const uint32_t k = in ? key_at(i + lane) : 0;
-    const bool up = in && k > prefix, eq = in && k == prefix;
+  each([&](int i, uint32_t k) {
+    const bool up = i < n && k >> shift > prefix, eq = i < n && k >> shift == prefix;
     const uint64_t mu = __ballot(up), me = __ballot(eq);
     const int ub = at + __popcll(mu & below), eb = tied + __popcll(me & below);
-    if (up || (eq && eb < need)) out[ub + min(eb, need)] = i + lane;
+    if (up || (eq && eb < need)) out[ub + min(eb, need)] = i;
     at += __popcll(mu);
     tied += __popcll(me);
-  }
+  });
 }
 
 // ------------------------------------------------------------------ attention
@@ -850,23 +922,40 @@ extern "C" int aia_select_blocks(const void* query, int64_t q_token_stride, int6
   a.tok = reinterpret_cast<const int4*>(ws + L.tok);
   a.scores = reinterpret_cast<float*>(ws + L.scores);
   a.hkv = num_kv_heads; a.group = group; a.nb = num_blocks; a.width = table_width;
-  // tokens of a tile share their request's bounds: worth it where requests have several
-  a.per = num_tokens >= 4 * batch ? 16 / lanes : 1;
+  a.lanes = lanes;
+  // Tokens of a tile share their request's bounds: worth it where requests have several.
+  const bool many = num_tokens >= 4 * batch && group <= 16;
+  const int hblocks = (group + 15) / 16;
+  a.per = many ? 16 / lanes : 1;
+  a.tiles = many && num_tokens >= 8 * a.per ? 8 : 1;
+  a.heads = a.tiles > 1 || hblocks > 4 ? 1 : std::min(num_kv_heads, kSparseThreads / 64);
   SelectArgs s;
   s.scores = a.scores; s.tok = a.tok; s.out = selected; s.out_ts = sel_token_stride; s.out_hs = sel_head_stride;
   s.hkv = num_kv_heads; s.width = table_width; s.selected = num_selected; s.sink = sink; s.local = local;
-  const size_t lds = (size_t)((group + 15) / 16) * (2 * head_dim / 64) * 64 * 16;
+  const size_t lds = (size_t)a.heads * a.tiles * hblocks * (2 * head_dim / 64) * 64 * 16;
+  const int batch_blocks = 64 * (kSparseThreads / 64 / a.heads);         // blocks that a work-group's waves take at once
+  hipStream_t st = (hipStream_t)stream;
   for (int t0 = 0; t0 < num_tokens; t0 += L.score_tokens) {
     const int t1 = std::min(num_tokens, t0 + L.score_tokens);
-    a.t0 = t0; a.t1 = t1; s.t0 = t0;
-    const int tiles = (t1 - t0 + a.per - 1) / a.per;
-    // work-groups: about eight per compute unit, each of 256 blocks or more
-    const int64_t cuts = std::max<int64_t>(1, std::min<int64_t>(2048 / std::max<int64_t>(1, (int64_t)tiles * num_kv_heads), (table_width + 255) / 256));
-    a.chunk = (int)(((table_width + cuts - 1) / cuts + 255) / 256 * 256);
-    const dim3 grid((unsigned)tiles, (unsigned)num_kv_heads, (unsigned)((table_width + a.chunk - 1) / a.chunk));
-    (head_dim == 128 ? score_kernel<128> : score_kernel<64>)<<<grid, kSparseThreads, lds, (hipStream_t)stream>>>(a);
+    a.t0 = t0; a.t1 = t1; s.t0 = t0; s.rows = (t1 - t0) * num_kv_heads;
+    const unsigned gx = (unsigned)((t1 - t0 + a.per * a.tiles - 1) / (a.per * a.tiles));
+    const unsigned gy = (unsigned)((num_kv_heads + a.heads - 1) / a.heads);
+    // work-groups: about eight per compute unit, of whole batches of blocks
+    const int64_t batches = (table_width + batch_blocks - 1) / batch_blocks;
+    const int64_t cuts = std::max<int64_t>(1, std::min<int64_t>(2048 / std::max<int64_t>(1, (int64_t)gx * gy), batches));
+    a.chunk = (int)((batches + cuts - 1) / cuts * batch_blocks);
+    const dim3 grid(gx, gy, (unsigned)((table_width + a.chunk - 1) / a.chunk));
+    (head_dim == 128 ? score_kernel<128> : score_kernel<64>)<<<grid, kSparseThreads, lds, st>>>(a);
     if (int rc = check_hip(hipGetLastError(), "aia_select_blocks: score launch")) return rc;
-    select_kernel<<<dim3((unsigned)(t1 - t0), (unsigned)num_kv_heads), kSelThreads, 0, (hipStream_t)stream>>>(s);
+    if (table_width <= 1024) {
+      auto* kernel = table_width <= 256 ? select_wave_kernel<4> : table_width <= 512 ? select_wave_kernel<8>
+                     : table_width <= 768 ? select_wave_kernel<12> : select_wave_kernel<16>;
+      kernel<<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
+    } else {
+      auto* kernel = table_width <= 4 * kSelThreads ? select_kernel<4> : table_width <= 16 * kSelThreads ? select_kernel<16>
+                     : select_kernel<0>;
+      kernel<<<(unsigned)s.rows, kSelThreads, 0, st>>>(s);
+    }
     if (int rc = check_hip(hipGetLastError(), "aia_select_blocks: select launch")) return rc;
   }
   return AIA_OK;

@@ -163,22 +163,43 @@ def test_selection(step, hq, hkv, d, ties):
                 assert out[t, h].tolist() == want + [-1] * (selected - len(want)), (t, h)
 
 
-def test_selection_of_long_contexts():
-    """Many blocks per row, values of the query that are not finite, strided queries."""
+@pytest.mark.parametrize("most", [200, 300, 600, 900, 1500, 4097, 9000])
+def test_selection_of_long_contexts(most):
+    """Many blocks per row (every kernel that selects), values of the query that are not
+    finite, strided queries."""
     from auto_infer_amd import ops
-    s = make([(1, 4097), (2, 3001)], 4, 2, 128, 1, seed=9)
+    s = make([(1, most), (2, 3 * most // 4 + 1)], 4, 2, 128, 1, seed=9)
     s["q"][0, 0, 3], s["q"][0, 1, 4], s["q"][1] = float("inf"), float("nan"), 0.0
     b, e = random_bounds(s, 6)
     g = on_gpu(s)
     wide = torch.zeros(s["t"], 9, 128, dtype=torch.bfloat16, device=DEV)
     wide[:, 2:6] = g["q"]
-    out = ops.select_blocks(wide[:, 2:6], make_plan(g, 200, 3, 5), b.to(DEV),
+    out = ops.select_blocks(wide[:, 2:6], make_plan(g, 150, 3, 5), b.to(DEV),
                             (e + 127).to(torch.uint8).to(DEV).view(torch.float8_e8m0fnu)).cpu()
     for t, r, pos in tokens_of(s):
         rows = s["table"][r].long()
         for h in range(2):
-            want = ref.select(s["q"][t, 2 * h:2 * h + 2], b[rows, h, 0], b[rows, h, 1], e[rows, h], pos + 1, 200, 3, 5)
+            want = ref.select(s["q"][t, 2 * h:2 * h + 2], b[rows, h, 0], b[rows, h, 1], e[rows, h], pos + 1, 150, 3, 5)
             assert out[t, h].tolist() == want
+
+
+@pytest.mark.parametrize("hq,hkv,d", SHAPES)
+def test_selection_of_prompts(hq, hkv, d):
+    """Many tokens per request: tiles of several tokens, and of several requests."""
+    from auto_infer_amd import ops
+    s = make([(61, 300), (0, 9), (37, 37), (1, 200), (50, 90)], hq, hkv, d, 3, seed=hq + 1)
+    b, e = random_bounds(s, 8)
+    g = on_gpu(s)
+    out = ops.select_blocks(g["q"], make_plan(g, 9, 1, 2), b.to(DEV),
+                            (e + 127).to(torch.uint8).to(DEV).view(torch.float8_e8m0fnu)).cpu()
+    for t, r, pos in tokens_of(s):
+        if t % 5 and t not in (60, 61, 97, 98, 99):
+            continue
+        rows = s["table"][r].long()
+        for h in range(hkv):
+            q = s["q"][t, h * (hq // hkv):(h + 1) * (hq // hkv)]
+            want = ref.select(q, b[rows, h, 0], b[rows, h, 1], e[rows, h], pos // 3 + 1, 9, 1, 2)
+            assert out[t, h].tolist() == want + [-1] * (9 - len(want)), (t, h)
 
 
 def random_selection(s, selected, seed):
