@@ -302,24 +302,28 @@ struct ScoreKernelArgs {
   const int4* tok;
   float* scores;             // (tokens of this launch, hkv, width)
   int32_t t0, t1, hkv, group, nb, width;               // tokens [t0, t1)
-  int32_t lanes, per, tiles, heads, chunk;             // see score_kernel
+  int32_t lanes, per, tiles, chunk;                    // see score_kernel
 };
 
-// One work-group: `tiles` tiles of 16 query rows, each of `per` tokens (per token `lanes`
-// rows, the group's heads padded to a power of two; groups of more than 16 heads take 16
-// at a time, a token per tile), for `heads` KV heads, against `chunk` blocks.  Its four
-// waves are dealt to the KV heads and, where there are fewer, to 64 blocks each.
-//   The queries become whole numbers in LDS first, in MFMA order; then each wave holds 64
-// blocks' bounds in registers and goes over the tiles: S = Q B^T on
-// v_mfma_i32_16x16x64_i8, lane (row or block n, group g) with bytes 64 j + 16 g .. of
-// [q+ (D), q- (D)] and of [hi, nlo]; the four accumulators are rows 4 g .. 4 g + 3 of
+constexpr int kScoreTiles = 4, kTileTokens = 16 * kScoreTiles;
+
+// One work-group: `tiles` tiles of 16 query rows of a KV head, each of `per` tokens (per
+// token `lanes` rows, the group's heads padded to a power of two; groups of more than 16
+// heads take 16 at a time, a token per tile), against `chunk` blocks.
+//   A wave holds 64 blocks' bounds in registers; while the first of them arrive, the
+// queries become whole numbers in LDS, in MFMA order.  Then it goes over the tiles: S =
+// Q B^T on v_mfma_i32_16x16x64_i8, lane (row or block n, group g) with bytes 64 j + 16 g ..
+// of [q+ (D), q- (D)] and of [hi, nlo]; the four accumulators are rows 4 g .. 4 g + 3 of
 // block n.  Tokens of several requests are taken one request at a time.
-//   Few tokens: one tile, several KV heads, whose bounds of a block are neighbours in
-// memory; many tokens: many tiles of one KV head, so the bounds are read once for them.
+//   Few tokens: one tile; many: four, so that the bounds are read once for them (512
+// tokens, 28/4 heads, 513 blocks, with the selection: 28.0 us, 30.6 with eight, 32.5 with
+// two).  Waves of one work-group on four KV heads, whose bounds of a block are
+// neighbours, were no faster on single tokens.
 template <int D>
 __global__ __launch_bounds__(kSparseThreads) void score_kernel(ScoreKernelArgs a) {
   constexpr int KS = 2 * D / 64;             // MFMA steps
-  extern __shared__ uint4 qfrag[];           // [KV head][tile][head block][step][lane]
+  extern __shared__ uint4 qfrag[];           // [tile][head block][step][lane]
+  __shared__ int2 info[kTileTokens];         // the tokens' requests and visible blocks
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int lanes = a.lanes, hblocks = (a.group + 15) / 16;
@@ -328,12 +332,40 @@ __global__ __launch_bounds__(kSparseThreads) void score_kernel(ScoreKernelArgs a
   const int c0 = blockIdx.z * a.chunk;
   // (nothing to do where no token sees the chunk's blocks)
   int see = 0;
-  for (int i = lane; i < tokens; i += 64) see = max(see, a.tok[tb + i].z);
+  for (int i = lane; i < tokens; i += 64) {
+    const int4 x = a.tok[tb + i];
+    see = max(see, x.z);
+    if (wid == 0) info[i] = make_int2(x.x, x.z);
+  }
   if (__ballot(see > c0) == 0) return;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) see = max(see, __shfl_xor(see, d));
+  see = __builtin_amdgcn_readfirstlane(see);
+  const int kvh = blockIdx.y, own = 64 * wid;
+  // the bounds of 64 blocks from b0 on of a request's table row, up to c1
+  int4v_t bf[4][KS];
+  int eb[4];
+  auto load_bounds = [&](int req, int b0, int c1) {
+    const int32_t* btrow = a.bt + (int64_t)req * a.bt_stride;
+    const int id = b0 + lane < c1 ? min(max(btrow[b0 + lane], 0), a.nb - 1) : 0;
+    const int ebyte = a.scale[(int64_t)id * a.hkv + kvh];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int blk = __shfl(id, 16 * s + n);
+      eb[s] = __shfl(ebyte, 16 * s + n) - 127;
+      const uint4* bp = reinterpret_cast<const uint4*>(a.bounds + ((int64_t)blk * a.hkv + kvh) * 2 * D) + g;
+#pragma unroll
+      for (int j = 0; j < KS; ++j) bf[s][j] = __builtin_bit_cast(int4v_t, as_u4(bp[4 * j]));
+    }
+  };
+  // The first ones arrive while the queries are prepared.
+  const int first_req = __builtin_amdgcn_readfirstlane(a.tok[tb].x);
+  const bool ahead = first_req >= 0 && c0 + own < see;
+  if (ahead) load_bounds(first_req, c0 + own, min(see, c0 + a.chunk));
   const int tn = n / lanes, hn = n - tn * lanes;       // this lane's row: token of the tile, head
-  for (int u = wid; u < a.heads * a.tiles; u += kSparseThreads / 64) {
-    const int kvh = blockIdx.y * a.heads + u / a.tiles, ti = u % a.tiles * a.per + tn;
-    const bool row = ti < tokens && kvh < a.hkv && tn < a.per;
+  for (int u = wid; u < a.tiles; u += kSparseThreads / 64) {
+    const int ti = u * a.per + tn;
+    const bool row = ti < tokens && tn < a.per;
     const uint16_t* qt = a.q + (int64_t)(tb + ti) * a.q_ts + (int64_t)kvh * a.group * a.q_hs;
     uint32_t amax = 0;                       // largest finite |q| of the token's heads
     for (int hb = 0; hb < hblocks; ++hb) {
@@ -381,38 +413,27 @@ __global__ __launch_bounds__(kSparseThreads) void score_kernel(ScoreKernelArgs a
     }
   }
   __syncthreads();
-  const int hw = wid % a.heads, kvh = blockIdx.y * a.heads + hw;
-  if (wid >= kSparseThreads / 64 / a.heads * a.heads || kvh >= a.hkv) return;
-  const int stride = 64 * (kSparseThreads / 64 / a.heads), own = 64 * (wid / a.heads);
   auto frag = [&](int m, int hb, int j) {
-    return __builtin_bit_cast(int4v_t, as_u4(qfrag[(((hw * a.tiles + m) * hblocks + hb) * KS + j) * 64 + lane]));
+    return __builtin_bit_cast(int4v_t, as_u4(qfrag[((m * hblocks + hb) * KS + j) * 64 + lane]));
   };
   for (int done = 0; done < tokens;) {
-    const int4 lead = a.tok[tb + done];
-    const int from = done;
+    const int from = done, req = __builtin_amdgcn_readfirstlane(info[from].x);
     int vis = 0;                             // tokens [from, done) of one request
-    while (done < tokens) {
-      const int4 x = a.tok[tb + done];
-      if (x.x != lead.x) break;
-      vis = max(vis, x.z);
-      ++done;
+    for (bool more = true; more && done < tokens;) {         // 64 at a time
+      const int2 x = done + lane < tokens ? info[done + lane] : make_int2(-2, 0);
+      const uint64_t other = __ballot(x.x != req);
+      const int here = other ? __builtin_ctzll(other) : 64;
+      int v = lane < here ? x.y : 0;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) v = max(v, __shfl_xor(v, d));
+      vis = max(vis, __builtin_amdgcn_readfirstlane(v));
+      done += here;
+      more = here == 64;
     }
     const int c1 = min(vis, c0 + a.chunk);
-    if (lead.x < 0) continue;
-    const int32_t* btrow = a.bt + (int64_t)lead.x * a.bt_stride;
-    for (int b0 = c0 + own; b0 < c1; b0 += stride) {
-      const int id = b0 + lane < c1 ? min(max(btrow[b0 + lane], 0), a.nb - 1) : 0;
-      const int ebyte = a.scale[(int64_t)id * a.hkv + kvh];
-      int4v_t bf[4][KS];
-      int eb[4];
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int blk = __shfl(id, 16 * s + n);
-        eb[s] = __shfl(ebyte, 16 * s + n) - 127;
-        const uint4* bp = reinterpret_cast<const uint4*>(a.bounds + ((int64_t)blk * a.hkv + kvh) * 2 * D) + g;
-#pragma unroll
-        for (int j = 0; j < KS; ++j) bf[s][j] = __builtin_bit_cast(int4v_t, as_u4(bp[4 * j]));
-      }
+    if (req < 0) continue;
+    for (int b0 = c0 + own; b0 < c1; b0 += kSparseThreads) {
+      if (from > 0 || b0 > c0 + own || !ahead) load_bounds(req, b0, c1);
       for (int m = from / a.per; m * a.per < done; ++m) {
         int4v_t acc[4];
 #pragma unroll
@@ -927,24 +948,21 @@ extern "C" int aia_select_blocks(const void* query, int64_t q_token_stride, int6
   const bool many = num_tokens >= 4 * batch && group <= 16;
   const int hblocks = (group + 15) / 16;
   a.per = many ? 16 / lanes : 1;
-  a.tiles = many && num_tokens >= 8 * a.per ? 8 : 1;
-  a.heads = a.tiles > 1 || hblocks > 4 ? 1 : std::min(num_kv_heads, kSparseThreads / 64);
+  a.tiles = many && num_tokens >= kScoreTiles * a.per ? kScoreTiles : 1;
   SelectArgs s;
   s.scores = a.scores; s.tok = a.tok; s.out = selected; s.out_ts = sel_token_stride; s.out_hs = sel_head_stride;
   s.hkv = num_kv_heads; s.width = table_width; s.selected = num_selected; s.sink = sink; s.local = local;
-  const size_t lds = (size_t)a.heads * a.tiles * hblocks * (2 * head_dim / 64) * 64 * 16;
-  const int batch_blocks = 64 * (kSparseThreads / 64 / a.heads);         // blocks that a work-group's waves take at once
+  const size_t lds = (size_t)a.tiles * hblocks * (2 * head_dim / 64) * 64 * 16;
   hipStream_t st = (hipStream_t)stream;
   for (int t0 = 0; t0 < num_tokens; t0 += L.score_tokens) {
     const int t1 = std::min(num_tokens, t0 + L.score_tokens);
     a.t0 = t0; a.t1 = t1; s.t0 = t0; s.rows = (t1 - t0) * num_kv_heads;
     const unsigned gx = (unsigned)((t1 - t0 + a.per * a.tiles - 1) / (a.per * a.tiles));
-    const unsigned gy = (unsigned)((num_kv_heads + a.heads - 1) / a.heads);
-    // work-groups: about eight per compute unit, of whole batches of blocks
-    const int64_t batches = (table_width + batch_blocks - 1) / batch_blocks;
-    const int64_t cuts = std::max<int64_t>(1, std::min<int64_t>(2048 / std::max<int64_t>(1, (int64_t)gx * gy), batches));
-    a.chunk = (int)((batches + cuts - 1) / cuts * batch_blocks);
-    const dim3 grid(gx, gy, (unsigned)((table_width + a.chunk - 1) / a.chunk));
+    // work-groups: about eight per compute unit, each of 256 blocks (64 a wave) or more
+    const int64_t batches = (table_width + kSparseThreads - 1) / kSparseThreads;
+    const int64_t cuts = std::max<int64_t>(1, std::min<int64_t>(2048 / std::max<int64_t>(1, (int64_t)gx * num_kv_heads), batches));
+    a.chunk = (int)((batches + cuts - 1) / cuts * kSparseThreads);
+    const dim3 grid(gx, (unsigned)num_kv_heads, (unsigned)((table_width + a.chunk - 1) / a.chunk));
     (head_dim == 128 ? score_kernel<128> : score_kernel<64>)<<<grid, kSparseThreads, lds, st>>>(a);
     if (int rc = check_hip(hipGetLastError(), "aia_select_blocks: score launch")) return rc;
     if (table_width <= 1024) {
