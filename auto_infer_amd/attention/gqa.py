@@ -21,14 +21,19 @@ scores, ``rope`` (an ``ops.RotaryEmbedding``) turns Q and K from
 ``ctx.positions`` instead of ``ctx.cos`` / ``ctx.sin`` (``rope=False``: a model
 without rotary positions, Q and K stay as they are), and a context with
 ``aia_prefix_lens`` (one per request; a host list or device int32) lets all rows of a request
-see its first keys.
+see its first keys.  ``share_prefixes=True`` reads the cache blocks that requests have in
+common once for all of them (``ops.paged_attention_shared``; ``ctx.aia_group_ids`` names
+the groups, else the first blocks do).  ``sparse_blocks=n`` lets every query token and KV
+head attend n cache blocks that an upper bound of their scores selects
+(``ops.select_blocks``), always the first ``sparse_sink`` and the last ``sparse_local``;
+the layers' caches then carry the blocks' bounds.
 """
 import torch
 
 from auto_infer_amd import ops
 from auto_infer_amd.attention.base import AttentionBackend
 from auto_infer_amd.attention.layers import lin, rms_norm, rotate_half
-from auto_infer_amd.attention.metadata import step_plan
+from auto_infer_amd.attention.metadata import step_plan, step_shared_plan, step_sparse_plan
 
 
 class GqaHipBackend(AttentionBackend):
@@ -37,7 +42,8 @@ class GqaHipBackend(AttentionBackend):
                  num_layers: int, device, dtype, w: dict = None, layer_prefix=None,
                  rms_eps=None, fuse_kv_write: bool = True, fuse_pre_attention: bool = True,
                  kv_layout: str = "nd", kv_dtype: str = "bf16", softcap: float = 0.0,
-                 alibi_slopes=None, rope=None):
+                 alibi_slopes=None, rope=None, share_prefixes: bool = False,
+                 sparse_blocks: int = 0, sparse_sink: int = 1, sparse_local: int = 2):
         self.n_q_heads = n_q_heads
         self.n_kv_heads = n_kv_heads
         self.head_dim = head_dim
@@ -74,9 +80,32 @@ class GqaHipBackend(AttentionBackend):
             raise ValueError("rope must be an ops.RotaryEmbedding, False (no rotary positions) or None "
                              "(ctx.cos / ctx.sin)")
         self.rope = rope
+        self.share_prefixes, self.sparse = bool(share_prefixes), None
+        if sparse_blocks:
+            if not (sparse_sink >= 0 and sparse_local >= 1 and sparse_sink + sparse_local <= sparse_blocks):
+                raise ValueError(f"sparse_sink {sparse_sink} and sparse_local {sparse_local} do not fit "
+                                 f"{sparse_blocks} blocks (sparse_local at least 1)")
+            self.sparse = (int(sparse_blocks), int(sparse_sink), int(sparse_local))
+        if self.share_prefixes or self.sparse:
+            if self.share_prefixes and self.sparse:
+                raise ValueError("share_prefixes and sparse_blocks exclude each other")
+            if kv_layout != "nd":
+                raise NotImplementedError("shared prefixes and sparse blocks have no NZ layout")
+            if softcap != 0 or alibi_slopes is not None:
+                raise NotImplementedError("shared prefixes and sparse blocks take no modified scores")
+            self.fuse_kv_write = False      # the cache is written before it is read
         self._pending = None
 
     def alloc_kv_caches(self, num_blocks: int, block_size: int) -> list:
+        if not self.sparse:
+            return self._alloc(num_blocks, block_size)
+        # per layer (k, v, ...) and the blocks' bounds and their scales
+        shape = (num_blocks, self.n_kv_heads)
+        return [(*cache, torch.zeros(*shape, 2, self.head_dim, device=self.device, dtype=torch.int8),
+                 torch.zeros(shape, device=self.device, dtype=torch.uint8).view(ops.FP8_KV_SCALE))
+                for cache in self._alloc(num_blocks, block_size)]
+
+    def _alloc(self, num_blocks, block_size):
         if self.fp8:      # per layer (k, v, k scales, v scales)
             shape = (num_blocks, block_size, self.n_kv_heads, self.head_dim)
 
@@ -97,7 +126,7 @@ class GqaHipBackend(AttentionBackend):
 
     def _write(self, k, v, cache, slot_mapping):
         if self.fp8:
-            ops.write_kv_fp8(k, v, *cache, slot_mapping)
+            ops.write_kv_fp8(k, v, *cache[:4], slot_mapping)
         elif self.kv_layout == "nz":
             ops.write_kv_nz(k, v, cache[0], cache[1], slot_mapping)
         else:
@@ -114,6 +143,16 @@ class GqaHipBackend(AttentionBackend):
             raise ValueError("the context has no cos / sin: give the backend a rope, or rope=False "
                              "for a model without rotary positions")
         if self.rope is not None and self.rope is not False:
+            if self.fuse_pre_attention and not self._deferred(T, ctx):
+                cache = ctx.kv_caches[layer_idx]
+                scales = dict(key_scale=cache[2], value_scale=cache[3]) if self.fp8 else {}
+                q = ops.rope_append(qkv, n_q, n_kv, ctx.positions, self.rope, cache[0], cache[1],
+                                    ctx.slot_mapping, qn,
+                                    w.get(p + "k_norm.weight") if qn is not None else None,
+                                    self.rms_eps if self.rms_eps is not None else 1e-6,
+                                    kv_layout=self.kv_layout, **scales)
+                o = self._attn(layer_idx, q, None, None, ctx).reshape(T, n_q * hd)
+                return lin(o, w[p + "o_proj.weight"])
             q, k, v = ops.rope_qk(qkv, n_q, n_kv, ctx.positions, self.rope, qn,
                                   w.get(p + "k_norm.weight") if qn is not None else None,
                                   self.rms_eps if self.rms_eps is not None else 1e-6)
@@ -147,16 +186,22 @@ class GqaHipBackend(AttentionBackend):
                 and all(t.dtype == torch.bfloat16 and t.numel() == T * hd and t.stride(-1) == 1
                         and aligned(t) for t in (ctx.cos, ctx.sin)))
 
+    def _deferred(self, T, ctx):
+        """Whether the attention kernel writes the new rows."""
+        return (self.fuse_kv_write and not self.fp8 and getattr(ctx, "aia_slots_from_block_table", False)
+                and T == ctx.slot_mapping.shape[0])
+
     def _write_kv(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, ctx) -> None:
         cache = ctx.kv_caches[layer_idx]
-        if (self.fuse_kv_write and not self.fp8 and getattr(ctx, "aia_slots_from_block_table", False)
-                and k.shape[0] == ctx.slot_mapping.shape[0]):
+        if self._deferred(k.shape[0], ctx):
             self._pending = (layer_idx, id(ctx), k, v)
             return
         self._write(k, v, cache, ctx.slot_mapping)
 
     def _attn(self, layer_idx: int, q, k, v, ctx) -> torch.Tensor:
         cache = ctx.kv_caches[layer_idx]
+        if self.share_prefixes or self.sparse:
+            return self._attn_blocks(q, cache, ctx)
         plan = step_plan(ctx, self.n_q_heads, self.n_kv_heads, self.head_dim, cache[0].shape[1])
         pending, self._pending = self._pending, None
         if pending is not None and pending[:2] == (layer_idx, id(ctx)):
@@ -171,3 +216,16 @@ class GqaHipBackend(AttentionBackend):
                                            key_scale=cache[2], value_scale=cache[3], **self.scores)
         return ops.paged_attention_gqa(q, cache[0], cache[1], plan, self.scale,
                                        kv_layout=self.kv_layout, **self.scores)
+
+    def _attn_blocks(self, q, cache, ctx):
+        """Attention over shared prefixes or selected blocks of written caches."""
+        sizes = (self.n_q_heads, self.n_kv_heads, self.head_dim, cache[0].shape[1])
+        scales = dict(key_scale=cache[2], value_scale=cache[3]) if self.fp8 else {}
+        if self.share_prefixes:
+            return ops.paged_attention_shared(q, cache[0], cache[1], step_shared_plan(ctx, *sizes),
+                                              self.scale, **scales)
+        plan = step_sparse_plan(ctx, *sizes, *self.sparse)
+        bounds, bounds_scale = cache[-2:]
+        ops.summarize_blocks(cache[0], plan, bounds, bounds_scale, key_scale=scales.get("key_scale"))
+        selected = ops.select_blocks(q, plan, bounds, bounds_scale)
+        return ops.paged_attention_sparse(q, cache[0], cache[1], plan, selected, self.scale, **scales)

@@ -50,13 +50,19 @@ def _gqa_options(model):
     """What a model may ask for beyond the reference's backends:
     ``KV_CACHE_DTYPE`` ("bf16" or "fp8"), ``attn_scale`` (of the scores; default
     head_dim ** -0.5), ``attn_softcap``, ``alibi_slopes`` (device float32, one per
-    local query head) and ``aia_rope`` (an ``ops.RotaryEmbedding``; False for a model
-    without rotary positions)."""
+    local query head), ``aia_rope`` (an ``ops.RotaryEmbedding``; False for a model
+    without rotary positions), ``attn_share_prefixes`` (True: cache blocks that requests
+    have in common are read once for them) and ``attn_sparse_blocks`` with
+    ``attn_sparse_sink`` / ``attn_sparse_local`` (cache blocks that a query token attends)."""
     return dict(scale=getattr(model, "attn_scale", model.cfg.head_dim ** -0.5),
                 kv_dtype=getattr(model, "KV_CACHE_DTYPE", "bf16"),
                 softcap=getattr(model, "attn_softcap", 0.0),
                 alibi_slopes=getattr(model, "alibi_slopes", None),
-                rope=getattr(model, "aia_rope", None))
+                rope=getattr(model, "aia_rope", None),
+                share_prefixes=getattr(model, "attn_share_prefixes", False),
+                sparse_blocks=getattr(model, "attn_sparse_blocks", 0),
+                sparse_sink=getattr(model, "attn_sparse_sink", 1),
+                sparse_local=getattr(model, "attn_sparse_local", 2))
 
 
 def _gqa_hip(model, mode: str, kv_layout: str = "nd", family: str = GQA_FAMILY):

@@ -54,16 +54,25 @@ class DecodeGraph(_GearGraph):
     ``GqaHipBackend(kv_dtype="fp8")`` allocates them: the graph then writes the
     new rows at the stager's slots in a launch of its own.  ``softcap`` /
     ``alibi_slopes``: as ``ops.paged_attention_gqa`` takes them.
+    ``share_prefixes=True``: cache blocks that the step's requests have in common
+    (those with the same first block) are read once for them; the new rows are
+    written in a launch of their own.
     """
 
     def __init__(self, stager, caches, *, num_q_heads, num_kv_heads, head_dim=128, scale=None,
-                 stream=None, kv_layout="nd", softcap=0.0, alibi_slopes=None):
+                 stream=None, kv_layout="nd", softcap=0.0, alibi_slopes=None,
+                 share_prefixes=False):
         if kv_layout not in ops.KV_LAYOUTS:
             raise ValueError(f"kv_layout must be one of {sorted(ops.KV_LAYOUTS)}")
         self.kv_layout = kv_layout
         self.scores = dict(softcap=softcap, alibi_slopes=alibi_slopes)
         if kv_layout != "nd" and any(len(c) == 4 for c in caches):
             raise NotImplementedError("8-bit caches have no NZ layout")
+        if any(len(c) > 4 or (len(c) == 4 and c[2].dtype != ops.FP8_KV_SCALE) for c in caches):
+            raise NotImplementedError("DecodeGraph takes no caches with block bounds")
+        if share_prefixes and (kv_layout != "nd" or softcap != 0 or alibi_slopes is not None):
+            raise NotImplementedError("shared prefixes take no NZ layout or modified scores")
+        self.share_prefixes = share_prefixes
         self.stager = stager
         self.caches = caches
         dev = stager.block_table.device
@@ -77,14 +86,18 @@ class DecodeGraph(_GearGraph):
         self.stream = stream or torch.cuda.Stream(device=dev)
         block_size = caches[0][0].shape[1]
         with torch.cuda.stream(self.stream):
-            self.plan = ops.AttentionPlan(stager.block_table, stager._cu, stager._kv, T,
-                                          num_q_heads, num_kv_heads, head_dim, block_size)
+            plan = ops.SharedPrefixPlan if share_prefixes else ops.AttentionPlan
+            self.plan = plan(stager.block_table, stager._cu, stager._kv, T, num_q_heads,
+                             num_kv_heads, head_dim, block_size)
         self.graph = None
 
     def _body(self):
         self.plan.replan()
         for layer, cache in enumerate(self.caches):
             kc, vc, *scales = cache
+            if self.share_prefixes:
+                self._write_and_share(layer, kc, vc, scales)
+                continue
             if scales:
                 ops.write_kv_fp8(self.k_new[layer], self.v_new[layer], *cache, self.stager.slots)
                 ops.paged_attention_gqa(self.q[layer], kc, vc, self.plan, self.scale,
@@ -95,6 +108,17 @@ class DecodeGraph(_GearGraph):
                                     out=self.out[layer], key_new=self.k_new[layer],
                                     value_new=self.v_new[layer], kv_layout=self.kv_layout,
                                     **self.scores)
+
+
+    def _write_and_share(self, layer, kc, vc, scales):
+        k, v = self.k_new[layer], self.v_new[layer]
+        if scales:
+            ops.write_kv_fp8(k, v, kc, vc, *scales, self.stager.slots)
+        else:
+            ops.write_kv(k, v, kc, vc, self.stager.slots)
+        more = dict(key_scale=scales[0], value_scale=scales[1]) if scales else {}
+        ops.paged_attention_shared(self.q[layer], kc, vc, self.plan, self.scale, out=self.out[layer],
+                                   **more)
 
 
 class LatentDecodeGraph(_GearGraph):

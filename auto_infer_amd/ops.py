@@ -948,12 +948,13 @@ class _StepPlan:
         # (a single row's stride means nothing)
         self._table_stride = block_table.stride(0) if block_table.shape[0] > 1 else block_table.shape[1]
 
-    def _make(self, nbytes, workspace):
+    def _make(self, nbytes, workspace, owned):
         if workspace is None:
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         _check_on(workspace, "workspace", torch.uint8, self.device.index)
         _require(workspace.is_contiguous() and workspace.numel() >= nbytes, "workspace too small")
         self.workspace = workspace
+        self._owned = [workspace, *(owned or ())]      # as AttentionPlan keeps them
         self._streams = {torch.cuda.current_stream(self.device)}
         self.replan()
 
@@ -968,7 +969,8 @@ class _StepPlan:
     def _use_on(self, stream):
         if stream not in self._streams:
             self._streams.add(stream)
-            self.workspace.record_stream(stream)
+            for t in self._owned:
+                t.record_stream(stream)
 
 
 def _attention_inputs(what, query, key_cache, value_cache, plan, key_scale, value_scale, out):
@@ -1014,7 +1016,7 @@ class SharedPrefixPlan(_StepPlan):
     """
 
     def __init__(self, block_table, cu_seqlens_q, seqlens_kv, num_tokens, num_q_heads, num_kv_heads,
-                 head_dim, block_size, group_ids=None, workspace=None):
+                 head_dim, block_size, group_ids=None, workspace=None, owned=None):
         self._take(block_table, cu_seqlens_q, seqlens_kv, num_tokens, num_q_heads, num_kv_heads,
                    head_dim, block_size)
         if group_ids is not None:
@@ -1028,7 +1030,7 @@ class SharedPrefixPlan(_StepPlan):
         _native.call("aia_shared_workspace_bytes", self.batch, self.num_tokens, self.num_q_heads,
                      self.num_kv_heads, self.head_dim, self.block_size, block_table.shape[1],
                      ctypes.byref(nbytes))
-        self._make(nbytes.value, workspace)
+        self._make(nbytes.value, workspace, owned)
 
     def _plan(self, stream):
         _call_on(self.device.index, "aia_shared_plan", self.cu_seqlens_q.data_ptr(),
@@ -1076,7 +1078,7 @@ class BlockSparsePlan(_StepPlan):
     """
 
     def __init__(self, block_table, cu_seqlens_q, seqlens_kv, num_tokens, num_q_heads, num_kv_heads,
-                 head_dim, block_size, num_selected, sink=1, local=1, workspace=None):
+                 head_dim, block_size, num_selected, sink=1, local=1, workspace=None, owned=None):
         self._take(block_table, cu_seqlens_q, seqlens_kv, num_tokens, num_q_heads, num_kv_heads,
                    head_dim, block_size)
         self.num_selected, self.sink, self.local = int(num_selected), int(sink), int(local)
@@ -1089,7 +1091,7 @@ class BlockSparsePlan(_StepPlan):
         _native.call("aia_sparse_workspace_bytes", self.batch, self.num_tokens, self.num_q_heads,
                      self.num_kv_heads, self.head_dim, self.block_size, block_table.shape[1],
                      self.num_selected, ctypes.byref(nbytes))
-        self._make(nbytes.value, workspace)
+        self._make(nbytes.value, workspace, owned)
 
     def _plan(self, stream):
         width, bs, batch, *rest = self._sizes
