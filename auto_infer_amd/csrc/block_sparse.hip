@@ -301,41 +301,172 @@ struct ScoreKernelArgs {
   int64_t bt_stride;
   const int4* tok;
   float* scores;             // (tokens of this launch, hkv, width)
-  int32_t t0, t1, hkv, group, nb, width;               // tokens [t0, t1)
-  int32_t lanes, per, tiles, chunk;                    // see score_kernel
+  int32_t t0, t1, hkv, group, nb, width, chunk;        // tokens [t0, t1)
 };
 
-constexpr int kScoreTiles = 4, kTileTokens = 16 * kScoreTiles;
+// A token's query heads of a KV head are added up before the products: with q+ and q- the
+// positive and negative parts of the whole numbers, the sum over the heads of
+// q+ . hi + q- . nlo is (sum q+) . hi + (sum q-) . nlo, in whole numbers without a
+// difference.  The sums, up to 127 * 256, go as two bytes: s = 256 up + low with low in
+// [-128, 127] and up <= 127.
 
-// One work-group: `tiles` tiles of 16 query rows of a KV head, each of `per` tokens (per
-// token `lanes` rows, the group's heads padded to a power of two; groups of more than 16
-// heads take 16 at a time, a token per tile), against `chunk` blocks.
+// Numbers 2 i and 2 i + 1 of eight words in order, low or upper bytes, four a word.
+__device__ __forceinline__ uint4 low_bytes(const uint32_t s[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(s[2 * i + 1], s[2 * i], 0x06040200u);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 up_bytes(const uint32_t s[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = __builtin_amdgcn_perm(s[2 * i + 1] + 0x00800080u, s[2 * i] + 0x00800080u, 0x07050301u);
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint32_t finite_max(const uint4& w, uint32_t most) {
+  const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = p[i] & 0x7fffu, up = (p[i] >> 16) & 0x7fffu;
+    most = max(most, max(lo < 0x7f80u ? lo : 0u, up < 0x7f80u ? up : 0u));
+  }
+  return most;
+}
+// Adds the whole numbers of one sign (f: the factor with it) of 8 bf16 to 4 words.
+__device__ __forceinline__ void add_whole(const uint4& w, float f, uint32_t s[4]) {
+  const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = aia::bf16_lo(p[i]), y = aia::bf16_hi(p[i]);
+    const int u = __builtin_fabsf(x) < INFINITY ? max((int)__builtin_rintf(x * f), 0) : 0;
+    const int v = __builtin_fabsf(y) < INFINITY ? max((int)__builtin_rintf(y * f), 0) : 0;
+    s[i] += (uint32_t)(u | v << 16);
+  }
+}
+
+// Sums over rows of CH lanes: lane c of a row gets the row's sum of x[c].  Each step
+// exchanges half of the values with the lane across a bit of c.
+template <int CTRL>
+__device__ __forceinline__ int from_lane(int x) {
+  return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xf, 0xf, true);
+}
+template <int CTRL, int H>
+__device__ __forceinline__ void fold(int* x, bool upper) {
+#pragma unroll
+  for (int i = 0; i < H; ++i) x[i] = (upper ? x[i + H] : x[i]) + from_lane<CTRL>(upper ? x[i] : x[i + H]);
+}
+template <int CH>
+__device__ __forceinline__ int sum_of_own(int* x, int c) {
+  if constexpr (CH == 16) fold<0x128, 8>(x, c & 8);        // rotate by 8 lanes
+  fold<0x141, 4>(x, c & 4);                                // mirror eight
+  fold<0x4e, 2>(x, c & 2);                                 // swap pairs
+  fold<0xb1, 1>(x, c & 1);                                 // swap neighbours
+  return x[0];
+}
+
+// Few tokens of a request: a work-group is a token, a KV head and `chunk` blocks.  A
+// wave takes 64 blocks at a time, each load 1 KB of whole rows of bounds, lane (row, c)
+// with bytes 16 c .. of [hi, nlo] against the same bytes of [sum q+, sum q-] on
+// v_dot4_i32_i8.  8 tokens, 32/8 heads, 1875 to 4096 blocks: 45 MB of bounds in 13.2 us,
+// 3.4 TB/s, the chain plan, table, bounds being a third of it.  (The matrix kernel below with
+// one token a tile: 18; its loads take 64 bytes of a row at a time.)
+template <int D>
+__global__ __launch_bounds__(kSparseThreads) void score_token_kernel(ScoreKernelArgs a) {
+  constexpr int CH = 2 * D / 16, RP = 64 / CH;             // lanes of a row, rows of a load
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & (CH - 1), r = lane / CH;
+  const int t = a.t0 + blockIdx.x, kvh = blockIdx.y;
+  const int4 tok = a.tok[t];
+  const int c0 = blockIdx.z * a.chunk + 64 * wid, c1 = min(tok.z, (int)(blockIdx.z + 1) * a.chunk);
+  if (tok.x < 0 || c0 >= c1) return;
+  const int32_t* btrow = a.bt + (int64_t)tok.x * a.bt_stride;
+  uint4 w[CH];
+  int ebyte;
+  const int own = RP * c + r;                // this lane's block of 64
+  auto load = [&](int b0) {
+    const int blk = b0 + own < c1 ? min(max(btrow[b0 + own], 0), a.nb - 1) : 0;
+    ebyte = a.scale[(int64_t)blk * a.hkv + kvh];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {           // rows RP i .. RP i + RP - 1
+      const int at = __shfl(blk, (lane & ~(CH - 1)) + i);
+      w[i] = reinterpret_cast<const uint4*>(a.bounds + ((int64_t)at * a.hkv + kvh) * 2 * D)[c];
+    }
+  };
+  load(c0);
+  // the queries, while the bounds arrive: heads r, r + RP, .. of the group
+  const uint16_t* qt = a.q + (int64_t)t * a.q_ts + (int64_t)kvh * a.group * a.q_hs + 16 * (c & (CH / 2 - 1));
+  uint32_t amax = 0;
+  for (int h = r; h < a.group; h += RP) {
+    const uint4* qp = reinterpret_cast<const uint4*>(qt + (int64_t)h * a.q_hs);
+    amax = finite_max(qp[1], finite_max(qp[0], amax));
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, d));
+  const float f = __builtin_ldexpf(c < CH / 2 ? 1.f : -1.f, -bound_exp(amax));
+  uint32_t s[8] = {};
+  for (int h = r; h < a.group; h += RP) {
+    const uint4* qp = reinterpret_cast<const uint4*>(qt + (int64_t)h * a.q_hs);
+    add_whole(qp[0], f, s);
+    add_whole(qp[1], f, s + 4);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int d = CH; d < 64; d <<= 1) s[i] += (uint32_t)__shfl_xor((int)s[i], d);
+  }
+  const uint4 low = low_bytes(s), up = up_bytes(s);
+  float* out = a.scores + ((int64_t)(t - a.t0) * a.hkv + kvh) * a.width;
+  for (int b0 = c0;;) {
+    int x[CH];
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const uint32_t k[4] = {w[i].x, w[i].y, w[i].z, w[i].w}, l[4] = {low.x, low.y, low.z, low.w},
+                     u[4] = {up.x, up.y, up.z, up.w};
+      int ls = 0, us = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        ls = __builtin_amdgcn_sdot4((int)l[j], (int)k[j], ls, false);
+        us = __builtin_amdgcn_sdot4((int)u[j], (int)k[j], us, false);
+      }
+      x[i] = ls + (us << 8);
+    }
+    const int sum = sum_of_own<CH>(x, c), e = ebyte - 127, blk = b0 + own;
+    b0 += kSparseThreads;
+    if (b0 < c1) load(b0);
+    if (blk < c1) out[blk] = __builtin_ldexpf((float)sum, e);
+    if (b0 >= c1) break;
+  }
+}
+
+constexpr int kScoreTiles = 4, kTileTokens = 8 * kScoreTiles;
+
+// Many tokens of a request: a work-group is `tiles` tiles of 8 tokens of a KV head, two
+// rows each, low and upper bytes, against `chunk` blocks.
 //   A wave holds 64 blocks' bounds in registers; while the first of them arrive, the
 // queries become whole numbers in LDS, in MFMA order.  Then it goes over the tiles: S =
 // Q B^T on v_mfma_i32_16x16x64_i8, lane (row or block n, group g) with bytes 64 j + 16 g ..
-// of [q+ (D), q- (D)] and of [hi, nlo]; the four accumulators are rows 4 g .. 4 g + 3 of
-// block n.  Tokens of several requests are taken one request at a time.
-//   Few tokens: one tile; many: four, so that the bounds are read once for them (512
-// tokens, 28/4 heads, 513 blocks, with the selection: 28.0 us, 30.6 with eight, 32.5 with
-// two).  Waves of one work-group on four KV heads, whose bounds of a block are
-// neighbours, were no faster on single tokens.
+// of [sum q+ (D), sum q- (D)] and of [hi, nlo]; the four accumulators are tokens 2 g and
+// 2 g + 1 against block n.  Tokens of several requests are taken one request at a time.
+//   512 tokens, 28/4 heads, 513 blocks: 14.5 us, with the selection 23.0; 23.4 with one
+// tile a work-group, 24.8 with two, 37 with eight.  Waiting bounds it, for queries and
+// bounds one after the other; a row per head instead of two per token took 28.0.
 template <int D>
 __global__ __launch_bounds__(kSparseThreads) void score_kernel(ScoreKernelArgs a) {
   constexpr int KS = 2 * D / 64;             // MFMA steps
-  extern __shared__ uint4 qfrag[];           // [tile][head block][step][lane]
+  __shared__ uint4 qfrag[kScoreTiles * KS * 64];           // [tile][step][lane]
   __shared__ int2 info[kTileTokens];         // the tokens' requests and visible blocks
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int lanes = a.lanes, hblocks = (a.group + 15) / 16;
-  const int tb = a.t0 + blockIdx.x * a.per * a.tiles;
-  const int tokens = min(a.per * a.tiles, a.t1 - tb);
+  const int tb = a.t0 + blockIdx.x * kTileTokens;
+  const int tokens = min(kTileTokens, a.t1 - tb);
   const int c0 = blockIdx.z * a.chunk;
   // (nothing to do where no token sees the chunk's blocks)
   int see = 0;
-  for (int i = lane; i < tokens; i += 64) {
-    const int4 x = a.tok[tb + i];
-    see = max(see, x.z);
-    if (wid == 0) info[i] = make_int2(x.x, x.z);
+  if (lane < tokens) {
+    const int4 x = a.tok[tb + lane];
+    see = x.z;
+    if (wid == 0) info[lane] = make_int2(x.x, x.z);
   }
   if (__ballot(see > c0) == 0) return;
 #pragma unroll
@@ -362,105 +493,93 @@ __global__ __launch_bounds__(kSparseThreads) void score_kernel(ScoreKernelArgs a
   const int first_req = __builtin_amdgcn_readfirstlane(a.tok[tb].x);
   const bool ahead = first_req >= 0 && c0 + own < see;
   if (ahead) load_bounds(first_req, c0 + own, min(see, c0 + a.chunk));
-  const int tn = n / lanes, hn = n - tn * lanes;       // this lane's row: token of the tile, head
-  for (int u = wid; u < a.tiles; u += kSparseThreads / 64) {
-    const int ti = u * a.per + tn;
-    const bool row = ti < tokens && tn < a.per;
-    const uint16_t* qt = a.q + (int64_t)(tb + ti) * a.q_ts + (int64_t)kvh * a.group * a.q_hs;
+  // lane (token n / 2 of the tile, sign n % 2, g) adds up dims 64 j + 16 g .. + 15
+  const int tn = n >> 1, sign = n & 1;
+  for (int u = wid; 8 * u < tokens; u += kSparseThreads / 64) {
+    const int ti = 8 * u + tn;
+    const int heads = ti < tokens ? a.group : 0;
+    const uint16_t* qt = a.q + (int64_t)(tb + ti) * a.q_ts + (int64_t)kvh * a.group * a.q_hs + 16 * g;
     uint32_t amax = 0;                       // largest finite |q| of the token's heads
-    for (int hb = 0; hb < hblocks; ++hb) {
-      if (!row || hn + 16 * hb >= a.group) continue;
-      const uint4* qp = reinterpret_cast<const uint4*>(qt + (int64_t)(hn + 16 * hb) * a.q_hs);
+    for (int h0 = 0; h0 < heads; h0 += 4) {  // (four heads' loads at a time; each sign takes half)
+      uint4 w[4][D / 64];
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        const uint4 w = qp[4 * j + g];
-        const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+      for (int i = 0; i < 4; ++i) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t lo = p[i] & 0x7fffu, up = (p[i] >> 16) & 0x7fffu;
-          amax = max(amax, lo < 0x7f80u ? lo : 0u);
-          amax = max(amax, up < 0x7f80u ? up : 0u);
+        for (int j = 0; j < D / 64; ++j)
+          w[i][j] = reinterpret_cast<const uint4*>(qt + (int64_t)min(h0 + i, heads - 1) * a.q_hs + 64 * j)[sign];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) amax = finite_max(w[i][j], amax);
+      }
+    }
+    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 1));
+    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
+    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
+    const float f = __builtin_ldexpf(sign ? -1.f : 1.f, -bound_exp(amax));
+    uint32_t s[D / 64][8] = {};
+    for (int h0 = 0; h0 < heads; h0 += 2) {
+      uint4 w[2][D / 64][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+          const uint4* qp = reinterpret_cast<const uint4*>(qt + (int64_t)min(h0 + i, heads - 1) * a.q_hs + 64 * j);
+          w[i][j][0] = qp[0];
+          w[i][j][1] = qp[1];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float fi = h0 + i < heads ? f : 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) {
+          add_whole(w[i][j][0], fi, s[j]);
+          add_whole(w[i][j][1], fi, s[j] + 4);
         }
       }
     }
-    for (int d = 1; d < lanes; d <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, d));
-    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
-    amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
-    const float f = __builtin_ldexpf(1.f, -bound_exp(amax));
-    for (int hb = 0; hb < hblocks; ++hb) {
-      const bool live = row && hn + 16 * hb < a.group;
-      const uint16_t* qp = qt + (int64_t)(hn + 16 * hb) * a.q_hs;
 #pragma unroll
-      for (int j = 0; j < KS / 2; ++j) {
-        uint32_t pos[4] = {0, 0, 0, 0}, neg[4] = {0, 0, 0, 0};
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint4 w = make_uint4(0, 0, 0, 0);
-          if (live) w = reinterpret_cast<const uint4*>(qp + 64 * j + 16 * g)[half];
-          const uint32_t p[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float x = i & 1 ? aia::bf16_hi(p[i >> 1]) : aia::bf16_lo(p[i >> 1]);
-            const int v = __builtin_fabsf(x) < INFINITY ? (int)__builtin_rintf(x * f) : 0;
-            pos[2 * half + (i >> 2)] |= (uint32_t)max(v, 0) << (8 * (i & 3));
-            neg[2 * half + (i >> 2)] |= (uint32_t)max(-v, 0) << (8 * (i & 3));
-          }
-        }
-        uint4* to = qfrag + (int64_t)((u * hblocks + hb) * KS) * 64 + lane;
-        to[j * 64] = make_uint4(pos[0], pos[1], pos[2], pos[3]);
-        to[(KS / 2 + j) * 64] = make_uint4(neg[0], neg[1], neg[2], neg[3]);
-      }
+    for (int j = 0; j < D / 64; ++j) {
+      uint4* to = qfrag + (u * KS + sign * (D / 64) + j) * 64 + 16 * g + 2 * tn;
+      to[0] = low_bytes(s[j]);
+      to[1] = up_bytes(s[j]);
     }
   }
   __syncthreads();
-  auto frag = [&](int m, int hb, int j) {
-    return __builtin_bit_cast(int4v_t, as_u4(qfrag[((m * hblocks + hb) * KS + j) * 64 + lane]));
-  };
   for (int done = 0; done < tokens;) {
     const int from = done, req = __builtin_amdgcn_readfirstlane(info[from].x);
-    int vis = 0;                             // tokens [from, done) of one request
-    for (bool more = true; more && done < tokens;) {         // 64 at a time
-      const int2 x = done + lane < tokens ? info[done + lane] : make_int2(-2, 0);
-      const uint64_t other = __ballot(x.x != req);
-      const int here = other ? __builtin_ctzll(other) : 64;
-      int v = lane < here ? x.y : 0;
+    // tokens [from, done) of one request (a work-group has at most 64)
+    const int2 x = from + lane < tokens ? info[from + lane] : make_int2(-2, 0);
+    const uint64_t other = __ballot(x.x != req);
+    const int here = other ? __builtin_ctzll(other) : 64;
+    int vis = lane < here ? x.y : 0;
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) v = max(v, __shfl_xor(v, d));
-      vis = max(vis, __builtin_amdgcn_readfirstlane(v));
-      done += here;
-      more = here == 64;
-    }
-    const int c1 = min(vis, c0 + a.chunk);
+    for (int d = 1; d < 64; d <<= 1) vis = max(vis, __shfl_xor(vis, d));
+    done += here;
+    const int c1 = min(__builtin_amdgcn_readfirstlane(vis), c0 + a.chunk);
     if (req < 0) continue;
     for (int b0 = c0 + own; b0 < c1; b0 += kSparseThreads) {
       if (from > 0 || b0 > c0 + own || !ahead) load_bounds(req, b0, c1);
-      for (int m = from / a.per; m * a.per < done; ++m) {
+      for (int m = from / 8; m * 8 < done; ++m) {
         int4v_t acc[4];
 #pragma unroll
         for (int s = 0; s < 4; ++s) acc[s] = int4v_t{0, 0, 0, 0};
-        for (int hb = 0; hb < hblocks; ++hb) {
 #pragma unroll
-          for (int j = 0; j < KS; ++j) {
-            const int4v_t qf = frag(m, hb, j);
+        for (int j = 0; j < KS; ++j) {
+          const int4v_t qf = __builtin_bit_cast(int4v_t, as_u4(qfrag[(m * KS + j) * 64 + lane]));
 #pragma unroll
-            for (int s = 0; s < 4; ++s) acc[s] = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf, bf[s][j], acc[s], 0, 0, 0);
-          }
+          for (int s = 0; s < 4; ++s) acc[s] = __builtin_amdgcn_mfma_i32_16x16x64_i8(qf, bf[s][j], acc[s], 0, 0, 0);
         }
+        const int t = 8 * m + 2 * g;
+        float* out = a.scores + ((int64_t)(tb + t - a.t0) * a.hkv + kvh) * a.width + b0 + n;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          // sums over a token's rows: `lanes` of the rows 4 g + v
-          int sum[4] = {acc[s][0], acc[s][1], acc[s][2], acc[s][3]};
-          if (lanes > 1) { sum[0] += sum[1]; sum[2] += sum[3]; }
-          if (lanes > 2) sum[0] += sum[2];
-          if (lanes > 4) sum[0] += __shfl_xor(sum[0], 16);
-          if (lanes > 8) sum[0] += __shfl_xor(sum[0], 32);
-          const int blk = b0 + 16 * s + n;
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const int r = 4 * g + v, t = m * a.per + r / lanes;
-            if (r % lanes || t < from || t >= done || r / lanes >= a.per || blk >= c1) continue;
-            a.scores[((int64_t)(tb + t - a.t0) * a.hkv + kvh) * a.width + blk] = __builtin_ldexpf((float)sum[v], eb[s]);
-          }
+          if (b0 + 16 * s + n >= c1) continue;
+          if (t >= from && t < done) out[16 * s] = __builtin_ldexpf((float)(acc[s][0] + (acc[s][1] << 8)), eb[s]);
+          if (t + 1 >= from && t + 1 < done)
+            out[(int64_t)a.hkv * a.width + 16 * s] = __builtin_ldexpf((float)(acc[s][2] + (acc[s][3] << 8)), eb[s]);
         }
       }
     }
@@ -482,16 +601,16 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t u = __float_as_uint(x);
   return min(u & 0x80000000u ? ~u : u | 0x80000000u, 0xfffffffeu);
 }
-__device__ __forceinline__ uint32_t key_at(const SelectArgs& a, const float* sc, int i, int n) {
-  if (i >= n) return 0;
-  return i < a.sink || i >= n - a.local ? 0xffffffffu : order_key(sc[i]);
+__device__ __forceinline__ uint32_t key_of(const SelectArgs& a, float score, int i, int n) {
+  const uint32_t k = i < a.sink || i >= n - a.local ? 0xffffffffu : order_key(score);
+  return i < n ? k : 0;
 }
 
 // A wave per row, for tables of up to 64 NK blocks: the key of the `selected`-th largest
-// score bit by bit from the top, counting by ballots, until a bound has exactly so many
-// above it; then the blocks above it and the first of those at it, in order.  No
-// barriers, no LDS.  (A work-group per row that counts digits in LDS: 17.0 us for 2048
-// rows of 513 blocks.)
+// score bit by bit, from the highest bit in which the scores differ, counting by ballots,
+// until a bound has exactly so many above it; then the blocks above it and the first of those at it, in order.  No
+// barriers, no LDS.  2048 rows of 513 blocks: 8.8 us; a work-group per row that counts
+// digits in LDS: 17.0.
 template <int NK>
 __global__ __launch_bounds__(256) void select_wave_kernel(SelectArgs a) {
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -505,13 +624,34 @@ __global__ __launch_bounds__(256) void select_wave_kernel(SelectArgs a) {
     return;
   }
   const float* sc = a.scores + (int64_t)row * a.width;
+  float x[NK];                               // (all loads in flight: none under a condition)
+#pragma unroll
+  for (int j = 0; j < NK; ++j) x[j] = sc[min(64 * j + lane, n - 1)];
   uint32_t k[NK];
 #pragma unroll
-  for (int j = 0; j < NK; ++j) k[j] = key_at(a, sc, 64 * j + lane, n);
+  for (int j = 0; j < NK; ++j) k[j] = key_of(a, x[j], 64 * j + lane, n);
   // (keys behind the row's end are 0, below every bound that is tried)
-  uint32_t p = 0;
+  uint32_t p = 0xfffffffeu;                  // (all that is taken are blocks that always are)
+  int top = -1;
+  if (a.selected > a.sink + a.local) {
+    uint32_t most = 0, least = 0xfffffffeu;
+#pragma unroll
+    for (int j = 0; j < NK; ++j) {
+      if (k[j] < 0xffffffffu) most = max(most, k[j]);
+      if (64 * j + lane < n) least = min(least, k[j]);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      most = max(most, (uint32_t)__shfl_xor((int)most, d));
+      least = min(least, (uint32_t)__shfl_xor((int)least, d));
+    }
+    most = (uint32_t)__builtin_amdgcn_readfirstlane((int)most);
+    least = (uint32_t)__builtin_amdgcn_readfirstlane((int)least);
+    top = most > least ? 31 - __builtin_clz(most ^ least) : -1;
+    p = top < 0 ? most : most >> top >> 1 << top << 1;     // the bits in common
+  }
 #pragma unroll 1
-  for (int bit = 31; bit >= 0; --bit) {
+  for (int bit = top; bit >= 0; --bit) {
     const uint32_t bound = p | 1u << bit;
     int count = 0;
 #pragma unroll
@@ -539,9 +679,12 @@ __global__ __launch_bounds__(256) void select_wave_kernel(SelectArgs a) {
 constexpr int kSelThreads = 512, kSelWaves = kSelThreads / 64;
 constexpr int kDigits = 2048;
 
-// A work-group per row, for longer tables: the same key by 11 bits at a time, counted in
-// LDS.  A wave has a run of the row's blocks, up to 64 NK of them in registers (NK 0:
-// any number, read again in every pass).
+// A work-group per row, for longer tables: the same key by up to 11 bits at a time of what
+// it is above the row's least one, counted in LDS.  (Without the least taken off, the
+// first digit is mostly the exponent: one pass more and counters that many lanes hit at
+// once, 10.5 us for 64 rows of 1875 to 4096 blocks; 9.5 so, of which waiting for the scores
+// and the launch are most.)  A wave has a run of the row's blocks,
+// up to 64 NK of them in registers (NK 0: any number, read again in every pass).
 template <int NK>
 __global__ __launch_bounds__(kSelThreads) void select_kernel(SelectArgs a) {
   __shared__ int hist[kDigits];
@@ -557,27 +700,52 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(SelectArgs a) {
   const float* sc = a.scores + (int64_t)blockIdx.x * a.width;
   const int rounds = (n + kSelThreads - 1) / kSelThreads, first = wid * 64 * rounds + lane;
   uint32_t held[NK > 0 ? NK : 1];
+  if constexpr (NK > 0) {                    // (all loads in flight: none under a condition)
+    float x[NK];
 #pragma unroll
-  for (int j = 0; j < NK; ++j) held[j] = j < rounds ? key_at(a, sc, first + 64 * j, n) : 0;
+    for (int j = 0; j < NK; ++j) x[j] = sc[min(first + 64 * min(j, rounds - 1), n - 1)];
+#pragma unroll
+    for (int j = 0; j < NK; ++j) held[j] = key_of(a, x[j], first + 64 * j, n);
+  }
   auto each = [&](auto f) {
     if constexpr (NK > 0) {
 #pragma unroll
       for (int j = 0; j < NK; ++j)
         if (j < rounds) f(first + 64 * j, held[j]);
     } else {
-      for (int j = 0; j < rounds; ++j) f(first + 64 * j, key_at(a, sc, first + 64 * j, n));
+      for (int j = 0; j < rounds; ++j) f(first + 64 * j, key_of(a, sc[min(first + 64 * j, n - 1)], first + 64 * j, n));
     }
   };
-  uint32_t prefix = 0;                       // the digits found so far
-  int need = a.selected, shift = 32;         // blocks to take among those of the prefix
+  for (int i = tid; i < kDigits; i += kSelThreads) hist[i] = 0;
+  uint32_t most = 0, least = 0xfffffffeu;
+  each([&](int i, uint32_t k) {
+    if (k < 0xffffffffu) most = max(most, k);
+    if (i < n) least = min(least, k);
+  });
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    most = max(most, (uint32_t)__shfl_xor((int)most, d));
+    least = min(least, (uint32_t)__shfl_xor((int)least, d));
+  }
+  if (lane == 0) { wave_a[wid] = (int)most; wave_b[wid] = (int)least; }
+  __syncthreads();
+  for (int w = 0; w < kSelWaves; ++w) {
+    most = max(most, (uint32_t)wave_a[w]);
+    least = min(least, (uint32_t)wave_b[w]);
+  }
+  __syncthreads();
+  // The always kept blocks are counted apart: `need` of the others are left to take.
+  int need = a.selected - a.sink - a.local;
+  uint32_t prefix = need > 0 ? 0u : 0xffffffffu;           // the digits found so far
+  int shift = 0;
+  int left = need > 0 && most > least ? 32 - __builtin_clz(most - least) : 0;
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int bits = pass == 2 ? 10 : 11;
-    shift -= bits;
-    for (int i = tid; i < kDigits; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
+  for (bool all = true; left > 0; all = false) {
+    const int bits = min(left, 11);
+    shift = left - bits;
     each([&](int i, uint32_t k) {
-      if (i < n && (pass == 0 || k >> (shift + bits) == prefix)) atomicAdd(&hist[k >> shift & ((1 << bits) - 1)], 1);
+      if (i < n && k < 0xffffffffu && (all || (k - least) >> left == prefix))
+        atomicAdd(&hist[(k - least) >> shift & ((1 << bits) - 1)], 1);
     });
     __syncthreads();
     // digits from the largest down: thread tid has kDigits / kSelThreads of them
@@ -585,7 +753,11 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(SelectArgs a) {
     const int top = kDigits - 1 - PER * tid;
     int c[PER], sum = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) { c[i] = hist[top - i]; sum += c[i]; }
+    for (int i = 0; i < PER; ++i) {
+      c[i] = hist[top - i];
+      hist[top - i] = 0;
+      sum += c[i];
+    }
     int upto = sum;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -606,13 +778,15 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(SelectArgs a) {
     __syncthreads();
     prefix = prefix << bits | (uint32_t)found[0];
     need = found[1];
-    if (found[2] == need) break;             // all of the digit's blocks are taken
+    left = found[2] == need ? 0 : shift;     // (all of the digit's blocks are taken)
   }
-  // blocks above the prefix, and the first `need` of those of it
+  // the always kept ones, the blocks above the prefix, and the first `need` of those of it
+  auto upper = [&](int i, uint32_t k) { return i < n && (k == 0xffffffffu || (k - least) >> shift > prefix); };
+  auto equal = [&](int i, uint32_t k) { return i < n && k != 0xffffffffu && (k - least) >> shift == prefix; };
   int more = 0, ties = 0;
   each([&](int i, uint32_t k) {
-    more += __popcll(__ballot(i < n && k >> shift > prefix));
-    ties += __popcll(__ballot(i < n && k >> shift == prefix));
+    more += __popcll(__ballot(upper(i, k)));
+    ties += __popcll(__ballot(equal(i, k)));
   });
   __syncthreads();
   if (lane == 0) { wave_a[wid] = more; wave_b[wid] = ties; }
@@ -621,7 +795,7 @@ __global__ __launch_bounds__(kSelThreads) void select_kernel(SelectArgs a) {
   for (int w = 0; w < wid; ++w) { at += wave_a[w]; tied += wave_b[w]; }
   const uint64_t below = (1ull << lane) - 1;
   each([&](int i, uint32_t k) {
-    const bool up = i < n && k >> shift > prefix, eq = i < n && k >> shift == prefix;
+    const bool up = upper(i, k), eq = equal(i, k);
     const uint64_t mu = __ballot(up), me = __ballot(eq);
     const int ub = at + __popcll(mu & below), eb = tied + __popcll(me & below);
     if (up || (eq && eb < need)) out[ub + min(eb, need)] = i;
@@ -933,37 +1107,32 @@ extern "C" int aia_select_blocks(const void* query, int64_t q_token_stride, int6
   if (!aligned16(query) || !aligned16(bounds) || q_token_stride % 8 || q_head_stride % 8)
     return fail(AIA_ERR_INVALID, "aia_select_blocks: tensors must be 16-byte aligned with strides a multiple of 8");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  const int group = num_q_heads / num_kv_heads;
-  int lanes = 1;
-  while (lanes < group && lanes < 16) lanes <<= 1;
   ScoreKernelArgs a;
   a.q = static_cast<const uint16_t*>(query); a.q_ts = q_token_stride; a.q_hs = q_head_stride;
   a.bounds = static_cast<const int8_t*>(bounds); a.scale = static_cast<const uint8_t*>(bounds_scale);
   a.bt = block_table; a.bt_stride = block_table_stride;
   a.tok = reinterpret_cast<const int4*>(ws + L.tok);
   a.scores = reinterpret_cast<float*>(ws + L.scores);
-  a.hkv = num_kv_heads; a.group = group; a.nb = num_blocks; a.width = table_width;
-  a.lanes = lanes;
+  a.hkv = num_kv_heads; a.group = num_q_heads / num_kv_heads; a.nb = num_blocks; a.width = table_width;
   // Tokens of a tile share their request's bounds: worth it where requests have several.
-  const bool many = num_tokens >= 4 * batch && group <= 16;
-  const int hblocks = (group + 15) / 16;
-  a.per = many ? 16 / lanes : 1;
-  a.tiles = many && num_tokens >= kScoreTiles * a.per ? kScoreTiles : 1;
+  const bool many = num_tokens >= 4 * batch;
+  const int per = many ? kTileTokens : 1;
   SelectArgs s;
   s.scores = a.scores; s.tok = a.tok; s.out = selected; s.out_ts = sel_token_stride; s.out_hs = sel_head_stride;
   s.hkv = num_kv_heads; s.width = table_width; s.selected = num_selected; s.sink = sink; s.local = local;
-  const size_t lds = (size_t)a.tiles * hblocks * (2 * head_dim / 64) * 64 * 16;
   hipStream_t st = (hipStream_t)stream;
   for (int t0 = 0; t0 < num_tokens; t0 += L.score_tokens) {
     const int t1 = std::min(num_tokens, t0 + L.score_tokens);
     a.t0 = t0; a.t1 = t1; s.t0 = t0; s.rows = (t1 - t0) * num_kv_heads;
-    const unsigned gx = (unsigned)((t1 - t0 + a.per * a.tiles - 1) / (a.per * a.tiles));
+    const unsigned gx = (unsigned)((t1 - t0 + per - 1) / per);
     // work-groups: about eight per compute unit, each of 256 blocks (64 a wave) or more
     const int64_t batches = (table_width + kSparseThreads - 1) / kSparseThreads;
     const int64_t cuts = std::max<int64_t>(1, std::min<int64_t>(2048 / std::max<int64_t>(1, (int64_t)gx * num_kv_heads), batches));
     a.chunk = (int)((batches + cuts - 1) / cuts * kSparseThreads);
     const dim3 grid(gx, (unsigned)num_kv_heads, (unsigned)((table_width + a.chunk - 1) / a.chunk));
-    (head_dim == 128 ? score_kernel<128> : score_kernel<64>)<<<grid, kSparseThreads, lds, st>>>(a);
+    auto* score = many ? (head_dim == 128 ? score_kernel<128> : score_kernel<64>)
+                       : (head_dim == 128 ? score_token_kernel<128> : score_token_kernel<64>);
+    score<<<grid, kSparseThreads, 0, st>>>(a);
     if (int rc = check_hip(hipGetLastError(), "aia_select_blocks: score launch")) return rc;
     if (table_width <= 1024) {
       auto* kernel = table_width <= 256 ? select_wave_kernel<4> : table_width <= 512 ? select_wave_kernel<8>
