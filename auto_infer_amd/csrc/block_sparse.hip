@@ -844,19 +844,24 @@ struct SparseRow {
     for (int i = 0; i < a.selected; i += 64) {
       const int e = i + lane < a.selected ? sel[i + lane] : -1;
       int upto = e;                          // the largest entry up to this lane's
+      int prev = __shfl_up(upto, 1);
+      int last = __popcll(__ballot(e >= 0)) - 1;       // in order: the largest entry's lane
+      if (__any(lane && e >= 0 && (prev < 0 || prev >= e))) {
+        last = 63;
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int x = __shfl_up(upto, d);
-        if (lane >= d) upto = max(upto, x);
+        for (int d = 1; d < 64; d <<= 1) {
+          const int x = __shfl_up(upto, d);
+          if (lane >= d) upto = max(upto, x);
+        }
+        prev = __shfl_up(upto, 1);
       }
-      const int prev = __shfl_up(upto, 1);
       const int before = lane ? max(most, prev) : most;
       const bool ok = e >= b0 && e < min(b1, tk.z) && e > before;
       const uint64_t m = __ballot(ok);
       if (ok) list[count + __popcll(m & ((1ull << lane) - 1))] = btrow[e];
       count += __popcll(m);
       own |= __any(ok && e == tk.y / a.c.bs) != 0;
-      most = max(most, __shfl(upto, 63));
+      if (last >= 0) most = max(most, __shfl(upto, last));
       if (most >= b1) break;                 // (the rest is behind the range)
     }
     keys = count * a.c.bs - (own ? a.c.bs - 1 - tk.y % a.c.bs : 0);
@@ -940,6 +945,8 @@ __global__ __launch_bounds__(64 * kSpWaves) __attribute__((amdgpu_waves_per_eu(3
   const int t = a.t0 + i / hblocks / a.c.hkv, kvh = i / hblocks % a.c.hkv;
   if (t >= a.t1) return;
   const SparseRow r(a, t, kvh, i % hblocks);
+  uint4 qf[D / 32];                          // (arrives while the list is made)
+  load_q<D>(r.query(a, n), g, qf);
   int keys;
   const int blocks = min(kRangeBlocks, (a.hdr[1] + a.parts - 1) / a.parts), b0 = part * blocks;
   const int count = r.blocks(a, b0, b0 + blocks, list[wid], lane, keys);
@@ -949,8 +956,6 @@ __global__ __launch_bounds__(64 * kSpWaves) __attribute__((amdgpu_waves_per_eu(3
     if (live && g == 0) a.part_ml[row] = make_float2(-INFINITY, 0.f);
     return;
   }
-  uint4 qf[D / 32];
-  load_q<D>(r.query(a, n), g, qf);
   RowState<D> s;
   s.clear();
   __builtin_amdgcn_wave_barrier();           // the list is the wave's own
