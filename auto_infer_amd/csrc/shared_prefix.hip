@@ -25,18 +25,14 @@ constexpr int kLightRows = 64;                            // up to here a unit w
 constexpr int kKeys = 64;                                 // keys of a tile
 constexpr int kMaxShared = 4096;                          // requests: the planner's LDS arrays
 constexpr int kShPlanT = 1024;
-#ifndef SH_TARGET
-#define SH_TARGET 512
-#endif
-#ifndef SH_MINW
-#define SH_MINW 8
-#endif
-#ifndef SH_TURN
-#define SH_TURN 256
-#endif
-constexpr int kTargetGroups = SH_TARGET;                  // units to aim at: two per compute unit
-constexpr int kMinCut = SH_MINW;                          // tiles of a cut
-constexpr int kTurn = SH_TURN;
+constexpr int kTargetGroups = 512;                        // units to aim at: two per compute unit
+// Tiles of a cut: fewer make a unit's queries and its join cost more, more leave small
+// steps few units.  16 requests on a prefix of 4K: 21.6 us with eight, 20.4 with four; 40
+// requests of three tokens on five prefixes, 8-bit: 21.8 and 23.2.
+constexpr int kMinCut = 8;
+// Units of a kind in a row.  128 requests on a prefix of 32K, before later steps: 262 us
+// with 256 (a unit per compute unit), 272 with all heavy ones first, 281 with 512.
+constexpr int kTurn = 256;
 constexpr int kMinShare = 128;                            // keys worth a part of their own
 constexpr int kRecord = 12, kHdr = 64;
 
@@ -416,6 +412,11 @@ __device__ __forceinline__ void finish_row(const ShArgs& a, const Unit& u, int k
 // chunk c at c ^ 2 (r % (RC / 2)) (RC = D / 8 chunks a row), which spreads the fragment
 // reads over the banks.  8-bit caches: a thread's chunks wait in registers and become
 // bf16 on their way to the same places, once per work-group.
+//   128 requests on a prefix of 32K with 100 to 2048 keys of their own (64/8 heads, D 128):
+// 228 us with the join.  The prefix's 1024 rows a KV head alone take 149 us, 0.92 PFLOP/s,
+// bound by the softmax between the matrix products; the requests' own keys alone 137 us,
+// 2.6 TB/s, bound by the two tiles in flight per work-group.  16 requests on a prefix of
+// 4K: 21.6 us, of which a launch each for units and join and their first loads are most.
 template <int D, bool F8, bool ONE_BLOCK, int WK>
 __device__ __forceinline__ void unit_rows(const ShArgs& a, const Unit& u, uint16_t* k0b, uint16_t* k1b,
                                           uint16_t* v0b, uint16_t* v1b, int* odd_tile, float2 (*share)[16 * kRt]) {
