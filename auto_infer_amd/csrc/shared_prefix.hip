@@ -415,7 +415,7 @@ __device__ __forceinline__ void finish_row(const ShArgs& a, const Unit& u, int k
 //   128 requests on a prefix of 32K with 100 to 2048 keys of their own (64/8 heads, D 128):
 // 228 us with the join.  The prefix's 1024 rows a KV head alone take 149 us, 0.92 PFLOP/s,
 // bound by the softmax between the matrix products; the requests' own keys alone 137 us,
-// 2.6 TB/s, bound by the two tiles in flight per work-group.  16 requests on a prefix of
+// 4.2 TB/s, bound by the two tiles in flight per work-group.  16 requests on a prefix of
 // 4K: 21.6 us, of which a launch each for units and join and their first loads are most.
 template <int D, bool F8, bool ONE_BLOCK, int WK>
 __device__ __forceinline__ void unit_rows(const ShArgs& a, const Unit& u, uint16_t* k0b, uint16_t* k1b,
