@@ -106,15 +106,20 @@ __device__ __forceinline__ void attend(const CacheArgs& a, int kvh, const uint4 
   p1 = __builtin_amdgcn_readfirstlane(p1);
   entries = __builtin_amdgcn_readfirstlane(entries);
   if (p0 >= p1) return;
+  const int block_tiles = a.bs / kTile;      // of whole blocks
   const int row_bytes = a.hkv * D * CELL, head_bytes = kvh * D * CELL;
-  const uint8_t* kc = reinterpret_cast<const uint8_t*>(a.kc) + head_bytes + 16 * lc;
-  const uint8_t* vc = reinterpret_cast<const uint8_t*>(a.vc) + head_bytes + 16 * lc;
+  const uint8_t* kc = reinterpret_cast<const uint8_t*>(a.kc) + head_bytes;
+  const uint8_t* vc = reinterpret_cast<const uint8_t*>(a.vc) + head_bytes;
   int base = 0, bend = 0, ids = 0, sev = 0;  // list entries held by the lanes: [base, bend)
   int end = 0;                               // places of the window
 
   uint4 kk[kNt][LD], vv[kNt][LD];
   int64_t at[kNt][WHOLE ? 1 : LD];           // byte offsets of the rows being loaded
-  int off[kNt][WHOLE ? LD : 1];
+  uint32_t off[kNt][WHOLE ? LD : 1];
+  uint32_t full[LD];                         // this lane's offsets in a tile
+#pragma unroll
+  for (int i = 0; i < LD; ++i) full[i] = (uint32_t)((i * RPL + lr) * row_bytes + 16 * lc);
+  int le = 0, lt = 0;                        // whole blocks: the next tile's entry from base on, its place there
   int ek[kNt][WHOLE ? 1 : LD], ev[kNt][WHOLE ? 1 : LD];      // 8-bit caches: scales of the keys in kk, vv
   // Tiles behind the window read its first row again (an L1 hit); keys behind the end
   // the last one (never a slot that may hold stale bytes).
@@ -124,23 +129,24 @@ __device__ __forceinline__ void attend(const CacheArgs& a, int kvh, const uint4 
       const int first = (t + st) * kTile;
       const bool in = first < end;
       if (WHOLE) {
-        const int p = in ? first : base * a.bs, e = p / a.bs;
-        const int blk = __builtin_amdgcn_readlane(ids, e - base);
-        if (F8) ek[st][0] = __builtin_amdgcn_readlane(sev, e - base);
-        at[st][0] = ((int64_t)blk * a.bs + (p - e * a.bs)) * row_bytes;
-        const int last = in ? end - 1 - first : 0;
+        const int e = in ? le : 0, blk = __builtin_amdgcn_readlane(ids, e);
+        if (F8) ek[st][0] = __builtin_amdgcn_readlane(sev, e);
+        at[st][0] = ((int64_t)blk * a.bs + (in ? lt * kTile : 0)) * row_bytes;
+        // (the least of the offsets is that of the least of the rows)
+        const uint32_t last = (uint32_t)((in ? min(end - 1 - first, kTile - 1) : 0) * row_bytes + 16 * lc);
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
-          off[st][i] = min(i * RPL + lr, last) * row_bytes;
+          off[st][i] = min(full[i], last);
           kk[st][i] = *reinterpret_cast<const uint4*>(kc + at[st][0] + off[st][i]);
         }
+        if (++lt == block_tiles) { lt = 0; ++le; }
       } else {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
           const int p = in ? min(first + i * RPL + lr, end - 1) : base * a.bs, e = p / a.bs;
           const int blk = __shfl(ids, e - base);
           if (F8) ek[st][i] = __shfl(sev, e - base);
-          at[st][i] = ((int64_t)blk * a.bs + (p - e * a.bs)) * row_bytes;
+          at[st][i] = ((int64_t)blk * a.bs + (p - e * a.bs)) * row_bytes + 16 * lc;
           kk[st][i] = *reinterpret_cast<const uint4*>(kc + at[st][i]);
         }
       }
@@ -183,6 +189,8 @@ __device__ __forceinline__ void attend(const CacheArgs& a, int kvh, const uint4 
       const int64_t se = (int64_t)ids * a.hkv + kvh;
       sev = a.ks[se] | a.vs[se] << 8;
     }
+    le = 0;
+    lt = WHOLE ? t0 - base * block_tiles : 0;
     load_k(t0);
     load_v();
     for (int t = t0; t < t1; t += kNt) {
