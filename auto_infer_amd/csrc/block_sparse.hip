@@ -335,16 +335,34 @@ __device__ __forceinline__ uint32_t finite_max(const uint4& w, uint32_t most) {
   }
   return most;
 }
-// Adds the whole numbers of one sign (f: the factor with it) of 8 bf16 to 4 words.
-__device__ __forceinline__ void add_whole(const uint4& w, float f, uint32_t s[4]) {
+// Largest |x| of 8 bf16, as their bits, packed in two halves; infinities and NaN count.
+typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ ushort2_t any_max(const uint4& w, ushort2_t most) {
   const uint32_t p[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float x = aia::bf16_lo(p[i]), y = aia::bf16_hi(p[i]);
-    const int u = __builtin_fabsf(x) < INFINITY ? max((int)__builtin_rintf(x * f), 0) : 0;
-    const int v = __builtin_fabsf(y) < INFINITY ? max((int)__builtin_rintf(y * f), 0) : 0;
-    s[i] += (uint32_t)(u | v << 16);
+  for (int i = 0; i < 4; ++i)
+    most = __builtin_elementwise_max(most, __builtin_bit_cast(ushort2_t, p[i] & 0x7fff7fffu));
+  return most;
+}
+// Adds kWhole + the whole numbers of one sign (f: the factor with it) of 8 bf16: |x f| <=
+// 127, and adding 1.5 * 2^23 rounds it to a whole number, to even, in the sum's low bits.
+// ODD: values that are not finite count as zero.  (With a check, a rounding and a
+// conversion for every value, 512 tokens take 23.1 us instead of 20.5.)
+constexpr uint32_t kWhole = 0x4b400000u;
+template <bool ODD>
+__device__ __forceinline__ void add_whole(const uint4& w, float f, uint32_t s[8]) {
+  const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float x = i & 1 ? aia::bf16_hi(p[i >> 1]) : aia::bf16_lo(p[i >> 1]);
+    if (ODD && !(__builtin_fabsf(x) < INFINITY)) x = 0.f;
+    s[i] += (uint32_t)max((int)__float_as_uint(__builtin_fmaf(x, f, 12582912.f)), (int)kWhole);
   }
+}
+// The sums of 16 numbers, n of them each, in pairs.
+__device__ __forceinline__ void pair_up(const uint32_t s[16], int n, uint32_t (&w)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = (s[2 * i] - n * kWhole) | (s[2 * i + 1] - n * kWhole) << 16;
 }
 
 // Sums over rows of CH lanes: lane c of a row gets the row's sum of x[c].  Each step
@@ -406,12 +424,14 @@ __global__ __launch_bounds__(kSparseThreads) void score_token_kernel(ScoreKernel
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) amax = max(amax, (uint32_t)__shfl_xor((int)amax, d));
   const float f = __builtin_ldexpf(c < CH / 2 ? 1.f : -1.f, -bound_exp(amax));
-  uint32_t s[8] = {};
-  for (int h = r; h < a.group; h += RP) {
+  uint32_t sum[16] = {}, s[8];
+  int heads = 0;
+  for (int h = r; h < a.group; h += RP, ++heads) {
     const uint4* qp = reinterpret_cast<const uint4*>(qt + (int64_t)h * a.q_hs);
-    add_whole(qp[0], f, s);
-    add_whole(qp[1], f, s + 4);
+    add_whole<true>(qp[0], f, sum);
+    add_whole<true>(qp[1], f, sum + 8);
   }
+  pair_up(sum, heads, s);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
 #pragma unroll
@@ -450,9 +470,9 @@ constexpr int kScoreTiles = 4, kTileTokens = 8 * kScoreTiles;
 // Q B^T on v_mfma_i32_16x16x64_i8, lane (row or block n, group g) with bytes 64 j + 16 g ..
 // of [sum q+ (D), sum q- (D)] and of [hi, nlo]; the four accumulators are tokens 2 g and
 // 2 g + 1 against block n.  Tokens of several requests are taken one request at a time.
-//   512 tokens, 28/4 heads, 513 blocks: 14.5 us, with the selection 23.0; 23.4 with one
-// tile a work-group, 24.8 with two, 37 with eight.  Waiting bounds it, for queries and
-// bounds one after the other; a row per head instead of two per token took 28.0.
+//   512 tokens, 28/4 heads, 513 blocks: 12 us, with the selection 20.5; 25.1 with one tile a
+// work-group, 20.6 with two, 26.2 with eight.  Waiting bounds it, and the instructions that
+// turn the queries to whole numbers; a row per head instead of two per token took 28.0.
 template <int D>
 __global__ __launch_bounds__(kSparseThreads) void score_kernel(ScoreKernelArgs a) {
   constexpr int KS = 2 * D / 64;             // MFMA steps
@@ -501,47 +521,61 @@ __global__ __launch_bounds__(kSparseThreads) void score_kernel(ScoreKernelArgs a
     const int ti = 8 * u + tn;
     const int heads = ti < tokens ? a.group : 0;
     const uint16_t* qt = a.q + (int64_t)(tb + ti) * a.q_ts + (int64_t)kvh * a.group * a.q_hs + 16 * g;
-    uint32_t amax = 0;                       // largest finite |q| of the token's heads
-    for (int h0 = 0; h0 < heads; h0 += 4) {  // (four heads' loads at a time; each sign takes half)
-      uint4 w[4][D / 64];
+    // largest |q| of the token's heads (four heads' loads at a time; each sign takes half)
+    auto largest = [&](auto most, auto of) {
+      for (int h0 = 0; h0 < heads; h0 += 4) {
+        uint4 w[4][D / 64];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 4; ++i) {
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j)
-          w[i][j] = reinterpret_cast<const uint4*>(qt + (int64_t)min(h0 + i, heads - 1) * a.q_hs + 64 * j)[sign];
+          for (int j = 0; j < D / 64; ++j)
+            w[i][j] = reinterpret_cast<const uint4*>(qt + (int64_t)min(h0 + i, heads - 1) * a.q_hs + 64 * j)[sign];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int j = 0; j < D / 64; ++j) most = of(w[i][j], most);
+        }
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int j = 0; j < D / 64; ++j) amax = finite_max(w[i][j], amax);
-      }
-    }
+      return most;
+    };
+    const ushort2_t both = largest(ushort2_t{0, 0}, [](const uint4& w, ushort2_t m) { return any_max(w, m); });
+    uint32_t amax = max((uint32_t)both[0], (uint32_t)both[1]);
+    const bool odd = __any(amax >= 0x7f80u);
+    if (odd) amax = largest(0u, [](const uint4& w, uint32_t m) { return finite_max(w, m); });
     amax = max(amax, (uint32_t)__shfl_xor((int)amax, 1));
     amax = max(amax, (uint32_t)__shfl_xor((int)amax, 16));
     amax = max(amax, (uint32_t)__shfl_xor((int)amax, 32));
     const float f = __builtin_ldexpf(sign ? -1.f : 1.f, -bound_exp(amax));
-    uint32_t s[D / 64][8] = {};
-    for (int h0 = 0; h0 < heads; h0 += 2) {
-      uint4 w[2][D / 64][2];
+    uint32_t sum[D / 64][16] = {};
+    auto add_up = [&](auto tag) {
+      for (int h0 = 0; h0 < heads; h0 += 2) {
+        uint4 w[2][D / 64][2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int j = 0; j < D / 64; ++j) {
-          const uint4* qp = reinterpret_cast<const uint4*>(qt + (int64_t)min(h0 + i, heads - 1) * a.q_hs + 64 * j);
-          w[i][j][0] = qp[0];
-          w[i][j][1] = qp[1];
+          for (int j = 0; j < D / 64; ++j) {
+            const uint4* qp = reinterpret_cast<const uint4*>(qt + (int64_t)min(h0 + i, heads - 1) * a.q_hs + 64 * j);
+            w[i][j][0] = qp[0];
+            w[i][j][1] = qp[1];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float fi = h0 + i < heads ? f : 0.f;
+#pragma unroll
+          for (int j = 0; j < D / 64; ++j) {
+            add_whole<decltype(tag)::value>(w[i][j][0], fi, sum[j]);
+            add_whole<decltype(tag)::value>(w[i][j][1], fi, sum[j] + 8);
+          }
         }
       }
+    };
+    if (odd) add_up(std::true_type{});
+    else add_up(std::false_type{});
+    uint32_t s[D / 64][8];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float fi = h0 + i < heads ? f : 0.f;
-#pragma unroll
-        for (int j = 0; j < D / 64; ++j) {
-          add_whole(w[i][j][0], fi, s[j]);
-          add_whole(w[i][j][1], fi, s[j] + 4);
-        }
-      }
-    }
+    for (int j = 0; j < D / 64; ++j) pair_up(sum[j], (heads + 1) / 2 * 2, s[j]);
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) {
       uint4* to = qfrag + (u * KS + sign * (D / 64) + j) * 64 + 16 * g + 2 * tn;

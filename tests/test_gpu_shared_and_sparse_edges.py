@@ -176,3 +176,21 @@ def test_drawn_steps(seed):
     out = ops.paged_attention_sparse(g["q"], g["kc"], g["vc"], plan, sel.to(DEV), d ** -0.5, key_scale=g["ks"],
                                      value_scale=g["vs"])
     sparse.check_attention(s, sel, out.cpu(), d ** -0.5, some)
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(28, 4, 128), (14, 2, 64)])
+def test_prompts_with_query_values_that_are_not_finite(hq, hkv, d):
+    """They count as zero, beside tokens of the same tile that have none."""
+    s = sparse.make([(45, 200)], hq, hkv, d, 3, seed=12)
+    s["q"][3, 1, 5], s["q"][3, 2, 9], s["q"][20, 0, 0] = float("nan"), float("-inf"), float("inf")
+    s["q"][21] = float("nan")
+    s["q"][33, :, :] *= 2.0 ** 100
+    s["q"][34, :, :] *= 2.0 ** -120
+    b, e = sparse.random_bounds(s, 3)
+    g = sparse.on_gpu(s)
+    out = ops.select_blocks(g["q"], sparse.make_plan(g, 7, 1, 2), b.to(DEV), e8m0(e)).cpu()
+    for t, r, pos in sparse.tokens_of(s):
+        rows = s["table"][r].long()
+        for h in range(hkv):
+            q = s["q"][t, h * (hq // hkv):(h + 1) * (hq // hkv)]
+            assert out[t, h].tolist() == ref.select(q, b[rows, h, 0], b[rows, h, 1], e[rows, h], pos // 3 + 1, 7, 1, 2), t
