@@ -168,6 +168,8 @@ __global__ __launch_bounds__(kPlanT) void sparse_plan_kernel(PlanArgs a) {
 
 // ------------------------------------------------------------------ bounds
 
+typedef int16_t short2_t __attribute__((ext_vector_type(2)));
+
 struct SummaryArgs {
   const uint16_t* kc;
   const uint8_t* ks;
@@ -192,9 +194,11 @@ __device__ __forceinline__ int bound_exp(uint32_t amax) {
 
 // WPB waves take a (block, KV head): 64 / (D / 8) rows a pass, a lane 8 dims of one.
 // Blocks of 64 keys and more are cut over the work-group's four waves: a decode step
-// has few blocks, and the rows of one are loaded at once.  Waiting bounds it: plan,
-// touched block, keys.  A decode step's 64 blocks of 64 keys, 8 heads: 5.8 us; a prompt
-// step's 1,000 blocks of 16: 14.0.
+// has few blocks, and the rows of one are loaded at once.  Waiting bounds it (plan,
+// touched block, keys), and instructions where there are many blocks, so values are
+// compared two at a time as whole numbers; only a wave that meets one that is not finite
+// goes over its rows again, one by one.  A decode step's 64 blocks of 64 keys, 8 heads:
+// 4.4 us; a prompt step's 1,000 blocks of 16: 10.4 (5.8 and 13.9 one by one).
 template <int D, bool F8, int WPB>
 __global__ __launch_bounds__(kSparseThreads) void summarize_kernel(SummaryArgs a) {
   constexpr int CH = D / 8, RPW = 64 / CH, DEEP = 8;
@@ -212,28 +216,71 @@ __global__ __launch_bounds__(kSparseThreads) void summarize_kernel(SummaryArgs a
   if (WPB == 1 && !live) return;
   const int64_t row = (int64_t)a.hkv * D;
   const int64_t at = (int64_t)t.x * a.bs * row + (int64_t)h * D + 8 * c;
-  float hi[8], nlo[8];
-  uint32_t bad = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) hi[i] = nlo[i] = -INFINITY;
   const float f8 = F8 && live ? __uint_as_float((uint32_t)a.ks[(int64_t)t.x * a.hkv + h] << 23) : 0.f;
-  const int rows = live ? held : 0;
-  for (int j0 = sub * RPW + r; j0 < rows; j0 += DEEP * WPB * RPW) {
-    uint4 w[DEEP];
+  const int rows = __builtin_amdgcn_readfirstlane(live ? held : 0);
+  // f of each row's 8 dims, some rows (the last one) more than once
+  auto each = [&](auto f) {
+    for (int j0 = __builtin_amdgcn_readfirstlane(sub) * RPW; j0 < rows; j0 += DEEP * WPB * RPW) {
+      uint4 w[DEEP];
 #pragma unroll
-    for (int u = 0; u < DEEP; ++u) {
-      const int j = min(j0 + u * WPB * RPW, rows - 1);         // (the last row again)
-      if constexpr (F8) {
-        const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(a.kc) + at + j * row);
-        const uint2 lo = fp8x4_to_bf16(x.x, f8), up = fp8x4_to_bf16(x.y, f8);
-        w[u] = make_uint4(lo.x, lo.y, up.x, up.y);
-      } else {
-        w[u] = *reinterpret_cast<const uint4*>(a.kc + at + j * row);
+      for (int u = 0; u < DEEP; ++u) {
+        if (j0 + u * WPB * RPW >= rows) continue;
+        const int j = min(j0 + r + u * WPB * RPW, rows - 1);
+        if constexpr (F8) {
+          const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(a.kc) + at + j * row);
+          const uint2 lo = fp8x4_to_bf16(x.x, f8), up = fp8x4_to_bf16(x.y, f8);
+          w[u] = make_uint4(lo.x, lo.y, up.x, up.y);
+        } else {
+          w[u] = *reinterpret_cast<const uint4*>(a.kc + at + j * row);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < DEEP; ++u)
+        if (j0 + u * WPB * RPW < rows) f(w[u]);
+    }
+  };
+  // Two dims at a time, as whole numbers in the values' order: bits of negative values
+  // turned but for the sign (which turns them back, too).
+  auto turned = [](short2_t x) { return x ^ ((x >> 15) & (short2_t)(int16_t)0x7fff); };
+  short2_t top[4], low[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { top[i] = (short2_t)INT16_MIN; low[i] = (short2_t)INT16_MAX; }
+  each([&](const uint4& w) {
+    const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const short2_t x = turned(__builtin_bit_cast(short2_t, p[i]));
+      top[i] = __builtin_elementwise_max(top[i], x);
+      low[i] = __builtin_elementwise_min(low[i], x);
+    }
+  });
+  float hi[8], nlo[8];
+  uint32_t bad = 0;                          // dims with a value that is not finite
+  constexpr int16_t kMost = 0x7f7f;          // the largest finite value; the least is ~kMost
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) odd |= top[i][0] > kMost || top[i][1] > kMost || low[i][0] < ~kMost || low[i][1] < ~kMost;
+  if (!__any(odd && rows > 0)) {
+#pragma unroll
+    for (int d = CH; d < 64; d <<= 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        top[i] = __builtin_elementwise_max(top[i], __builtin_bit_cast(short2_t, __shfl_xor(__builtin_bit_cast(int, top[i]), d)));
+        low[i] = __builtin_elementwise_min(low[i], __builtin_bit_cast(short2_t, __shfl_xor(__builtin_bit_cast(int, low[i]), d)));
       }
     }
+    const bool some = sub * RPW < rows;      // (a wave without rows knows nothing)
 #pragma unroll
-    for (int u = 0; u < DEEP; ++u) {
-      const uint32_t p[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t x = __builtin_bit_cast(uint32_t, turned(top[i >> 1])), y = __builtin_bit_cast(uint32_t, turned(low[i >> 1]));
+      hi[i] = some ? (i & 1 ? aia::bf16_hi(x) : aia::bf16_lo(x)) : -INFINITY;
+      nlo[i] = some ? -(i & 1 ? aia::bf16_hi(y) : aia::bf16_lo(y)) : -INFINITY;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) hi[i] = nlo[i] = -INFINITY;
+    each([&](const uint4& w) {
+      const uint32_t p[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float x = i & 1 ? aia::bf16_hi(p[i >> 1]) : aia::bf16_lo(p[i >> 1]);
@@ -242,16 +289,16 @@ __global__ __launch_bounds__(kSparseThreads) void summarize_kernel(SummaryArgs a
         hi[i] = fmaxf(hi[i], ok ? x : -INFINITY);
         nlo[i] = fmaxf(nlo[i], ok ? -x : -INFINITY);
       }
-    }
-  }
+    });
 #pragma unroll
-  for (int d = CH; d < 64; d <<= 1) {
+    for (int d = CH; d < 64; d <<= 1) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], d));
-      nlo[i] = fmaxf(nlo[i], __shfl_xor(nlo[i], d));
+      for (int i = 0; i < 8; ++i) {
+        hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], d));
+        nlo[i] = fmaxf(nlo[i], __shfl_xor(nlo[i], d));
+      }
+      bad |= (uint32_t)__shfl_xor((int)bad, d);
     }
-    bad |= (uint32_t)__shfl_xor((int)bad, d);
   }
   if constexpr (WPB > 1) {
     if (r == 0) {
