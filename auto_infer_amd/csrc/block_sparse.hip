@@ -34,7 +34,7 @@ constexpr int64_t kPartRows = 1ll << 20;      // and partial rows
 // of the L2's channels.)  512 tokens behind 32K, 28/4 heads of 128, 32 of 513 blocks of 64
 // each, chosen by chance: 180 us in 16 ranges, 186 in 8, 199 in 24, 226 in 32, 345
 // without: a wave's start, four dependent round trips, costs as much as the ranges' L2
-// hits save.
+// hits save.  (Later steps took the 16 to 167.)
 struct SparseCut {
   int32_t parts, tokens;     // tokens per launch
   bool ranges;
@@ -1018,7 +1018,8 @@ __global__ __launch_bounds__(64 * kSpWaves) __attribute__((amdgpu_waves_per_eu(3
 
 // One wave: 16 query heads of a token and KV head and the selected blocks in one range
 // of the context.  A range is taken on one XCD (block ids are dealt to the eight in
-// turn).
+// turn).  Four of five lines come from L2, 14 TB/s in all; L1, LDS and VALU are busy a
+// third of the time each.
 template <int D, bool F8, bool WHOLE>
 __global__ __launch_bounds__(64 * kSpWaves) __attribute__((amdgpu_waves_per_eu(3, 3))) void sparse_range_kernel(SparseArgs a) {
   __shared__ __attribute__((aligned(16))) uint16_t vt[kSpWaves][kStep];
