@@ -517,7 +517,7 @@ constexpr int kScoreTiles = 4, kTileTokens = 8 * kScoreTiles;
 // Q B^T on v_mfma_i32_16x16x64_i8, lane (row or block n, group g) with bytes 64 j + 16 g ..
 // of [sum q+ (D), sum q- (D)] and of [hi, nlo]; the four accumulators are tokens 2 g and
 // 2 g + 1 against block n.  Tokens of several requests are taken one request at a time.
-//   512 tokens, 28/4 heads, 513 blocks: 12 us, with the selection 20.5; 25.1 with one tile a
+//   512 tokens, 28/4 heads, 513 blocks: 12 us, with the selection 19.4; before a later step 20.5, 25.1 with one tile a
 // work-group, 20.6 with two, 26.2 with eight.  Waiting bounds it, and the instructions that
 // turn the queries to whole numbers; a row per head instead of two per token took 28.0.
 template <int D>
@@ -692,7 +692,7 @@ __device__ __forceinline__ uint32_t key_of(const SelectArgs& a, float score, int
 // A wave per row, for tables of up to 64 NK blocks: the key of the `selected`-th largest
 // score bit by bit, from the highest bit in which the scores differ, counting by ballots,
 // until a bound has exactly so many above it; then the blocks above it and the first of those at it, in order.  No
-// barriers, no LDS.  2048 rows of 513 blocks: 8.8 us; a work-group per row that counts
+// barriers, no LDS.  2048 rows of 513 blocks: 7.9 us; a work-group per row that counts
 // digits in LDS: 17.0.
 template <int NK>
 __global__ __launch_bounds__(256) void select_wave_kernel(SelectArgs a) {
@@ -765,7 +765,7 @@ constexpr int kDigits = 2048;
 // A work-group per row, for longer tables: the same key by up to 11 bits at a time of what
 // it is above the row's least one, counted in LDS.  (Without the least taken off, the
 // first digit is mostly the exponent: one pass more and counters that many lanes hit at
-// once, 10.5 us for 64 rows of 1875 to 4096 blocks; 9.5 so, of which waiting for the scores
+// once, 10.5 us for 64 rows of 1875 to 4096 blocks; 7.5 so, of which waiting for the scores
 // and the launch are most.)  A wave has a run of the row's blocks,
 // up to 64 NK of them in registers (NK 0: any number, read again in every pass).
 template <int NK>
@@ -1225,13 +1225,21 @@ extern "C" int aia_select_blocks(const void* query, int64_t q_token_stride, int6
                        : (head_dim == 128 ? score_token_kernel<128> : score_token_kernel<64>);
     score<<<grid, kSparseThreads, 0, st>>>(a);
     if (int rc = check_hip(hipGetLastError(), "aia_select_blocks: score launch")) return rc;
+    // (keys held for the table's width and little more: places behind it cost what keys
+    // do, 22.2 us instead of 20.3 for 4,096 blocks with twice as many)
     if (table_width <= 1024) {
-      auto* kernel = table_width <= 256 ? select_wave_kernel<4> : table_width <= 512 ? select_wave_kernel<8>
-                     : table_width <= 768 ? select_wave_kernel<12> : select_wave_kernel<16>;
+      auto* kernel = table_width <= 256   ? select_wave_kernel<4>
+                     : table_width <= 384 ? select_wave_kernel<6>
+                     : table_width <= 512 ? select_wave_kernel<8>
+                     : table_width <= 640 ? select_wave_kernel<10>
+                     : table_width <= 768 ? select_wave_kernel<12>
+                                          : select_wave_kernel<16>;
       kernel<<<(unsigned)((s.rows + 3) / 4), 256, 0, st>>>(s);
     } else {
-      auto* kernel = table_width <= 4 * kSelThreads ? select_kernel<4> : table_width <= 16 * kSelThreads ? select_kernel<16>
-                     : select_kernel<0>;
+      auto* kernel = table_width <= 4 * kSelThreads    ? select_kernel<4>
+                     : table_width <= 8 * kSelThreads  ? select_kernel<8>
+                     : table_width <= 16 * kSelThreads ? select_kernel<16>
+                                                       : select_kernel<0>;
       kernel<<<(unsigned)s.rows, kSelThreads, 0, st>>>(s);
     }
     if (int rc = check_hip(hipGetLastError(), "aia_select_blocks: select launch")) return rc;

@@ -194,3 +194,16 @@ def test_prompts_with_query_values_that_are_not_finite(hq, hkv, d):
         for h in range(hkv):
             q = s["q"][t, h * (hq // hkv):(h + 1) * (hq // hkv)]
             assert out[t, h].tolist() == ref.select(q, b[rows, h, 0], b[rows, h, 1], e[rows, h], pos // 3 + 1, 7, 1, 2), t
+
+
+@pytest.mark.parametrize("most", [250, 383, 500, 639, 760, 1023, 2000, 4000, 8000, 8300])
+def test_selections_over_tables_of_many_widths(most):
+    s = sparse.make([(1, most), (1, most // 2), (1, 70)], 4, 2, 64, 1, seed=most)
+    b, e = sparse.random_bounds(s, most)
+    g = sparse.on_gpu(s)
+    out = ops.select_blocks(g["q"], sparse.make_plan(g, 64, 1, 2), b.to(DEV), e8m0(e)).cpu()
+    for t, r, pos in sparse.tokens_of(s):
+        rows = s["table"][r].long()
+        for h in range(2):
+            want = ref.select(s["q"][t, 2 * h:2 * h + 2], b[rows, h, 0], b[rows, h, 1], e[rows, h], pos + 1, 64, 1, 2)
+            assert out[t, h].tolist() == want, (t, h)
