@@ -517,9 +517,10 @@ constexpr int kScoreTiles = 4, kTileTokens = 8 * kScoreTiles;
 // Q B^T on v_mfma_i32_16x16x64_i8, lane (row or block n, group g) with bytes 64 j + 16 g ..
 // of [sum q+ (D), sum q- (D)] and of [hi, nlo]; the four accumulators are tokens 2 g and
 // 2 g + 1 against block n.  Tokens of several requests are taken one request at a time.
-//   512 tokens, 28/4 heads, 513 blocks: 12 us, with the selection 19.4; before a later step 20.5, 25.1 with one tile a
-// work-group, 20.6 with two, 26.2 with eight.  Waiting bounds it, and the instructions that
-// turn the queries to whole numbers; a row per head instead of two per token took 28.0.
+//   512 tokens, 28/4 heads, 513 blocks: 12 us, with the selection 19.4.  (Before the
+// selection's last step 20.5, and 25.1 with one tile a work-group, 20.6 with two, 26.2 with
+// eight.)  Waiting bounds it, and the instructions that turn the queries to whole numbers;
+// a row per head instead of two per token took 28.0.
 template <int D>
 __global__ __launch_bounds__(kSparseThreads) void score_kernel(ScoreKernelArgs a) {
   constexpr int KS = 2 * D / 64;             // MFMA steps
