@@ -20,8 +20,8 @@ is checked for the first and uploaded; a device int32 tensor is taken as it is
 Device metadata attached by a packer is not checked on the host.  Query
 lengths that do not add up to the step's token count make the planner plan
 nothing (status -1); the attention call then fills its output with NaN.
-With ``AIA_CHECK_PLAN=1`` in the environment, ``step_plan`` also reads the
-status back after planning (one device synchronisation per step) and raises
+With ``AIA_CHECK_PLAN=1`` in the environment, the step plans also read the
+status back after planning (one device synchronisation per step) and raise
 the ValueError of the reference's stager contract
 (prefill_input_stager.py:77-81).
 
@@ -116,8 +116,11 @@ def step_shared_plan(ctx, num_q_heads, num_kv_heads, head_dim, block_size):
 def step_sparse_plan(ctx, num_q_heads, num_kv_heads, head_dim, block_size, num_selected, sink, local):
     def make():
         _no_prefixes(ctx, "block-sparse attention")
-        bt, cu, kv, T, owned, _ = _metadata(ctx, block_size)
-        return ops.BlockSparsePlan(bt, cu, kv, T, num_q_heads, num_kv_heads, head_dim, block_size,
+        bt, cu, kv, T, owned, packed = _metadata(ctx, block_size)
+        plan = ops.BlockSparsePlan(bt, cu, kv, T, num_q_heads, num_kv_heads, head_dim, block_size,
                                    num_selected, sink, local, owned=owned)
+        if packed and _checking():
+            plan.status()
+        return plan
     return _plan_of(ctx, ("sparse", num_q_heads, num_kv_heads, head_dim, block_size, num_selected, sink,
                           local), make)

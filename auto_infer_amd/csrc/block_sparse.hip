@@ -94,16 +94,19 @@ struct PlanArgs {
   const int32_t* bt;
   int64_t bt_stride;
   int32_t batch, tokens, bs, width;
-  int32_t* hdr;              // {blocks written to by the step, most blocks that a token sees}
-  int4* tok;                 // {request or -1, position, visible blocks, 0}
+  int32_t* hdr;              // {blocks written to by the step, most blocks that a token sees, status}
+  int4* tok;                 // {request, -1 or kBadStep, position, visible blocks, 0}
   int4* touched;             // {block id, keys that it holds, 0, 0}
   int32_t touched_cap;
 };
 
 constexpr int kPlanT = 1024;
+constexpr int kBadStep = -2;               // request of all tokens where the lengths describe more than the step
 
 // Every work-group counts the blocks that each request's new tokens fall into (and
-// those of the requests before it), then places its own kPlanT tokens.
+// those of the requests before it), then places its own kPlanT tokens.  Every block that is
+// counted is written by the first of its tokens, so lengths whose tokens are not all the
+// step's give no blocks at all and a status.
 __global__ __launch_bounds__(kPlanT) void sparse_plan_kernel(PlanArgs a) {
   extern __shared__ int lds[];               // cu (batch + 1), first touched entry (batch)
   int* cu = lds;
@@ -113,6 +116,14 @@ __global__ __launch_bounds__(kPlanT) void sparse_plan_kernel(PlanArgs a) {
   if (tid == 0) { carry = 0; most = 0; }
   for (int b = tid; b <= a.batch; b += kPlanT) cu[b] = a.cu[b];
   __syncthreads();
+  bool wrong = cu[0] != 0 || cu[a.batch] > a.tokens;
+  for (int b = tid; b < a.batch; b += kPlanT) wrong |= cu[b + 1] < cu[b];
+  const int t = blockIdx.x * kPlanT + tid;
+  if (__syncthreads_or(wrong)) {
+    if (blockIdx.x == 0 && tid == 0) { a.hdr[0] = 0; a.hdr[1] = 0; a.hdr[2] = -1; }
+    if (t < a.tokens) a.tok[t] = make_int4(kBadStep, -1, 0, 0);
+    return;
+  }
   for (int b0 = 0; b0 < a.batch; b0 += kPlanT) {
     const int b = b0 + tid;
     int n = 0;
@@ -139,8 +150,7 @@ __global__ __launch_bounds__(kPlanT) void sparse_plan_kernel(PlanArgs a) {
     if (tid == kPlanT - 1) carry = before + sum;
     __syncthreads();
   }
-  if (blockIdx.x == 0 && tid == 0) { a.hdr[0] = min(carry, a.touched_cap); a.hdr[1] = most; }
-  const int t = blockIdx.x * kPlanT + tid;
+  if (blockIdx.x == 0 && tid == 0) { a.hdr[0] = min(carry, a.touched_cap); a.hdr[1] = most; a.hdr[2] = 0; }
   if (t >= a.tokens) return;
   int lo = 0, hi = a.batch;                  // the last request that begins at or before t
   while (hi - lo > 1) {
@@ -953,6 +963,8 @@ struct SparseRow {
   }
   // row n's query head within the KV head's group
   __device__ __forceinline__ int head(int n) const { return hb * kRows + n; }
+  // what a row without keys has for a sum: NaN where the plan has none
+  __device__ __forceinline__ float no_keys() const { return tk.x == kBadStep ? __builtin_nanf("") : 0.f; }
   __device__ __forceinline__ const uint16_t* query(const SparseArgs& a, int n) const {
     return head(n) < a.c.group ? a.q + (int64_t)t * a.q_ts + (int64_t)(kvh * a.c.group + head(n)) * a.q_hs : nullptr;
   }
@@ -993,6 +1005,7 @@ __global__ __launch_bounds__(64 * kSpWaves) __attribute__((amdgpu_waves_per_eu(3
   attend<D, F8, WHOLE>(a.c, r.kvh, qf, t0 * kTile, min(keys, t1 * kTile), count, [&](int i) { return list[i]; },
                 reinterpret_cast<uint16_t*>(lds) + wid * kStep, lane, s);
   s.finish();
+  if (keys == 0) s.l = r.no_keys();
   __syncthreads();
   if (g == 0) { wave_m[wid][n] = s.m; wave_l[wid][n] = s.l; }
 #pragma unroll
@@ -1040,7 +1053,7 @@ __global__ __launch_bounds__(64 * kSpWaves) __attribute__((amdgpu_waves_per_eu(3
   const int64_t row = part_row(a, t, kvh, r.hb, part) + n;
   const bool live = r.head(n) < a.c.group;
   if (count == 0) {
-    if (live && g == 0) a.part_ml[row] = make_float2(-INFINITY, 0.f);
+    if (live && g == 0) a.part_ml[row] = make_float2(-INFINITY, r.no_keys());
     return;
   }
   RowState<D> s;

@@ -1100,6 +1100,15 @@ class BlockSparsePlan(_StepPlan):
                  batch, *rest, self.num_selected, self.workspace.data_ptr(), self.workspace.numel(),
                  stream)
 
+    def status(self):
+        """Synchronising check of the last plan: raises ValueError if cu_seqlens_q does not
+        begin at 0, decreases or ends behind ``num_tokens``; ``summarize_blocks`` then
+        wrote no bounds, nothing was selected and attention outputs are NaN."""
+        code = int(self.workspace[8:12].view(torch.int32).item())
+        if code != 0:
+            raise ValueError(f"block-sparse planner (status {code}): cu_seqlens_q does not describe "
+                             f"{self.num_tokens} query tokens")
+
 
 def _check_bounds(bounds, bounds_scale, plan, dev):
     _check_on(bounds, "bounds", torch.int8, dev)

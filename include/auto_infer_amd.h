@@ -281,7 +281,10 @@ int aia_paged_attention_shared(const void* query, int64_t q_token_stride, int64_
  * block_size * table_width below 2^31.  head_dim 128 or 64, at most 8192 requests, 256
  * query heads per KV head and 1024 selected blocks (AIA_ERR_UNSUPPORTED otherwise).
  * Query token i of request b stands at position Lk - Lq + i; tokens that no request
- * covers (cu_seqlens_q ends before num_tokens) select nothing and give zeros. */
+ * covers (cu_seqlens_q ends before num_tokens) select nothing and give zeros.  The
+ * int32 at byte offset 8 of the workspace is the plan's status: 0, or -1 where
+ * cu_seqlens_q does not begin at 0, decreases or ends behind num_tokens (no bounds are
+ * then written, nothing is selected and the outputs are NaN). */
 int aia_sparse_workspace_bytes(int32_t batch, int32_t num_tokens, int32_t num_q_heads,
                                int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
                                int32_t table_width, int32_t num_selected, int64_t* bytes);
