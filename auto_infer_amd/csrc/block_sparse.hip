@@ -62,7 +62,7 @@ SparseCut sparse_cut(int32_t batch, int32_t tokens, int32_t hkv, int32_t hblocks
 }
 
 struct SparseLayout {
-  int64_t hdr, tok, touched, scores, part_o, part_ml, total;
+  int64_t hdr, tok, touched, scores, part_o, part_head, total;
   int32_t touched_cap, score_tokens, hblocks;
   SparseCut cut;
 };
@@ -81,8 +81,8 @@ SparseLayout sparse_layout(int32_t batch, int32_t tokens, int32_t hq, int32_t hk
   L.scores = L.touched + up(16ll * L.touched_cap);
   L.part_o = L.scores + up(4ll * L.score_tokens * hkv * width);
   const int64_t rows = L.cut.parts > 1 ? (int64_t)L.cut.parts * L.cut.tokens * hkv * L.hblocks * kRows : 0;
-  L.part_ml = L.part_o + up(2 * rows * d);
-  L.total = L.part_ml + up(8 * rows);
+  L.part_head = L.part_o + up(2 * rows * d);
+  L.total = L.part_head + up((int64_t)sizeof(PartHead) * rows);
   return L;
 }
 
@@ -914,7 +914,7 @@ struct SparseArgs {
   uint16_t* out;
   int64_t o_ts, o_hs;
   uint16_t* part_o;          // (token, KV head, head block, part): 16 rows of D
-  float2* part_ml;
+  PartHead* part_head;
 };
 
 constexpr int kSpWaves = 4;
@@ -1026,7 +1026,7 @@ __global__ __launch_bounds__(64 * kSpWaves) __attribute__((amdgpu_waves_per_eu(3
     for (int dt = 0; dt < DT; ++dt) o[dt] += join[i][dt][lane] * w;
   }
   const bool live = r.head(n) < a.c.group;
-  if (a.parts > 1) write_part<D>(a.part_o, a.part_ml, part_row(a, r.t, r.kvh, r.hb, part) + n, o, m, l, live, g);
+  if (a.parts > 1) write_part<D>(a.part_o, a.part_head, part_row(a, r.t, r.kvh, r.hb, part) + n, o, m, l, live, g);
   else if (live) write_out<D>(r.output(a, n), o, l, g);
 }
 
@@ -1053,7 +1053,7 @@ __global__ __launch_bounds__(64 * kSpWaves) __attribute__((amdgpu_waves_per_eu(3
   const int64_t row = part_row(a, t, kvh, r.hb, part) + n;
   const bool live = r.head(n) < a.c.group;
   if (count == 0) {
-    if (live && g == 0) a.part_ml[row] = make_float2(-INFINITY, r.no_keys());
+    if (live && g == 0) a.part_head[row] = no_part(r.no_keys());
     return;
   }
   RowState<D> s;
@@ -1061,7 +1061,7 @@ __global__ __launch_bounds__(64 * kSpWaves) __attribute__((amdgpu_waves_per_eu(3
   __builtin_amdgcn_wave_barrier();           // the list is the wave's own
   attend<D, F8, WHOLE>(a.c, kvh, qf, 0, keys, count, [&](int j) { return list[wid][j]; }, vt[wid], lane, s);
   s.finish();
-  write_part<D>(a.part_o, a.part_ml, row, s.o, s.m, s.l, live, g);
+  write_part<D>(a.part_o, a.part_head, row, s.o, s.m, s.l, live, g);
 }
 
 // The parts of each row, joined.
@@ -1072,7 +1072,7 @@ __global__ __launch_bounds__(256) void sparse_join_kernel(SparseArgs a) {
   if (head >= hq) return;
   const int kvh = head / a.c.group, hh = head - kvh * a.c.group;
   const int64_t first = part_row(a, t, kvh, hh / kRows, 0) + hh % kRows;
-  join_row<D, W>(a.part_o, a.part_ml, a.parts, [&](int i) { return first + i * kRows; },
+  join_row<D, W>(a.part_o, a.part_head, a.parts, [&](int i) { return first + i * kRows; },
                  a.out + (int64_t)t * a.o_ts + (int64_t)head * a.o_hs);
 }
 
@@ -1299,7 +1299,7 @@ extern "C" int aia_paged_attention_sparse(const void* query, int64_t q_token_str
   a.sel = selected; a.sel_ts = sel_token_stride; a.sel_hs = sel_head_stride; a.selected = num_selected;
   a.parts = L.cut.parts; a.hdr = reinterpret_cast<const int32_t*>(ws + L.hdr);
   a.out = static_cast<uint16_t*>(out); a.o_ts = out_token_stride; a.o_hs = out_head_stride;
-  a.part_o = reinterpret_cast<uint16_t*>(ws + L.part_o); a.part_ml = reinterpret_cast<float2*>(ws + L.part_ml);
+  a.part_o = reinterpret_cast<uint16_t*>(ws + L.part_o); a.part_head = reinterpret_cast<PartHead*>(ws + L.part_head);
   hipStream_t s = (hipStream_t)stream;
   for (int t0 = 0; t0 < num_tokens; t0 += L.cut.tokens) {
     a.t0 = t0;

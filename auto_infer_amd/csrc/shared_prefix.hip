@@ -55,7 +55,7 @@ struct Entity {
 };
 
 struct ShLayout {
-  int64_t hdr, lead, common, place, tokreq, order, ent, rec, part_ml, part_o, total;
+  int64_t hdr, lead, common, place, tokreq, order, ent, rec, part_head, part_o, total;
   int32_t wg_cap;
   int64_t part_cap;
 };
@@ -74,8 +74,8 @@ ShLayout sh_layout(int32_t batch, int32_t tokens, int32_t hq, int32_t hkv, int32
   L.order = L.tokreq + up(16ll * tokens);
   L.ent = L.order + up(4ll * tokens);
   L.rec = L.ent + up((int64_t)sizeof(Entity) * 2 * batch);
-  L.part_ml = L.rec + up(4ll * kRecord * L.wg_cap);
-  L.part_o = L.part_ml + up(8 * L.part_cap);
+  L.part_head = L.rec + up(4ll * kRecord * L.wg_cap);
+  L.part_o = L.part_head + up((int64_t)sizeof(PartHead) * L.part_cap);
   L.total = L.part_o + up(2 * L.part_cap * d);
   return L;
 }
@@ -343,7 +343,7 @@ struct ShArgs {
   uint16_t* out;
   int64_t o_ts, o_hs;
   uint16_t* part_o;
-  float2* part_ml;
+  PartHead* part_head;
   int64_t part_cap;
   // for the join
   const Entity* ent;
@@ -397,7 +397,7 @@ __device__ __forceinline__ void finish_row(const ShArgs& a, const Unit& u, int k
     return;
   }
   const int64_t prow = u.part + (int64_t)kvh * u.rows + row;
-  write_part<D>(a.part_o, a.part_ml, prow, o, m, l, live && prow < a.part_cap, g);
+  write_part<D>(a.part_o, a.part_head, prow, o, m, l, live && prow < a.part_cap, g);
 }
 
 // A unit: K and V in tiles of 64 keys, staged once for the four waves in one of two
@@ -840,7 +840,7 @@ __global__ __launch_bounds__(256) void shared_join_kernel(ShArgs a) {
   int n0, n1 = 0;
   parts_of(own, tk.y * a.c.group + hh, kvh, a.hkv, at0, step0, n0);
   if (sh.rows > 0) parts_of(sh, (tk.w + tk.y) * a.c.group + hh, kvh, a.hkv, at1, step1, n1);
-  join_row<D, W>(a.part_o, a.part_ml, n0 + n1, [&](int i) { return i < n0 ? at0 + i * step0 : at1 + (i - n0) * step1; }, op);
+  join_row<D, W>(a.part_o, a.part_head, n0 + n1, [&](int i) { return i < n0 ? at0 + i * step0 : at1 + (i - n0) * step1; }, op);
 }
 
 int sh_check(const char* what, int32_t batch, int32_t tokens, int32_t hq, int32_t hkv, int32_t d, int32_t bs,
@@ -963,7 +963,7 @@ extern "C" int aia_paged_attention_shared(const void* query, int64_t q_token_str
   a.bt = block_table; a.bt_stride = block_table_stride; a.batch = batch; a.tokens = num_tokens; a.width = table_width;
   a.hdr = ints(L.hdr); a.rec = ints(L.rec); a.order = ints(L.order);
   a.out = static_cast<uint16_t*>(out); a.o_ts = out_token_stride; a.o_hs = out_head_stride;
-  a.part_o = reinterpret_cast<uint16_t*>(ws + L.part_o); a.part_ml = reinterpret_cast<float2*>(ws + L.part_ml);
+  a.part_o = reinterpret_cast<uint16_t*>(ws + L.part_o); a.part_head = reinterpret_cast<PartHead*>(ws + L.part_head);
   a.part_cap = L.part_cap;
   a.ent = reinterpret_cast<const Entity*>(ws + L.ent);
   a.tokreq = reinterpret_cast<const int4*>(ws + L.tokreq); a.hq = num_q_heads; a.hkv = num_kv_heads;
