@@ -853,8 +853,8 @@ int sh_check(const char* what, int32_t batch, int32_t tokens, int32_t hq, int32_
   if (batch > kMaxShared) return fail(AIA_ERR_UNSUPPORTED, "%s: %d requests (at most %d)", what, batch, kMaxShared);
   if ((int64_t)bs * width > INT32_MAX - 128 * kKeys)
     return fail(AIA_ERR_UNSUPPORTED, "%s: contexts of 2^31 tokens and more", what);
-  // partial rows are numbered in 32 bits
-  if (2ll * tokens * hq * kShWaves + 2ll * kTargetGroups * kUnitRows > INT32_MAX / 2)
+  // partial rows (part_cap of them at most) are numbered in 32 bits
+  if (2ll * tokens * hq + (int64_t)kTargetGroups * kUnitRows > INT32_MAX)
     return fail(AIA_ERR_UNSUPPORTED, "%s: %d tokens of %d heads in one step", what, tokens, hq);
   return AIA_OK;
 }
