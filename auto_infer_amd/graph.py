@@ -55,7 +55,7 @@ class DecodeGraph(_GearGraph):
     new rows at the stager's slots in a launch of its own.  ``softcap`` /
     ``alibi_slopes``: as ``ops.paged_attention_gqa`` takes them.
     ``share_prefixes=True``: cache blocks that the step's requests have in common
-    (those with the same first block) are read once for them; the new rows are
+    (``ops.SharedPrefixPlan``, by their tables) are read once for them; the new rows are
     written in a launch of their own.
     """
 

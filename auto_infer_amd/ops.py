@@ -1008,10 +1008,11 @@ class SharedPrefixPlan(_StepPlan):
     layers, for ``paged_attention_shared``.
 
     Metadata as ``AttentionPlan`` takes it.  ``group_ids`` (B,) int32 on the device
-    names each request's group (negative: alone); without it, requests with the same
-    first block form a group.  What a group shares is found on the GPU: the leading
-    keys, in front of the new tokens, for which the block table rows agree, from 128
-    keys on.  A wrong group costs speed, never the result.  The plan holds scratch
+    names requests that may share (negative: alone); without it, those with the same
+    first block may.  What they share is found on the GPU: each goes with the ones that
+    agree with it in most keys times requests, from 128 keys on and in powers of two, and
+    such a group shares the leading keys, in front of the new tokens, for which all its
+    block table rows agree.  A wrong group costs speed, never the result.  The plan holds scratch
     space, so its calls run on one stream at a time.
     """
 

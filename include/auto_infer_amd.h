@@ -239,11 +239,13 @@ int aia_paged_attention_gqa_ex(const void* query, int64_t q_token_stride, int64_
  * (standard layout, bf16 or 8-bit caches, no modified scores), with the keys that
  * requests have in common read once for all of them.  No counterpart in the reference.
  * Same results as one request at a time, but for roundings.
- * aia_shared_plan, once per step, finds what is shared: requests of one group_ids entry
- * (negative: alone; NULL: of one first block id) share the leading keys, in front of
- * their new tokens, for which their block table rows hold the same block ids as the
- * group's first request, at least 128 keys.  A wrong group costs speed, never the
- * result.  Requests of 128 query rows (tokens x heads per KV head) and more, which use
+ * aia_shared_plan, once per step, finds what is shared.  Requests of one group_ids entry
+ * (negative: alone; NULL: of one first block id) are compared in the blocks of their
+ * 128th, 256th, 512th, .. key, as far as those lie in front of their new tokens; each
+ * takes the length at which keys times requests that agree with it are most, and those
+ * of one length and block form a group.  A group shares the leading keys, in front of
+ * its requests' new tokens, for which their block table rows hold the same block ids as
+ * its first one's.  A wrong group costs speed, never the result.  Requests of 128 query rows (tokens x heads per KV head) and more, which use
  * every key that often anyway, do not share.
  * Workspace: aia_shared_workspace_bytes long, 256-byte aligned, the same sizes in every
  * call; it holds the plan and the partials, so it serves one stream at a time.  The
