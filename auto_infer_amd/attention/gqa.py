@@ -143,7 +143,7 @@ class GqaHipBackend(AttentionBackend):
             raise ValueError("the context has no cos / sin: give the backend a rope, or rope=False "
                              "for a model without rotary positions")
         if self.rope is not None and self.rope is not False:
-            if self.fuse_pre_attention and not self._deferred(T, ctx):
+            if self.fuse_pre_attention and self._own_pair() and not self._deferred(T, ctx):
                 cache = ctx.kv_caches[layer_idx]
                 scales = dict(key_scale=cache[2], value_scale=cache[3]) if self.fp8 else {}
                 q = ops.rope_append(qkv, n_q, n_kv, ctx.positions, self.rope, cache[0], cache[1],
@@ -185,6 +185,11 @@ class GqaHipBackend(AttentionBackend):
                 and qkv.is_cuda and qkv.stride(-1) == 1 and aligned(qkv)
                 and all(t.dtype == torch.bfloat16 and t.numel() == T * hd and t.stride(-1) == 1
                         and aligned(t) for t in (ctx.cos, ctx.sin)))
+
+    def _own_pair(self):
+        """Whether the op pair is this class's: one that replaces either gets K and V."""
+        return (getattr(self._write_kv, "__func__", None) is GqaHipBackend._write_kv
+                and getattr(self._attn, "__func__", None) is GqaHipBackend._attn)
 
     def _deferred(self, T, ctx):
         """Whether the attention kernel writes the new rows."""
