@@ -29,12 +29,19 @@ constexpr int64_t kPartRows = 1ll << 20;      // and partial rows
 // more.  Many tokens of a request: their selections overlap in a context that no L2
 // holds, so the context (as long as the longest that a token sees, which the plan
 // knows) is cut into `parts` equal ranges, a multiple of the eight XCDs, so many that a
-// range's K and V fit an XCD's L2 in the longest context, and all tokens and KV heads
-// take a range there together.  (All KV heads: the rows of one of four lie in a quarter
-// of the L2's channels.)  512 tokens behind 32K, 28/4 heads of 128, 32 of 513 blocks of 64
-// each, chosen by chance: 180 us in 16 ranges, 186 in 8, 199 in 24, 226 in 32, 345
-// without: a wave's start, four dependent round trips, costs as much as the ranges' L2
-// hits save.  (Later steps took the 16 to 167.)
+// range's K and V fit an XCD's L2 in a context as long as the table, and all tokens and
+// KV heads take a range there together.  (All KV heads: the rows of one of four lie in a
+// quarter of the L2's channels.)  512 tokens behind 32K, 28/4 heads of 128, 32 of 513
+// blocks of 64 each, chosen by chance: 180 us in 16 ranges, 186 in 8, 199 in 24, 226 in
+// 32, 345 without: a wave's start, four dependent round trips, costs as much as the
+// ranges' L2 hits save.  (Later steps took the 16 to 154.)
+//   Ranges against parts, same heads and blocks, us: 32 tokens at 32K 28 and 29, 64 tokens
+// 39 and 37, 128 tokens 55 and 54, 256 tokens 86 and 117; at 16K two requests of 64 tokens
+// 53 and 48, eight of 16 80 and 72.
+//   There are 64 ranges at most: those of 131K tokens of 8 heads of 128 are 8.4 MB.  And the
+// table's width is what the host knows: in one much wider than the contexts ranges are
+// short and launches many.  512 tokens of 2K, 32/8 heads, 32 blocks of 16: 99 us in a table
+// of 128 columns, 370 in one of 8,192.
 struct SparseCut {
   int32_t parts, tokens;     // tokens per launch
   bool ranges;

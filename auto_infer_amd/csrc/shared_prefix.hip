@@ -680,7 +680,8 @@ __device__ __forceinline__ void unit_rows(const ShArgs& a, const Unit& u, uint16
     }
     __builtin_amdgcn_sched_barrier(0);
     if (MASK && *reinterpret_cast<volatile int*>(odd_tile + Bf) == t) {
-      // a masked tile with a value that is not finite: key by key (see attend())
+      // a masked tile with a value that is not finite, which a weight of zero would not
+      // take out: key by key, each row those that it sees
       for (int kk = 0; kk < 16 * ST; ++kk) {
         const int k = 16 * s0 + kk;
         const uint16_t* vs = vt + k * D + 4 * (g & 1);

@@ -89,7 +89,7 @@ __device__ __forceinline__ void soften(float (&x)[NT][4], float scale_log2, floa
 
 // Attends places [p0, p1) (p0 a multiple of 16) with rows qf, which all see them all.
 // id(i): the block id of list entry i, called with different i per lane, 0 <= i <
-// entries.  vt: kStep values of the wave's own LDS.  V behind p1 counts as zeros: a
+// entries.  lds: kStep values of the wave's own.  V behind p1 counts as zeros: a
 // weight of zero times an infinity or NaN there would not be zero.
 constexpr int kNt = 2;                           // tiles per step
 constexpr int kStep = kNt * kTile * kVStride;        // K or V values of a step in LDS

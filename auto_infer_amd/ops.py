@@ -1157,9 +1157,12 @@ def select_blocks(query, plan, bounds, bounds_scale, out=None):
 
     ``query`` (T, Hq, D) bf16 (rotated, as attention takes it); ``plan`` a
     ``BlockSparsePlan``; ``bounds`` / ``bounds_scale`` of ``summarize_blocks``.  A
-    block's score is an upper bound of the sum of the group's products with its keys,
-    in whole numbers (8-bit query values and bounds), so the selection does not
-    depend on any order of summation; of equal scores the lowest block wins."""
+    block's score bounds the sum of the group's products with its keys from above, up to
+    the query's rounding, in whole numbers (8-bit query values and bounds), so the selection
+    does not depend on any order of summation; of equal scores the lowest block wins.  The
+    query's values are rounded to whole numbers of up to 127 of one power of two for all of
+    the group's heads: a value below half of it, 1/127 to 1/254 of the group's largest,
+    counts as zero, and so does all of a head whose values are."""
     _check_device_tensor(query, "query", _BF16)
     dev = query.get_device()
     if query.shape != (plan.num_tokens, plan.num_q_heads, plan.head_dim) or query.stride(2) != 1:
