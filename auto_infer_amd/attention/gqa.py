@@ -26,7 +26,9 @@ common once for all of them (``ops.paged_attention_shared``; ``ctx.aia_group_ids
 the groups, else the first blocks do).  ``sparse_blocks=n`` lets every query token and KV
 head attend n cache blocks that an upper bound of their scores selects
 (``ops.select_blocks``), always the first ``sparse_sink`` and the last ``sparse_local``;
-the layers' caches then carry the blocks' bounds.
+the layers' caches then carry the blocks' bounds.  With a ``rope``, one launch turns Q
+and K and writes the caches (``ops.rope_append``) where the op pair is this class's own;
+a replaced ``_write_kv`` or ``_attn`` is given K and V.
 """
 import torch
 
